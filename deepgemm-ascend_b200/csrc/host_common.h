@@ -16,18 +16,23 @@ void count_kernel_launch(unsigned n = 1);
 bool overlap_launches_enabled();
 
 // Launch of a kernel that starts with griddepcontrol.wait: it may be scheduled while the kernel in front of it in the stream is
-// still draining.
-inline int launch_overlapped(const void* fn, dim3 grid, dim3 block, void** params, cudaStream_t stream, uint32_t smem_bytes = 0) {
+// still draining. `cluster`: CTAs of a thread-block cluster.
+inline int launch_overlapped(const void* fn, dim3 grid, dim3 block, void** params, cudaStream_t stream, uint32_t smem_bytes = 0, uint32_t cluster = 1) {
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
     cfg.blockDim = block;
     cfg.dynamicSmemBytes = smem_bytes;
     cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchAttribute attr[2];
     cfg.attrs = attr;
-    cfg.numAttrs = overlap_launches_enabled() ? 1 : 0;
+    if (overlap_launches_enabled()) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+    }
+    if (cluster > 1) {
+        attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        attr[cfg.numAttrs++].val.clusterDim = {cluster, 1, 1};
+    }
     const cudaError_t err = cudaLaunchKernelExC(&cfg, fn, params);
     if (err != cudaSuccess) {
         set_last_error("CUDA error %d (%s) at a kernel launch", (int)err, cudaGetErrorString(err));

@@ -1,0 +1,287 @@
+// Microscaled 4-bit operands: BF16 or FP32 values -> packed E2M1 with one UE8M0 scale per 32 values along K, in the layout the
+// GEMM reads, and back.
+//
+// Mathematics: over a block of 32 values, s = the smallest power of two with amax <= 6 s and q = x / s rounded to the nearest of
+// {0, 0.5, 1, 1.5, 2, 3, 4, 6} and their negatives, halves to the even code (the hardware conversion); s is a power of two, so
+// x / s is exact and that is the only rounding. A block that holds an infinity or a NaN gets the scale byte of NaN.
+//
+// Two directions, because the contraction of a product runs along the row of a K-major operand and down the rows of an MN-major
+// one: blocks of 32 lie along a row (K-major) or down a column (MN-major). Codes are packed in pairs along the row either way,
+// as the GEMM wants them.
+//
+// HBM-bound: n values read (2 or 4 bytes each), n / 2 + n / 32 bytes written, or the reverse.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/dg_b200.h"
+#include "host_common.h"
+#include "ptx.cuh"
+#include "quant.cuh"
+
+namespace dg {
+
+struct Fp4Args {
+    const uint8_t* x; uint64_t x_stride, x_group_stride;                  // bytes
+    uint8_t* codes; uint64_t code_stride, code_group_stride;              // bytes; a row holds cols / 2
+    uint8_t* sf; uint64_t sf_stride, sf_group_stride;                     // bytes; K-major: [ceil(cols / 64)][rows], MN-major: [ceil(rows / 64)][cols]
+    const int32_t* psum; uint32_t num_experts, alignment;
+    uint32_t rows, cols, tiles_r, tiles_c;
+};
+
+// Eight values of a lane, as they lie in memory.
+template <typename T> struct Raw8;
+template <> struct Raw8<__nv_bfloat16> {
+    uint4 a;
+    __device__ __forceinline__ void clear() { a = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void load(const uint8_t* p) { a = ld_stream_v4(p); }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) { v[2 * j] = bf16_lo(w[j]); v[2 * j + 1] = bf16_hi(w[j]); }
+    }
+};
+template <> struct Raw8<float> {
+    uint4 a, b;
+    __device__ __forceinline__ void clear() { a = b = make_uint4(0u, 0u, 0u, 0u); }
+    __device__ __forceinline__ void load(const uint8_t* p) { a = ld_global_v4(p); b = ld_global_v4(p + 16); }
+    __device__ __forceinline__ void values(float (&v)[8]) const {
+        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+    }
+};
+
+// Magnitudes are compared as bit patterns: infinities and NaN come out on top by themselves.
+__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+
+constexpr uint32_t kFp4Threads = 256, kFp4Rows = 32, kFp4Cols = 256;
+
+// K-major: one CTA = 32 rows x 256 columns, a warp takes four rows (all loads issued before the first is used), a lane eight
+// columns, four lanes a block. Scales go through shared memory, so that every scale column of the tile is one 64-byte run.
+template <typename T>
+__global__ void __launch_bounds__(kFp4Threads) quant_fp4_kernel(const Fp4Args a) {
+    constexpr uint32_t kWarpRows = kFp4Rows / (kFp4Threads / 32);
+    __shared__ __align__(8) uint8_t sf_smem[kFp4Rows][kFp4Cols / 32];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t tiles = a.tiles_r * a.tiles_c, group = blockIdx.x / tiles, tile = blockIdx.x - group * tiles;
+    const uint32_t row_base = tile / a.tiles_c * kFp4Rows, c0 = tile % a.tiles_c * kFp4Cols;
+    griddep_wait();
+    griddep_launch_dependents();
+    uint32_t row_end = min(a.rows, row_base + kFp4Rows);
+    if (a.psum != nullptr) row_end = min(row_end, group_end_of(a.psum, a.num_experts, a.alignment, row_base, lane).valid);
+    if (row_end <= row_base) return;                      // the whole tile is padding (uniform over the CTA)
+
+    const uint32_t c = c0 + lane * 8, r0 = row_base + warp * kWarpRows;
+    Raw8<T> raw[kWarpRows];
+    #pragma unroll
+    for (uint32_t i = 0; i < kWarpRows; ++i) {
+        raw[i].clear();
+        if (r0 + i < row_end && c < a.cols) raw[i].load(a.x + group * a.x_group_stride + (uint64_t)(r0 + i) * a.x_stride + (uint64_t)c * sizeof(T));
+    }
+    #pragma unroll
+    for (uint32_t i = 0; i < kWarpRows; ++i) {
+        float v[8];
+        raw[i].values(v);
+        uint32_t amax = 0;
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) amax = max(amax, magnitude_bits(v[j]));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const uint32_t e = e2m1_scale_byte(amax);
+        if (r0 + i < row_end && c < a.cols)
+            *reinterpret_cast<uint32_t*>(a.codes + group * a.code_group_stride + (uint64_t)(r0 + i) * a.code_stride + c / 2) = e2m1_pack8(v, e2m1_inverse(e));
+        // (the second block of a last, half-used scale column is zero)
+        if ((lane & 3u) == 0) sf_smem[warp * kWarpRows + i][lane / 4] = c < a.cols ? (uint8_t)e : (uint8_t)0;
+    }
+    __syncthreads();
+    const uint32_t col = threadIdx.x / kFp4Rows, r = threadIdx.x % kFp4Rows;
+    if (col < kFp4Cols / 64 && c0 + col * 64 < a.cols && r < row_end - row_base)
+        *reinterpret_cast<uint16_t*>(a.sf + group * a.sf_group_stride + (uint64_t)(c0 / 64 + col) * a.sf_stride + (uint64_t)(row_base + r) * 2) =
+            *reinterpret_cast<const uint16_t*>(&sf_smem[r][col * 2]);
+}
+
+// MN-major: one CTA = 64 rows x 256 columns. A warp takes one block of 32 rows x 64 columns: lane = (eight rows, eight columns), so
+// that a row of the warp's tile is a whole 128-byte line of BF16 and the maximum down a column takes two shuffles.
+template <typename T>
+__global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args a) {
+    __shared__ uint8_t sf_smem[2][kFp4Cols];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t tiles = a.tiles_r * a.tiles_c, group = blockIdx.x / tiles, tile = blockIdx.x - group * tiles;
+    const uint32_t row_base = tile / a.tiles_c * 64, c0 = tile % a.tiles_c * kFp4Cols;
+    const uint32_t half = warp / 4, tc = warp % 4 * 64 + lane % 8 * 8, c = c0 + tc;
+    const uint32_t r0 = row_base + half * 32 + lane / 8 * 8;
+    griddep_wait();
+    griddep_launch_dependents();
+    uint32_t row_end = min(a.rows, row_base + 64), write_end = row_end;
+    if (a.psum != nullptr) {
+        // (groups start on multiples of 64 rows: a tile lies in one) Rows of the padding count as zeros and are written as zeros
+        const GroupEnd end = group_end_of(a.psum, a.num_experts, a.alignment, row_base, lane);
+        if (end.whole <= row_base) return;                // behind the last group (uniform over the CTA)
+        row_end = min(row_end, end.valid);
+    }
+    Raw8<T> raw[8];
+    #pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        raw[i].clear();
+        if (r0 + i < row_end && c < a.cols) raw[i].load(a.x + group * a.x_group_stride + (uint64_t)(r0 + i) * a.x_stride + (uint64_t)c * sizeof(T));
+    }
+    uint32_t amax[8] = {};
+    #pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        float v[8];
+        raw[i].values(v);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) amax[j] = max(amax[j], magnitude_bits(v[j]));
+    }
+    float inv[8];
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], 8));
+        amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], 16));
+        const uint32_t e = e2m1_scale_byte(amax[j]);
+        inv[j] = e2m1_inverse(e);
+        // (blocks behind the last row are zero)
+        if (lane < 8) sf_smem[half][tc + j] = r0 < a.rows ? (uint8_t)e : (uint8_t)0;
+    }
+    #pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        float v[8];
+        raw[i].values(v);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= inv[j];
+        if (r0 + i < write_end && c < a.cols)
+            *reinterpret_cast<uint32_t*>(a.codes + group * a.code_group_stride + (uint64_t)(r0 + i) * a.code_stride + c / 2) = e2m1_pack8(v, 1.0f);
+    }
+    __syncthreads();
+    if (c0 + threadIdx.x < a.cols)
+        *reinterpret_cast<uint16_t*>(a.sf + group * a.sf_group_stride + (uint64_t)(row_base / 64) * a.sf_stride + (uint64_t)(c0 + threadIdx.x) * 2) =
+            (uint16_t)(sf_smem[0][threadIdx.x] | ((uint32_t)sf_smem[1][threadIdx.x] << 8));
+}
+
+// The way back: code x 2^(byte - 127), exact in FP32 and rounded once to BF16 (which changes it only where BF16 has subnormals).
+template <typename T>
+__device__ __forceinline__ void store8(uint8_t* p, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
+        uint32_t w[4];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            w[j] = *reinterpret_cast<const uint32_t*>(&b);
+        }
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+        *reinterpret_cast<float4*>(p + 16) = make_float4(v[4], v[5], v[6], v[7]);
+    }
+}
+__device__ __forceinline__ void e2m1_values8(uint32_t q, float (&v)[8]) {
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((q >> (8 * j)) & 0xffu), __NV_E2M1);
+        const float2 f = __half22float2(__half2(h));
+        v[2 * j] = f.x;
+        v[2 * j + 1] = f.y;
+    }
+}
+
+// One CTA = 32 rows x 256 columns, tiles and lanes as in the quantisers. The scales of a K-major tile come in runs down the rows,
+// through shared memory; an MN-major tile lies in one block of rows, whose scales lie along the columns.
+template <typename T, bool kMnMajor>
+__global__ void __launch_bounds__(kFp4Threads) dequant_fp4_kernel(const Fp4Args a, uint8_t* out) {
+    constexpr uint32_t kWarpRows = kFp4Rows / (kFp4Threads / 32);
+    __shared__ __align__(8) uint8_t sf_smem[kFp4Rows][kFp4Cols / 32];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t tiles = a.tiles_r * a.tiles_c, group = blockIdx.x / tiles, tile = blockIdx.x - group * tiles;
+    const uint32_t row_base = tile / a.tiles_c * kFp4Rows, c0 = tile % a.tiles_c * kFp4Cols;
+    const uint32_t c = c0 + lane * 8, r0 = row_base + warp * kWarpRows;
+    griddep_wait();
+    griddep_launch_dependents();
+    uint32_t q[kWarpRows];
+    #pragma unroll
+    for (uint32_t i = 0; i < kWarpRows; ++i)
+        q[i] = r0 + i < a.rows && c < a.cols ? ld_stream_u32(a.codes + group * a.code_group_stride + (uint64_t)(r0 + i) * a.code_stride + c / 2) : 0u;
+    const uint8_t* sf = a.sf + group * a.sf_group_stride;
+    float scale[8];
+    if constexpr (kMnMajor) {
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t pair = c < a.cols ? ld_global_u16(sf + (uint64_t)(row_base / 64) * a.sf_stride + (uint64_t)(c + j) * 2) : 0u;
+            scale[j] = ue8m0_value((pair >> (row_base / 32 % 2 * 8)) & 0xffu);
+        }
+    } else {
+        const uint32_t col = threadIdx.x / kFp4Rows, r = threadIdx.x % kFp4Rows;
+        if (col < kFp4Cols / 64 && c0 + col * 64 < a.cols && row_base + r < a.rows)
+            *reinterpret_cast<uint16_t*>(&sf_smem[r][col * 2]) = ld_global_u16(sf + (uint64_t)(c0 / 64 + col) * a.sf_stride + (uint64_t)(row_base + r) * 2);
+        __syncthreads();
+    }
+    #pragma unroll
+    for (uint32_t i = 0; i < kWarpRows; ++i) {
+        if (r0 + i >= a.rows || c >= a.cols) continue;
+        float v[8];
+        e2m1_values8(q[i], v);
+        const float s = kMnMajor ? 1.0f : ue8m0_value(sf_smem[warp * kWarpRows + i][lane / 4]);
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] *= kMnMajor ? scale[j] : s;
+        store8<T>(out + group * a.x_group_stride + (uint64_t)(r0 + i) * a.x_stride + (uint64_t)c * sizeof(T), v);
+    }
+}
+
+}  // namespace dg
+
+using namespace dg;
+
+// What both directions check: the float side is `x`, strides in elements of each side.
+static int fp4_args(Fp4Args& a, uint32_t tile_rows, uint32_t& tiles, const void* x, int is_fp32, uint64_t x_stride, uint64_t x_group_stride,
+                    uint32_t groups, uint32_t rows, uint32_t cols, const void* codes, uint64_t code_stride, uint64_t code_group_stride,
+                    const int16_t* sf, uint64_t sf_stride, uint64_t sf_group_stride, int mn_major) {
+    const uint64_t es = is_fp32 ? 4 : 2;
+    DG_CHECK_ARG(x != nullptr && codes != nullptr && sf != nullptr, "fp4: null pointer");
+    DG_CHECK_ARG(cols % 32 == 0, "fp4: the row length must be a multiple of 32");
+    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(x) & 15) == 0 && x_stride * es % 16 == 0 && x_group_stride * es % 16 == 0,
+                 "fp4: rows of values must start on 16-byte boundaries");
+    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(codes) & 3) == 0 && code_stride % 4 == 0 && code_group_stride % 4 == 0,
+                 "fp4: rows of codes must start on 4-byte boundaries");
+    DG_CHECK_ARG(sf_stride >= (mn_major ? cols : rows), "fp4: scale stride smaller than the rows (columns when MN-major)");
+    a.x = static_cast<const uint8_t*>(x); a.x_stride = x_stride * es; a.x_group_stride = x_group_stride * es;
+    a.codes = static_cast<uint8_t*>(const_cast<void*>(codes)); a.code_stride = code_stride; a.code_group_stride = code_group_stride;
+    a.sf = reinterpret_cast<uint8_t*>(const_cast<int16_t*>(sf)); a.sf_stride = sf_stride * 2; a.sf_group_stride = sf_group_stride * 2;
+    a.rows = rows; a.cols = cols;
+    a.tiles_r = (rows + tile_rows - 1) / tile_rows;
+    a.tiles_c = (cols + kFp4Cols - 1) / kFp4Cols;
+    DG_CHECK_ARG((uint64_t)a.tiles_r * a.tiles_c <= 0x7fffffffull / groups, "fp4: too many values");
+    tiles = groups * a.tiles_r * a.tiles_c;
+    return DG_OK;
+}
+
+extern "C" int dg_quant_fp4_launch(const void* x, int x_is_fp32, uint64_t x_stride, uint64_t x_group_stride, uint32_t groups, uint32_t rows,
+                                   uint32_t cols, int mn_major, const int32_t* psum, uint32_t num_experts, uint32_t alignment,
+                                   void* out, uint64_t out_stride, uint64_t out_group_stride,
+                                   int16_t* sf, uint64_t sf_stride, uint64_t sf_group_stride, void* stream) {
+    if (groups == 0 || rows == 0 || cols == 0) return DG_OK;
+    DG_CHECK_ARG(psum == nullptr || (groups == 1 && num_experts > 0 && alignment > 0 && alignment % (mn_major ? 64u : kFp4Rows) == 0),
+                 "quant_fp4: a psum layout needs one matrix, experts, and an alignment that is a multiple of %u", mn_major ? 64u : kFp4Rows);
+    Fp4Args a{};
+    uint32_t tiles = 0;
+    if (int rc = fp4_args(a, mn_major ? 64 : kFp4Rows, tiles, x, x_is_fp32, x_stride, x_group_stride, groups, rows, cols, out, out_stride,
+                          out_group_stride, sf, sf_stride, sf_group_stride, mn_major)) return rc;
+    a.psum = psum; a.num_experts = psum ? num_experts : 0; a.alignment = alignment;
+    const void* fn = mn_major ? (x_is_fp32 ? (const void*)quant_fp4_mn_kernel<float> : (const void*)quant_fp4_mn_kernel<__nv_bfloat16>)
+                              : (x_is_fp32 ? (const void*)quant_fp4_kernel<float> : (const void*)quant_fp4_kernel<__nv_bfloat16>);
+    void* params[] = {&a};
+    return launch_overlapped(fn, dim3(tiles), dim3(kFp4Threads), params, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int dg_dequant_fp4_launch(const void* codes, uint64_t code_stride, uint64_t code_group_stride, const int16_t* sf, uint64_t sf_stride,
+                                     uint64_t sf_group_stride, uint32_t groups, uint32_t rows, uint32_t cols, int mn_major,
+                                     void* out, int out_is_fp32, uint64_t out_stride, uint64_t out_group_stride, void* stream) {
+    if (groups == 0 || rows == 0 || cols == 0) return DG_OK;
+    Fp4Args a{};
+    uint32_t tiles = 0;
+    if (int rc = fp4_args(a, kFp4Rows, tiles, out, out_is_fp32, out_stride, out_group_stride, groups, rows, cols, codes, code_stride,
+                          code_group_stride, sf, sf_stride, sf_group_stride, mn_major)) return rc;
+    const void* fn = mn_major ? (out_is_fp32 ? (const void*)dequant_fp4_kernel<float, true> : (const void*)dequant_fp4_kernel<__nv_bfloat16, true>)
+                              : (out_is_fp32 ? (const void*)dequant_fp4_kernel<float, false> : (const void*)dequant_fp4_kernel<__nv_bfloat16, false>);
+    uint8_t* to = static_cast<uint8_t*>(out);
+    void* params[] = {&a, &to};
+    return launch_overlapped(fn, dim3(tiles), dim3(kFp4Threads), params, static_cast<cudaStream_t>(stream));
+}

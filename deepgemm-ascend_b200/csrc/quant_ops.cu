@@ -10,14 +10,13 @@
 // the padding of a psum layout skipped (:263-268).
 //
 // HBM-bound: 4 H bytes read and H + H/32 bytes written per token (2 H + H + H/32 without SwiGLU).
-#include <cuda_bf16.h>
-#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
 
 #include "../../include/dg_b200.h"
 #include "host_common.h"
 #include "ptx.cuh"
+#include "quant.cuh"
 
 namespace dg {
 
@@ -36,20 +35,6 @@ struct QuantArgs {
     float clamp; uint32_t has_clamp, swiglu;
 };
 
-// End of the valid tokens of the group [token_base, token_base + 32) in the psum layout (token_base when it is all
-// padding). The lanes of a warp look at 32 experts at a time, so the look-up is one round trip and not a binary search's five.
-__device__ __forceinline__ uint32_t valid_end_of(const QuantArgs& a, uint32_t token_base, uint32_t end, uint32_t lane) {
-    for (uint32_t e0 = 0; e0 < a.num_experts; e0 += 32) {
-        const uint32_t p = e0 + lane < a.num_experts ? (uint32_t)max((int32_t)ld_stream_u32(a.psum + e0 + lane), 0) : 0u;
-        const uint32_t hit = __ballot_sync(0xffffffffu, (p + a.alignment - 1) / a.alignment * a.alignment > token_base);
-        if (hit != 0) return min(end, __shfl_sync(0xffffffffu, p, __ffs(hit) - 1));
-    }
-    return token_base;
-}
-
-__device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
-
 // One CTA = 32 tokens x 256 channels. A warp takes four tokens and issues the loads of all of them (4 or 8 x 16 bytes per
 // lane) before it uses the first. Cutting the channels as well as the tokens is what gives a decoding step its parallelism:
 // a CTA that ran through the whole row left 64 tokens x 7168 channels to two CTAs. Bound by HBM for many tokens, by one
@@ -66,7 +51,7 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp8_kernel(const QuantArg
     griddep_wait();
     griddep_launch_dependents();
     uint32_t valid_end = min(a.tokens, token_base + kTokenGroup);
-    if (a.psum != nullptr) valid_end = max(valid_end_of(a, token_base, valid_end, lane), token_base);
+    if (a.psum != nullptr) valid_end = min(valid_end, max(group_end_of(a.psum, a.num_experts, a.alignment, token_base, lane).valid, token_base));
     if (valid_end <= token_base) return;                  // the whole group is padding (uniform over the CTA)
 
     const uint32_t c = c0 + lane * 8, t0 = token_base + warp * kWarpTokens;
@@ -115,20 +100,9 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp8_kernel(const QuantArg
         for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[j]));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        // scale = max(amax, 1e-4) * (1/448) rounded up to a power of two; exponent byte from the bit pattern
-        const uint32_t bits = __float_as_uint(fmaxf(amax, 1e-4f) * (1.0f / 448.0f));
-        const uint32_t e = ((bits - 1u) >> 23) + 1u;
-        const float inv = __uint_as_float((254u - e) << 23);
-        if (t0 + i < valid_end && c < a.hidden) {
-            uint32_t q[2];
-            #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const __nv_fp8x2_storage_t p0 = __nv_cvt_float2_to_fp8x2(make_float2(v[h * 4] * inv, v[h * 4 + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-                const __nv_fp8x2_storage_t p1 = __nv_cvt_float2_to_fp8x2(make_float2(v[h * 4 + 2] * inv, v[h * 4 + 3] * inv), __NV_SATFINITE, __NV_E4M3);
-                q[h] = (uint32_t)p0 | ((uint32_t)p1 << 16);
-            }
-            *reinterpret_cast<uint2*>(a.out + (uint64_t)(t0 + i) * a.out_stride + c) = make_uint2(q[0], q[1]);
-        }
+        const uint32_t e = e4m3_scale_byte(amax);
+        if (t0 + i < valid_end && c < a.hidden)
+            *reinterpret_cast<uint2*>(a.out + (uint64_t)(t0 + i) * a.out_stride + c) = e4m3_pack8(v, e);
         // (the second block of a last, half-used scale column is zero)
         if ((lane & 3u) == 0) sf_smem[warp * kWarpTokens + i][lane / 4] = c < a.hidden ? (uint8_t)e : (uint8_t)0;
     }

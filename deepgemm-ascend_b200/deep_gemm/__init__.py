@@ -45,8 +45,9 @@ for _name in _HOT_PATH_NAMES:
     globals()[_name] = getattr(_C if _C is not None else _api, _name)
 del _name
 
-from . import epilogue, quant_ops, testing  # noqa: E402,F401
-from .quant_ops import cast_to_fp8, swiglu_apply_weight_to_fp8  # noqa: F401
+from . import epilogue, moe_ops, quant_ops, testing  # noqa: E402,F401
+from .quant_ops import cast_from_fp4, cast_to_fp4, cast_to_fp8, swiglu_apply_weight_to_fp8  # noqa: F401
+from .moe_ops import moe_combine, moe_combine_grad, moe_dispatch, moe_dispatch_to_fp8, moe_sort  # noqa: F401
 from .locality_domain import (  # noqa: F401
     destroy_localizer,
     get_num_locality_domains,

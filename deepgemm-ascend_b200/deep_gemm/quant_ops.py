@@ -1,10 +1,10 @@
-"""Producers of block-scaled FP8 operands whose scale factors come out in the layout the GEMM reads.
+"""Producers of block-scaled FP8 and FP4 operands whose scale factors come out in the layout the GEMM reads.
 
 `swiglu_apply_weight_to_fp8` mirrors the reference's third-party/tilelang_ops/swiglu_apply_weight_to_fp8.py:411-449
 (same arguments, same return pair); `cast_to_fp8` is the same kernel without the SwiGLU step and has no counterpart in
 the reference. Both return `(out, out_sf)` with `out` E4M3 [tokens, hidden] and `out_sf` int16 [tokens, hidden / 64]
 whose stride(0) == 1: pass them to `fp8_gemm_*` / `m_grouped_fp8_gemm_*` as `(out, out_sf)` with `recipe_a=(1, 32)`
-and no scale-factor transform runs.
+and no scale-factor transform runs. `cast_to_fp4` does the same for packed E2M1, in both majors, and `cast_from_fp4` is the way back.
 """
 
 from __future__ import annotations
@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib as L
-from ._api import _C, _host_assert, _stream_ptr
+from ._api import _C, _ceil_div, _host_assert, _stream_ptr
 
 
 def _launch(x, hidden, swiglu, topk_weights, psum, clamp_value, expert_alignment):
@@ -55,6 +55,70 @@ def cast_to_fp8(x: torch.Tensor, psum_num_tokens_per_expert: Optional[torch.Tens
     return _launch(x, x.size(1), False, None, psum_num_tokens_per_expert, None, expert_alignment)
 
 
-# The compiled host layer has the same two functions (csrc/apis/quant.hpp): 5 to 6 us of host time a call instead of 15.
+def cast_to_fp4(x: torch.Tensor, psum_num_tokens_per_expert: Optional[torch.Tensor] = None, expert_alignment: int = 128, mn_major: bool = False):
+    """x [rows, cols] or [groups, rows, cols] BF16 or FP32 -> (packed E2M1 int8 [.., rows, cols / 2], packed UE8M0 scales), one scale per
+    32 values along K, in the layout that the GEMMs read:
+
+      mn_major=False   K runs along the row. Scales int16 [.., rows, ceil(cols / 64)] with consecutive rows contiguous: either operand of
+                       an "NT" GEMM, the experts' weights of a grouped one
+      mn_major=True    K runs down the rows. Scales int16 [.., ceil(rows / 64), cols]: the operands that the "NN" and "TN" spellings
+                       take with K in front (weights for the gradient of the activations, both sides of a weight gradient)
+
+    The scale is the smallest power of two with which the block's largest magnitude is at most 6 (2^-126 or more); values are rounded to the
+    nearest code, halves to the even one. A block that holds an infinity or a NaN gets the scale NaN. Rows in the padding of a psum layout
+    are not written; with mn_major they count as zeros and are written as zeros (`expert_alignment` is a multiple of 64 then)."""
+    _host_assert(x.is_cuda and x.dim() in (2, 3) and x.stride(-1) == 1 and x.dtype in (torch.bfloat16, torch.float32),
+                 'x must be a row-major 2-D or 3-D BF16 or FP32 tensor on a CUDA device')
+    groups, rows, cols = x.size(0) if x.dim() == 3 else 1, x.size(-2), x.size(-1)
+    _host_assert(cols % 32 == 0, 'the row length of x must be a multiple of 32')
+    _host_assert(max(groups, rows, cols) < 2 ** 31, 'x is too large')
+    psum = psum_num_tokens_per_expert
+    if psum is not None:
+        _host_assert(psum.dtype == torch.int32 and psum.dim() == 1 and psum.is_contiguous() and psum.device == x.device,
+                     'psum_num_tokens_per_expert must be a contiguous int32 vector on the device of x')
+        _host_assert(x.dim() == 2, 'a psum layout needs a 2-D x')
+        _host_assert(0 < expert_alignment < 2 ** 31 and expert_alignment % (64 if mn_major else 32) == 0,
+                     'expert_alignment must be a positive multiple of 32 (64 when mn_major)')
+    with torch.cuda.device(x.device):
+        out = torch.empty((*x.shape[:-1], cols // 2), dtype=torch.int8, device=x.device)
+        k64, run = _ceil_div(rows if mn_major else cols, 64), cols if mn_major else rows
+        storage = torch.empty((groups, k64, run), dtype=torch.int16, device=x.device)
+        if x.numel():
+            L.check(L.lib().dg_quant_fp4_launch(
+                x.data_ptr(), int(x.dtype == torch.float32), x.stride(-2) if rows > 1 else cols, x.stride(0) if groups > 1 else 0, groups, rows, cols,
+                int(mn_major), psum.data_ptr() if psum is not None else None, psum.numel() if psum is not None else 0, int(expert_alignment),
+                out.data_ptr(), cols // 2, rows * (cols // 2), storage.data_ptr(), run, k64 * run, _stream_ptr(x.device)))
+    sf = storage if mn_major else storage.transpose(1, 2)
+    return out, sf if x.dim() == 3 else sf.squeeze(0)
+
+
+def cast_from_fp4(x, out_dtype: torch.dtype = torch.bfloat16, mn_major: bool = False):
+    """The pair that `cast_to_fp4` makes (or the quantised weights of a GEMM) -> [.., rows, cols] BF16 or FP32: the values that a product with
+    it sees, code times scale."""
+    codes, sf = x
+    _host_assert(codes.is_cuda and codes.dim() in (2, 3) and codes.dtype == torch.int8 and codes.stride(-1) == 1,
+                 'x must be a row-major 2-D or 3-D tensor of packed FP4 on a CUDA device, with its scales')
+    _host_assert(out_dtype in (torch.bfloat16, torch.float32), 'out_dtype must be bf16 or fp32')
+    groups, rows, cols = codes.size(0) if codes.dim() == 3 else 1, codes.size(-2), codes.size(-1) * 2
+    _host_assert(cols % 32 == 0, 'the row length of x must be a multiple of 32')
+    _host_assert(max(groups, rows, cols) < 2 ** 31, 'x is too large')
+    k64, run = _ceil_div(rows if mn_major else cols, 64), cols if mn_major else rows
+    along_k, along_mn = (-2, -1) if mn_major else (-1, -2)
+    _host_assert(sf.dtype == torch.int16 and sf.device == codes.device and sf.dim() == codes.dim() and (sf.dim() == 2 or sf.size(0) == groups) and
+                 sf.size(along_k) == k64 and sf.size(along_mn) == run,
+                 'the scales must be packed int16 on the device of x, one byte for each 32 values along K')
+    _host_assert(sf.stride(along_mn) == 1 or run <= 1, 'the scales must be contiguous along MN')
+    with torch.cuda.device(codes.device):
+        out = torch.empty((*codes.shape[:-1], cols), dtype=out_dtype, device=codes.device)
+        if out.numel():
+            L.check(L.lib().dg_dequant_fp4_launch(
+                codes.data_ptr(), codes.stride(-2) if rows > 1 else cols // 2, codes.stride(0) if groups > 1 else 0, sf.data_ptr(),
+                sf.stride(along_k) if k64 > 1 else run, sf.stride(0) if groups > 1 else 0, groups, rows, cols, int(mn_major),
+                out.data_ptr(), int(out_dtype == torch.float32), cols, rows * cols, _stream_ptr(codes.device)))
+    return out
+
+
+# The compiled host layer has the same functions (csrc/apis/quant.hpp): 5 to 6 us of host time a call instead of 15.
 if _C is not None:
     cast_to_fp8, swiglu_apply_weight_to_fp8 = _C.cast_to_fp8, _C.swiglu_apply_weight_to_fp8
+    cast_to_fp4, cast_from_fp4 = _C.cast_to_fp4, _C.cast_from_fp4

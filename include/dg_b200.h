@@ -287,6 +287,59 @@ int dg_quant_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint3
                         int has_clamp, float clamp_value, void* out, uint64_t out_stride,
                         int16_t* out_sf, uint64_t sf_col_stride, void* stream);
 
+/* BF16 or FP32 values <-> packed E2M1 (two codes per byte along the row, low nibble first) plus UE8M0 scales, one per 32 values along
+ * K, in the layout the GEMM reads. No reference counterpart (tests/generators.py:34-95 quantises on the host). `groups` matrices of
+ * [rows, cols]; strides of values in elements, of codes in bytes, of scales in int16 elements. cols % 32 == 0; rows of values
+ * 16-byte aligned, of codes 4-byte aligned.
+ *   mn_major = 0   K runs along the row: sf[g * sf_group_stride + c * sf_stride + row], c = K64 column, ceil(cols / 64) of them
+ *   mn_major = 1   K runs down the rows: sf[g * sf_group_stride + c * sf_stride + col], c = K64 row, ceil(rows / 64) of them
+ * The scale of a block is the smallest power of two s with amax <= 6 s (at least 2^-126; the byte 255, NaN, where the block holds an
+ * infinity or a NaN); codes are x / s rounded to the nearest, halves to the even code. `psum` / `num_experts` / `alignment`
+ * (groups = 1): rows in the padding of a psum layout are skipped, or (mn_major) count as zeros and are written as zeros; the
+ * alignment is a multiple of 32 (64 when mn_major). */
+int dg_quant_fp4_launch(const void* x, int x_is_fp32, uint64_t x_stride, uint64_t x_group_stride, uint32_t groups, uint32_t rows,
+                        uint32_t cols, int mn_major, const int32_t* psum, uint32_t num_experts, uint32_t alignment,
+                        void* out, uint64_t out_stride, uint64_t out_group_stride,
+                        int16_t* sf, uint64_t sf_stride, uint64_t sf_group_stride, void* stream);
+int dg_dequant_fp4_launch(const void* codes, uint64_t code_stride, uint64_t code_group_stride, const int16_t* sf, uint64_t sf_stride,
+                          uint64_t sf_group_stride, uint32_t groups, uint32_t rows, uint32_t cols, int mn_major,
+                          void* out, int out_is_fp32, uint64_t out_stride, uint64_t out_group_stride, void* stream);
+
+/* From the router's choices to the rows of a grouped layout and back; no reference counterpart (its fused MoE does both inside).
+ * Choice t * topk + j is the j-th expert of token t; experts outside [0, num_experts) (another rank's, -1) have no row.
+ *
+ * dg_moe_sort_launch: `layout` int32[num_experts] is what the m-grouped GEMMs take as grouped_layout: the psum layout, whose
+ * groups start on multiples of `alignment`, or with max_m > 0 the number of rows of each expert (at most max_m; choices behind those
+ * are dropped). `token_rows` int32[tokens * topk]: the row of every choice, -1 where it has none. `row_choices`
+ * int32[num_rows]: the choice of every row, -1 where it holds none. Rows of a group are in the order of the choices. num_rows is
+ * num_experts * max_m, or dg_moe_num_rows: the most that any choices need. At most 1024 experts.
+ *
+ * The others take token_rows; entries outside [0, num_rows) are skipped, no two may be equal. Rows that hold no choice are neither read nor
+ * written, except that `zero_padding` writes zeros to the rows between each group's end and the next multiple of the alignment
+ * (with max_m > 0: to the rest of each expert's slots). Rows start on 16-byte boundaries and hold a multiple of 16 bytes.
+ *
+ * dg_moe_dispatch_launch copies rows of `row_bytes` bytes, dg_moe_dispatch_fp8_launch quantises BF16 rows as dg_quant_fp8_launch does
+ * (scales of row r at out_sf[r / sf_rows * sf_group_stride + c * sf_col_stride + r % sf_rows]).
+ * dg_moe_combine_launch: out[t] = sum over j of topk_weights[t, j] (1 when NULL) x rows[token_rows[t, j]], summed in FP32.
+ * dg_moe_combine_grad_launch: its gradients, grad_rows[token_rows[t, j]] = topk_weights[t, j] x grad_out[t] and grad_weights[t, j] =
+ * <rows[token_rows[t, j]], grad_out[t]> (0 for a choice without a row); grad_rows may be `rows` itself. Strides in elements. */
+uint64_t dg_moe_num_rows(uint32_t choices, uint32_t num_experts, uint32_t alignment);
+int dg_moe_sort_launch(const void* topk_idx, int idx_is_int64, uint32_t tokens, uint32_t topk, uint32_t num_experts, uint32_t alignment,
+                       uint32_t max_m, int32_t* layout, int32_t* token_rows, int32_t* row_choices, uint64_t num_rows, void* stream);
+int dg_moe_dispatch_launch(const void* x, uint64_t x_stride_bytes, uint32_t tokens, uint32_t topk, uint64_t row_bytes,
+                           const int32_t* token_rows, uint64_t num_rows, void* out, uint64_t out_stride_bytes,
+                           const int32_t* layout, uint32_t num_experts, uint32_t alignment, uint32_t max_m, int zero_padding, void* stream);
+int dg_moe_dispatch_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t topk, uint32_t hidden,
+                               const int32_t* token_rows, uint64_t num_rows, void* out, uint64_t out_stride,
+                               int16_t* out_sf, uint64_t sf_col_stride, uint64_t sf_group_stride, uint32_t sf_rows, void* stream);
+int dg_moe_combine_launch(const void* rows, int is_fp32, uint64_t rows_stride, uint64_t num_rows, uint32_t hidden, const int32_t* token_rows,
+                          uint32_t tokens, uint32_t topk, const float* topk_weights, void* out, uint64_t out_stride, void* stream);
+int dg_moe_combine_grad_launch(const void* grad_out, int is_fp32, uint64_t grad_stride, const void* rows, uint64_t rows_stride,
+                               uint64_t num_rows, uint32_t hidden, const int32_t* token_rows, uint32_t tokens, uint32_t topk,
+                               const float* topk_weights, void* grad_rows, uint64_t grad_rows_stride, float* grad_weights,
+                               const int32_t* layout, uint32_t num_experts, uint32_t alignment, uint32_t max_m, int zero_padding,
+                               void* stream);
+
 /* Copy a 2-D byte matrix into a buffer whose row pitch satisfies the 16-byte rule of TMA, zero
  * filling the tail of each row. Used for operands whose contiguous extent is not a multiple of 16
  * bytes (the unaligned-K / unaligned-MN cases of tests/generators.py:491-541). */

@@ -33,7 +33,8 @@ from .mxgemm import (  # noqa: F401
     quantize_e4m3,
     stochastic_round_bf16,
 )
-from .quant import swiglu_quant_ref  # noqa: F401
+from .moe import moe_combine_grad_ref, moe_combine_ref, moe_padding, moe_rows, moe_sort_ref  # noqa: F401
+from .quant import cast_fp4_ref, swiglu_quant_ref  # noqa: F401
 from .sf_layout import (  # noqa: F401
     align,
     ceil_div,

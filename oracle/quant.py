@@ -53,3 +53,33 @@ def swiglu_quant_ref(x: torch.Tensor, topk_weights=None, psum=None, clamp_value=
             valid[start:min(int(p), t)] = True
             start = (int(p) + alignment - 1) // alignment * alignment
     return q.view(torch.uint8), sf, valid, deq
+
+
+def cast_fp4_ref(x: torch.Tensor, axis: int, valid=None):
+    """Microscaled E2M1 of x (any float type) in 64 bits, blocks of 32 along `axis` (-1 or -2), the last one perhaps short: (codes uint8 like
+    x, scale bytes uint8 with `axis` divided by 32, values float64). The scale is the smallest power of two (2^-126 or more) with which the
+    largest magnitude is at most 6; the nearest code, halves to the even one; scale byte 255 where a block holds an infinity or a
+    NaN. `valid` (bool along axis -2): rows that do not count and are zero."""
+    x = x.double()
+    if valid is not None:
+        x = torch.where(valid[:, None], x, 0.0)
+    x = x.movedim(axis, -1)
+    n = x.size(-1)
+    blocks = torch.nn.functional.pad(x, (0, -n % 32)).unflatten(-1, (-1, 32))
+    finite = torch.isfinite(blocks).all(-1)
+    blocks = torch.where(finite[..., None], blocks, 0.0)
+    mantissa, exponent = torch.frexp(blocks.abs().amax(-1) / 6)
+    exponent = (exponent - (mantissa == 0.5).int()).clamp(min=-126)
+    exponent = torch.where(blocks.abs().amax(-1) == 0, torch.full_like(exponent, -126), exponent)
+    scaled = torch.ldexp(blocks, -exponent[..., None])
+    grid = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], dtype=torch.float64)
+    distance = (scaled.abs()[..., None] - grid).abs()
+    best = distance.amin(-1, keepdim=True)
+    tied = distance == best                                              # one code, or two neighbours: the even one of them
+    code = torch.where(tied & (torch.arange(8) % 2 == 0), 2, torch.where(tied, 1, 0)).argmax(-1)
+    values = torch.ldexp(grid[code], exponent[..., None]) * torch.where(torch.signbit(blocks), -1.0, 1.0)
+    values = torch.where(finite[..., None], values, float('nan'))
+    code = (code + 8 * torch.signbit(blocks)).to(torch.uint8)
+    byte = torch.where(finite, exponent + 127, 255).to(torch.uint8)
+    back = lambda t: t.flatten(-2)[..., :n].movedim(-1, axis)            # noqa: E731
+    return back(code), byte.movedim(-1, axis), back(values)
