@@ -120,10 +120,13 @@ inline TensorPair moe_dispatch_to_fp8(const torch::Tensor& x, const MoePlan& pla
         if (!plan.max_m) sf = sf.squeeze(0);
     }
     const int64_t stride = plan.check_rows(out, "out must hold a row for each of the layout's, at one distance");
+    const uint64_t nbytes = dg_moe_dispatch_fp8_scratch_bytes((uint32_t)plan.tokens, (uint32_t)plan.topk, (uint32_t)hidden);
+    const auto scratch = nbytes ? torch::empty({(int64_t)nbytes}, x.options().dtype(torch::kUInt8)) : torch::Tensor();
     check(dg_moe_dispatch_fp8_launch(x.data_ptr(), (uint64_t)stride_of_rows(x), (uint32_t)plan.tokens, (uint32_t)plan.topk, (uint32_t)hidden,
-                                     plan.token_rows_ptr(), (uint64_t)plan.rows, out.data_ptr(), (uint64_t)stride, static_cast<int16_t*>(sf.data_ptr()),
+                                     plan.token_rows_ptr(), static_cast<const int32_t*>(plan.row_choices.data_ptr()), (uint64_t)plan.rows,
+                                     out.data_ptr(), (uint64_t)stride, static_cast<int16_t*>(sf.data_ptr()),
                                      (uint64_t)(cols > 1 ? sf.stride(-1) : per_group), sf.dim() == 3 && plan.experts > 1 ? (uint64_t)sf.stride(0) : 0,
-                                     (uint32_t)per_group, stream_of(x)));
+                                     (uint32_t)per_group, nbytes ? scratch.data_ptr() : nullptr, nbytes, stream_of(x)));
     return {out, sf};
 }
 

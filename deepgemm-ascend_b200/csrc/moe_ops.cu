@@ -12,6 +12,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/dg_b200.h"
 #include "host_common.h"
 #include "ptx.cuh"
@@ -20,7 +22,7 @@
 namespace dg {
 
 // ---------------------------------------------------------------------------------------------------------- sort
-constexpr uint32_t kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortMaxExperts = 1024, kSortMaxCluster = 8;
+constexpr uint32_t kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortMaxExperts = 1024, kSortMaxCluster = 16, kSortBatch = 8;
 
 struct SortArgs {
     const void* idx;                                    // [n] int32 or int64
@@ -30,25 +32,47 @@ struct SortArgs {
     uint32_t warps;                                     // warps of a CTA that hold choices
 };
 
-template <typename T>
-__device__ __forceinline__ uint32_t expert_of(const SortArgs& a, uint32_t i, uint32_t end) {
-    if (i >= end) return 0xffffffffu;
-    T e;
-    if constexpr (sizeof(T) == 8) asm volatile("ld.global.s64 %0, [%1];" : "=l"(e) : "l"(static_cast<const T*>(a.idx) + i));
-    else asm volatile("ld.global.s32 %0, [%1];" : "=r"(e) : "l"(static_cast<const T*>(a.idx) + i));
-    return e >= 0 && e < (T)a.experts ? (uint32_t)e : 0xffffffffu;
+// The experts of kBatch runs of 32 choices from `i` on (all loads on their way at once); `experts` stands for none.
+template <typename T, uint32_t kBatch>
+__device__ __forceinline__ void load_experts(const SortArgs& a, uint32_t i, uint32_t end, uint32_t (&expert)[kBatch]) {
+    T e[kBatch];
+    #pragma unroll
+    for (uint32_t k = 0; k < kBatch; ++k) {
+        e[k] = -1;
+        if (i + k * 32 < end) {
+            const T* p = static_cast<const T*>(a.idx) + i + k * 32;
+            if constexpr (sizeof(T) == 8) asm volatile("ld.global.s64 %0, [%1];" : "=l"(e[k]) : "l"(p));
+            else asm volatile("ld.global.s32 %0, [%1];" : "=r"(e[k]) : "l"(p));
+        }
+    }
+    #pragma unroll
+    for (uint32_t k = 0; k < kBatch; ++k) expert[k] = e[k] >= 0 && e[k] < (T)a.experts ? (uint32_t)e[k] : a.experts;
+}
+// The lanes that hold the same expert, bit by bit (a match over 32 lanes takes a turn for every value that occurs: three times as long).
+__device__ __forceinline__ uint32_t same_expert(uint32_t e, uint32_t bits) {
+    uint32_t peers = 0xffffffffu;
+    for (uint32_t b = 0; b < bits; ++b) {
+        const bool set = (e >> b) & 1u;
+        const uint32_t with = __ballot_sync(0xffffffffu, set);
+        peers &= set ? with : ~with;
+    }
+    return peers;
 }
 
 // A stable counting sort in one launch: one CTA, or a cluster whose CTAs exchange their counts through distributed shared memory.
 // Every warp owns a run of choices and a row of counters of its own (no atomics): it counts, the counters become offsets (over the
 // warps of the CTA, the CTAs of the cluster, and the experts with their alignment), and it walks its run a second time to hand
-// out rows. Within 32 choices the order is that of the lanes (match).
-template <typename T>
+// out rows. Within 32 choices the order is that of the lanes. Runs that fit kBatch are read once; kBatch is 1 where 32 choices for each
+// of a CTA's warps are all (1024 choices: 3.6 us against 4.4 with 8). 131072 choices of 256 experts: 12.2 us with 16 CTAs, 19 with 8; 40 with
+// one load at a time and a match for the peers.
+template <typename T, uint32_t kBatch>
 __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a) {
     extern __shared__ uint32_t smem[];
     uint32_t* const counts = smem;                                      // [warps][experts]
     uint32_t* const totals = smem + a.warps * a.experts;                // [experts]: of this CTA
     uint32_t* const bases = totals + a.experts;                         // [experts]: row of this CTA's first choice
+    // experts of the batch whose rows a thread hands out (kept here, the loop over them need not be unrolled)
+    uint16_t* const held = reinterpret_cast<uint16_t*>(bases + a.experts);      // [kBatch][threads]
     __shared__ uint32_t scan[kSortWarps];
     const uint32_t tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     const uint32_t cta = blockIdx.x, ctas = gridDim.x;
@@ -60,11 +84,12 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a
     __syncthreads();
     const uint32_t first = min(a.n, (cta * a.warps + warp) * a.segment), last = warp < a.warps ? min(a.n, first + a.segment) : first;
     uint32_t* const mine = counts + warp * a.experts;
-    for (uint32_t i0 = first; i0 < last; i0 += 32) {
-        const uint32_t e = expert_of<T>(a, i0 + lane, last);
-        const uint32_t peers = __match_any_sync(0xffffffffu, e);
-        if (e != 0xffffffffu && lane == (uint32_t)__ffs(peers) - 1) mine[e] += __popc(peers);
-        __syncwarp();
+    uint32_t expert[kBatch];
+    for (uint32_t i0 = first; i0 < last; i0 += 32 * kBatch) {
+        load_experts<T>(a, i0 + lane, last, expert);
+        #pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k)
+            if (expert[k] < a.experts) atomicAdd(mine + expert[k], 1u);
     }
     __syncthreads();
     uint32_t total = 0;
@@ -118,19 +143,25 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a
         if (cta == 0) a.layout[tid] = (int32_t)(a.max_m ? min(total, a.max_m) : start + total);
     }
     __syncthreads();
-    for (uint32_t i0 = first; i0 < last; i0 += 32) {
-        const uint32_t i = i0 + lane, e = expert_of<T>(a, i, last);
-        const uint32_t peers = __match_any_sync(0xffffffffu, e);
-        uint32_t row = 0xffffffffu;
-        if (e != 0xffffffffu) {
-            row = bases[e] + mine[e] + __popc(peers & ((1u << lane) - 1u));
-            if (a.max_m && row >= (e + 1) * a.max_m) row = 0xffffffffu;
+    const uint32_t bits = 32 - __clz(a.experts);
+    for (uint32_t i0 = first; i0 < last; i0 += 32 * kBatch) {
+        if (last - first > 32 * kBatch) load_experts<T>(a, i0 + lane, last, expert);
+        #pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k) held[k * kSortThreads + tid] = (uint16_t)expert[k];
+        #pragma unroll 1
+        for (uint32_t k = 0; k < kBatch && i0 + k * 32 < last; ++k) {
+            const uint32_t i = i0 + k * 32 + lane, e = held[k * kSortThreads + tid], peers = same_expert(e, bits);
+            uint32_t row = 0xffffffffu;
+            if (e < a.experts) {
+                row = bases[e] + mine[e] + __popc(peers & ((1u << lane) - 1u));
+                if (a.max_m && row >= (e + 1) * a.max_m) row = 0xffffffffu;
+            }
+            __syncwarp();
+            if (e < a.experts && lane == (uint32_t)__ffs(peers) - 1) mine[e] += __popc(peers);
+            __syncwarp();
+            if (i < last) a.token_rows[i] = (int32_t)row;
+            if (row < a.rows) a.row_choices[row] = (int32_t)i;
         }
-        __syncwarp();
-        if (e != 0xffffffffu && lane == (uint32_t)__ffs(peers) - 1) mine[e] += __popc(peers);
-        __syncwarp();
-        if (i < last) a.token_rows[i] = (int32_t)row;
-        if (row < a.rows) a.row_choices[row] = (int32_t)i;
     }
     if (ctas > 1) cluster_wait();                       // the others have read this CTA's totals
 }
@@ -167,6 +198,9 @@ struct DispatchArgs {
     uint64_t token_items, items;                        // warps that copy, and with those that zero the padding
     uint8_t* sf; uint64_t sf_col_stride, sf_group_stride;          // E4M3 only: bytes between scale columns and groups
     uint32_t sf_rows, hidden;                                      // rows of a group of scales
+    uint8_t* scratch;                                              // scale bytes by token, [tokens][scratch_stride], or nullptr
+    uint32_t scratch_stride;
+    const int32_t* row_choices;                                    // where the scales go through the scratch
 };
 
 // A warp takes 32 x kCopyUnits pieces of a token's row, reads them once and writes them to the rows of all its choices.
@@ -196,7 +230,10 @@ __global__ void __launch_bounds__(kMoeThreads) moe_dispatch_kernel(const Dispatc
     }
 }
 
-// The same with a quantisation on the way: a warp takes 256 channels of a token, eight to a lane, four lanes to a block of 32.
+// The same with a quantisation on the way: a warp takes 256 channels of a token, eight to a lane, four lanes to a block of 32. The
+// scales of a row lie num_rows elements apart, and the rows of a token far from one another: written from here, each is a store of two
+// bytes with a sector of L2 to itself. That suits a few tokens. For many (65536 rows of 7168: 127 us, 93 without the scales), the
+// bytes go to a scratch, by token, and moe_scales_kernel behind this one turns them into runs.
 __global__ void __launch_bounds__(kMoeThreads) moe_dispatch_fp8_kernel(const DispatchArgs a) {
     const uint32_t lane = threadIdx.x % 32;
     const uint64_t item = (uint64_t)blockIdx.x * kMoeWarps + threadIdx.x / 32;
@@ -226,6 +263,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_dispatch_fp8_kernel(const Dis
             const uint32_t row = __shfl_sync(0xffffffffu, mine, j);
             if (row < a.r.rows && c < a.hidden) *reinterpret_cast<uint2*>(a.out + row * a.out_stride + c) = q;
         }
+        if (a.scratch != nullptr) continue;
         // eight rows' scales at a time, four columns each
         for (uint32_t j = 0; j < some; j += 8) {
             const uint32_t row = __shfl_sync(0xffffffffu, mine, min(31u, j + lane / 4));
@@ -235,6 +273,43 @@ __global__ void __launch_bounds__(kMoeThreads) moe_dispatch_fp8_kernel(const Dis
             }
         }
     }
+    if (a.scratch != nullptr && lane < 4 && c0 + col * 64 < a.hidden)
+        *reinterpret_cast<uint16_t*>(a.scratch + (uint64_t)token * a.scratch_stride + c0 / 32 + col * 2) = (uint16_t)pair;
+}
+
+// Scale bytes by token -> the layout that the GEMM reads. One CTA = 64 rows: their tokens' bytes are read 16 at a time into shared memory
+// (rows an odd number of words apart: the columns are read without conflicts), and every scale column of the tile is a run of 128 bytes.
+constexpr uint32_t kScaleRows = 64, kScaleChunk = 128;  // rows of a CTA, scale bytes of a row that it holds at a time
+__global__ void __launch_bounds__(kMoeThreads) moe_scales_kernel(const DispatchArgs a) {
+    __shared__ uint32_t bytes[kScaleRows][kScaleChunk / 4 + 1];
+    __shared__ uint32_t token_of[kScaleRows];
+    const uint32_t row0 = blockIdx.x * kScaleRows, b0 = blockIdx.y * kScaleChunk, tid = threadIdx.x;
+    griddep_wait();
+    griddep_launch_dependents();
+    bool some = false;
+    if (tid < kScaleRows) {
+        const uint32_t choice = row0 + tid < a.r.rows ? ld_global_u32(a.row_choices + row0 + tid) : 0xffffffffu;
+        const uint32_t token = choice / max(a.r.topk, 1u);
+        some = (int32_t)choice >= 0 && token < a.r.tokens;
+        token_of[tid] = some ? token : 0xffffffffu;
+    }
+    if (!__syncthreads_or(some)) return;
+    const uint32_t words = min(kScaleChunk, a.scratch_stride - b0) / 16;       // pieces of 16 bytes
+    for (uint32_t i = tid; i < kScaleRows * words; i += kMoeThreads) {
+        const uint32_t r = i / words, w = i - r * words, token = token_of[r];
+        if (token == 0xffffffffu) continue;
+        const uint4 v = ld_global_v4(a.scratch + (uint64_t)token * a.scratch_stride + b0 + w * 16);
+        uint32_t* to = &bytes[r][w * 4];
+        to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
+    }
+    __syncthreads();
+    const uint32_t r = tid % kScaleRows, row = row0 + r;
+    if (token_of[r] == 0xffffffffu) return;
+    const uint32_t g = row / a.sf_rows;
+    uint8_t* const to = a.sf + g * a.sf_group_stride + (uint64_t)(row - g * a.sf_rows) * 2;
+    const uint32_t cols = (a.hidden + 63) / 64, c0 = b0 / 2;
+    for (uint32_t c = tid / kScaleRows; c < kScaleChunk / 2 && c0 + c < cols; c += kMoeThreads / kScaleRows)
+        *reinterpret_cast<uint16_t*>(to + (uint64_t)(c0 + c) * a.sf_col_stride) = (uint16_t)(bytes[r][c / 2] >> (c % 2 * 16));
 }
 
 // -------------------------------------------------------------------------------------------------- combine
@@ -323,46 +398,52 @@ struct CombineGradArgs {
 };
 
 // One CTA a token: its gradient is read once and multiplied with eight rows at a time; the products with the rows are summed over the
-// CTA. The CTAs behind the last token zero the padding.
+// CTA. The CTAs behind the last token zero the padding. Where the rows begin is kept in shared memory: as registers those 32 words
+// left one CTA on an SM.
 template <typename T>
-__global__ void __launch_bounds__(kMoeThreads) moe_combine_grad_kernel(const CombineGradArgs a) {
+__global__ void __launch_bounds__(kMoeThreads, 3) moe_combine_grad_kernel(const CombineGradArgs a) {
     __shared__ float partial[kMoeWarps][8];
+    __shared__ const uint8_t* from[8];
+    __shared__ uint8_t* to[8];
+    __shared__ float weights[8];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, token = blockIdx.x;
     griddep_wait();
     griddep_launch_dependents();
     if (token >= a.r.tokens) {
-        zero_padding_row(a.r, (uint64_t)(token - a.r.tokens) * kMoeWarps + warp, a.dy, a.dy_stride, a.units, lane);
+        zero_padding_row(a.r, (uint64_t)(token - a.r.tokens) * (blockDim.x / 32) + warp, a.dy, a.dy_stride, a.units, lane);
         return;
     }
     for (uint32_t j0 = 0; j0 < a.r.topk; j0 += 8) {
-        uint32_t row[8];
-        float weight[8], dot[8];
-        #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
-            const bool is = j0 + j < a.r.topk;
-            row[j] = is ? ld_global_u32(a.r.token_rows + (uint64_t)token * a.r.topk + j0 + j) : 0xffffffffu;
-            weight[j] = is ? __uint_as_float(ld_global_u32(a.w + (uint64_t)token * a.r.topk + j0 + j)) : 0.f;
-            dot[j] = 0.f;
+        if (threadIdx.x < 8) {
+            const uint32_t j = j0 + threadIdx.x;
+            const uint32_t row = j < a.r.topk ? ld_global_u32(a.r.token_rows + (uint64_t)token * a.r.topk + j) : 0xffffffffu;
+            const bool is = row < a.r.rows;
+            from[threadIdx.x] = is ? a.y + row * a.y_stride : nullptr;
+            to[threadIdx.x] = a.dy + row * a.dy_stride;
+            weights[threadIdx.x] = is ? __uint_as_float(ld_global_u32(a.w + (uint64_t)token * a.r.topk + j)) : 0.f;
         }
-        for (uint32_t u = threadIdx.x; u < a.units; u += kMoeThreads) {
+        __syncthreads();
+        float dot[8] = {};
+        for (uint32_t u = threadIdx.x; u < a.units; u += blockDim.x) {
             uint4 q[8];
             const uint4 gq = ld_global_v4(a.g + token * a.g_stride + (uint64_t)u * 16);
             #pragma unroll
             for (uint32_t j = 0; j < 8; ++j)
-                if (row[j] < a.r.rows) q[j] = ld_stream_v4(a.y + row[j] * a.y_stride + (uint64_t)u * 16);
+                if (from[j] != nullptr) q[j] = ld_stream_v4(from[j] + (uint64_t)u * 16);
             float g[Unit<T>::kValues];
             Unit<T>::values(gq, g);
             #pragma unroll
             for (uint32_t j = 0; j < 8; ++j) {
-                if (row[j] >= a.r.rows) continue;
+                if (from[j] == nullptr) continue;
                 float v[Unit<T>::kValues], d[Unit<T>::kValues];
                 Unit<T>::values(q[j], v);
+                const float w = weights[j];
                 #pragma unroll
                 for (int k = 0; k < Unit<T>::kValues; ++k) {
                     dot[j] = fmaf(v[k], g[k], dot[j]);
-                    d[k] = weight[j] * g[k];
+                    d[k] = w * g[k];
                 }
-                *reinterpret_cast<uint4*>(a.dy + row[j] * a.dy_stride + (uint64_t)u * 16) = Unit<T>::pack(d);
+                *reinterpret_cast<uint4*>(to[j] + (uint64_t)u * 16) = Unit<T>::pack(d);
             }
         }
         #pragma unroll
@@ -374,17 +455,56 @@ __global__ void __launch_bounds__(kMoeThreads) moe_combine_grad_kernel(const Com
         __syncthreads();
         if (threadIdx.x < 8 && j0 + threadIdx.x < a.r.topk) {
             float s = 0.f;
-            #pragma unroll
-            for (uint32_t w = 0; w < kMoeWarps; ++w) s += partial[w][threadIdx.x];
+            for (uint32_t w = 0; w < blockDim.x / 32; ++w) s += partial[w][threadIdx.x];
             a.dw[(uint64_t)token * a.r.topk + j0 + threadIdx.x] = s;
         }
-        __syncthreads();
     }
 }
 
 }  // namespace dg
 
 using namespace dg;
+
+static const void* sort_kernel(bool int64, bool small) {
+    return int64 ? small ? (const void*)moe_sort_kernel<int64_t, 1> : (const void*)moe_sort_kernel<int64_t, kSortBatch>
+                 : small ? (const void*)moe_sort_kernel<int32_t, 1> : (const void*)moe_sort_kernel<int32_t, kSortBatch>;
+}
+
+// CTAs of the sort's cluster on the current device: 16 where it keeps that many together (they have to share a GPC), else the portable 8.
+// The first call on a device gives the kernels leave for it, and for the shared memory of the most experts (once and for all: a
+// limit set before each launch could be lowered by another thread in between).
+static int sort_cluster(uint32_t* out) {
+    constexpr int kMaxDevices = 64;
+    static std::atomic<uint8_t> known[kMaxDevices];
+    int device = 0;
+    DG_CHECK_CUDA(cudaGetDevice(&device));
+    uint32_t ctas = device < kMaxDevices ? known[device].load(std::memory_order_acquire) : 0;
+    if (ctas == 0) {
+        const int smem = (int)((kSortWarps + 2) * kSortMaxExperts * 4 + kSortBatch * kSortThreads * 2);
+        int fits = 1;
+        for (int k = 0; k < 4; ++k) {
+            const void* fn = sort_kernel(k & 1, k & 2);
+            DG_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+            DG_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+            cudaLaunchConfig_t cfg{};
+            cfg.gridDim = dim3(kSortMaxCluster);
+            cfg.blockDim = dim3(kSortThreads);
+            cfg.dynamicSmemBytes = smem;
+            cudaLaunchAttribute attr[1];
+            attr[0].id = cudaLaunchAttributeClusterDimension;
+            attr[0].val.clusterDim = {kSortMaxCluster, 1, 1};
+            cfg.attrs = attr;
+            cfg.numAttrs = 1;
+            int clusters = 0;
+            DG_CHECK_CUDA(cudaOccupancyMaxActiveClusters(&clusters, fn, &cfg));
+            fits = fits && clusters > 0;
+        }
+        ctas = fits ? kSortMaxCluster : kSortMaxCluster / 2;
+        if (device < kMaxDevices) known[device].store((uint8_t)ctas, std::memory_order_release);
+    }
+    *out = ctas;
+    return DG_OK;
+}
 
 extern "C" uint64_t dg_moe_num_rows(uint32_t choices, uint32_t num_experts, uint32_t alignment) {
     const uint64_t used = choices < num_experts ? choices : num_experts;
@@ -404,12 +524,17 @@ extern "C" int dg_moe_sort_launch(const void* topk_idx, int idx_is_int64, uint32
     SortArgs a{};
     a.idx = topk_idx; a.layout = layout; a.token_rows = token_rows; a.row_choices = row_choices;
     a.n = n; a.experts = num_experts; a.alignment = max_m ? 1 : alignment; a.max_m = max_m; a.rows = (uint32_t)num_rows;
-    const uint32_t ctas = n <= 4096 && num_rows <= 16384 ? 1 : kSortMaxCluster;
+    // One CTA where the cluster's barriers cost more than its other 15 CTAs take off (measured, one CTA against 16: 1024 choices of 32 experts,
+    // 8960 rows, 4.0 against 4.6 us; 2048 5.2 against 4.5; 64 of 256 experts, 16384 rows, 3.5 against 3.9; 128, 32768 rows to clear, 4.7
+    // against 4.0).
+    uint32_t ctas = 1;
+    if (int rc = sort_cluster(&ctas)) return rc;
+    if (n <= 1024 && num_rows <= 16384) ctas = 1;
     a.segment = ((n + ctas * kSortWarps - 1) / (ctas * kSortWarps) + 31) / 32 * 32;
     a.warps = a.segment == 0 ? 0 : (n + a.segment - 1) / a.segment < kSortWarps ? (n + a.segment - 1) / a.segment : kSortWarps;
-    const uint32_t smem = (a.warps + 2) * num_experts * 4;
-    const void* fn = idx_is_int64 ? (const void*)moe_sort_kernel<int64_t> : (const void*)moe_sort_kernel<int32_t>;
-    if (smem > 48 * 1024) DG_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    const bool small = a.segment <= 32;
+    const void* fn = sort_kernel(idx_is_int64, small);
+    const uint32_t smem = (a.warps + 2) * num_experts * 4 + (small ? 1 : kSortBatch) * kSortThreads * 2;
     void* params[] = {&a};
     return launch_overlapped(fn, dim3(ctas), dim3(kSortThreads), params, static_cast<cudaStream_t>(stream), smem, ctas);
 }
@@ -425,6 +550,9 @@ static int rows_args(RowsArgs& r, const int32_t* token_rows, uint32_t tokens, ui
     return DG_OK;
 }
 static uint64_t padding_items(const RowsArgs& r) { return (uint64_t)r.experts * (r.max_m ? r.max_m : r.alignment); }
+// Bytes that a token's scales take in the scratch, and from how many scale elements on they go through it.
+static uint32_t scale_bytes_of(uint32_t hidden) { return (hidden / 32 + 15) / 16 * 16; }
+constexpr uint64_t kScatteredScales = 1ull << 18;
 static bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride_bytes % 16 == 0; }
 
 extern "C" int dg_moe_dispatch_launch(const void* x, uint64_t x_stride_bytes, uint32_t tokens, uint32_t topk, uint64_t row_bytes,
@@ -450,27 +578,41 @@ extern "C" int dg_moe_dispatch_launch(const void* x, uint64_t x_stride_bytes, ui
     return launch_overlapped((const void*)moe_dispatch_kernel, dim3((uint32_t)ctas), dim3(kMoeThreads), params, static_cast<cudaStream_t>(stream));
 }
 
+extern "C" uint64_t dg_moe_dispatch_fp8_scratch_bytes(uint32_t tokens, uint32_t topk, uint32_t hidden) {
+    // (see moe_dispatch_fp8_kernel) the second launch costs more than a few scales written one by one
+    const uint64_t scales = (uint64_t)tokens * topk * ((hidden + 63) / 64);
+    return scales < kScatteredScales ? 0 : (uint64_t)tokens * scale_bytes_of(hidden);
+}
+
 extern "C" int dg_moe_dispatch_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t topk, uint32_t hidden,
-                                          const int32_t* token_rows, uint64_t num_rows, void* out, uint64_t out_stride,
-                                          int16_t* out_sf, uint64_t sf_col_stride, uint64_t sf_group_stride, uint32_t sf_rows, void* stream) {
+                                          const int32_t* token_rows, const int32_t* row_choices, uint64_t num_rows, void* out, uint64_t out_stride,
+                                          int16_t* out_sf, uint64_t sf_col_stride, uint64_t sf_group_stride, uint32_t sf_rows,
+                                          void* scratch, uint64_t scratch_bytes, void* stream) {
     if (tokens == 0 || topk == 0 || hidden == 0 || num_rows == 0) return DG_OK;
     DG_CHECK_ARG(x != nullptr && out != nullptr && out_sf != nullptr, "moe_dispatch_fp8: null pointer");
     DG_CHECK_ARG(hidden % 32 == 0, "moe_dispatch_fp8: hidden must be a multiple of 32");
     DG_CHECK_ARG(aligned16(x, x_stride * 2), "moe_dispatch_fp8: input rows must start on 16-byte boundaries");
     DG_CHECK_ARG((reinterpret_cast<uintptr_t>(out) & 7) == 0 && out_stride % 8 == 0, "moe_dispatch_fp8: output rows must start on 8-byte boundaries");
     DG_CHECK_ARG(sf_rows > 0 && sf_col_stride >= sf_rows, "moe_dispatch_fp8: scale column stride smaller than the rows of a group");
+    DG_CHECK_ARG(scratch == nullptr || (row_choices != nullptr && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0 &&
+                                        scratch_bytes >= (uint64_t)tokens * scale_bytes_of(hidden)),
+                 "moe_dispatch_fp8: the scratch must be 16-byte aligned, hold dg_moe_dispatch_fp8_scratch_bytes, and come with the rows' choices");
     DispatchArgs a{};
     if (int rc = rows_args(a.r, token_rows, tokens, topk, num_rows, nullptr, 0, 0, 0, 0)) return rc;
     a.x = static_cast<const uint8_t*>(x); a.x_stride = x_stride * 2;
     a.out = static_cast<uint8_t*>(out); a.out_stride = out_stride;
     a.sf = reinterpret_cast<uint8_t*>(out_sf); a.sf_col_stride = sf_col_stride * 2; a.sf_group_stride = sf_group_stride * 2;
     a.sf_rows = sf_rows; a.hidden = hidden;
+    a.scratch = static_cast<uint8_t*>(scratch); a.scratch_stride = scale_bytes_of(hidden); a.row_choices = row_choices;
     a.chunks = (hidden + 255) / 256;
     a.token_items = (uint64_t)tokens * a.chunks;
-    const uint64_t ctas = (a.token_items + kMoeWarps - 1) / kMoeWarps;
-    DG_CHECK_ARG(ctas <= 0x7fffffffull, "moe_dispatch_fp8: too many tokens");
+    const uint64_t ctas = (a.token_items + kMoeWarps - 1) / kMoeWarps, tiles = (num_rows + kScaleRows - 1) / kScaleRows;
+    const uint32_t pieces = (a.scratch_stride + kScaleChunk - 1) / kScaleChunk;
+    DG_CHECK_ARG(ctas <= 0x7fffffffull && pieces <= 65535, "moe_dispatch_fp8: too many tokens or channels");
     void* params[] = {&a};
-    return launch_overlapped((const void*)moe_dispatch_fp8_kernel, dim3((uint32_t)ctas), dim3(kMoeThreads), params, static_cast<cudaStream_t>(stream));
+    if (int rc = launch_overlapped((const void*)moe_dispatch_fp8_kernel, dim3((uint32_t)ctas), dim3(kMoeThreads), params, static_cast<cudaStream_t>(stream))) return rc;
+    if (scratch == nullptr) return DG_OK;
+    return launch_overlapped((const void*)moe_scales_kernel, dim3((uint32_t)tiles, pieces), dim3(kMoeThreads), params, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dg_moe_combine_launch(const void* rows, int is_fp32, uint64_t rows_stride, uint64_t num_rows, uint32_t hidden, const int32_t* token_rows,
@@ -514,10 +656,13 @@ extern "C" int dg_moe_combine_grad_launch(const void* grad_out, int is_fp32, uin
     a.dy = static_cast<uint8_t*>(grad_rows); a.dy_stride = grad_rows_stride * es;
     a.dw = grad_weights;
     a.units = (uint32_t)(hidden * es / 16);
-    const uint64_t ctas = tokens + (padding_items(a.r) + kMoeWarps - 1) / kMoeWarps;
+    // as few threads as take a row in the same number of turns
+    const uint32_t turns = a.units > kMoeThreads ? (a.units + kMoeThreads - 1) / kMoeThreads : 1;
+    const uint32_t threads = a.units == 0 ? 32 : ((a.units + turns - 1) / turns + 31) / 32 * 32;
+    const uint64_t ctas = tokens + (padding_items(a.r) + threads / 32 - 1) / (threads / 32);
     if (ctas == 0) return DG_OK;
     DG_CHECK_ARG(ctas <= 0x7fffffffull, "moe_combine_grad: too many rows");
     const void* fn = is_fp32 ? (const void*)moe_combine_grad_kernel<float> : (const void*)moe_combine_grad_kernel<__nv_bfloat16>;
     void* params[] = {&a};
-    return launch_overlapped(fn, dim3((uint32_t)ctas), dim3(kMoeThreads), params, static_cast<cudaStream_t>(stream));
+    return launch_overlapped(fn, dim3((uint32_t)ctas), dim3(threads), params, static_cast<cudaStream_t>(stream));
 }

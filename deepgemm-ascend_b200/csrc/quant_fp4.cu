@@ -100,19 +100,24 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_kernel(const Fp4Args a)
             *reinterpret_cast<const uint16_t*>(&sf_smem[r][col * 2]);
 }
 
-// MN-major: one CTA = 64 rows x 256 columns. A warp takes one block of 32 rows x 64 columns: lane = (eight rows, eight columns), so
-// that a row of the warp's tile is a whole 128-byte line of BF16 and the maximum down a column takes two shuffles.
+// MN-major: one CTA = 64 rows x 256 columns. A warp takes one block of 32 rows x 64 columns: lane = (every fourth row, eight columns), so
+// that a row of the warp's tile is a whole 128-byte line of BF16 and the maximum down a column takes two shuffles. The codes go through
+// shared memory and out as lines of 128 bytes (written by the lanes as they are, a row of a warp's tile is one sector of 32 bytes, and
+// the number of stores bounds the kernel); its rows are 40 words apart, which keeps the four rows of a store in banks of their own.
+constexpr uint32_t kFp4StageWords = 40;
 template <typename T>
 __global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args a) {
     __shared__ uint8_t sf_smem[2][kFp4Cols];
+    __shared__ __align__(16) uint32_t stage[64][kFp4StageWords];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t tiles = a.tiles_r * a.tiles_c, group = blockIdx.x / tiles, tile = blockIdx.x - group * tiles;
     const uint32_t row_base = tile / a.tiles_c * 64, c0 = tile % a.tiles_c * kFp4Cols;
     const uint32_t half = warp / 4, tc = warp % 4 * 64 + lane % 8 * 8, c = c0 + tc;
-    const uint32_t r0 = row_base + half * 32 + lane / 8 * 8;
+    const uint32_t tr = half * 32 + lane / 8, r0 = row_base + tr;
     griddep_wait();
     griddep_launch_dependents();
-    uint32_t row_end = min(a.rows, row_base + 64), write_end = row_end;
+    const uint32_t write_end = min(a.rows, row_base + 64);
+    uint32_t row_end = write_end;
     if (a.psum != nullptr) {
         // (groups start on multiples of 64 rows: a tile lies in one) Rows of the padding count as zeros and are written as zeros
         const GroupEnd end = group_end_of(a.psum, a.num_experts, a.alignment, row_base, lane);
@@ -123,7 +128,7 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args
     #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
         raw[i].clear();
-        if (r0 + i < row_end && c < a.cols) raw[i].load(a.x + group * a.x_group_stride + (uint64_t)(r0 + i) * a.x_stride + (uint64_t)c * sizeof(T));
+        if (r0 + i * 4 < row_end && c < a.cols) raw[i].load(a.x + group * a.x_group_stride + (uint64_t)(r0 + i * 4) * a.x_stride + (uint64_t)c * sizeof(T));
     }
     uint32_t amax[8] = {};
     #pragma unroll
@@ -141,7 +146,7 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args
         const uint32_t e = e2m1_scale_byte(amax[j]);
         inv[j] = e2m1_inverse(e);
         // (blocks behind the last row are zero)
-        if (lane < 8) sf_smem[half][tc + j] = r0 < a.rows ? (uint8_t)e : (uint8_t)0;
+        if (lane < 8) sf_smem[half][tc + j] = row_base + half * 32 < a.rows ? (uint8_t)e : (uint8_t)0;
     }
     #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
@@ -149,10 +154,16 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args
         raw[i].values(v);
         #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] *= inv[j];
-        if (r0 + i < write_end && c < a.cols)
-            *reinterpret_cast<uint32_t*>(a.codes + group * a.code_group_stride + (uint64_t)(r0 + i) * a.code_stride + c / 2) = e2m1_pack8(v, 1.0f);
+        stage[tr + i * 4][tc / 8] = e2m1_pack8(v, 1.0f);
     }
     __syncthreads();
+    #pragma unroll
+    for (uint32_t i = 0; i < 2; ++i) {
+        const uint32_t r = threadIdx.x / 8 + i * 32, part = threadIdx.x % 8;
+        if (row_base + r < write_end && c0 + part * 32 < a.cols)
+            *reinterpret_cast<uint4*>(a.codes + group * a.code_group_stride + (uint64_t)(row_base + r) * a.code_stride + (c0 + part * 32) / 2) =
+                *reinterpret_cast<const uint4*>(&stage[r][part * 4]);
+    }
     if (c0 + threadIdx.x < a.cols)
         *reinterpret_cast<uint16_t*>(a.sf + group * a.sf_group_stride + (uint64_t)(row_base / 64) * a.sf_stride + (uint64_t)(c0 + threadIdx.x) * 2) =
             (uint16_t)(sf_smem[0][threadIdx.x] | ((uint32_t)sf_smem[1][threadIdx.x] << 8));
@@ -170,8 +181,9 @@ __device__ __forceinline__ void store8(uint8_t* p, const float (&v)[8]) {
         }
         *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
-        *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(p + 16) = make_float4(v[4], v[5], v[6], v[7]);
+        // (one store of 32 bytes: as two, each leaves half of every sector to the other)
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+                     "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
     }
 }
 __device__ __forceinline__ void e2m1_values8(uint32_t q, float (&v)[8]) {
@@ -184,15 +196,15 @@ __device__ __forceinline__ void e2m1_values8(uint32_t q, float (&v)[8]) {
     }
 }
 
-// One CTA = 32 rows x 256 columns, tiles and lanes as in the quantisers. The scales of a K-major tile come in runs down the rows,
-// through shared memory; an MN-major tile lies in one block of rows, whose scales lie along the columns.
+// One CTA = 64 rows x 256 columns, a warp eight rows, a lane eight columns. The scales of a K-major tile come in runs down the rows, through
+// shared memory; an MN-major tile lies in two blocks of rows, whose scales lie along the columns.
 template <typename T, bool kMnMajor>
 __global__ void __launch_bounds__(kFp4Threads) dequant_fp4_kernel(const Fp4Args a, uint8_t* out) {
-    constexpr uint32_t kWarpRows = kFp4Rows / (kFp4Threads / 32);
-    __shared__ __align__(8) uint8_t sf_smem[kFp4Rows][kFp4Cols / 32];
+    constexpr uint32_t kWarpRows = 8;
+    __shared__ __align__(8) uint8_t sf_smem[64][kFp4Cols / 32];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t tiles = a.tiles_r * a.tiles_c, group = blockIdx.x / tiles, tile = blockIdx.x - group * tiles;
-    const uint32_t row_base = tile / a.tiles_c * kFp4Rows, c0 = tile % a.tiles_c * kFp4Cols;
+    const uint32_t row_base = tile / a.tiles_c * 64, c0 = tile % a.tiles_c * kFp4Cols;
     const uint32_t c = c0 + lane * 8, r0 = row_base + warp * kWarpRows;
     griddep_wait();
     griddep_launch_dependents();
@@ -206,11 +218,11 @@ __global__ void __launch_bounds__(kFp4Threads) dequant_fp4_kernel(const Fp4Args 
         #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t pair = c < a.cols ? ld_global_u16(sf + (uint64_t)(row_base / 64) * a.sf_stride + (uint64_t)(c + j) * 2) : 0u;
-            scale[j] = ue8m0_value((pair >> (row_base / 32 % 2 * 8)) & 0xffu);
+            scale[j] = ue8m0_value((pair >> (warp / 4 * 8)) & 0xffu);
         }
     } else {
-        const uint32_t col = threadIdx.x / kFp4Rows, r = threadIdx.x % kFp4Rows;
-        if (col < kFp4Cols / 64 && c0 + col * 64 < a.cols && row_base + r < a.rows)
+        const uint32_t col = threadIdx.x / 64, r = threadIdx.x % 64;
+        if (c0 + col * 64 < a.cols && row_base + r < a.rows)
             *reinterpret_cast<uint16_t*>(&sf_smem[r][col * 2]) = ld_global_u16(sf + (uint64_t)(c0 / 64 + col) * a.sf_stride + (uint64_t)(row_base + r) * 2);
         __syncthreads();
     }
@@ -230,17 +242,18 @@ __global__ void __launch_bounds__(kFp4Threads) dequant_fp4_kernel(const Fp4Args 
 
 using namespace dg;
 
-// What both directions check: the float side is `x`, strides in elements of each side.
-static int fp4_args(Fp4Args& a, uint32_t tile_rows, uint32_t& tiles, const void* x, int is_fp32, uint64_t x_stride, uint64_t x_group_stride,
+// What both directions check: the float side is `x`, strides in elements of each side. `x_bytes`, `code_bytes`: the alignment that the
+// kernel's loads and stores need.
+static int fp4_args(Fp4Args& a, uint32_t tile_rows, uint32_t& tiles, uint32_t x_bytes, uint32_t code_bytes, const void* x, int is_fp32, uint64_t x_stride, uint64_t x_group_stride,
                     uint32_t groups, uint32_t rows, uint32_t cols, const void* codes, uint64_t code_stride, uint64_t code_group_stride,
                     const int16_t* sf, uint64_t sf_stride, uint64_t sf_group_stride, int mn_major) {
     const uint64_t es = is_fp32 ? 4 : 2;
     DG_CHECK_ARG(x != nullptr && codes != nullptr && sf != nullptr, "fp4: null pointer");
     DG_CHECK_ARG(cols % 32 == 0, "fp4: the row length must be a multiple of 32");
-    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(x) & 15) == 0 && x_stride * es % 16 == 0 && x_group_stride * es % 16 == 0,
-                 "fp4: rows of values must start on 16-byte boundaries");
-    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(codes) & 3) == 0 && code_stride % 4 == 0 && code_group_stride % 4 == 0,
-                 "fp4: rows of codes must start on 4-byte boundaries");
+    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(x) | x_stride * es | x_group_stride * es) % x_bytes == 0,
+                 "fp4: rows of values must start on %u-byte boundaries", x_bytes);
+    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(codes) | code_stride | code_group_stride) % code_bytes == 0,
+                 "fp4: rows of codes must start on %u-byte boundaries", code_bytes);
     DG_CHECK_ARG(sf_stride >= (mn_major ? cols : rows), "fp4: scale stride smaller than the rows (columns when MN-major)");
     a.x = static_cast<const uint8_t*>(x); a.x_stride = x_stride * es; a.x_group_stride = x_group_stride * es;
     a.codes = static_cast<uint8_t*>(const_cast<void*>(codes)); a.code_stride = code_stride; a.code_group_stride = code_group_stride;
@@ -262,7 +275,7 @@ extern "C" int dg_quant_fp4_launch(const void* x, int x_is_fp32, uint64_t x_stri
                  "quant_fp4: a psum layout needs one matrix, experts, and an alignment that is a multiple of %u", mn_major ? 64u : kFp4Rows);
     Fp4Args a{};
     uint32_t tiles = 0;
-    if (int rc = fp4_args(a, mn_major ? 64 : kFp4Rows, tiles, x, x_is_fp32, x_stride, x_group_stride, groups, rows, cols, out, out_stride,
+    if (int rc = fp4_args(a, mn_major ? 64 : kFp4Rows, tiles, 16, mn_major ? 16 : 4, x, x_is_fp32, x_stride, x_group_stride, groups, rows, cols, out, out_stride,
                           out_group_stride, sf, sf_stride, sf_group_stride, mn_major)) return rc;
     a.psum = psum; a.num_experts = psum ? num_experts : 0; a.alignment = alignment;
     const void* fn = mn_major ? (x_is_fp32 ? (const void*)quant_fp4_mn_kernel<float> : (const void*)quant_fp4_mn_kernel<__nv_bfloat16>)
@@ -277,7 +290,7 @@ extern "C" int dg_dequant_fp4_launch(const void* codes, uint64_t code_stride, ui
     if (groups == 0 || rows == 0 || cols == 0) return DG_OK;
     Fp4Args a{};
     uint32_t tiles = 0;
-    if (int rc = fp4_args(a, kFp4Rows, tiles, out, out_is_fp32, out_stride, out_group_stride, groups, rows, cols, codes, code_stride,
+    if (int rc = fp4_args(a, 64, tiles, out_is_fp32 ? 32 : 16, 4, out, out_is_fp32, out_stride, out_group_stride, groups, rows, cols, codes, code_stride,
                           code_group_stride, sf, sf_stride, sf_group_stride, mn_major)) return rc;
     const void* fn = mn_major ? (out_is_fp32 ? (const void*)dequant_fp4_kernel<float, true> : (const void*)dequant_fp4_kernel<__nv_bfloat16, true>)
                               : (out_is_fp32 ? (const void*)dequant_fp4_kernel<float, false> : (const void*)dequant_fp4_kernel<__nv_bfloat16, false>);

@@ -151,9 +151,12 @@ def moe_dispatch_to_fp8(x: torch.Tensor, plan, out=None):
             sf = torch.empty((p.experts if p.max_m else 1, cols, per_group), dtype=torch.int16, device=x.device).transpose(1, 2)
             sf = sf if p.max_m else sf.squeeze(0)
         stride = p.check_rows(out, _OUT_ROWS)
+        nbytes = L.lib().dg_moe_dispatch_fp8_scratch_bytes(p.tokens, p.topk, hidden)
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         L.check(L.lib().dg_moe_dispatch_fp8_launch(
-            x.data_ptr(), _row_stride(x), p.tokens, p.topk, hidden, p.token_rows.data_ptr(), p.rows, out.data_ptr(), stride, sf.data_ptr(),
-            sf.stride(-1) if cols > 1 else per_group, sf.stride(0) if sf.dim() == 3 and p.experts > 1 else 0, per_group, _stream_ptr(x.device)))
+            x.data_ptr(), _row_stride(x), p.tokens, p.topk, hidden, p.token_rows.data_ptr(), p.row_choices.data_ptr(), p.rows, out.data_ptr(), stride,
+            sf.data_ptr(), sf.stride(-1) if cols > 1 else per_group, sf.stride(0) if sf.dim() == 3 and p.experts > 1 else 0, per_group,
+            scratch.data_ptr() if nbytes else None, nbytes, _stream_ptr(x.device)))
     return out, sf
 
 

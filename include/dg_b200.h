@@ -290,7 +290,7 @@ int dg_quant_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint3
 /* BF16 or FP32 values <-> packed E2M1 (two codes per byte along the row, low nibble first) plus UE8M0 scales, one per 32 values along
  * K, in the layout the GEMM reads. No reference counterpart (tests/generators.py:34-95 quantises on the host). `groups` matrices of
  * [rows, cols]; strides of values in elements, of codes in bytes, of scales in int16 elements. cols % 32 == 0; rows of values
- * 16-byte aligned, of codes 4-byte aligned.
+ * 16-byte aligned (32 where FP32 is written), of codes 4-byte aligned (16 where mn_major codes are written).
  *   mn_major = 0   K runs along the row: sf[g * sf_group_stride + c * sf_stride + row], c = K64 column, ceil(cols / 64) of them
  *   mn_major = 1   K runs down the rows: sf[g * sf_group_stride + c * sf_stride + col], c = K64 row, ceil(rows / 64) of them
  * The scale of a block is the smallest power of two s with amax <= 6 s (at least 2^-126; the byte 255, NaN, where the block holds an
@@ -319,7 +319,9 @@ int dg_dequant_fp4_launch(const void* codes, uint64_t code_stride, uint64_t code
  * (with max_m > 0: to the rest of each expert's slots). Rows start on 16-byte boundaries and hold a multiple of 16 bytes.
  *
  * dg_moe_dispatch_launch copies rows of `row_bytes` bytes, dg_moe_dispatch_fp8_launch quantises BF16 rows as dg_quant_fp8_launch does
- * (scales of row r at out_sf[r / sf_rows * sf_group_stride + c * sf_col_stride + r % sf_rows]).
+ * (scales of row r at out_sf[r / sf_rows * sf_group_stride + c * sf_col_stride + r % sf_rows]). `scratch`: device memory of
+ * dg_moe_dispatch_fp8_scratch_bytes (0 for small problems) that the call may use until it has run; with it `row_choices` says which
+ * choice a row holds, and must agree with token_rows. NULL works for any size, slower for many tokens.
  * dg_moe_combine_launch: out[t] = sum over j of topk_weights[t, j] (1 when NULL) x rows[token_rows[t, j]], summed in FP32.
  * dg_moe_combine_grad_launch: its gradients, grad_rows[token_rows[t, j]] = topk_weights[t, j] x grad_out[t] and grad_weights[t, j] =
  * <rows[token_rows[t, j]], grad_out[t]> (0 for a choice without a row); grad_rows may be `rows` itself. Strides in elements. */
@@ -329,9 +331,11 @@ int dg_moe_sort_launch(const void* topk_idx, int idx_is_int64, uint32_t tokens, 
 int dg_moe_dispatch_launch(const void* x, uint64_t x_stride_bytes, uint32_t tokens, uint32_t topk, uint64_t row_bytes,
                            const int32_t* token_rows, uint64_t num_rows, void* out, uint64_t out_stride_bytes,
                            const int32_t* layout, uint32_t num_experts, uint32_t alignment, uint32_t max_m, int zero_padding, void* stream);
+uint64_t dg_moe_dispatch_fp8_scratch_bytes(uint32_t tokens, uint32_t topk, uint32_t hidden);
 int dg_moe_dispatch_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t topk, uint32_t hidden,
-                               const int32_t* token_rows, uint64_t num_rows, void* out, uint64_t out_stride,
-                               int16_t* out_sf, uint64_t sf_col_stride, uint64_t sf_group_stride, uint32_t sf_rows, void* stream);
+                               const int32_t* token_rows, const int32_t* row_choices, uint64_t num_rows, void* out, uint64_t out_stride,
+                               int16_t* out_sf, uint64_t sf_col_stride, uint64_t sf_group_stride, uint32_t sf_rows,
+                               void* scratch, uint64_t scratch_bytes, void* stream);
 int dg_moe_combine_launch(const void* rows, int is_fp32, uint64_t rows_stride, uint64_t num_rows, uint32_t hidden, const int32_t* token_rows,
                           uint32_t tokens, uint32_t topk, const float* topk_weights, void* out, uint64_t out_stride, void* stream);
 int dg_moe_combine_grad_launch(const void* grad_out, int is_fp32, uint64_t grad_stride, const void* rows, uint64_t rows_stride,

@@ -130,6 +130,32 @@ def test_dispatch_to_fp8(host, layout, hidden):
     assert (flat[~live] == 0x11).all() and (flat_sf[~live] == 0x2222).all()
 
 
+@pytest.mark.parametrize('tokens,topk,experts,max_m,hidden', [(700, 6, 16, None, 7168), (1001, 8, 40, None, 4128), (2000, 2, 7, 333, 8224), (300, 33, 64, 130, 3200),
+                                                              (5000, 1, 3, None, 65568)])
+def test_dispatch_to_fp8_of_many_tokens(tokens, topk, experts, max_m, hidden):
+    """Where the scales take a second launch."""
+    assert deep_gemm._lib.lib().dg_moe_dispatch_fp8_scratch_bytes(tokens, topk, hidden) > 0
+    seed_all(hidden)
+    idx = _choices(tokens, topk, 2 * experts, 5)
+    plan, (_, _, row_choices) = _sort(torch.where(idx < experts, idx, -1), experts, max_m=max_m)
+    x = (torch.randn(tokens, hidden, device='cuda') * 3).bfloat16()
+    codes, sf = deep_gemm.cast_to_fp8(x)
+    choice = row_choices.view(-1).long().cuda()
+    live = choice >= 0
+    cols = sf.size(1)
+    data = torch.full((*row_choices.shape, hidden), 0x11, dtype=torch.uint8, device='cuda').view(torch.float8_e4m3fn)
+    groups, per = (experts, max_m) if max_m else (1, row_choices.numel())
+    room = torch.full((groups, cols + 1, per + 5), 0x2222, dtype=torch.int16, device='cuda')
+    scales = room[:, :cols, :per].transpose(1, 2)
+    for host in moe_hosts:
+        got, got_sf = host.moe_dispatch_to_fp8(x, plan, out=(data, scales if max_m else scales[0]))
+        flat, flat_sf = got.view(torch.uint8).view(-1, hidden), got_sf.reshape(-1, cols)
+        assert torch.equal(flat[live], codes.view(torch.uint8)[choice[live] // topk]) and torch.equal(flat_sf[live], sf[choice[live] // topk])
+        assert (flat[~live] == 0x11).all() and (flat_sf[~live] == 0x2222).all() and (room[:, cols] == 0x2222).all() and (room[:, :, per:] == 0x2222).all()
+        fresh, fresh_sf = host.moe_dispatch_to_fp8(x, plan)
+        assert torch.equal(fresh_sf.reshape(-1, cols)[live], flat_sf[live])
+
+
 def test_rows_with_strides():
     """Views of wider tensors on both sides, and one token's row broadcast to all."""
     seed_all(3)

@@ -62,14 +62,17 @@ def test_the_c_abi_checks_its_arguments():
     for bad in (dict(layout=None), dict(e=0), dict(align=0)):
         _refused(copy(zero=1, **bad), 'zeros in the padding need the layout')
     _refused(copy(rows=1 << 31), 'too many choices or rows')
-    fp8 = lambda x=p, xs=64, hidden=64, out=p, os=64, sf=p, col=512, per=512: lib.dg_moe_dispatch_fp8_launch(  # noqa: E731
-        x, xs, 4, 2, hidden, p, 512, out, os, sf, col, 0, per, None)
+    fp8 = lambda x=p, xs=64, hidden=64, out=p, os=64, sf=p, col=512, per=512, rc=p, scratch=None, nbytes=0: lib.dg_moe_dispatch_fp8_launch(  # noqa: E731
+        x, xs, 4, 2, hidden, p, rc, 512, out, os, sf, col, 0, per, scratch, nbytes, None)
     _refused(fp8(hidden=48), 'multiple of 32')
     _refused(fp8(xs=60), 'input rows must start on 16-byte boundaries')
     _refused(fp8(os=60), 'output rows must start on 8-byte boundaries')
     _refused(fp8(col=500), 'scale column stride')
     _refused(fp8(per=0, col=0), 'scale column stride')
     _refused(fp8(sf=None), 'null pointer')
+    for bad in (dict(nbytes=63), dict(scratch=p + 8, nbytes=64), dict(rc=None, nbytes=64)):
+        _refused(fp8(**{'scratch': p, **bad}), 'the scratch must be')
+    assert lib.dg_moe_dispatch_fp8_scratch_bytes(64, 8, 7168) == 0 and lib.dg_moe_dispatch_fp8_scratch_bytes(8191, 8, 7200) == 8191 * 240
     combine = lambda y=p, ys=64, hidden=64, out=p, os=64: lib.dg_moe_combine_launch(y, 0, ys, 512, hidden, p, 4, 2, p, out, os, None)  # noqa: E731
     for bad in (dict(y=p + 2), dict(ys=60), dict(hidden=60), dict(out=p + 2), dict(os=60)):
         _refused(combine(**bad), '16-byte boundaries')
@@ -83,7 +86,8 @@ def test_the_c_abi_checks_its_arguments():
         x, 0, xs, 0, groups, rows, cols, mn, psum, e, align, out, os, 0, sf, ss, 0, None)
     _refused(fp4(cols=48), 'multiple of 32')
     _refused(fp4(xs=60), '16-byte boundaries')
-    _refused(fp4(os=30), '4-byte boundaries')
+    _refused(fp4(os=30), 'codes must start on 4-byte boundaries')
+    _refused(fp4(os=36, mn=1), 'codes must start on 16-byte boundaries')
     _refused(fp4(ss=7), 'scale stride')
     _refused(fp4(mn=1, ss=63), 'scale stride')
     _refused(fp4(psum=p, e=4, align=48), 'multiple of 32')
