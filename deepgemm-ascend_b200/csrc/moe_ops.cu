@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_dispatch_fp8_kernel(const Dis
 
 // Scale bytes by token -> the layout that the GEMM reads. One CTA = 64 rows: their tokens' bytes are read 16 at a time into shared memory
 // (rows an odd number of words apart: the columns are read without conflicts), and every scale column of the tile is a run of 128 bytes.
-constexpr uint32_t kScaleRows = 64, kScaleChunk = 128;  // rows of a CTA, scale bytes of a row that it holds at a time
+constexpr uint32_t kScaleRows = 64, kScaleChunk = 256;  // rows of a CTA, scale bytes of a row that it holds at a time
 __global__ void __launch_bounds__(kMoeThreads) moe_scales_kernel(const DispatchArgs a) {
     __shared__ uint32_t bytes[kScaleRows][kScaleChunk / 4 + 1];
     __shared__ uint32_t token_of[kScaleRows];
@@ -399,10 +399,11 @@ struct CombineGradArgs {
 
 // One CTA a token: its gradient is read once and multiplied with eight rows at a time; the products with the rows are summed over the
 // CTA. The CTAs behind the last token zero the padding. Where the rows begin is kept in shared memory: as registers those 32 words
-// left one CTA on an SM.
+// left eight warps on an SM (4096 tokens x 7168, 8 rows each: 210 us; three CTAs of 256 threads 160, six of 128 158, eight of 128 161).
+constexpr uint32_t kGradThreads = 128;
 template <typename T>
-__global__ void __launch_bounds__(kMoeThreads, 3) moe_combine_grad_kernel(const CombineGradArgs a) {
-    __shared__ float partial[kMoeWarps][8];
+__global__ void __launch_bounds__(kGradThreads, 6) moe_combine_grad_kernel(const CombineGradArgs a) {
+    __shared__ float partial[kGradThreads / 32][8];
     __shared__ const uint8_t* from[8];
     __shared__ uint8_t* to[8];
     __shared__ float weights[8];
@@ -657,7 +658,7 @@ extern "C" int dg_moe_combine_grad_launch(const void* grad_out, int is_fp32, uin
     a.dw = grad_weights;
     a.units = (uint32_t)(hidden * es / 16);
     // as few threads as take a row in the same number of turns
-    const uint32_t turns = a.units > kMoeThreads ? (a.units + kMoeThreads - 1) / kMoeThreads : 1;
+    const uint32_t turns = a.units > kGradThreads ? (a.units + kGradThreads - 1) / kGradThreads : 1;
     const uint32_t threads = a.units == 0 ? 32 : ((a.units + turns - 1) / turns + 31) / 32 * 32;
     const uint64_t ctas = tokens + (padding_items(a.r) + threads / 32 - 1) / (threads / 32);
     if (ctas == 0) return DG_OK;

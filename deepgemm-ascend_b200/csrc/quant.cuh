@@ -57,19 +57,41 @@ __device__ __forceinline__ uint32_t e2m1_scale_byte(uint32_t amax_bits) {
     const int32_t e = (int32_t)((amax_bits + 0x3fffffu) >> 23) - 2;
     return (uint32_t)max(e, 1);
 }
-// Factor that brings a block of scale byte `e` into E2M1's range (0 where the scale is NaN: the codes do not matter then).
-__device__ __forceinline__ float e2m1_inverse(uint32_t e) { return e == 255u ? 0.0f : __uint_as_float((254u - e) << 23); }
-// Eight values times `inv`, rounded to the nearest E2M1 (halves to the even code), the first in the lowest bits.
-__device__ __forceinline__ uint32_t e2m1_pack8(const float (&v)[8], float inv) {
+// Exponent field of the factor that brings a block of scale byte `e` into E2M1's range (0 where the scale is NaN: the codes do not
+// matter then).
+__device__ __forceinline__ uint32_t e2m1_inverse(uint32_t e) { return e == 255u ? 0u : 254u - e; }
+// Eight values, rounded to the nearest E2M1 (halves to the even code), the first in the lowest bits.
+__device__ __forceinline__ uint32_t e2m1_pack8(const float (&v)[8]) {
     uint32_t q = 0;
     #pragma unroll
     for (int h = 0; h < 4; ++h)
-        q |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(v[2 * h] * inv, v[2 * h + 1] * inv), __NV_E2M1, cudaRoundNearest) << (8 * h);
+        q |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(v[2 * h], v[2 * h + 1]), __NV_E2M1, cudaRoundNearest) << (8 * h);
     return q;
 }
-// A power of two from its exponent byte: 2^-127 is a subnormal number, 255 is NaN.
+// Eight codes as BF16 pairs, exactly: the two bytes of a magnitude are looked up by its three bits in tables of eight bytes (a byte permute
+// takes four of them at a time), the sign bits by a permute that repeats the top bit of its source where a code's fourth bit is set.
+__device__ __forceinline__ void e2m1_to_bf16(uint32_t q, uint32_t (&w)[4]) {
+    #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t four = q >> (16 * h), magnitude = four & 0x7777u;
+        const uint32_t low = __byte_perm(0xc0800000u, 0xc0804000u, magnitude);        // 0, .5, 1, 1.5 and 2, 3, 4, 6
+        uint32_t high = __byte_perm(0x3f3f3f00u, 0x40404040u, magnitude);
+        uint32_t sign;                                                                // 0x80 where positive, 0xff where negative
+        asm("prmt.b32 %0, %1, %1, %2;" : "=r"(sign) : "r"(0x80808080u), "r"(four));
+        high |= (sign << 7) & 0x80808080u;
+        w[2 * h] = __byte_perm(low, high, 0x5140);
+        w[2 * h + 1] = __byte_perm(low, high, 0x7362);
+    }
+}
+// A power of two from its exponent byte, as FP32 or BF16 bits: 2^-127 is a subnormal number, 255 is NaN.
 __device__ __forceinline__ float ue8m0_value(uint32_t e) {
     return e == 0u ? __uint_as_float(0x00400000u) : e == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(e << 23);
+}
+__device__ __forceinline__ uint32_t ue8m0_bf16(uint32_t e) { return e == 0u ? 0x0040u : e == 255u ? 0x7fffu : e << 7; }
+// Two products of BF16 values. (One factor is a power of two here: exact but where the result is subnormal.)
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+    const __nv_bfloat162 p = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&p);
 }
 
 }  // namespace dg

@@ -28,31 +28,60 @@ struct Fp4Args {
     uint32_t rows, cols, tiles_r, tiles_c;
 };
 
-// Eight values of a lane, as they lie in memory.
+// Eight values of a lane, as they lie in memory: kWords words of one or two values. Magnitudes are compared as bit patterns (infinities
+// and NaN come out on top by themselves), BF16 two at a time; so are the products with the inverse scales, which are exact (down to where
+// BF16 has subnormals, all of which round to zero), so that half of the arithmetic per value is gone: an MN-major quantiser that
+// turned every BF16 into FP32 first kept the SMs at 67 % and HBM at 58 %.
 template <typename T> struct Raw8;
 template <> struct Raw8<__nv_bfloat16> {
-    uint4 a;
-    __device__ __forceinline__ void clear() { a = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ void load(const uint8_t* p) { a = ld_stream_v4(p); }
-    __device__ __forceinline__ void values(float (&v)[8]) const {
-        const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    static constexpr int kWords = 4;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void clear() { w[0] = w[1] = w[2] = w[3] = 0u; }
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        const uint4 q = ld_stream_v4(p);
+        w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+    }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return __vmaxu2(a, b); }
+    static __device__ __forceinline__ uint32_t magnitude(uint32_t w) { return w & 0x7fff7fffu; }
+    // FP32 bits of column `j` of the magnitudes, factors of the columns of a word from the exponent fields of the inverse scales
+    static __device__ __forceinline__ uint32_t bits(const uint32_t (&m)[kWords], int j) { return j % 2 ? m[j / 2] & 0xffff0000u : m[j / 2] << 16; }
+    static __device__ __forceinline__ uint32_t factor(const uint32_t (&field)[8], int word) { return field[2 * word] << 7 | field[2 * word + 1] << 23; }
+    static __device__ __forceinline__ uint32_t factor(uint32_t field) { return field << 7 | field << 23; }
+    __device__ __forceinline__ uint32_t codes(const uint32_t (&f)[kWords]) const {
+        float v[8];
         #pragma unroll
-        for (int j = 0; j < 4; ++j) { v[2 * j] = bf16_lo(w[j]); v[2 * j + 1] = bf16_hi(w[j]); }
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t p = mul_bf16x2(w[j], f[j]);
+            v[2 * j] = bf16_lo(p);
+            v[2 * j + 1] = bf16_hi(p);
+        }
+        return e2m1_pack8(v);
     }
 };
 template <> struct Raw8<float> {
-    uint4 a, b;
-    __device__ __forceinline__ void clear() { a = b = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ void load(const uint8_t* p) { a = ld_global_v4(p); b = ld_global_v4(p + 16); }
-    __device__ __forceinline__ void values(float (&v)[8]) const {
-        const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    static constexpr int kWords = 8;
+    uint32_t w[kWords];
+    __device__ __forceinline__ void clear() {
         #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+        for (int j = 0; j < 8; ++j) w[j] = 0u;
+    }
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        const uint4 q = ld_global_v4(p), r = ld_global_v4(p + 16);
+        w[0] = q.x; w[1] = q.y; w[2] = q.z; w[3] = q.w;
+        w[4] = r.x; w[5] = r.y; w[6] = r.z; w[7] = r.w;
+    }
+    static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return max(a, b); }
+    static __device__ __forceinline__ uint32_t magnitude(uint32_t w) { return w & 0x7fffffffu; }
+    static __device__ __forceinline__ uint32_t bits(const uint32_t (&m)[kWords], int j) { return m[j]; }
+    static __device__ __forceinline__ uint32_t factor(const uint32_t (&field)[8], int word) { return field[word] << 23; }
+    static __device__ __forceinline__ uint32_t factor(uint32_t field) { return field << 23; }
+    __device__ __forceinline__ uint32_t codes(const uint32_t (&f)[kWords]) const {
+        float v[8];
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]) * __uint_as_float(f[j]);
+        return e2m1_pack8(v);
     }
 };
-
-// Magnitudes are compared as bit patterns: infinities and NaN come out on top by themselves.
-__device__ __forceinline__ uint32_t magnitude_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 constexpr uint32_t kFp4Threads = 256, kFp4Rows = 32, kFp4Cols = 256;
 
@@ -80,16 +109,20 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_kernel(const Fp4Args a)
     }
     #pragma unroll
     for (uint32_t i = 0; i < kWarpRows; ++i) {
-        float v[8];
-        raw[i].values(v);
-        uint32_t amax = 0;
+        uint32_t m[Raw8<T>::kWords], f[Raw8<T>::kWords];
         #pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max(amax, magnitude_bits(v[j]));
+        for (int j = 0; j < Raw8<T>::kWords; ++j) {
+            m[j] = Raw8<T>::magnitude(raw[i].w[j]);
+            if (j > 0) m[0] = Raw8<T>::larger(m[0], m[j]);
+        }
+        uint32_t amax = sizeof(T) == 2 ? max(Raw8<T>::bits(m, 0), Raw8<T>::bits(m, 1)) : m[0];
         amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         const uint32_t e = e2m1_scale_byte(amax);
+        #pragma unroll
+        for (int j = 0; j < Raw8<T>::kWords; ++j) f[j] = Raw8<T>::factor(e2m1_inverse(e));
         if (r0 + i < row_end && c < a.cols)
-            *reinterpret_cast<uint32_t*>(a.codes + group * a.code_group_stride + (uint64_t)(r0 + i) * a.code_stride + c / 2) = e2m1_pack8(v, e2m1_inverse(e));
+            *reinterpret_cast<uint32_t*>(a.codes + group * a.code_group_stride + (uint64_t)(r0 + i) * a.code_stride + c / 2) = raw[i].codes(f);
         // (the second block of a last, half-used scale column is zero)
         if ((lane & 3u) == 0) sf_smem[warp * kWarpRows + i][lane / 4] = c < a.cols ? (uint8_t)e : (uint8_t)0;
     }
@@ -107,7 +140,7 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_kernel(const Fp4Args a)
 constexpr uint32_t kFp4StageWords = 40;
 template <typename T>
 __global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args a) {
-    __shared__ uint8_t sf_smem[2][kFp4Cols];
+    __shared__ __align__(8) uint8_t sf_smem[2][kFp4Cols];
     __shared__ __align__(16) uint32_t stage[64][kFp4StageWords];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t tiles = a.tiles_r * a.tiles_c, group = blockIdx.x / tiles, tile = blockIdx.x - group * tiles;
@@ -130,32 +163,29 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args
         raw[i].clear();
         if (r0 + i * 4 < row_end && c < a.cols) raw[i].load(a.x + group * a.x_group_stride + (uint64_t)(r0 + i * 4) * a.x_stride + (uint64_t)c * sizeof(T));
     }
-    uint32_t amax[8] = {};
+    uint32_t m[Raw8<T>::kWords] = {}, f[Raw8<T>::kWords], field[8];
     #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        float v[8];
-        raw[i].values(v);
+    for (uint32_t i = 0; i < 8; ++i)
         #pragma unroll
-        for (int j = 0; j < 8; ++j) amax[j] = max(amax[j], magnitude_bits(v[j]));
+        for (int j = 0; j < Raw8<T>::kWords; ++j) m[j] = Raw8<T>::larger(m[j], Raw8<T>::magnitude(raw[i].w[j]));
+    #pragma unroll
+    for (int j = 0; j < Raw8<T>::kWords; ++j) {
+        m[j] = Raw8<T>::larger(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
+        m[j] = Raw8<T>::larger(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
     }
-    float inv[8];
+    uint32_t bytes[2] = {};
     #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], 8));
-        amax[j] = max(amax[j], __shfl_xor_sync(0xffffffffu, amax[j], 16));
-        const uint32_t e = e2m1_scale_byte(amax[j]);
-        inv[j] = e2m1_inverse(e);
-        // (blocks behind the last row are zero)
-        if (lane < 8) sf_smem[half][tc + j] = row_base + half * 32 < a.rows ? (uint8_t)e : (uint8_t)0;
+        const uint32_t e = e2m1_scale_byte(Raw8<T>::bits(m, j));
+        field[j] = e2m1_inverse(e);
+        bytes[j / 4] |= e << (j % 4 * 8);
     }
     #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        float v[8];
-        raw[i].values(v);
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= inv[j];
-        stage[tr + i * 4][tc / 8] = e2m1_pack8(v, 1.0f);
-    }
+    for (int j = 0; j < Raw8<T>::kWords; ++j) f[j] = Raw8<T>::factor(field, j);
+    // (blocks behind the last row are zero)
+    if (lane < 8) *reinterpret_cast<uint2*>(&sf_smem[half][tc]) = row_base + half * 32 < a.rows ? make_uint2(bytes[0], bytes[1]) : make_uint2(0u, 0u);
+    #pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) stage[tr + i * 4][tc / 8] = raw[i].codes(f);
     __syncthreads();
     #pragma unroll
     for (uint32_t i = 0; i < 2; ++i) {
@@ -169,32 +199,35 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args
             (uint16_t)(sf_smem[0][threadIdx.x] | ((uint32_t)sf_smem[1][threadIdx.x] << 8));
 }
 
-// The way back: code x 2^(byte - 127), exact in FP32 and rounded once to BF16 (which changes it only where BF16 has subnormals).
-template <typename T>
-__device__ __forceinline__ void store8(uint8_t* p, const float (&v)[8]) {
-    if constexpr (sizeof(T) == 2) {
+// The way back: code x 2^(byte - 127), in the type of the result (exact, but rounded once where that has subnormals).
+template <typename T> struct Out8;
+template <> struct Out8<__nv_bfloat16> {
+    static __device__ __forceinline__ uint32_t scale(uint32_t byte) { return ue8m0_bf16(byte) * 0x10001u; }
+    static __device__ __forceinline__ uint32_t scale_pair(uint32_t b0, uint32_t b1) { return ue8m0_bf16(b0) | ue8m0_bf16(b1) << 16; }
+    static __device__ __forceinline__ void store(uint8_t* p, uint32_t q, const uint32_t (&s)[4]) {
         uint32_t w[4];
+        e2m1_to_bf16(q, w);
+        *reinterpret_cast<uint4*>(p) = make_uint4(mul_bf16x2(w[0], s[0]), mul_bf16x2(w[1], s[1]), mul_bf16x2(w[2], s[2]), mul_bf16x2(w[3], s[3]));
+    }
+};
+template <> struct Out8<float> {
+    // (the scales are held as BF16 pairs too, which holds every power of two that a byte stands for)
+    static __device__ __forceinline__ uint32_t scale(uint32_t byte) { return Out8<__nv_bfloat16>::scale(byte); }
+    static __device__ __forceinline__ uint32_t scale_pair(uint32_t b0, uint32_t b1) { return Out8<__nv_bfloat16>::scale_pair(b0, b1); }
+    static __device__ __forceinline__ void store(uint8_t* p, uint32_t q, const uint32_t (&s)[4]) {
+        uint32_t w[4];
+        e2m1_to_bf16(q, w);
+        float v[8];
         #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-            w[j] = *reinterpret_cast<const uint32_t*>(&b);
+            v[2 * j] = bf16_lo(w[j]) * bf16_lo(s[j]);
+            v[2 * j + 1] = bf16_hi(w[j]) * bf16_hi(s[j]);
         }
-        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
-    } else {
         // (one store of 32 bytes: as two, each leaves half of every sector to the other)
         asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
                      "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
     }
-}
-__device__ __forceinline__ void e2m1_values8(uint32_t q, float (&v)[8]) {
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const __half2_raw h = __nv_cvt_fp4x2_to_halfraw2((__nv_fp4x2_storage_t)((q >> (8 * j)) & 0xffu), __NV_E2M1);
-        const float2 f = __half22float2(__half2(h));
-        v[2 * j] = f.x;
-        v[2 * j + 1] = f.y;
-    }
-}
+};
 
 // One CTA = 64 rows x 256 columns, a warp eight rows, a lane eight columns. The scales of a K-major tile come in runs down the rows, through
 // shared memory; an MN-major tile lies in two blocks of rows, whose scales lie along the columns.
@@ -213,13 +246,16 @@ __global__ void __launch_bounds__(kFp4Threads) dequant_fp4_kernel(const Fp4Args 
     for (uint32_t i = 0; i < kWarpRows; ++i)
         q[i] = r0 + i < a.rows && c < a.cols ? ld_stream_u32(a.codes + group * a.code_group_stride + (uint64_t)(r0 + i) * a.code_stride + c / 2) : 0u;
     const uint8_t* sf = a.sf + group * a.sf_group_stride;
-    float scale[8];
+    uint32_t scale[4];
     if constexpr (kMnMajor) {
+        uint32_t byte[8];
         #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const uint32_t pair = c < a.cols ? ld_global_u16(sf + (uint64_t)(row_base / 64) * a.sf_stride + (uint64_t)(c + j) * 2) : 0u;
-            scale[j] = ue8m0_value((pair >> (warp / 4 * 8)) & 0xffu);
+            byte[j] = (pair >> (warp / 4 * 8)) & 0xffu;
         }
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) scale[j] = Out8<T>::scale_pair(byte[2 * j], byte[2 * j + 1]);
     } else {
         const uint32_t col = threadIdx.x / 64, r = threadIdx.x % 64;
         if (c0 + col * 64 < a.cols && row_base + r < a.rows)
@@ -229,12 +265,8 @@ __global__ void __launch_bounds__(kFp4Threads) dequant_fp4_kernel(const Fp4Args 
     #pragma unroll
     for (uint32_t i = 0; i < kWarpRows; ++i) {
         if (r0 + i >= a.rows || c >= a.cols) continue;
-        float v[8];
-        e2m1_values8(q[i], v);
-        const float s = kMnMajor ? 1.0f : ue8m0_value(sf_smem[warp * kWarpRows + i][lane / 4]);
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] *= kMnMajor ? scale[j] : s;
-        store8<T>(out + group * a.x_group_stride + (uint64_t)(r0 + i) * a.x_stride + (uint64_t)c * sizeof(T), v);
+        if constexpr (!kMnMajor) scale[0] = scale[1] = scale[2] = scale[3] = Out8<T>::scale(sf_smem[warp * kWarpRows + i][lane / 4]);
+        Out8<T>::store(out + group * a.x_group_stride + (uint64_t)(r0 + i) * a.x_stride + (uint64_t)c * sizeof(T), q[i], scale);
     }
 }
 
