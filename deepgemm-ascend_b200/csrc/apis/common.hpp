@@ -43,6 +43,13 @@ inline void check(int rc) {
     }
 }
 
+// Packed scales of `shape` [.., rows, cols], consecutive rows contiguous: the layout that the GEMMs read.
+inline torch::Tensor empty_scales(const std::vector<int64_t>& shape, const torch::Tensor& like) {
+    const int64_t rows = std::max<int64_t>(shape[shape.size() - 2], 1), cols = std::max<int64_t>(shape.back(), 1);
+    const auto options = like.options().dtype(torch::kInt16);
+    return shape.size() == 3 ? torch::empty_strided(shape, {rows * cols, 1, rows}, options) : torch::empty_strided(shape, {1, rows}, options);
+}
+
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 inline int64_t align_up(int64_t a, int64_t b) { return ceil_div(a, b) * b; }
 

@@ -71,10 +71,19 @@ inline MoePlan moe_sort(const torch::Tensor& topk_idx, int64_t num_experts, int6
     const int64_t rows = slots ? num_experts * slots : (int64_t)dg_moe_num_rows((uint32_t)topk_idx.numel(), (uint32_t)num_experts, (uint32_t)expert_alignment);
     host_assert(rows <= INT32_MAX, "the layout has too many rows");
     const c10::cuda::CUDAGuard guard(topk_idx.device());
-    const auto int32 = topk_idx.options().dtype(torch::kInt32);
-    auto layout = torch::empty({num_experts}, int32);
-    auto token_rows = torch::empty(topk_idx.sizes(), int32);
-    auto row_choices = slots ? torch::empty({num_experts, slots}, int32) : torch::empty({rows}, int32);
+    // one allocation for the three (about a microsecond of host time each); every part starts on 16 bytes
+    const int64_t part[3] = {num_experts, topk_idx.numel(), rows};
+    int64_t offset = 0;
+    const auto buffer = torch::empty({align_up(part[0], 4) + align_up(part[1], 4) + part[2]}, topk_idx.options().dtype(torch::kInt32));
+    const auto take = [&](int k, at::IntArrayRef sizes) {
+        auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), buffer.dtype());
+        t.unsafeGetTensorImpl()->set_storage_offset(offset);
+        t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+        offset += align_up(part[k], 4);
+        return t;
+    };
+    const auto layout = take(0, {num_experts}), token_rows = take(1, topk_idx.sizes());
+    const auto row_choices = slots ? take(2, {num_experts, slots}) : take(2, {rows});
     check(dg_moe_sort_launch(topk_idx.data_ptr(), topk_idx.scalar_type() == torch::kInt64, (uint32_t)topk_idx.size(0), (uint32_t)topk_idx.size(1),
                              (uint32_t)num_experts, (uint32_t)expert_alignment, (uint32_t)slots, static_cast<int32_t*>(layout.data_ptr()),
                              static_cast<int32_t*>(token_rows.data_ptr()), static_cast<int32_t*>(row_choices.data_ptr()), (uint64_t)rows, stream_of(topk_idx)));
@@ -115,9 +124,7 @@ inline TensorPair moe_dispatch_to_fp8(const torch::Tensor& x, const MoePlan& pla
                     "the scales of out must be int16, one element for 64 channels of each row, contiguous along the rows");
     } else {
         out = torch::empty(plan.shape(hidden), x.options().dtype(torch::kFloat8_e4m3fn));
-        const auto storage = torch::empty({plan.max_m ? plan.experts : 1, cols, per_group}, x.options().dtype(torch::kInt16));
-        sf = storage.transpose(1, 2);
-        if (!plan.max_m) sf = sf.squeeze(0);
+        sf = empty_scales(plan.shape(cols), x);
     }
     const int64_t stride = plan.check_rows(out, "out must hold a row for each of the layout's, at one distance");
     const uint64_t nbytes = dg_moe_dispatch_fp8_scratch_bytes((uint32_t)plan.tokens, (uint32_t)plan.topk, (uint32_t)hidden);

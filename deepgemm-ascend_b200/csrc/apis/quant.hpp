@@ -55,15 +55,16 @@ inline TensorPair cast_to_fp4(const torch::Tensor& x, const std::optional<torch:
     shape.back() = cols / 2;
     auto out = torch::empty(shape, x.options().dtype(torch::kInt8));
     const int64_t k64 = ceil_div(mn_major ? rows : cols, 64), run = mn_major ? cols : rows;
-    auto storage = torch::empty({groups, k64, run}, x.options().dtype(torch::kInt16));
+    auto sf_shape = x.sizes().vec();
+    (mn_major ? sf_shape[sf_shape.size() - 2] : sf_shape.back()) = k64;
+    auto sf = mn_major ? torch::empty(sf_shape, x.options().dtype(torch::kInt16)) : empty_scales(sf_shape, x);
     if (x.numel() != 0)
         check(dg_quant_fp4_launch(x.data_ptr(), x.scalar_type() == torch::kFloat32, rows > 1 ? (uint64_t)x.stride(-2) : (uint64_t)cols,
                                   groups > 1 ? (uint64_t)x.stride(0) : 0, (uint32_t)groups, (uint32_t)rows, (uint32_t)cols, mn_major,
                                   psum.has_value() ? static_cast<const int32_t*>(psum->data_ptr()) : nullptr,
                                   psum.has_value() ? (uint32_t)psum->numel() : 0u, (uint32_t)expert_alignment, out.data_ptr(), (uint64_t)(cols / 2),
-                                  (uint64_t)(rows * (cols / 2)), static_cast<int16_t*>(storage.data_ptr()), (uint64_t)run, (uint64_t)(k64 * run), stream_of(x)));
-    auto sf = mn_major ? storage : storage.transpose(1, 2);
-    return {out, x.dim() == 3 ? sf : sf.squeeze(0)};
+                                  (uint64_t)(rows * (cols / 2)), static_cast<int16_t*>(sf.data_ptr()), (uint64_t)run, (uint64_t)(k64 * run), stream_of(x)));
+    return {out, sf};
 }
 
 inline torch::Tensor cast_from_fp4(const TensorPair& x, const torch::Dtype& out_dtype, bool mn_major) {

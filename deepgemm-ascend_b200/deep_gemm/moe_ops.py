@@ -29,6 +29,7 @@ import torch
 
 from . import _lib as L
 from ._api import MK_ALIGNMENT, _C, _ceil_div, _host_assert, _stream_ptr
+from .quant_ops import _empty_scales
 
 _INT_MAX = 2 ** 31 - 1
 _OUT_ROWS = "out must hold a row for each of the layout's, at one distance"
@@ -148,8 +149,7 @@ def moe_dispatch_to_fp8(x: torch.Tensor, plan, out=None):
                          'the scales of out must be int16, one element for 64 channels of each row, contiguous along the rows')
         else:
             out = torch.empty(p.shape(hidden), dtype=torch.float8_e4m3fn, device=x.device)
-            sf = torch.empty((p.experts if p.max_m else 1, cols, per_group), dtype=torch.int16, device=x.device).transpose(1, 2)
-            sf = sf if p.max_m else sf.squeeze(0)
+            sf = _empty_scales(p.shape(cols), x.device)
         stride = p.check_rows(out, _OUT_ROWS)
         nbytes = L.lib().dg_moe_dispatch_fp8_scratch_bytes(p.tokens, p.topk, hidden)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None

@@ -55,6 +55,12 @@ def cast_to_fp8(x: torch.Tensor, psum_num_tokens_per_expert: Optional[torch.Tens
     return _launch(x, x.size(1), False, None, psum_num_tokens_per_expert, None, expert_alignment)
 
 
+def _empty_scales(shape, device):
+    """Packed scales [.., rows, cols] with consecutive rows contiguous."""
+    rows, cols = max(shape[-2], 1), max(shape[-1], 1)
+    return torch.empty_strided(shape, (rows * cols, 1, rows)[-len(shape):], dtype=torch.int16, device=device)
+
+
 def cast_to_fp4(x: torch.Tensor, psum_num_tokens_per_expert: Optional[torch.Tensor] = None, expert_alignment: int = 128, mn_major: bool = False):
     """x [rows, cols] or [groups, rows, cols] BF16 or FP32 -> (packed E2M1 int8 [.., rows, cols / 2], packed UE8M0 scales), one scale per
     32 values along K, in the layout that the GEMMs read:
@@ -82,14 +88,14 @@ def cast_to_fp4(x: torch.Tensor, psum_num_tokens_per_expert: Optional[torch.Tens
     with torch.cuda.device(x.device):
         out = torch.empty((*x.shape[:-1], cols // 2), dtype=torch.int8, device=x.device)
         k64, run = _ceil_div(rows if mn_major else cols, 64), cols if mn_major else rows
-        storage = torch.empty((groups, k64, run), dtype=torch.int16, device=x.device)
+        sf = (torch.empty((*x.shape[:-2], k64, cols), dtype=torch.int16, device=x.device) if mn_major else
+              _empty_scales((*x.shape[:-1], k64), x.device))
         if x.numel():
             L.check(L.lib().dg_quant_fp4_launch(
                 x.data_ptr(), int(x.dtype == torch.float32), x.stride(-2) if rows > 1 else cols, x.stride(0) if groups > 1 else 0, groups, rows, cols,
                 int(mn_major), psum.data_ptr() if psum is not None else None, psum.numel() if psum is not None else 0, int(expert_alignment),
-                out.data_ptr(), cols // 2, rows * (cols // 2), storage.data_ptr(), run, k64 * run, _stream_ptr(x.device)))
-    sf = storage if mn_major else storage.transpose(1, 2)
-    return out, sf if x.dim() == 3 else sf.squeeze(0)
+                out.data_ptr(), cols // 2, rows * (cols // 2), sf.data_ptr(), run, k64 * run, _stream_ptr(x.device)))
+    return out, sf
 
 
 def cast_from_fp4(x, out_dtype: torch.dtype = torch.bfloat16, mn_major: bool = False):
