@@ -90,7 +90,7 @@ def build_extension(force: bool = False, verbose: bool = False) -> str:
            os.path.join(CSRC, 'python_api.cpp'), '-o', EXT_OUT,
            *['-I' + p for p in cpp_extension.include_paths()], '-I' + sysconfig.get_paths()['include'],
            '-I/usr/local/cuda/include',
-           '-L' + torch_lib, '-ltorch_python', '-ltorch', '-ltorch_cpu', '-lc10', '-lc10_cuda',
+           '-L' + torch_lib, '-ltorch_python', '-ltorch', '-ltorch_cuda', '-ltorch_cpu', '-lc10', '-lc10_cuda',
            '-L' + os.path.dirname(OUT), '-l:libdg_b200.so', '-Wl,-rpath,$ORIGIN', '-Wl,-rpath,' + torch_lib]
     proc = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
     if verbose or proc.returncode != 0:

@@ -74,7 +74,7 @@ inline MoePlan moe_sort(const torch::Tensor& topk_idx, int64_t num_experts, int6
     // one allocation for the three (about a microsecond of host time each); every part starts on 16 bytes
     const int64_t part[3] = {num_experts, topk_idx.numel(), rows};
     int64_t offset = 0;
-    const auto buffer = torch::empty({align_up(part[0], 4) + align_up(part[1], 4) + part[2]}, topk_idx.options().dtype(torch::kInt32));
+    const auto buffer = empty_on({align_up(part[0], 4) + align_up(part[1], 4) + part[2]}, torch::kInt32, topk_idx);
     const auto take = [&](int k, at::IntArrayRef sizes) {
         auto t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buffer.storage()), buffer.key_set(), buffer.dtype());
         t.unsafeGetTensorImpl()->set_storage_offset(offset);
@@ -98,7 +98,7 @@ inline torch::Tensor moe_dispatch(const torch::Tensor& x, const MoePlan& plan_in
     const c10::cuda::CUDAGuard guard(x.device());
     if (out_in.has_value()) host_assert(out_in->scalar_type() == x.scalar_type() && out_in->device() == x.device() && out_in->size(-1) == x.size(1),
                                         "out must have the type, the device and the row length of x");
-    const auto out = out_in.has_value() ? out_in.value() : torch::empty(plan.shape(x.size(1)), x.options());
+    const auto out = out_in.has_value() ? out_in.value() : empty_on(plan.shape(x.size(1)), x.scalar_type(), x);
     const int64_t stride = plan.check_rows(out, "out must hold a row for each of the layout's, at one distance"), es = x.element_size();
     check(dg_moe_dispatch_launch(x.data_ptr(), (uint64_t)(stride_of_rows(x) * es), (uint32_t)plan.tokens, (uint32_t)plan.topk, (uint64_t)(x.size(1) * es),
                                  plan.token_rows_ptr(), (uint64_t)plan.rows, out.data_ptr(), (uint64_t)(stride * es), plan.layout_ptr(),
@@ -123,12 +123,12 @@ inline TensorPair moe_dispatch_to_fp8(const torch::Tensor& x, const MoePlan& pla
                     (sf.dim() == 2 || plan.experts <= 1 || sf.stride(0) >= (cols > 1 ? (cols - 1) * sf.stride(-1) : 0) + per_group),
                     "the scales of out must be int16, one element for 64 channels of each row, contiguous along the rows");
     } else {
-        out = torch::empty(plan.shape(hidden), x.options().dtype(torch::kFloat8_e4m3fn));
+        out = empty_on(plan.shape(hidden), torch::kFloat8_e4m3fn, x);
         sf = empty_scales(plan.shape(cols), x);
     }
     const int64_t stride = plan.check_rows(out, "out must hold a row for each of the layout's, at one distance");
     const uint64_t nbytes = dg_moe_dispatch_fp8_scratch_bytes((uint32_t)plan.tokens, (uint32_t)plan.topk, (uint32_t)hidden);
-    const auto scratch = nbytes ? torch::empty({(int64_t)nbytes}, x.options().dtype(torch::kUInt8)) : torch::Tensor();
+    const auto scratch = nbytes ? empty_on({(int64_t)nbytes}, torch::kUInt8, x) : torch::Tensor();
     check(dg_moe_dispatch_fp8_launch(x.data_ptr(), (uint64_t)stride_of_rows(x), (uint32_t)plan.tokens, (uint32_t)plan.topk, (uint32_t)hidden,
                                      plan.token_rows_ptr(), static_cast<const int32_t*>(plan.row_choices.data_ptr()), (uint64_t)plan.rows,
                                      out.data_ptr(), (uint64_t)stride, static_cast<int16_t*>(sf.data_ptr()),
@@ -149,7 +149,7 @@ inline torch::Tensor moe_combine(const torch::Tensor& rows, const MoePlan& plan_
         host_assert(out_in->scalar_type() == rows.scalar_type() && out_in->device() == rows.device() && out_in->dim() == 2 && out_in->size(0) == plan.tokens &&
                     out_in->size(1) == hidden && out_in->stride(1) == 1 && stride_of_rows(out_in.value()) >= hidden,
                     "out must be a row-major [tokens, hidden] tensor of the type and the device of rows");
-    const auto out = out_in.has_value() ? out_in.value() : torch::empty({plan.tokens, hidden}, rows.options());
+    const auto out = out_in.has_value() ? out_in.value() : empty_on({plan.tokens, hidden}, rows.scalar_type(), rows);
     check(dg_moe_combine_launch(rows.data_ptr(), rows.scalar_type() == torch::kFloat32, (uint64_t)stride, (uint64_t)plan.rows, (uint32_t)hidden, plan.token_rows_ptr(),
                                 (uint32_t)plan.tokens, (uint32_t)plan.topk, topk_weights.has_value() ? static_cast<const float*>(topk_weights->data_ptr()) : nullptr,
                                 out.data_ptr(), (uint64_t)stride_of_rows(out), stream_of(rows)));
@@ -171,9 +171,9 @@ inline TensorPair moe_combine_grad(const torch::Tensor& grad_out, const torch::T
     if (out_in.has_value())
         host_assert(out_in->scalar_type() == rows.scalar_type() && out_in->device() == rows.device() && out_in->size(-1) == hidden,
                     "out must have the type, the device and the row length of rows");
-    const auto out = out_in.has_value() ? out_in.value() : torch::empty(plan.shape(hidden), rows.options());
+    const auto out = out_in.has_value() ? out_in.value() : empty_on(plan.shape(hidden), rows.scalar_type(), rows);
     const int64_t out_stride = plan.check_rows(out, "out must hold a row for each of the layout's, at one distance");
-    const auto grad_weights = torch::empty(topk_weights.sizes(), topk_weights.options());
+    const auto grad_weights = empty_on(topk_weights.sizes(), topk_weights.scalar_type(), topk_weights);
     check(dg_moe_combine_grad_launch(grad_out.data_ptr(), rows.scalar_type() == torch::kFloat32, (uint64_t)stride_of_rows(grad_out), rows.data_ptr(), (uint64_t)stride,
                                      (uint64_t)plan.rows, (uint32_t)hidden, plan.token_rows_ptr(), (uint32_t)plan.tokens, (uint32_t)plan.topk,
                                      static_cast<const float*>(topk_weights.data_ptr()), out.data_ptr(), (uint64_t)out_stride,

@@ -53,11 +53,11 @@ inline TensorPair cast_to_fp4(const torch::Tensor& x, const std::optional<torch:
     const c10::cuda::CUDAGuard guard(x.device());
     auto shape = x.sizes().vec();
     shape.back() = cols / 2;
-    auto out = torch::empty(shape, x.options().dtype(torch::kInt8));
+    auto out = empty_on(shape, torch::kInt8, x);
     const int64_t k64 = ceil_div(mn_major ? rows : cols, 64), run = mn_major ? cols : rows;
     auto sf_shape = x.sizes().vec();
     (mn_major ? sf_shape[sf_shape.size() - 2] : sf_shape.back()) = k64;
-    auto sf = mn_major ? torch::empty(sf_shape, x.options().dtype(torch::kInt16)) : empty_scales(sf_shape, x);
+    auto sf = mn_major ? empty_on(sf_shape, torch::kInt16, x) : empty_scales(sf_shape, x);
     if (x.numel() != 0)
         check(dg_quant_fp4_launch(x.data_ptr(), x.scalar_type() == torch::kFloat32, rows > 1 ? (uint64_t)x.stride(-2) : (uint64_t)cols,
                                   groups > 1 ? (uint64_t)x.stride(0) : 0, (uint32_t)groups, (uint32_t)rows, (uint32_t)cols, mn_major,
@@ -83,7 +83,7 @@ inline torch::Tensor cast_from_fp4(const TensorPair& x, const torch::Dtype& out_
     const c10::cuda::CUDAGuard guard(codes.device());
     auto shape = codes.sizes().vec();
     shape.back() = cols;
-    auto out = torch::empty(shape, codes.options().dtype(out_dtype));
+    auto out = empty_on(shape, out_dtype, codes);
     if (out.numel() != 0)
         check(dg_dequant_fp4_launch(codes.data_ptr(), rows > 1 ? (uint64_t)codes.stride(-2) : (uint64_t)(cols / 2), groups > 1 ? (uint64_t)codes.stride(0) : 0,
                                     static_cast<const int16_t*>(sf.data_ptr()), k64 > 1 ? (uint64_t)sf.stride(mn_major ? -2 : -1) : (uint64_t)run,

@@ -284,8 +284,8 @@ __global__ void __launch_bounds__(kMoeThreads) moe_scales_kernel(const DispatchA
     __shared__ uint32_t bytes[kScaleRows][kScaleChunk / 4 + 1];
     __shared__ uint32_t token_of[kScaleRows];
     const uint32_t row0 = blockIdx.x * kScaleRows, b0 = blockIdx.y * kScaleChunk, tid = threadIdx.x;
-    griddep_wait();
-    griddep_launch_dependents();
+    // (the choices come from in front of the dispatch, whose CTAs have all passed their own wait when this kernel is let in: they may be read
+    // before the bytes that it writes are there)
     bool some = false;
     if (tid < kScaleRows) {
         const uint32_t choice = row0 + tid < a.r.rows ? ld_global_u32(a.row_choices + row0 + tid) : 0xffffffffu;
@@ -293,7 +293,10 @@ __global__ void __launch_bounds__(kMoeThreads) moe_scales_kernel(const DispatchA
         some = (int32_t)choice >= 0 && token < a.r.tokens;
         token_of[tid] = some ? token : 0xffffffffu;
     }
-    if (!__syncthreads_or(some)) return;
+    some = __syncthreads_or(some);
+    griddep_wait();
+    griddep_launch_dependents();
+    if (!some) return;
     const uint32_t words = min(kScaleChunk, a.scratch_stride - b0) / 16;       // pieces of 16 bytes
     for (uint32_t i = tid; i < kScaleRows * words; i += kMoeThreads) {
         const uint32_t r = i / words, w = i - r * words, token = token_of[r];
