@@ -400,16 +400,81 @@ struct CombineGradArgs {
     uint32_t units;
 };
 
-// One CTA a token: its gradient is read once and multiplied with eight rows at a time; the products with the rows are summed over the
-// CTA. The CTAs behind the last token zero the padding. Where the rows begin is kept in shared memory: as registers those 32 words
-// left eight warps on an SM (4096 tokens x 7168, 8 rows each: 210 us; three CTAs of 256 threads 160, six of 128 158, eight of 128 161).
-constexpr uint32_t kGradThreads = 128;
+constexpr uint32_t kGradThreads = 128, kGradCtas = 6;   // of a CTA; CTAs that an SM has the registers for
+
+// Where the rows of up to eight choices begin. In shared memory: as registers these words left eight
+// warps on an SM.
+struct GradRows {
+    const uint8_t* from[8];
+    uint8_t* to[8];
+    float weight[8];
+    uint32_t choice[8];
+};
+
+// kRows rows at a time, kTurns turns of the CTA over the row together: 8 to 10 pieces of 16 bytes on their way, however few rows there are.
+template <typename T, int kRows, int kTurns>
+__device__ __forceinline__ void grad_rows(const CombineGradArgs& a, const uint8_t* grad, const GradRows& rows, uint32_t n, float (&dot)[kRows]) {
+    #pragma unroll
+    for (int r = 0; r < kRows; ++r) dot[r] = 0.f;
+    for (uint32_t u0 = threadIdx.x; u0 < a.units; u0 += blockDim.x * kTurns) {
+        uint4 gq[kTurns], q[kTurns][kRows];
+        #pragma unroll
+        for (int t = 0; t < kTurns; ++t) {
+            const uint32_t u = u0 + t * blockDim.x;
+            gq[t] = make_uint4(0u, 0u, 0u, 0u);
+            if (u < a.units) gq[t] = ld_global_v4(grad + (uint64_t)u * 16);
+            #pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r)
+                if (u < a.units && (kRows <= 2 || r < n)) q[t][r] = ld_stream_v4(rows.from[r] + (uint64_t)u * 16);
+        }
+        #pragma unroll
+        for (int t = 0; t < kTurns; ++t) {
+            const uint32_t u = u0 + t * blockDim.x;
+            float g[Unit<T>::kValues];
+            Unit<T>::values(gq[t], g);
+            #pragma unroll
+            for (uint32_t r = 0; r < kRows; ++r) {
+                if (u >= a.units || !(kRows <= 2 || r < n)) continue;
+                float v[Unit<T>::kValues], d[Unit<T>::kValues];
+                Unit<T>::values(q[t][r], v);
+                const float w = rows.weight[r];
+                #pragma unroll
+                for (int k = 0; k < Unit<T>::kValues; ++k) {
+                    dot[r] = fmaf(v[k], g[k], dot[r]);
+                    d[k] = w * g[k];
+                }
+                *reinterpret_cast<uint4*>(rows.to[r] + (uint64_t)u * 16) = Unit<T>::pack(d);
+            }
+        }
+    }
+}
+
+// The sums of `dot` over the CTA, of which thread r < n writes the r-th.
+template <int kRows>
+__device__ __forceinline__ void write_sums(const CombineGradArgs& a, const GradRows& rows, uint32_t n, float (&partial)[kGradThreads / 32][8],
+                                           float (&dot)[kRows]) {
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    #pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        #pragma unroll
+        for (uint32_t d = 16; d > 0; d /= 2) dot[r] += __shfl_xor_sync(0xffffffffu, dot[r], d);
+        if (lane == 0) partial[warp][r] = dot[r];
+    }
+    __syncthreads();
+    if (threadIdx.x < n) {
+        float s = 0.f;
+        for (uint32_t w = 0; w < blockDim.x / 32; ++w) s += partial[w][threadIdx.x];
+        a.dw[rows.choice[threadIdx.x]] = s;
+    }
+}
+
+// One CTA a token: its gradient is read once and multiplied with the rows of its choices, up to eight at a time, and the products with the
+// rows are summed over the CTA. Choices without a row are passed over: a rank that has an eighth of the experts sees one of eight. The
+// CTAs behind the last token zero the padding.
 template <typename T>
-__global__ void __launch_bounds__(kGradThreads, 6) moe_combine_grad_kernel(const CombineGradArgs a) {
+__global__ void __launch_bounds__(kGradThreads, kGradCtas) moe_combine_grad_kernel(const CombineGradArgs a) {
     __shared__ float partial[kGradThreads / 32][8];
-    __shared__ const uint8_t* from[8];
-    __shared__ uint8_t* to[8];
-    __shared__ float weights[8];
+    __shared__ GradRows rows;
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, token = blockIdx.x;
     griddep_wait();
     griddep_launch_dependents();
@@ -417,50 +482,41 @@ __global__ void __launch_bounds__(kGradThreads, 6) moe_combine_grad_kernel(const
         zero_padding_row(a.r, (uint64_t)(token - a.r.tokens) * (blockDim.x / 32) + warp, a.dy, a.dy_stride, a.units, lane);
         return;
     }
-    for (uint32_t j0 = 0; j0 < a.r.topk; j0 += 8) {
-        if (threadIdx.x < 8) {
-            const uint32_t j = j0 + threadIdx.x;
-            const uint32_t row = j < a.r.topk ? ld_global_u32(a.r.token_rows + (uint64_t)token * a.r.topk + j) : 0xffffffffu;
-            const bool is = row < a.r.rows;
-            from[threadIdx.x] = is ? a.y + row * a.y_stride : nullptr;
-            to[threadIdx.x] = a.dy + row * a.dy_stride;
-            weights[threadIdx.x] = is ? __uint_as_float(ld_global_u32(a.w + (uint64_t)token * a.r.topk + j)) : 0.f;
-        }
-        __syncthreads();
-        float dot[8] = {};
-        for (uint32_t u = threadIdx.x; u < a.units; u += blockDim.x) {
-            uint4 q[8];
-            const uint4 gq = ld_global_v4(a.g + token * a.g_stride + (uint64_t)u * 16);
-            #pragma unroll
-            for (uint32_t j = 0; j < 8; ++j)
-                if (from[j] != nullptr) q[j] = ld_stream_v4(from[j] + (uint64_t)u * 16);
-            float g[Unit<T>::kValues];
-            Unit<T>::values(gq, g);
-            #pragma unroll
-            for (uint32_t j = 0; j < 8; ++j) {
-                if (from[j] == nullptr) continue;
-                float v[Unit<T>::kValues], d[Unit<T>::kValues];
-                Unit<T>::values(q[j], v);
-                const float w = weights[j];
-                #pragma unroll
-                for (int k = 0; k < Unit<T>::kValues; ++k) {
-                    dot[j] = fmaf(v[k], g[k], dot[j]);
-                    d[k] = w * g[k];
-                }
-                *reinterpret_cast<uint4*>(to[j] + (uint64_t)u * 16) = Unit<T>::pack(d);
+    for (uint32_t j0 = 0; j0 < a.r.topk; j0 += 32) {
+        const uint32_t choice = token * a.r.topk + j0 + lane;
+        const uint32_t row = j0 + lane < a.r.topk ? ld_global_u32(a.r.token_rows + choice) : 0xffffffffu;
+        const float weight = warp == 0 && j0 + lane < a.r.topk ? __uint_as_float(ld_global_u32(a.w + choice)) : 0.f;
+        uint32_t live = __ballot_sync(0xffffffffu, row < a.r.rows);
+        if (warp == 0 && row >= a.r.rows && j0 + lane < a.r.topk) a.dw[choice] = 0.f;
+        while (live != 0) {
+            const uint32_t n = min(8u, (uint32_t)__popc(live)), rank = __popc(live & ((1u << lane) - 1u));
+            const bool taken = ((live >> lane) & 1u) && rank < 8;
+            if (warp == 0 && taken) {
+                rows.from[rank] = a.y + row * a.y_stride;
+                rows.to[rank] = a.dy + row * a.dy_stride;
+                rows.weight[rank] = weight;
+                rows.choice[rank] = choice;
             }
-        }
-        #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) {
-            #pragma unroll
-            for (uint32_t d = 16; d > 0; d /= 2) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], d);
-            if (lane == 0) partial[warp][j] = dot[j];
-        }
-        __syncthreads();
-        if (threadIdx.x < 8 && j0 + threadIdx.x < a.r.topk) {
-            float s = 0.f;
-            for (uint32_t w = 0; w < blockDim.x / 32; ++w) s += partial[w][threadIdx.x];
-            a.dw[(uint64_t)token * a.r.topk + j0 + threadIdx.x] = s;
+            live &= ~__ballot_sync(0xffffffffu, taken);
+            __syncthreads();
+            const uint8_t* grad = a.g + token * a.g_stride;
+            if (n > 4) {
+                float dot[8];
+                grad_rows<T, 8, 1>(a, grad, rows, n, dot);
+                write_sums(a, rows, n, partial, dot);
+            } else if (n > 2) {
+                float dot[4];
+                grad_rows<T, 4, 1>(a, grad, rows, n, dot);
+                write_sums(a, rows, n, partial, dot);
+            } else if (n == 2) {
+                float dot[2];
+                grad_rows<T, 2, 1>(a, grad, rows, n, dot);
+                write_sums(a, rows, n, partial, dot);
+            } else {
+                float dot[1];
+                grad_rows<T, 1, 2>(a, grad, rows, n, dot);
+                write_sums(a, rows, n, partial, dot);
+            }
         }
     }
 }
