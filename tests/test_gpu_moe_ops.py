@@ -130,7 +130,7 @@ def test_dispatch_to_fp8(host, layout, hidden):
     assert (flat[~live] == 0x11).all() and (flat_sf[~live] == 0x2222).all()
 
 
-@pytest.mark.parametrize('tokens,topk,experts,max_m,hidden', [(700, 6, 16, None, 7168), (1001, 8, 40, None, 4128), (2000, 2, 7, 333, 8224), (300, 33, 64, 130, 3200),
+@pytest.mark.parametrize('tokens,topk,experts,max_m,hidden', [(1300, 6, 16, None, 7168), (1701, 8, 40, None, 4128), (3100, 2, 7, 333, 8224), (500, 33, 64, 130, 3200),
                                                               (5000, 1, 3, None, 65568)])
 def test_dispatch_to_fp8_of_many_tokens(tokens, topk, experts, max_m, hidden):
     """Where the scales take a second launch."""
