@@ -127,7 +127,7 @@ inline TensorPair moe_dispatch_to_fp8(const torch::Tensor& x, const MoePlan& pla
         sf = empty_scales(plan.shape(cols), x);
     }
     const int64_t stride = plan.check_rows(out, "out must hold a row for each of the layout's, at one distance");
-    const uint64_t nbytes = dg_moe_dispatch_fp8_scratch_bytes((uint32_t)plan.tokens, (uint32_t)plan.topk, (uint32_t)hidden);
+    const uint64_t nbytes = dg_moe_dispatch_fp8_scratch_bytes((uint32_t)plan.tokens, (uint32_t)hidden);
     const auto scratch = nbytes ? empty_on({(int64_t)nbytes}, torch::kUInt8, x) : torch::Tensor();
     check(dg_moe_dispatch_fp8_launch(x.data_ptr(), (uint64_t)stride_of_rows(x), (uint32_t)plan.tokens, (uint32_t)plan.topk, (uint32_t)hidden,
                                      plan.token_rows_ptr(), static_cast<const int32_t*>(plan.row_choices.data_ptr()), (uint64_t)plan.rows,

@@ -212,8 +212,8 @@ __device__ __forceinline__ uint32_t rows_of_token(const RowsArgs& a, uint32_t to
 __device__ __forceinline__ bool wanted(const RowsArgs& a, uint32_t mine) { return a.topk > 32 || __any_sync(0xffffffffu, mine < a.rows); }
 
 // A warp takes 32 x kCopyUnits pieces of a token's row, reads them once and writes them to the rows of all its choices. Tokens without a
-// choice here are not read (a rank with an eighth of the experts: 16384 tokens x 7168 @1 us, @2 when all are), unless there are so few tokens
-// that the second round trip to memory is what counts.
+// choice here are not read (a rank with an eighth of the experts, 16384 tokens x 7168: 66 us against 75 when all are), unless there are so
+// few tokens that the second round trip to memory is what counts. 4095 tokens x 2048 of 6 choices, with zeros in the padding: 24 us, 6.3 TB/s.
 __global__ void __launch_bounds__(kMoeThreads) moe_dispatch_kernel(const DispatchArgs a) {
     const uint32_t lane = threadIdx.x % 32;
     const uint32_t item = blockIdx.x * kMoeWarps + threadIdx.x / 32;
@@ -244,7 +244,9 @@ __global__ void __launch_bounds__(kMoeThreads) moe_dispatch_kernel(const Dispatc
 // The same with a quantisation on the way: a warp takes kTiles x 256 channels of a token, eight to a lane, four lanes to a block of 32. The
 // scales of a row lie num_rows elements apart, and the rows of a token far from one another: written from here, each is a store of two
 // bytes with a sector of L2 to itself. That suits a few tokens. For many (65536 rows of 7168: 127 us, 93 without the scales), the
-// bytes go to a scratch, by token, and moe_scales_kernel behind this one turns them into runs.
+// bytes go to a scratch, by token, and moe_scales_kernel behind this one turns them into runs: 101 us together, 5.9 TB/s. Two tiles to a
+// warp then: with one, 16384 tokens of which a rank has one choice of eight take 98 us, with two 66, with four 78. (A grid of one wave whose
+// warps take one piece after the other, the next on its way: 98 us, and 120 instead of 101.)
 constexpr uint32_t kFp8Tiles = 2;
 template <uint32_t kTiles>
 __global__ void __launch_bounds__(kMoeThreads) moe_dispatch_fp8_kernel(const DispatchArgs a) {
@@ -433,12 +435,14 @@ __device__ __forceinline__ void store_pieces(const CombineArgs& a, uint32_t toke
 }
 
 // A warp takes 32 x turns pieces of 16 bytes of a token's result (turns is 1, or kCombineTurns where there are tokens enough): eight pieces of rows
-// are on their way at once, of eight rows or of fewer and more turns.
-constexpr uint32_t kCombineTurns = 4;
+// are on their way at once, of eight rows or of fewer and more turns. 8192 tokens x 7168 of 8 rows each: 164 us, 6.4 TB/s; 16384 tokens of
+// which a rank has one row of eight: 186 us with one turn, 86 with four. Seven CTAs of 128 threads: with eight (64 registers) 167 and
+// 86 us, with five of 256 threads 171 and 97.
+constexpr uint32_t kCombineTurns = 4, kCombineThreads = 128;
 template <typename T>
-__global__ void __launch_bounds__(kMoeThreads, 4) moe_combine_kernel(const CombineArgs a) {
+__global__ void __launch_bounds__(kCombineThreads, 7) moe_combine_kernel(const CombineArgs a) {
     const uint32_t lane = threadIdx.x % 32;
-    const uint32_t item = blockIdx.x * kMoeWarps + threadIdx.x / 32;
+    const uint32_t item = blockIdx.x * (kCombineThreads / 32) + threadIdx.x / 32;
     griddep_wait();
     griddep_launch_dependents();
     if (item >= a.items) return;
@@ -704,9 +708,9 @@ static int rows_args(RowsArgs& r, const int32_t* token_rows, uint32_t tokens, ui
 }
 constexpr uint64_t kMaxItems = 0xfffffff0ull;          // warps of a launch, counted in 32 bits (a division by 64 costs more than the rest of an index)
 static uint64_t padding_items(const RowsArgs& r) { return (uint64_t)r.experts * (r.max_m ? r.max_m : r.alignment); }
-// Bytes that a token's scales take in the scratch, and from how many scale elements on they go through it.
+// Bytes that a token's scales take in the scratch, and from how many tokens and scale elements of theirs on they go through it.
 static uint32_t scale_bytes_of(uint32_t hidden) { return (hidden / 32 + 15) / 16 * 16; }
-constexpr uint64_t kScatteredScales = 3ull << 18;
+constexpr uint32_t kManyTokens = 2048, kManyScales = 1u << 16;
 static bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride_bytes % 16 == 0; }
 
 extern "C" int dg_moe_dispatch_launch(const void* x, uint64_t x_stride_bytes, uint32_t tokens, uint32_t topk, uint64_t row_bytes,
@@ -734,11 +738,11 @@ extern "C" int dg_moe_dispatch_launch(const void* x, uint64_t x_stride_bytes, ui
     return launch_overlapped((const void*)moe_dispatch_kernel, dim3((uint32_t)ctas), dim3(kMoeThreads), params, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" uint64_t dg_moe_dispatch_fp8_scratch_bytes(uint32_t tokens, uint32_t topk, uint32_t hidden) {
-    // The second launch against scales written one by one (8 choices, 32 experts): 7168 channels, 1024 tokens 20.4 against 18.6 us, 2048 tokens
-    // 32.4 against 34.2; 2048 channels, 2048 tokens 11.2 against 11.5 us, 4096 tokens 18.5 against 21.0.
-    const uint64_t scales = (uint64_t)tokens * topk * ((hidden + 63) / 64);
-    return scales < kScatteredScales ? 0 : (uint64_t)tokens * scale_bytes_of(hidden);
+extern "C" uint64_t dg_moe_dispatch_fp8_scratch_bytes(uint32_t tokens, uint32_t hidden) {
+    // Measured, the second launch against scales written one by one, 1024 / 2048 / 4096 tokens: 7168 channels, 8 choices 20.8 / 32.9 / 56.4 against
+    // 19.0 / 34.7 / 65.9 us, one choice 10.2 / 14.9 / 24.5 against 8.8 / 15.5 / 29.4, 8 choices of which a rank has one 9.6 / 13.9 / 22.3 against
+    // 7.5 / 13.2 / 25.6; 2048 channels, 8 choices 8.0 / 11.2 / 18.7 against 7.1 / 11.7 / 21.2; 512 channels 4.8 / 5.7 / 8.2 against 3.4 / 4.4 / 7.0.
+    return tokens < kManyTokens || (uint64_t)tokens * ((hidden + 63) / 64) < kManyScales ? 0 : (uint64_t)tokens * scale_bytes_of(hidden);
 }
 
 extern "C" int dg_moe_dispatch_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t topk, uint32_t hidden,
@@ -795,10 +799,10 @@ extern "C" int dg_moe_combine_launch(const void* rows, int is_fp32, uint64_t row
     const uint64_t items = (uint64_t)tokens * a.chunks;
     DG_CHECK_ARG(items <= kMaxItems, "moe_combine: too many tokens");
     a.items = (uint32_t)items;
-    const uint32_t ctas = (a.items + kMoeWarps - 1) / kMoeWarps;
+    const uint32_t ctas = (a.items + kCombineThreads / 32 - 1) / (kCombineThreads / 32);
     const void* fn = is_fp32 ? (const void*)moe_combine_kernel<float> : (const void*)moe_combine_kernel<__nv_bfloat16>;
     void* params[] = {&a};
-    return launch_overlapped(fn, dim3((uint32_t)ctas), dim3(kMoeThreads), params, static_cast<cudaStream_t>(stream));
+    return launch_overlapped(fn, dim3((uint32_t)ctas), dim3(kCombineThreads), params, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int dg_moe_combine_grad_launch(const void* grad_out, int is_fp32, uint64_t grad_stride, const void* rows, uint64_t rows_stride,

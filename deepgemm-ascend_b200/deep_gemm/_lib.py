@@ -102,7 +102,7 @@ _PROTOTYPES = {
     'dg_moe_dispatch_fp8_launch': (C.c_int, [
         C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64,
         C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p]),
-    'dg_moe_dispatch_fp8_scratch_bytes': (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint32]),
+    'dg_moe_dispatch_fp8_scratch_bytes': (C.c_uint64, [C.c_uint32, C.c_uint32]),
     'dg_moe_combine_launch': (C.c_int, [
         C.c_void_p, C.c_int, C.c_uint64, C.c_uint64, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
     'dg_moe_combine_grad_launch': (C.c_int, [

@@ -151,7 +151,7 @@ def moe_dispatch_to_fp8(x: torch.Tensor, plan, out=None):
             out = torch.empty(p.shape(hidden), dtype=torch.float8_e4m3fn, device=x.device)
             sf = _empty_scales(p.shape(cols), x.device)
         stride = p.check_rows(out, _OUT_ROWS)
-        nbytes = L.lib().dg_moe_dispatch_fp8_scratch_bytes(p.tokens, p.topk, hidden)
+        nbytes = L.lib().dg_moe_dispatch_fp8_scratch_bytes(p.tokens, hidden)
         scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         L.check(L.lib().dg_moe_dispatch_fp8_launch(
             x.data_ptr(), _row_stride(x), p.tokens, p.topk, hidden, p.token_rows.data_ptr(), p.row_choices.data_ptr(), p.rows, out.data_ptr(), stride,

@@ -331,7 +331,7 @@ int dg_moe_sort_launch(const void* topk_idx, int idx_is_int64, uint32_t tokens, 
 int dg_moe_dispatch_launch(const void* x, uint64_t x_stride_bytes, uint32_t tokens, uint32_t topk, uint64_t row_bytes,
                            const int32_t* token_rows, uint64_t num_rows, void* out, uint64_t out_stride_bytes,
                            const int32_t* layout, uint32_t num_experts, uint32_t alignment, uint32_t max_m, int zero_padding, void* stream);
-uint64_t dg_moe_dispatch_fp8_scratch_bytes(uint32_t tokens, uint32_t topk, uint32_t hidden);
+uint64_t dg_moe_dispatch_fp8_scratch_bytes(uint32_t tokens, uint32_t hidden);
 int dg_moe_dispatch_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t topk, uint32_t hidden,
                                const int32_t* token_rows, const int32_t* row_choices, uint64_t num_rows, void* out, uint64_t out_stride,
                                int16_t* out_sf, uint64_t sf_col_stride, uint64_t sf_group_stride, uint32_t sf_rows,

@@ -72,7 +72,7 @@ def test_the_c_abi_checks_its_arguments():
     _refused(fp8(sf=None), 'null pointer')
     for bad in (dict(nbytes=63), dict(scratch=p + 8, nbytes=64), dict(rc=None, nbytes=64)):
         _refused(fp8(**{'scratch': p, **bad}), 'the scratch must be')
-    assert lib.dg_moe_dispatch_fp8_scratch_bytes(64, 8, 7168) == 0 and lib.dg_moe_dispatch_fp8_scratch_bytes(8191, 8, 7200) == 8191 * 240
+    assert lib.dg_moe_dispatch_fp8_scratch_bytes(2047, 7168) == 0 and lib.dg_moe_dispatch_fp8_scratch_bytes(8191, 7200) == 8191 * 240
     combine = lambda y=p, ys=64, hidden=64, out=p, os=64: lib.dg_moe_combine_launch(y, 0, ys, 512, hidden, p, 4, 2, p, out, os, None)  # noqa: E731
     for bad in (dict(y=p + 2), dict(ys=60), dict(hidden=60), dict(out=p + 2), dict(os=60)):
         _refused(combine(**bad), '16-byte boundaries')
