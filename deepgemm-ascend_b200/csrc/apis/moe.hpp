@@ -27,12 +27,14 @@ struct MoeRows {
         tokens = token_rows.size(0); topk = token_rows.size(1); experts = layout.size(0);
         max_m = row_choices.dim() == 2 ? row_choices.size(1) : 0;
         rows = row_choices.numel();
+        host_assert(tokens <= INT32_MAX && topk <= INT32_MAX && token_rows.numel() <= INT32_MAX && rows <= INT32_MAX, "plan is too large");
         host_assert(num_tokens < 0 || tokens == num_tokens, "plan was made for another number of tokens");
     }
     std::vector<int64_t> shape(int64_t last) const {
         return row_choices.dim() == 2 ? std::vector<int64_t>{experts, max_m, last} : std::vector<int64_t>{rows, last};
     }
     const int32_t* token_rows_ptr() const { return static_cast<const int32_t*>(token_rows.data_ptr()); }
+    const int32_t* row_choices_ptr() const { return static_cast<const int32_t*>(row_choices.data_ptr()); }
     const int32_t* layout_ptr() const { return static_cast<const int32_t*>(layout.data_ptr()); }
     // Distance between the rows of a tensor of the grouped layout; `what` is the message where its rows do not lie at one distance
     // (or lie on one another).
@@ -101,7 +103,7 @@ inline torch::Tensor moe_dispatch(const torch::Tensor& x, const MoePlan& plan_in
     const auto out = out_in.has_value() ? out_in.value() : empty_on(plan.shape(x.size(1)), x.scalar_type(), x);
     const int64_t stride = plan.check_rows(out, "out must hold a row for each of the layout's, at one distance"), es = x.element_size();
     check(dg_moe_dispatch_launch(x.data_ptr(), (uint64_t)(stride_of_rows(x) * es), (uint32_t)plan.tokens, (uint32_t)plan.topk, (uint64_t)(x.size(1) * es),
-                                 plan.token_rows_ptr(), (uint64_t)plan.rows, out.data_ptr(), (uint64_t)(stride * es), plan.layout_ptr(),
+                                 plan.token_rows_ptr(), plan.row_choices_ptr(), (uint64_t)plan.rows, out.data_ptr(), (uint64_t)(stride * es), plan.layout_ptr(),
                                  (uint32_t)plan.experts, (uint32_t)expert_alignment, (uint32_t)plan.max_m, zero_padding, stream_of(x)));
     return out;
 }
@@ -130,7 +132,7 @@ inline TensorPair moe_dispatch_to_fp8(const torch::Tensor& x, const MoePlan& pla
     const uint64_t nbytes = dg_moe_dispatch_fp8_scratch_bytes((uint32_t)plan.tokens, (uint32_t)hidden);
     const auto scratch = nbytes ? empty_on({(int64_t)nbytes}, torch::kUInt8, x) : torch::Tensor();
     check(dg_moe_dispatch_fp8_launch(x.data_ptr(), (uint64_t)stride_of_rows(x), (uint32_t)plan.tokens, (uint32_t)plan.topk, (uint32_t)hidden,
-                                     plan.token_rows_ptr(), static_cast<const int32_t*>(plan.row_choices.data_ptr()), (uint64_t)plan.rows,
+                                     plan.token_rows_ptr(), plan.row_choices_ptr(), (uint64_t)plan.rows,
                                      out.data_ptr(), (uint64_t)stride, static_cast<int16_t*>(sf.data_ptr()),
                                      (uint64_t)(cols > 1 ? sf.stride(-1) : per_group), sf.dim() == 3 && plan.experts > 1 ? (uint64_t)sf.stride(0) : 0,
                                      (uint32_t)per_group, nbytes ? scratch.data_ptr() : nullptr, nbytes, stream_of(x)));
@@ -175,8 +177,8 @@ inline TensorPair moe_combine_grad(const torch::Tensor& grad_out, const torch::T
     const int64_t out_stride = plan.check_rows(out, "out must hold a row for each of the layout's, at one distance");
     const auto grad_weights = empty_on(topk_weights.sizes(), topk_weights.scalar_type(), topk_weights);
     check(dg_moe_combine_grad_launch(grad_out.data_ptr(), rows.scalar_type() == torch::kFloat32, (uint64_t)stride_of_rows(grad_out), rows.data_ptr(), (uint64_t)stride,
-                                     (uint64_t)plan.rows, (uint32_t)hidden, plan.token_rows_ptr(), (uint32_t)plan.tokens, (uint32_t)plan.topk,
-                                     static_cast<const float*>(topk_weights.data_ptr()), out.data_ptr(), (uint64_t)out_stride,
+                                     (uint64_t)plan.rows, (uint32_t)hidden, plan.token_rows_ptr(), plan.row_choices_ptr(), (uint32_t)plan.tokens,
+                                     (uint32_t)plan.topk, static_cast<const float*>(topk_weights.data_ptr()), out.data_ptr(), (uint64_t)out_stride,
                                      static_cast<float*>(grad_weights.data_ptr()), plan.layout_ptr(), (uint32_t)plan.experts, (uint32_t)expert_alignment,
                                      (uint32_t)plan.max_m, zero_padding, stream_of(grad_out)));
     return {out, grad_weights};

@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a
 // What the other kernels know of the layout.
 struct RowsArgs {
     const int32_t* token_rows;                          // [tokens][topk]
-    const int32_t* layout; uint32_t experts, alignment, max_m;     // of the padding, where it is to be zeroed
+    const int32_t* layout; uint32_t experts, alignment, max_m;     // of the padding, where it is to be zeroed,
+    const int32_t* row_choices;                                    // and which rows hold a choice
     uint32_t tokens, topk, rows;
 };
 
@@ -182,7 +183,8 @@ __device__ __forceinline__ void zero_padding_row(const RowsArgs& a, uint32_t ite
     const uint32_t p = ld_global_u32(a.layout + g);
     const uint64_t row = a.max_m ? (uint64_t)g * a.max_m + r : (uint64_t)p + r;
     if (a.max_m ? r < p : row >= ((uint64_t)p + a.alignment - 1) / a.alignment * a.alignment) return;
-    if (row >= a.rows) return;
+    // (a row that holds a choice is no padding, whatever the alignment says)
+    if (row >= a.rows || (int32_t)ld_global_u32(a.row_choices + row) >= 0) return;
     for (uint32_t u = lane; u < units; u += 32) *reinterpret_cast<uint4*>(out + row * stride + (uint64_t)u * 16) = make_uint4(0u, 0u, 0u, 0u);
 }
 
@@ -202,7 +204,6 @@ struct DispatchArgs {
     uint32_t sf_rows, hidden;                                      // rows of a group of scales
     uint8_t* scratch;                                              // scale bytes by token, [tokens][scratch_stride], or nullptr
     uint32_t scratch_stride;
-    const int32_t* row_choices;                                    // where the scales go through the scratch
 };
 
 // The rows of a token's first 32 choices, by lanes, and whether there is any (of the first 32: with more it cannot say no).
@@ -323,7 +324,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_scales_kernel(const DispatchA
     // before the bytes that it writes are there)
     bool some = false;
     if (tid < kScaleRows) {
-        const uint32_t choice = row0 + tid < a.r.rows ? ld_global_u32(a.row_choices + row0 + tid) : 0xffffffffu;
+        const uint32_t choice = row0 + tid < a.r.rows ? ld_global_u32(a.r.row_choices + row0 + tid) : 0xffffffffu;
         const uint32_t token = choice / max(a.r.topk, 1u);
         some = (int32_t)choice >= 0 && token < a.r.tokens;
         token_of[tid] = some ? token : 0xffffffffu;
@@ -697,13 +698,14 @@ extern "C" int dg_moe_sort_launch(const void* topk_idx, int idx_is_int64, uint32
 }
 
 // Checks of what the other three share; fills `r`.
-static int rows_args(RowsArgs& r, const int32_t* token_rows, uint32_t tokens, uint32_t topk, uint64_t num_rows, const int32_t* layout,
-                     uint32_t num_experts, uint32_t alignment, uint32_t max_m, int zero_padding) {
+static int rows_args(RowsArgs& r, const int32_t* token_rows, const int32_t* row_choices, uint32_t tokens, uint32_t topk, uint64_t num_rows,
+                     const int32_t* layout, uint32_t num_experts, uint32_t alignment, uint32_t max_m, int zero_padding) {
     DG_CHECK_ARG(token_rows != nullptr || (uint64_t)tokens * topk == 0, "moe: null pointer");
     DG_CHECK_ARG((uint64_t)tokens * topk <= 0x7fffffffull && num_rows <= 0x7fffffffull, "moe: too many choices or rows");
-    DG_CHECK_ARG(!zero_padding || (layout != nullptr && num_experts > 0 && (max_m > 0 || alignment > 0)), "moe: zeros in the padding need the layout");
-    r.token_rows = token_rows; r.tokens = tokens; r.topk = topk; r.rows = (uint32_t)num_rows;
-    r.layout = layout; r.experts = zero_padding ? num_experts : 0; r.alignment = alignment; r.max_m = max_m;
+    DG_CHECK_ARG(!zero_padding || num_rows == 0 || (layout != nullptr && row_choices != nullptr && num_experts > 0 && (max_m > 0 || alignment > 0)),
+                 "moe: zeros in the padding need the layout and the rows' choices");
+    r.token_rows = token_rows; r.row_choices = row_choices; r.tokens = tokens; r.topk = topk; r.rows = (uint32_t)num_rows;
+    r.layout = layout; r.experts = zero_padding && num_rows > 0 ? num_experts : 0; r.alignment = alignment; r.max_m = max_m;
     return DG_OK;
 }
 constexpr uint64_t kMaxItems = 0xfffffff0ull;          // warps of a launch, counted in 32 bits (a division by 64 costs more than the rest of an index)
@@ -714,7 +716,7 @@ constexpr uint32_t kManyTokens = 2048, kManyScales = 1u << 16;
 static bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && stride_bytes % 16 == 0; }
 
 extern "C" int dg_moe_dispatch_launch(const void* x, uint64_t x_stride_bytes, uint32_t tokens, uint32_t topk, uint64_t row_bytes,
-                                      const int32_t* token_rows, uint64_t num_rows, void* out, uint64_t out_stride_bytes,
+                                      const int32_t* token_rows, const int32_t* row_choices, uint64_t num_rows, void* out, uint64_t out_stride_bytes,
                                       const int32_t* layout, uint32_t num_experts, uint32_t alignment, uint32_t max_m, int zero_padding, void* stream) {
     if (row_bytes == 0 || num_rows == 0) return DG_OK;
     DG_CHECK_ARG(out != nullptr && (x != nullptr || tokens == 0), "moe_dispatch: null pointer");
@@ -722,7 +724,7 @@ extern "C" int dg_moe_dispatch_launch(const void* x, uint64_t x_stride_bytes, ui
                  "moe_dispatch: rows must start on 16-byte boundaries and hold a multiple of 16 bytes");
     DG_CHECK_ARG(row_bytes / 16 <= 0x7fffffffull, "moe_dispatch: rows too long");
     DispatchArgs a{};
-    if (int rc = rows_args(a.r, token_rows, tokens, topk, num_rows, layout, num_experts, alignment, max_m, zero_padding)) return rc;
+    if (int rc = rows_args(a.r, token_rows, row_choices, tokens, topk, num_rows, layout, num_experts, alignment, max_m, zero_padding)) return rc;
     a.x = static_cast<const uint8_t*>(x); a.x_stride = x_stride_bytes;
     a.out = static_cast<uint8_t*>(out); a.out_stride = out_stride_bytes;
     a.units = (uint32_t)(row_bytes / 16);
@@ -759,12 +761,12 @@ extern "C" int dg_moe_dispatch_fp8_launch(const void* x, uint64_t x_stride, uint
                                         scratch_bytes >= (uint64_t)tokens * scale_bytes_of(hidden)),
                  "moe_dispatch_fp8: the scratch must be 16-byte aligned, hold dg_moe_dispatch_fp8_scratch_bytes, and come with the rows' choices");
     DispatchArgs a{};
-    if (int rc = rows_args(a.r, token_rows, tokens, topk, num_rows, nullptr, 0, 0, 0, 0)) return rc;
+    if (int rc = rows_args(a.r, token_rows, row_choices, tokens, topk, num_rows, nullptr, 0, 0, 0, 0)) return rc;
     a.x = static_cast<const uint8_t*>(x); a.x_stride = x_stride * 2;
     a.out = static_cast<uint8_t*>(out); a.out_stride = out_stride;
     a.sf = reinterpret_cast<uint8_t*>(out_sf); a.sf_col_stride = sf_col_stride * 2; a.sf_group_stride = sf_group_stride * 2;
     a.sf_rows = sf_rows; a.hidden = hidden;
-    a.scratch = static_cast<uint8_t*>(scratch); a.scratch_stride = scale_bytes_of(hidden); a.row_choices = row_choices;
+    a.scratch = static_cast<uint8_t*>(scratch); a.scratch_stride = scale_bytes_of(hidden);
     // (many tokens, many stores: more bytes in each)
     const uint32_t tiles_of_warp = scratch == nullptr ? 1 : kFp8Tiles;
     a.chunks = (hidden + 256 * tiles_of_warp - 1) / (256 * tiles_of_warp);
@@ -789,7 +791,7 @@ extern "C" int dg_moe_combine_launch(const void* rows, int is_fp32, uint64_t row
     DG_CHECK_ARG(hidden * es % 16 == 0 && aligned16(rows, rows_stride * es) && aligned16(out, out_stride * es),
                  "moe_combine: rows must start on 16-byte boundaries and hold a multiple of 16 bytes");
     CombineArgs a{};
-    if (int rc = rows_args(a.r, token_rows, tokens, topk, num_rows, nullptr, 0, 0, 0, 0)) return rc;
+    if (int rc = rows_args(a.r, token_rows, nullptr, tokens, topk, num_rows, nullptr, 0, 0, 0, 0)) return rc;
     a.y = static_cast<const uint8_t*>(rows); a.y_stride = rows_stride * es;
     a.w = topk_weights;
     a.out = static_cast<uint8_t*>(out); a.out_stride = out_stride * es;
@@ -806,8 +808,8 @@ extern "C" int dg_moe_combine_launch(const void* rows, int is_fp32, uint64_t row
 }
 
 extern "C" int dg_moe_combine_grad_launch(const void* grad_out, int is_fp32, uint64_t grad_stride, const void* rows, uint64_t rows_stride,
-                                          uint64_t num_rows, uint32_t hidden, const int32_t* token_rows, uint32_t tokens, uint32_t topk,
-                                          const float* topk_weights, void* grad_rows, uint64_t grad_rows_stride, float* grad_weights,
+                                          uint64_t num_rows, uint32_t hidden, const int32_t* token_rows, const int32_t* row_choices,
+                                          uint32_t tokens, uint32_t topk, const float* topk_weights, void* grad_rows, uint64_t grad_rows_stride, float* grad_weights,
                                           const int32_t* layout, uint32_t num_experts, uint32_t alignment, uint32_t max_m, int zero_padding,
                                           void* stream) {
     if (tokens == 0 && !zero_padding) return DG_OK;
@@ -817,7 +819,7 @@ extern "C" int dg_moe_combine_grad_launch(const void* grad_out, int is_fp32, uin
     DG_CHECK_ARG(hidden * es % 16 == 0 && aligned16(grad_out, grad_stride * es) && aligned16(rows, rows_stride * es) &&
                  aligned16(grad_rows, grad_rows_stride * es), "moe_combine_grad: rows must start on 16-byte boundaries and hold a multiple of 16 bytes");
     CombineGradArgs a{};
-    if (int rc = rows_args(a.r, token_rows, tokens, topk, num_rows, layout, num_experts, alignment, max_m, zero_padding)) return rc;
+    if (int rc = rows_args(a.r, token_rows, row_choices, tokens, topk, num_rows, layout, num_experts, alignment, max_m, zero_padding)) return rc;
     a.g = static_cast<const uint8_t*>(grad_out); a.g_stride = grad_stride * es;
     a.y = static_cast<const uint8_t*>(rows); a.y_stride = rows_stride * es;
     a.w = topk_weights;

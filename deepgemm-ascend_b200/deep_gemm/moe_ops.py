@@ -52,6 +52,7 @@ class _Rows:
         self.max_m = self.row_choices.size(1) if masked else 0
         self.rows = self.row_choices.numel()
         self.masked = masked
+        _host_assert(max(self.tokens, self.topk, self.token_rows.numel(), self.rows) <= _INT_MAX, 'plan is too large')
         _host_assert(num_tokens is None or self.tokens == num_tokens, 'plan was made for another number of tokens')
 
     def shape(self, last):
@@ -109,7 +110,7 @@ def moe_sort(topk_idx: torch.Tensor, num_experts: int, expert_alignment: int = M
 
 def moe_dispatch(x: torch.Tensor, plan, out: Optional[torch.Tensor] = None, zero_padding: bool = False, expert_alignment: int = MK_ALIGNMENT):
     """x [tokens, hidden] BF16 or FP32 -> the rows of the layout, [rows, hidden] or [experts, max_m, hidden]: every token's row copied to
-    those of its choices. `zero_padding` writes zeros to the rows between each group's end and the next multiple of
+    those of its choices. `zero_padding` writes zeros to the rows without a choice between each group's end and the next multiple of
     `expert_alignment` (the k-grouped GEMM of a weight gradient reads them), or to the rest of an expert's `max_m`. `out` must not
     overlap x. Rows of x and out start on 16-byte boundaries."""
     _check_tokens(x, 'x must be a row-major 2-D BF16 or FP32 tensor on a CUDA device')
@@ -123,7 +124,7 @@ def moe_dispatch(x: torch.Tensor, plan, out: Optional[torch.Tensor] = None, zero
             out = torch.empty(p.shape(x.size(1)), dtype=x.dtype, device=x.device)
         stride, es = p.check_rows(out, _OUT_ROWS), x.element_size()
         L.check(L.lib().dg_moe_dispatch_launch(
-            x.data_ptr(), _row_stride(x) * es, p.tokens, p.topk, x.size(1) * es, p.token_rows.data_ptr(), p.rows, out.data_ptr(), stride * es,
+            x.data_ptr(), _row_stride(x) * es, p.tokens, p.topk, x.size(1) * es, p.token_rows.data_ptr(), p.row_choices.data_ptr(), p.rows, out.data_ptr(), stride * es,
             p.layout.data_ptr(), p.experts, expert_alignment, p.max_m, int(zero_padding), _stream_ptr(x.device)))
     return out
 
@@ -163,7 +164,7 @@ def moe_dispatch_to_fp8(x: torch.Tensor, plan, out=None):
 def moe_combine(rows: torch.Tensor, plan, topk_weights: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
     """rows [rows, hidden] or [experts, max_m, hidden] BF16 or FP32 -> [tokens, hidden]: the rows of a token's choices times their weights
     (float32 [tokens, k]; 1 without them), summed in FP32 in the order of the choices and rounded once. A choice without a row adds
-    nothing, whatever its weight."""
+    nothing, whatever its weight. `out` must not overlap rows."""
     _host_assert(rows.is_cuda and rows.dim() in (2, 3) and _is_float(rows), 'rows must be a 2-D or 3-D BF16 or FP32 tensor on a CUDA device')
     p = _Rows(plan, rows, None)
     stride, hidden = p.check_rows(rows, _IN_ROWS), rows.size(-1)
@@ -207,7 +208,7 @@ def moe_combine_grad(grad_out: torch.Tensor, rows: torch.Tensor, plan, topk_weig
         grad_weights = torch.empty_like(topk_weights)
         L.check(L.lib().dg_moe_combine_grad_launch(
             grad_out.data_ptr(), int(rows.dtype == torch.float32), _row_stride(grad_out), rows.data_ptr(), stride, p.rows, hidden,
-            p.token_rows.data_ptr(), p.tokens, p.topk, topk_weights.data_ptr(), out.data_ptr(), out_stride, grad_weights.data_ptr(),
+            p.token_rows.data_ptr(), p.row_choices.data_ptr(), p.tokens, p.topk, topk_weights.data_ptr(), out.data_ptr(), out_stride, grad_weights.data_ptr(),
             p.layout.data_ptr(), p.experts, expert_alignment, p.max_m, int(zero_padding), _stream_ptr(grad_out.device)))
     return out, grad_weights
 

@@ -315,8 +315,9 @@ int dg_dequant_fp4_launch(const void* codes, uint64_t code_stride, uint64_t code
  * num_experts * max_m, or dg_moe_num_rows: the most that any choices need. At most 1024 experts.
  *
  * The others take token_rows; entries outside [0, num_rows) are skipped, no two may be equal. Rows that hold no choice are neither read nor
- * written, except that `zero_padding` writes zeros to the rows between each group's end and the next multiple of the alignment
- * (with max_m > 0: to the rest of each expert's slots). Rows start on 16-byte boundaries and hold a multiple of 16 bytes.
+ * written, except that `zero_padding` writes zeros to those between each group's end and the next multiple of the alignment
+ * (with max_m > 0: to the rest of each expert's slots); it needs `layout` and `row_choices`, which may be NULL otherwise. Rows start on
+ * 16-byte boundaries and hold a multiple of 16 bytes.
  *
  * dg_moe_dispatch_launch copies rows of `row_bytes` bytes, dg_moe_dispatch_fp8_launch quantises BF16 rows as dg_quant_fp8_launch does
  * (scales of row r at out_sf[r / sf_rows * sf_group_stride + c * sf_col_stride + r % sf_rows]). `scratch`: device memory of
@@ -329,7 +330,7 @@ uint64_t dg_moe_num_rows(uint32_t choices, uint32_t num_experts, uint32_t alignm
 int dg_moe_sort_launch(const void* topk_idx, int idx_is_int64, uint32_t tokens, uint32_t topk, uint32_t num_experts, uint32_t alignment,
                        uint32_t max_m, int32_t* layout, int32_t* token_rows, int32_t* row_choices, uint64_t num_rows, void* stream);
 int dg_moe_dispatch_launch(const void* x, uint64_t x_stride_bytes, uint32_t tokens, uint32_t topk, uint64_t row_bytes,
-                           const int32_t* token_rows, uint64_t num_rows, void* out, uint64_t out_stride_bytes,
+                           const int32_t* token_rows, const int32_t* row_choices, uint64_t num_rows, void* out, uint64_t out_stride_bytes,
                            const int32_t* layout, uint32_t num_experts, uint32_t alignment, uint32_t max_m, int zero_padding, void* stream);
 uint64_t dg_moe_dispatch_fp8_scratch_bytes(uint32_t tokens, uint32_t hidden);
 int dg_moe_dispatch_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t topk, uint32_t hidden,
@@ -339,8 +340,8 @@ int dg_moe_dispatch_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens
 int dg_moe_combine_launch(const void* rows, int is_fp32, uint64_t rows_stride, uint64_t num_rows, uint32_t hidden, const int32_t* token_rows,
                           uint32_t tokens, uint32_t topk, const float* topk_weights, void* out, uint64_t out_stride, void* stream);
 int dg_moe_combine_grad_launch(const void* grad_out, int is_fp32, uint64_t grad_stride, const void* rows, uint64_t rows_stride,
-                               uint64_t num_rows, uint32_t hidden, const int32_t* token_rows, uint32_t tokens, uint32_t topk,
-                               const float* topk_weights, void* grad_rows, uint64_t grad_rows_stride, float* grad_weights,
+                               uint64_t num_rows, uint32_t hidden, const int32_t* token_rows, const int32_t* row_choices,
+                               uint32_t tokens, uint32_t topk, const float* topk_weights, void* grad_rows, uint64_t grad_rows_stride, float* grad_weights,
                                const int32_t* layout, uint32_t num_experts, uint32_t alignment, uint32_t max_m, int zero_padding,
                                void* stream);
 

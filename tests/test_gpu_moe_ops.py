@@ -369,6 +369,31 @@ def test_no_tokens(topk):
         assert dy.shape == y.shape and dw.shape == (0, topk) and (dy == 0).all()
 
 
+def test_zeros_spare_the_rows_that_hold_a_choice():
+    """Whatever alignment is given: groups on multiples of 32, zeros up to the next multiple of 256."""
+    plan, (psum, _, row_choices) = _plan(60, 3, 8, 8, None, alignment=32)
+    x = torch.randn(60, 64, device='cuda')
+    out = torch.full((row_choices.numel(), 64), 7.0, device='cuda')
+    deep_gemm.moe_dispatch(x, plan, out=out, zero_padding=True)
+    live, pad = row_choices >= 0, oracle.moe_padding(psum, row_choices.numel(), 256)
+    assert torch.equal(out.cpu()[live], x.cpu()[row_choices[live].long() // 3]) and (out.cpu()[pad & ~live] == 0).all()
+    assert (out.cpu()[~pad & ~live] == 7).all()
+    g, w = torch.randn(60, 64, device='cuda'), torch.rand(60, 3, device='cuda')
+    dy, _ = deep_gemm.moe_combine_grad(g, out, plan, w, zero_padding=True)
+    assert torch.equal(dy.cpu()[live], (w.view(-1, 1) * g.repeat_interleave(3, 0)).cpu()[row_choices[live].long()]) and (dy.cpu()[pad & ~live] == 0).all()
+
+
+def test_no_choices_at_all():
+    idx, x = torch.empty(5, 0, dtype=torch.int64, device='cuda'), torch.randn(5, 64, device='cuda')
+    for max_m in (None, 4):
+        plan = deep_gemm.moe_sort(idx, 3, max_m=max_m)
+        y = deep_gemm.moe_dispatch(x, plan, zero_padding=True)
+        assert (y == 0).all() and (deep_gemm.moe_combine(y, plan) == 0).all()
+        deep_gemm.moe_dispatch_to_fp8(x.bfloat16(), plan)
+        _, dw = deep_gemm.moe_combine_grad(x, y, plan, torch.empty(5, 0, device='cuda'))
+        assert dw.shape == (5, 0)
+
+
 def test_tokens_without_choices():
     idx = torch.full((9, 3), -1, device='cuda')
     plan = deep_gemm.moe_sort(idx, 4)
@@ -415,6 +440,41 @@ def test_another_stream_and_a_captured_run():
             if k in (4, 6, 7):
                 a, b = a.view(torch.int16 if k != 6 else torch.uint8)[live], b.view(torch.int16 if k != 6 else torch.uint8)[live]
             assert torch.equal(a, b), k
+
+
+def test_two_streams_at_once_and_launches_that_do_not_overlap():
+    """Calls in turn on two streams, nothing waited for in between, a sort over a cluster and the scales' second launch among them; then the same
+    one after the other with every launch waiting for the one in front of it."""
+    sizes = ((2500, 4, 16, 2048), (64, 8, 32, 512))
+    inputs = [[(_choices(t, k, e, seed).cuda(), torch.randn(t, h, device='cuda').bfloat16(), torch.rand(t, k, device='cuda')) for seed in range(4)] for t, k, e, h in sizes]
+
+    def way(n, i, x, w):
+        plan = deep_gemm.moe_sort(i, sizes[n][2])
+        y = deep_gemm.moe_dispatch(x, plan, out=torch.zeros(plan[2].numel(), x.size(1), dtype=x.dtype, device='cuda'))
+        q, sf = deep_gemm.moe_dispatch_to_fp8(x, plan)
+        live = plan[2] >= 0
+        return (*plan, y, deep_gemm.moe_combine(y, plan, w), *deep_gemm.moe_combine_grad(x, y, plan, w, out=y.clone()),
+                torch.where(live[:, None], q.view(torch.uint8), 0), torch.where(live[:, None], sf, 0))
+
+    want = [[way(n, *case) for case in inputs[n]] for n in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for k in range(4):
+        for n, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[n].append(way(n, *inputs[n][k]))
+    torch.cuda.synchronize()
+    lib = deep_gemm._lib.lib()
+    lib.dg_set_overlap_launches(0)
+    try:
+        alone = [[way(n, *case) for case in inputs[n]] for n in range(2)]
+    finally:
+        lib.dg_set_overlap_launches(1)
+    for n in range(2):
+        for k in range(4):
+            for a, b, c in zip(want[n][k], got[n][k], alone[n][k]):
+                assert torch.equal(a, b) and torch.equal(a, c)
 
 
 def test_offsets_beyond_32_bits():

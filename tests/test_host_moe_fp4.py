@@ -53,15 +53,16 @@ def test_the_c_abi_checks_its_arguments():
     _refused(sort(n=1 << 31, k=2), 'too many choices')
     _refused(sort(align=1 << 31, e=1, rows=1 << 31), 'too many rows')
     _refused(sort(idx=None), 'null pointer')
-    copy = lambda x=p, xs=128, nbytes=128, rows=512, out=p, os=128, layout=p, e=4, align=256, zero=0, of=p: lib.dg_moe_dispatch_launch(  # noqa: E731
-        x, xs, 4, 2, nbytes, of, rows, out, os, layout, e, align, 0, zero, None)
+    copy = lambda x=p, xs=128, nbytes=128, rows=512, out=p, os=128, layout=p, e=4, align=256, zero=0, of=p, rc=p: lib.dg_moe_dispatch_launch(  # noqa: E731
+        x, xs, 4, 2, nbytes, of, rc, rows, out, os, layout, e, align, 0, zero, None)
     for bad in (dict(nbytes=120), dict(x=p + 8), dict(xs=120), dict(out=p + 8), dict(os=136)):
         _refused(copy(**bad), '16-byte boundaries')
     for bad in (dict(x=None), dict(out=None), dict(of=None)):
         _refused(copy(**bad), 'null pointer')
-    for bad in (dict(layout=None), dict(e=0), dict(align=0)):
+    for bad in (dict(layout=None), dict(rc=None), dict(e=0), dict(align=0)):
         _refused(copy(zero=1, **bad), 'zeros in the padding need the layout')
     _refused(copy(rows=1 << 31), 'too many choices or rows')
+    _refused(copy(zero=1, e=1024, align=1 << 22), 'too many rows')
     fp8 = lambda x=p, xs=64, hidden=64, out=p, os=64, sf=p, col=512, per=512, rc=p, scratch=None, nbytes=0: lib.dg_moe_dispatch_fp8_launch(  # noqa: E731
         x, xs, 4, 2, hidden, p, rc, 512, out, os, sf, col, 0, per, scratch, nbytes, None)
     _refused(fp8(hidden=48), 'multiple of 32')
@@ -78,7 +79,7 @@ def test_the_c_abi_checks_its_arguments():
         _refused(combine(**bad), '16-byte boundaries')
     _refused(combine(y=None), 'null pointer')
     grad = lambda g=p, gs=64, y=p, w=p, dw=p, dy=p: lib.dg_moe_combine_grad_launch(  # noqa: E731
-        g, 0, gs, y, 64, 512, 64, p, 4, 2, w, dy, 64, dw, None, 0, 256, 0, 0, None)
+        g, 0, gs, y, 64, 512, 64, p, None, 4, 2, w, dy, 64, dw, None, 0, 256, 0, 0, None)
     for bad in (dict(g=None), dict(y=None), dict(w=None), dict(dw=None), dict(dy=None)):
         _refused(grad(**bad), 'null pointer')
     _refused(grad(gs=60), '16-byte boundaries')
