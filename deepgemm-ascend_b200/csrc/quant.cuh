@@ -2,7 +2,6 @@
 #pragma once
 
 #include <cuda_bf16.h>
-#include <cuda_fp4.h>
 #include <cuda_fp8.h>
 #include <stdint.h>
 
@@ -62,10 +61,14 @@ __device__ __forceinline__ uint32_t e2m1_scale_byte(uint32_t amax_bits) {
 __device__ __forceinline__ uint32_t e2m1_inverse(uint32_t e) { return e == 255u ? 0u : 254u - e; }
 // Eight values, rounded to the nearest E2M1 (halves to the even code), the first in the lowest bits.
 __device__ __forceinline__ uint32_t e2m1_pack8(const float (&v)[8]) {
-    uint32_t q = 0;
-    #pragma unroll
-    for (int h = 0; h < 4; ++h)
-        q |= (uint32_t)__nv_cvt_float2_to_fp4x2(make_float2(v[2 * h], v[2 * h + 1]), __NV_E2M1, cudaRoundNearest) << (8 * h);
+    uint32_t q;
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b0, %2, %1;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b1, %4, %3;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b2, %6, %5;\n\t"
+        "cvt.rn.satfinite.e2m1x2.f32 b3, %8, %7;\n\t"
+        "mov.b32 %0, {b0, b1, b2, b3};\n\t}"
+        : "=r"(q) : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return q;
 }
 // Eight codes as BF16 pairs, exactly: the two bytes of a magnitude are looked up by its three bits in tables of eight bytes (a byte permute

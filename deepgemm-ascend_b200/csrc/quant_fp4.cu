@@ -26,6 +26,7 @@ struct Fp4Args {
     uint8_t* sf; uint64_t sf_stride, sf_group_stride;                     // bytes; K-major: [ceil(cols / 64)][rows], MN-major: [ceil(rows / 64)][cols]
     const int32_t* psum; uint32_t num_experts, alignment;
     uint32_t rows, cols, tiles_r, tiles_c;
+    uint32_t sf_aligned;                                                  // eight scales of an MN-major matrix can be read at once
 };
 
 // Eight values of a lane, as they lie in memory: kWords words of one or two values. Magnitudes are compared as bit patterns (infinities
@@ -92,8 +93,8 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_kernel(const Fp4Args a)
     constexpr uint32_t kWarpRows = kFp4Rows / (kFp4Threads / 32);
     __shared__ __align__(8) uint8_t sf_smem[kFp4Rows][kFp4Cols / 32];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t tiles = a.tiles_r * a.tiles_c, group = blockIdx.x / tiles, tile = blockIdx.x - group * tiles;
-    const uint32_t row_base = tile / a.tiles_c * kFp4Rows, c0 = tile % a.tiles_c * kFp4Cols;
+    const uint64_t group = blockIdx.z;
+    const uint32_t row_base = blockIdx.x / a.tiles_c * kFp4Rows, c0 = blockIdx.x % a.tiles_c * kFp4Cols;
     griddep_wait();
     griddep_launch_dependents();
     uint32_t row_end = min(a.rows, row_base + kFp4Rows);
@@ -101,11 +102,13 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_kernel(const Fp4Args a)
     if (row_end <= row_base) return;                      // the whole tile is padding (uniform over the CTA)
 
     const uint32_t c = c0 + lane * 8, r0 = row_base + warp * kWarpRows;
+    const uint8_t* x = a.x + group * a.x_group_stride + (uint64_t)r0 * a.x_stride + (uint64_t)c * sizeof(T);
+    uint8_t* codes = a.codes + group * a.code_group_stride + (uint64_t)r0 * a.code_stride + c / 2;
     Raw8<T> raw[kWarpRows];
     #pragma unroll
-    for (uint32_t i = 0; i < kWarpRows; ++i) {
+    for (uint32_t i = 0; i < kWarpRows; ++i, x += a.x_stride) {
         raw[i].clear();
-        if (r0 + i < row_end && c < a.cols) raw[i].load(a.x + group * a.x_group_stride + (uint64_t)(r0 + i) * a.x_stride + (uint64_t)c * sizeof(T));
+        if (r0 + i < row_end && c < a.cols) raw[i].load(x);
     }
     #pragma unroll
     for (uint32_t i = 0; i < kWarpRows; ++i) {
@@ -121,8 +124,8 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_kernel(const Fp4Args a)
         const uint32_t e = e2m1_scale_byte(amax);
         #pragma unroll
         for (int j = 0; j < Raw8<T>::kWords; ++j) f[j] = Raw8<T>::factor(e2m1_inverse(e));
-        if (r0 + i < row_end && c < a.cols)
-            *reinterpret_cast<uint32_t*>(a.codes + group * a.code_group_stride + (uint64_t)(r0 + i) * a.code_stride + c / 2) = raw[i].codes(f);
+        if (r0 + i < row_end && c < a.cols) *reinterpret_cast<uint32_t*>(codes) = raw[i].codes(f);
+        codes += a.code_stride;
         // (the second block of a last, half-used scale column is zero)
         if ((lane & 3u) == 0) sf_smem[warp * kWarpRows + i][lane / 4] = c < a.cols ? (uint8_t)e : (uint8_t)0;
     }
@@ -143,8 +146,8 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args
     __shared__ __align__(8) uint8_t sf_smem[2][kFp4Cols];
     __shared__ __align__(16) uint32_t stage[64][kFp4StageWords];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t tiles = a.tiles_r * a.tiles_c, group = blockIdx.x / tiles, tile = blockIdx.x - group * tiles;
-    const uint32_t row_base = tile / a.tiles_c * 64, c0 = tile % a.tiles_c * kFp4Cols;
+    const uint64_t group = blockIdx.z;
+    const uint32_t row_base = blockIdx.x / a.tiles_c * 64, c0 = blockIdx.x % a.tiles_c * kFp4Cols;
     const uint32_t half = warp / 4, tc = warp % 4 * 64 + lane % 8 * 8, c = c0 + tc;
     const uint32_t tr = half * 32 + lane / 8, r0 = row_base + tr;
     griddep_wait();
@@ -157,11 +160,17 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args
         if (end.whole <= row_base) return;                // behind the last group (uniform over the CTA)
         row_end = min(row_end, end.valid);
     }
+    const uint8_t* x = a.x + group * a.x_group_stride + (uint64_t)r0 * a.x_stride + (uint64_t)c * sizeof(T);
     Raw8<T> raw[8];
-    #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        raw[i].clear();
-        if (r0 + i * 4 < row_end && c < a.cols) raw[i].load(a.x + group * a.x_group_stride + (uint64_t)(r0 + i * 4) * a.x_stride + (uint64_t)c * sizeof(T));
+    if (row_base + 64 <= row_end && c0 + kFp4Cols <= a.cols) {
+        #pragma unroll
+        for (uint32_t i = 0; i < 8; ++i, x += 4 * a.x_stride) raw[i].load(x);
+    } else {
+        #pragma unroll
+        for (uint32_t i = 0; i < 8; ++i, x += 4 * a.x_stride) {
+            raw[i].clear();
+            if (r0 + i * 4 < row_end && c < a.cols) raw[i].load(x);
+        }
     }
     uint32_t m[Raw8<T>::kWords] = {}, f[Raw8<T>::kWords], field[8];
     #pragma unroll
@@ -236,37 +245,50 @@ __global__ void __launch_bounds__(kFp4Threads) dequant_fp4_kernel(const Fp4Args 
     constexpr uint32_t kWarpRows = 8;
     __shared__ __align__(8) uint8_t sf_smem[64][kFp4Cols / 32];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t tiles = a.tiles_r * a.tiles_c, group = blockIdx.x / tiles, tile = blockIdx.x - group * tiles;
-    const uint32_t row_base = tile / a.tiles_c * 64, c0 = tile % a.tiles_c * kFp4Cols;
+    const uint64_t group = blockIdx.z;
+    const uint32_t row_base = blockIdx.x / a.tiles_c * 64, c0 = blockIdx.x % a.tiles_c * kFp4Cols;
     const uint32_t c = c0 + lane * 8, r0 = row_base + warp * kWarpRows;
     griddep_wait();
     griddep_launch_dependents();
+    const bool inside = row_base + 64 <= a.rows && c0 + kFp4Cols <= a.cols;
+    const uint8_t* codes = a.codes + group * a.code_group_stride + (uint64_t)r0 * a.code_stride + c / 2;
     uint32_t q[kWarpRows];
-    #pragma unroll
-    for (uint32_t i = 0; i < kWarpRows; ++i)
-        q[i] = r0 + i < a.rows && c < a.cols ? ld_stream_u32(a.codes + group * a.code_group_stride + (uint64_t)(r0 + i) * a.code_stride + c / 2) : 0u;
+    if (inside) {
+        #pragma unroll
+        for (uint32_t i = 0; i < kWarpRows; ++i, codes += a.code_stride) q[i] = ld_stream_u32(codes);
+    } else {
+        #pragma unroll
+        for (uint32_t i = 0; i < kWarpRows; ++i, codes += a.code_stride) q[i] = r0 + i < a.rows && c < a.cols ? ld_stream_u32(codes) : 0u;
+    }
     const uint8_t* sf = a.sf + group * a.sf_group_stride;
     uint32_t scale[4];
     if constexpr (kMnMajor) {
-        uint32_t byte[8];
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t pair = c < a.cols ? ld_global_u16(sf + (uint64_t)(row_base / 64) * a.sf_stride + (uint64_t)(c + j) * 2) : 0u;
-            byte[j] = (pair >> (warp / 4 * 8)) & 0xffu;
+        const uint8_t* pairs = sf + (uint64_t)(row_base / 64) * a.sf_stride + (uint64_t)c * 2;
+        uint32_t p[4] = {};
+        if (c < a.cols && a.sf_aligned) {
+            const uint4 v = ld_global_v4(pairs);
+            p[0] = v.x; p[1] = v.y; p[2] = v.z; p[3] = v.w;
+        } else if (c < a.cols) {
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) p[j] = ld_global_u16(pairs + 4 * j) | (uint32_t)ld_global_u16(pairs + 4 * j + 2) << 16;
         }
         #pragma unroll
-        for (int j = 0; j < 4; ++j) scale[j] = Out8<T>::scale_pair(byte[2 * j], byte[2 * j + 1]);
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t b = p[j] >> (warp / 4 * 8);
+            scale[j] = Out8<T>::scale_pair(b & 0xffu, (b >> 16) & 0xffu);
+        }
     } else {
         const uint32_t col = threadIdx.x / 64, r = threadIdx.x % 64;
         if (c0 + col * 64 < a.cols && row_base + r < a.rows)
             *reinterpret_cast<uint16_t*>(&sf_smem[r][col * 2]) = ld_global_u16(sf + (uint64_t)(c0 / 64 + col) * a.sf_stride + (uint64_t)(row_base + r) * 2);
         __syncthreads();
     }
+    uint8_t* to = out + group * a.x_group_stride + (uint64_t)r0 * a.x_stride + (uint64_t)c * sizeof(T);
     #pragma unroll
-    for (uint32_t i = 0; i < kWarpRows; ++i) {
-        if (r0 + i >= a.rows || c >= a.cols) continue;
+    for (uint32_t i = 0; i < kWarpRows; ++i, to += a.x_stride) {
+        if (!inside && (r0 + i >= a.rows || c >= a.cols)) continue;
         if constexpr (!kMnMajor) scale[0] = scale[1] = scale[2] = scale[3] = Out8<T>::scale(sf_smem[warp * kWarpRows + i][lane / 4]);
-        Out8<T>::store(out + group * a.x_group_stride + (uint64_t)(r0 + i) * a.x_stride + (uint64_t)c * sizeof(T), q[i], scale);
+        Out8<T>::store(to, q[i], scale);
     }
 }
 
@@ -276,12 +298,13 @@ using namespace dg;
 
 // What both directions check: the float side is `x`, strides in elements of each side. `x_bytes`, `code_bytes`: the alignment that the
 // kernel's loads and stores need.
-static int fp4_args(Fp4Args& a, uint32_t tile_rows, uint32_t& tiles, uint32_t x_bytes, uint32_t code_bytes, const void* x, int is_fp32, uint64_t x_stride, uint64_t x_group_stride,
-                    uint32_t groups, uint32_t rows, uint32_t cols, const void* codes, uint64_t code_stride, uint64_t code_group_stride,
+static int fp4_args(Fp4Args& a, uint32_t tile_rows, uint32_t x_bytes, uint32_t code_bytes, const void* x, int is_fp32, uint64_t x_stride, uint64_t x_group_stride,
+                    uint32_t rows, uint32_t cols, const void* codes, uint64_t code_stride, uint64_t code_group_stride,
                     const int16_t* sf, uint64_t sf_stride, uint64_t sf_group_stride, int mn_major) {
     const uint64_t es = is_fp32 ? 4 : 2;
     DG_CHECK_ARG(x != nullptr && codes != nullptr && sf != nullptr, "fp4: null pointer");
     DG_CHECK_ARG(cols % 32 == 0, "fp4: the row length must be a multiple of 32");
+    DG_CHECK_ARG(rows <= 0x7fffffffu && cols <= 0x7fffffffu, "fp4: too many values");
     DG_CHECK_ARG((reinterpret_cast<uintptr_t>(x) | x_stride * es | x_group_stride * es) % x_bytes == 0,
                  "fp4: rows of values must start on %u-byte boundaries", x_bytes);
     DG_CHECK_ARG((reinterpret_cast<uintptr_t>(codes) | code_stride | code_group_stride) % code_bytes == 0,
@@ -293,8 +316,22 @@ static int fp4_args(Fp4Args& a, uint32_t tile_rows, uint32_t& tiles, uint32_t x_
     a.rows = rows; a.cols = cols;
     a.tiles_r = (rows + tile_rows - 1) / tile_rows;
     a.tiles_c = (cols + kFp4Cols - 1) / kFp4Cols;
-    DG_CHECK_ARG((uint64_t)a.tiles_r * a.tiles_c <= 0x7fffffffull / groups, "fp4: too many values");
-    tiles = groups * a.tiles_r * a.tiles_c;
+    a.sf_aligned = (reinterpret_cast<uintptr_t>(sf) | a.sf_stride | a.sf_group_stride) % 16 == 0;
+    DG_CHECK_ARG((uint64_t)a.tiles_r * a.tiles_c <= 0x7fffffffull, "fp4: too many values");
+    return DG_OK;
+}
+
+// One launch for as many matrices as a grid holds. `out`: the float side, where it is written.
+static int launch_fp4(const void* fn, Fp4Args a, uint32_t groups, void* out, void* stream) {
+    constexpr uint32_t kMostGroups = 65535;
+    uint8_t* to = static_cast<uint8_t*>(out);
+    void* params[] = {&a, &to};
+    for (uint32_t g = 0; g < groups; g += kMostGroups) {
+        const dim3 grid(a.tiles_r * a.tiles_c, 1, groups - g < kMostGroups ? groups - g : kMostGroups);
+        if (int rc = launch_overlapped(fn, grid, dim3(kFp4Threads), params, static_cast<cudaStream_t>(stream))) return rc;
+        a.x += kMostGroups * a.x_group_stride; a.codes += kMostGroups * a.code_group_stride; a.sf += kMostGroups * a.sf_group_stride;
+        to += kMostGroups * a.x_group_stride;
+    }
     return DG_OK;
 }
 
@@ -306,14 +343,12 @@ extern "C" int dg_quant_fp4_launch(const void* x, int x_is_fp32, uint64_t x_stri
     DG_CHECK_ARG(psum == nullptr || (groups == 1 && num_experts > 0 && alignment > 0 && alignment % (mn_major ? 64u : kFp4Rows) == 0),
                  "quant_fp4: a psum layout needs one matrix, experts, and an alignment that is a multiple of %u", mn_major ? 64u : kFp4Rows);
     Fp4Args a{};
-    uint32_t tiles = 0;
-    if (int rc = fp4_args(a, mn_major ? 64 : kFp4Rows, tiles, 16, mn_major ? 16 : 4, x, x_is_fp32, x_stride, x_group_stride, groups, rows, cols, out, out_stride,
+    if (int rc = fp4_args(a, mn_major ? 64 : kFp4Rows, 16, mn_major ? 16 : 4, x, x_is_fp32, x_stride, x_group_stride, rows, cols, out, out_stride,
                           out_group_stride, sf, sf_stride, sf_group_stride, mn_major)) return rc;
     a.psum = psum; a.num_experts = psum ? num_experts : 0; a.alignment = alignment;
     const void* fn = mn_major ? (x_is_fp32 ? (const void*)quant_fp4_mn_kernel<float> : (const void*)quant_fp4_mn_kernel<__nv_bfloat16>)
                               : (x_is_fp32 ? (const void*)quant_fp4_kernel<float> : (const void*)quant_fp4_kernel<__nv_bfloat16>);
-    void* params[] = {&a};
-    return launch_overlapped(fn, dim3(tiles), dim3(kFp4Threads), params, static_cast<cudaStream_t>(stream));
+    return launch_fp4(fn, a, groups, nullptr, stream);
 }
 
 extern "C" int dg_dequant_fp4_launch(const void* codes, uint64_t code_stride, uint64_t code_group_stride, const int16_t* sf, uint64_t sf_stride,
@@ -321,12 +356,9 @@ extern "C" int dg_dequant_fp4_launch(const void* codes, uint64_t code_stride, ui
                                      void* out, int out_is_fp32, uint64_t out_stride, uint64_t out_group_stride, void* stream) {
     if (groups == 0 || rows == 0 || cols == 0) return DG_OK;
     Fp4Args a{};
-    uint32_t tiles = 0;
-    if (int rc = fp4_args(a, 64, tiles, out_is_fp32 ? 32 : 16, 4, out, out_is_fp32, out_stride, out_group_stride, groups, rows, cols, codes, code_stride,
+    if (int rc = fp4_args(a, 64, out_is_fp32 ? 32 : 16, 4, out, out_is_fp32, out_stride, out_group_stride, rows, cols, codes, code_stride,
                           code_group_stride, sf, sf_stride, sf_group_stride, mn_major)) return rc;
     const void* fn = mn_major ? (out_is_fp32 ? (const void*)dequant_fp4_kernel<float, true> : (const void*)dequant_fp4_kernel<__nv_bfloat16, true>)
                               : (out_is_fp32 ? (const void*)dequant_fp4_kernel<float, false> : (const void*)dequant_fp4_kernel<__nv_bfloat16, false>);
-    uint8_t* to = static_cast<uint8_t*>(out);
-    void* params[] = {&a, &to};
-    return launch_overlapped(fn, dim3(tiles), dim3(kFp4Threads), params, static_cast<cudaStream_t>(stream));
+    return launch_fp4(fn, a, groups, out, stream);
 }

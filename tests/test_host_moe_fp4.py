@@ -94,7 +94,7 @@ def test_the_c_abi_checks_its_arguments():
     _refused(fp4(psum=p, e=4, align=48), 'multiple of 32')
     _refused(fp4(psum=p, e=4, align=96, mn=1), 'multiple of 64')
     _refused(fp4(psum=p, e=4, align=128, groups=2), 'one matrix')
-    _refused(fp4(rows=1 << 31, ss=1 << 32, groups=64), 'too many values')
+    _refused(fp4(rows=(1 << 32) - 1, cols=1 << 13, ss=1 << 32), 'too many values')
     for bad in (dict(x=None), dict(out=None), dict(sf=None)):
         _refused(fp4(**bad), 'null pointer')
     assert lib.dg_moe_num_rows(0, 4, 256) == 0
