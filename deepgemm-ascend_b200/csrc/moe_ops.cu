@@ -48,23 +48,30 @@ __device__ __forceinline__ void load_experts(const SortArgs& a, uint32_t i, uint
     #pragma unroll
     for (uint32_t k = 0; k < kBatch; ++k) expert[k] = e[k] >= 0 && e[k] < (T)a.experts ? (uint32_t)e[k] : a.experts;
 }
-// The lanes that hold the same expert, bit by bit (a match over 32 lanes takes a turn for every value that occurs: three times as long).
-__device__ __forceinline__ uint32_t same_expert(uint32_t e, uint32_t bits) {
+// The lanes that hold the same expert, bit by bit (a match over 32 lanes takes a turn for every value that occurs). The number of bits is
+// rounded up to one that is unrolled: as a loop, the rest of it cost as much as the votes.
+template <uint32_t kBits>
+__device__ __forceinline__ uint32_t same_bits(uint32_t e) {
     uint32_t peers = 0xffffffffu;
-    for (uint32_t b = 0; b < bits; ++b) {
-        const bool set = (e >> b) & 1u;
+    #pragma unroll
+    for (uint32_t b = 0; b < kBits; ++b) {
+        const bool set = e & (1u << b);
         const uint32_t with = __ballot_sync(0xffffffffu, set);
-        peers &= set ? with : ~with;
+        peers &= with ^ (set ? 0u : 0xffffffffu);
     }
     return peers;
+}
+__device__ __forceinline__ uint32_t same_expert(uint32_t e, uint32_t bits) {
+    return bits <= 6 ? same_bits<6>(e) : bits <= 9 ? same_bits<9>(e) : same_bits<11>(e);
 }
 
 // A stable counting sort in one launch: one CTA, or a cluster whose CTAs exchange their counts through distributed shared memory.
 // Every warp owns a run of choices and a row of counters of its own (no atomics): it counts, the counters become offsets (over the
 // warps of the CTA, the CTAs of the cluster, and the experts with their alignment), and it walks its run a second time to hand
 // out rows. Within 32 choices the order is that of the lanes. Runs that fit kBatch are read once; kBatch is 1 where 32 choices for each
-// of a CTA's warps are all (1024 choices: 3.6 us against 4.4 with 8). 131072 choices of 256 experts: 12.2 us with 16 CTAs, 19 with 8; 40 with
-// one load at a time and a match for the peers.
+// of a CTA's warps are all (1024 choices: 3.5 us against 4.4 with 8). 131072 choices of 256 experts: 11.8 us with 16 CTAs, 19 with 8; 40 with
+// one load at a time and a match for the peers. What is left at that size is the second pass, 6 of the 11.8 us: the votes that find a choice's peers, and
+// one store to a place of its own for every choice, which 16 SMs have to make.
 template <typename T, uint32_t kBatch>
 __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a) {
     extern __shared__ uint32_t smem[];
@@ -79,14 +86,15 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a
     for (uint32_t i = tid; i < a.warps * a.experts; i += kSortThreads) counts[i] = 0;
     griddep_wait();
     griddep_launch_dependents();
-    // no row holds a choice until the second pass says so (the barrier in between orders the writes)
-    for (uint32_t i = cta * kSortThreads + tid; i < a.rows; i += ctas * kSortThreads) a.row_choices[i] = -1;
-    __syncthreads();
     const uint32_t first = min(a.n, (cta * a.warps + warp) * a.segment), last = warp < a.warps ? min(a.n, first + a.segment) : first;
     uint32_t* const mine = counts + warp * a.experts;
     uint32_t expert[kBatch];
+    load_experts<T>(a, first + lane, last, expert);
+    // no row holds a choice until the second pass says so (the barriers in between order the writes)
+    for (uint32_t i = cta * kSortThreads + tid; i < a.rows; i += ctas * kSortThreads) a.row_choices[i] = -1;
+    __syncthreads();
     for (uint32_t i0 = first; i0 < last; i0 += 32 * kBatch) {
-        load_experts<T>(a, i0 + lane, last, expert);
+        if (i0 > first) load_experts<T>(a, i0 + lane, last, expert);
         #pragma unroll
         for (uint32_t k = 0; k < kBatch; ++k)
             if (expert[k] < a.experts) atomicAdd(mine + expert[k], 1u);
@@ -106,13 +114,19 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a
         cluster_arrive();
         cluster_wait();
         if (tid < a.experts) {
-            total = 0;
+            // (all on their way at once: one after the other, sixteen of them took 2 us)
             const uint32_t at = smem_u32(totals + tid);
-            for (uint32_t r = 0; r < ctas; ++r) {
-                uint32_t c;
-                asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c) : "r"(mapa_shared(at, r)) : "memory");
-                before += r < cta ? c : 0u;
-                total += c;
+            uint32_t c[kSortMaxCluster];
+            #pragma unroll
+            for (uint32_t r = 0; r < kSortMaxCluster; ++r) {
+                c[r] = 0;
+                if (r < ctas) asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(c[r]) : "r"(mapa_shared(at, r)));
+            }
+            total = 0;
+            #pragma unroll
+            for (uint32_t r = 0; r < kSortMaxCluster; ++r) {
+                before += r < cta ? c[r] : 0u;
+                total += c[r];
             }
         }
         cluster_arrive();
