@@ -31,8 +31,8 @@ struct Fp4Args {
 
 // Eight values of a lane, as they lie in memory: kWords words of one or two values. Magnitudes are compared as bit patterns (infinities
 // and NaN come out on top by themselves), BF16 two at a time; so are the products with the inverse scales, which are exact (down to where
-// BF16 has subnormals, all of which round to zero), so that half of the arithmetic per value is gone: an MN-major quantiser that
-// turned every BF16 into FP32 first kept the SMs at 67 % and HBM at 58 %.
+// BF16 has subnormals, all of which round to zero). What is saved counts: an MN-major quantiser that turned every BF16 into FP32 first kept
+// the SMs at 67 % and HBM at 58 %, and in a long run arithmetic draws on the board's power limit.
 template <typename T> struct Raw8;
 template <> struct Raw8<__nv_bfloat16> {
     static constexpr int kWords = 4;
@@ -238,19 +238,22 @@ template <> struct Out8<float> {
     }
 };
 
-// One CTA = 64 rows x 256 columns, a warp eight rows, a lane eight columns. The scales of a K-major tile come in runs down the rows, through
-// shared memory; an MN-major tile lies in two blocks of rows, whose scales lie along the columns.
-template <typename T, bool kMnMajor>
+// One CTA = 8 kWarpRows rows x 256 columns, a warp kWarpRows (4 or 8) of the rows, a lane eight columns. The scales of a K-major tile come in runs
+// down the rows, through shared memory; a warp's rows of an MN-major tile lie in one block, whose scales lie along the columns. Four rows where
+// the tiles of eight would not fill the device a few times (with the quantiser in front, 2112 x 7168 FP32: 24.2 against 26.1 us, BF16 14.4 against
+// 15.1), else eight (8 x 4096 x 7168 BF16 in a long run, at the board's power limit: 187.8 against 191.3 us).
+constexpr uint32_t kFewBackTiles = 148 * 8 * 4;
+template <typename T, bool kMnMajor, uint32_t kWarpRows>
 __global__ void __launch_bounds__(kFp4Threads) dequant_fp4_kernel(const Fp4Args a, uint8_t* out) {
-    constexpr uint32_t kWarpRows = 8;
-    __shared__ __align__(8) uint8_t sf_smem[64][kFp4Cols / 32];
+    constexpr uint32_t kTileRows = kWarpRows * kFp4Threads / 32;
+    __shared__ __align__(8) uint8_t sf_smem[kTileRows][kFp4Cols / 32];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint64_t group = blockIdx.z;
-    const uint32_t row_base = blockIdx.x / a.tiles_c * 64, c0 = blockIdx.x % a.tiles_c * kFp4Cols;
+    const uint32_t row_base = blockIdx.x / a.tiles_c * kTileRows, c0 = blockIdx.x % a.tiles_c * kFp4Cols;
     const uint32_t c = c0 + lane * 8, r0 = row_base + warp * kWarpRows;
     griddep_wait();
     griddep_launch_dependents();
-    const bool inside = row_base + 64 <= a.rows && c0 + kFp4Cols <= a.cols;
+    const bool inside = row_base + kTileRows <= a.rows && c0 + kFp4Cols <= a.cols;
     const uint8_t* codes = a.codes + group * a.code_group_stride + (uint64_t)r0 * a.code_stride + c / 2;
     uint32_t q[kWarpRows];
     if (inside) {
@@ -263,7 +266,7 @@ __global__ void __launch_bounds__(kFp4Threads) dequant_fp4_kernel(const Fp4Args 
     const uint8_t* sf = a.sf + group * a.sf_group_stride;
     uint32_t scale[4];
     if constexpr (kMnMajor) {
-        const uint8_t* pairs = sf + (uint64_t)(row_base / 64) * a.sf_stride + (uint64_t)c * 2;
+        const uint8_t* pairs = sf + (uint64_t)(r0 / 64) * a.sf_stride + (uint64_t)c * 2;
         uint32_t p[4] = {};
         if (c < a.cols && a.sf_aligned) {
             const uint4 v = ld_global_v4(pairs);
@@ -274,12 +277,12 @@ __global__ void __launch_bounds__(kFp4Threads) dequant_fp4_kernel(const Fp4Args 
         }
         #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const uint32_t b = p[j] >> (warp / 4 * 8);
+            const uint32_t b = p[j] >> (r0 / 32 % 2 * 8);
             scale[j] = Out8<T>::scale_pair(b & 0xffu, (b >> 16) & 0xffu);
         }
     } else {
-        const uint32_t col = threadIdx.x / 64, r = threadIdx.x % 64;
-        if (c0 + col * 64 < a.cols && row_base + r < a.rows)
+        const uint32_t col = threadIdx.x / kTileRows, r = threadIdx.x % kTileRows;
+        if (col < kFp4Cols / 64 && c0 + col * 64 < a.cols && row_base + r < a.rows)
             *reinterpret_cast<uint16_t*>(&sf_smem[r][col * 2]) = ld_global_u16(sf + (uint64_t)(c0 / 64 + col) * a.sf_stride + (uint64_t)(row_base + r) * 2);
         __syncthreads();
     }
@@ -351,14 +354,20 @@ extern "C" int dg_quant_fp4_launch(const void* x, int x_is_fp32, uint64_t x_stri
     return launch_fp4(fn, a, groups, nullptr, stream);
 }
 
+template <uint32_t kWarpRows>
+static const void* back_kernel(bool fp32, bool mn_major) {
+    return mn_major ? (fp32 ? (const void*)dequant_fp4_kernel<float, true, kWarpRows> : (const void*)dequant_fp4_kernel<__nv_bfloat16, true, kWarpRows>)
+                    : (fp32 ? (const void*)dequant_fp4_kernel<float, false, kWarpRows> : (const void*)dequant_fp4_kernel<__nv_bfloat16, false, kWarpRows>);
+}
+
 extern "C" int dg_dequant_fp4_launch(const void* codes, uint64_t code_stride, uint64_t code_group_stride, const int16_t* sf, uint64_t sf_stride,
                                      uint64_t sf_group_stride, uint32_t groups, uint32_t rows, uint32_t cols, int mn_major,
                                      void* out, int out_is_fp32, uint64_t out_stride, uint64_t out_group_stride, void* stream) {
     if (groups == 0 || rows == 0 || cols == 0) return DG_OK;
+    const bool few = (uint64_t)groups * ((rows + 63) / 64) * ((cols + kFp4Cols - 1) / kFp4Cols) < kFewBackTiles;
     Fp4Args a{};
-    if (int rc = fp4_args(a, 64, out_is_fp32 ? 32 : 16, 4, out, out_is_fp32, out_stride, out_group_stride, rows, cols, codes, code_stride,
+    if (int rc = fp4_args(a, few ? 32 : 64, out_is_fp32 ? 32 : 16, 4, out, out_is_fp32, out_stride, out_group_stride, rows, cols, codes, code_stride,
                           code_group_stride, sf, sf_stride, sf_group_stride, mn_major)) return rc;
-    const void* fn = mn_major ? (out_is_fp32 ? (const void*)dequant_fp4_kernel<float, true> : (const void*)dequant_fp4_kernel<__nv_bfloat16, true>)
-                              : (out_is_fp32 ? (const void*)dequant_fp4_kernel<float, false> : (const void*)dequant_fp4_kernel<__nv_bfloat16, false>);
+    const void* fn = few ? back_kernel<4>(out_is_fp32, mn_major) : back_kernel<8>(out_is_fp32, mn_major);
     return launch_fp4(fn, a, groups, out, stream);
 }

@@ -113,6 +113,25 @@ def test_groups_and_strides(mn_major):
     assert torch.equal(deep_gemm.cast_from_fp4((room[:, :, 4:260], sf_view), mn_major=mn_major), deep_gemm.cast_from_fp4((codes, sf), mn_major=mn_major))
 
 
+@pytest.mark.parametrize('mn_major', [False, True])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_many_matrices_give_what_each_gives(mn_major, dtype):
+    """Enough of them for the larger tiles of the way back, and more than a grid holds."""
+    seed_all(14)
+    for shape in ((600, 67, 1056), (70001, 3, 32)):
+        x = torch.randn(shape, device='cuda', dtype=dtype)
+        codes, sf = deep_gemm.cast_to_fp4(x, mn_major=mn_major)
+        back = deep_gemm.cast_from_fp4((codes, sf), out_dtype=dtype, mn_major=mn_major)
+        for g in (*range(0, 600, 37), *range(65530, 65540), shape[0] - 1):
+            if g >= shape[0]:
+                continue
+            one, one_sf = deep_gemm.cast_to_fp4(x[g], mn_major=mn_major)
+            assert torch.equal(codes[g], one) and torch.equal(sf[g], one_sf), g
+            assert torch.equal(back[g], deep_gemm.cast_from_fp4((one, one_sf), out_dtype=dtype, mn_major=mn_major)), g
+            if g < 74:
+                _check(x[g].cpu(), mn_major)
+
+
 @pytest.mark.parametrize('mn_major,alignment', [(False, 32), (False, 256), (True, 64), (True, 256)])
 def test_psum_layout(mn_major, alignment):
     seed_all(alignment)
