@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kMoeThreads) moe_dispatch_kernel(const Dispatc
 // The same with a quantisation on the way: a warp takes kTiles x 256 channels of a token, eight to a lane, four lanes to a block of 32. The
 // scales of a row lie num_rows elements apart, and the rows of a token far from one another: written from here, each is a store of two
 // bytes with a sector of L2 to itself. That suits a few tokens. For many (65536 rows of 7168: 127 us, 93 without the scales), the
-// bytes go to a scratch, by token, and moe_scales_kernel behind this one turns them into runs: 101 us together, 5.9 TB/s. Two tiles to a
+// bytes go to a scratch, by token, and moe_scales_kernel behind this one turns them into runs: 100 us together, 6.0 TB/s. Two tiles to a
 // warp then: with one, 16384 tokens of which a rank has one choice of eight take 98 us, with two 66, with four 78. (A grid of one wave whose
 // warps take one piece after the other, the next on its way: 98 us, and 120 instead of 101.)
 constexpr uint32_t kFp8Tiles = 2;
@@ -347,22 +347,26 @@ __global__ void __launch_bounds__(kMoeThreads) moe_scales_kernel(const DispatchA
     griddep_wait();
     griddep_launch_dependents();
     if (!some) return;
-    const uint32_t words = min(kScaleChunk, a.scratch_stride - b0) / 16;       // pieces of 16 bytes
-    for (uint32_t i = tid; i < kScaleRows * words; i += kMoeThreads) {
-        const uint32_t r = i / words, w = i - r * words, token = token_of[r];
+    // (a thread keeps to its piece of the rows, and its row of the columns: what is left of an index is an addition)
+    const uint32_t pieces = min(kScaleChunk, a.scratch_stride - b0) / 16, piece = tid % (kScaleChunk / 16);
+    for (uint32_t r = tid / (kScaleChunk / 16); r < kScaleRows && piece < pieces; r += kMoeThreads / (kScaleChunk / 16)) {
+        const uint32_t token = token_of[r];
         if (token == 0xffffffffu) continue;
-        const uint4 v = ld_global_v4(a.scratch + (uint64_t)token * a.scratch_stride + b0 + w * 16);
-        uint32_t* to = &bytes[r][w * 4];
+        const uint4 v = ld_global_v4(a.scratch + (uint64_t)token * a.scratch_stride + b0 + piece * 16);
+        uint32_t* to = &bytes[r][piece * 4];
         to[0] = v.x; to[1] = v.y; to[2] = v.z; to[3] = v.w;
     }
     __syncthreads();
     const uint32_t r = tid % kScaleRows, row = row0 + r;
     if (token_of[r] == 0xffffffffu) return;
-    const uint32_t g = row / a.sf_rows;
-    uint8_t* const to = a.sf + g * a.sf_group_stride + (uint64_t)(row - g * a.sf_rows) * 2;
-    const uint32_t cols = (a.hidden + 63) / 64, c0 = b0 / 2;
-    for (uint32_t c = tid / kScaleRows; c < kScaleChunk / 2 && c0 + c < cols; c += kMoeThreads / kScaleRows)
-        *reinterpret_cast<uint16_t*>(to + (uint64_t)(c0 + c) * a.sf_col_stride) = (uint16_t)(bytes[r][c / 2] >> (c % 2 * 16));
+    const uint32_t g = row / a.sf_rows, cols = (a.hidden + 63) / 64, c0 = b0 / 2;
+    uint32_t word = tid / kScaleRows;                     // two columns
+    uint8_t* to = a.sf + g * a.sf_group_stride + (uint64_t)(row - g * a.sf_rows) * 2 + (uint64_t)(c0 + 2 * word) * a.sf_col_stride;
+    for (; word < pieces * 4; word += kMoeThreads / kScaleRows, to += 2 * (kMoeThreads / kScaleRows) * a.sf_col_stride) {
+        const uint32_t pair = bytes[r][word];
+        if (c0 + 2 * word < cols) *reinterpret_cast<uint16_t*>(to) = (uint16_t)pair;
+        if (c0 + 2 * word + 1 < cols) *reinterpret_cast<uint16_t*>(to + a.sf_col_stride) = (uint16_t)(pair >> 16);
+    }
 }
 
 // -------------------------------------------------------------------------------------------------- combine
