@@ -87,7 +87,8 @@ template <> struct Raw8<float> {
 constexpr uint32_t kFp4Threads = 256, kFp4Rows = 32, kFp4Cols = 256;
 
 // K-major: one CTA = 32 rows x 256 columns, a warp takes four rows (all loads issued before the first is used), a lane eight
-// columns, four lanes a block. Scales go through shared memory, so that every scale column of the tile is one 64-byte run.
+// columns, four lanes a block. Scales go through shared memory, so that every scale column of the tile is one 64-byte run. Bound by HBM for many
+// rows, by the launch for few: 64 x 7168 BF16 2.1 us, 2112 x 7168 FP32 12.4 us (5.5 TB/s, from HBM), 8 x 4096 x 7168 BF16 about 90 us (6.6 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(kFp4Threads) quant_fp4_kernel(const Fp4Args a) {
     constexpr uint32_t kWarpRows = kFp4Rows / (kFp4Threads / 32);
@@ -139,7 +140,8 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_kernel(const Fp4Args a)
 // MN-major: one CTA = 64 rows x 256 columns. A warp takes one block of 32 rows x 64 columns: lane = (every fourth row, eight columns), so
 // that a row of the warp's tile is a whole 128-byte line of BF16 and the maximum down a column takes two shuffles. The codes go through
 // shared memory and out as lines of 128 bytes (written by the lanes as they are, a row of a warp's tile is one sector of 32 bytes, and
-// the number of stores bounds the kernel); its rows are 40 words apart, which keeps the four rows of a store in banks of their own.
+// the number of stores bounds the kernel: 114 us against 110 for 8 x 4096 x 7168 BF16); its rows are 40 words apart, which keeps the four rows of a
+// store in banks of their own. That size now: 90 us, 6.6 TB/s, since whole tiles check no bounds and BF16 goes two at a time.
 constexpr uint32_t kFp4StageWords = 40;
 template <typename T>
 __global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args a) {
