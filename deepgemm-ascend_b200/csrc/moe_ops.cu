@@ -70,8 +70,9 @@ __device__ __forceinline__ uint32_t same_expert(uint32_t e, uint32_t bits) {
 // become offsets (over the warps of the CTA, the CTAs of the cluster, and the experts with their alignment), and it walks its run a
 // second time to hand out rows. Within 32 choices the order is that of the lanes. Runs that fit kBatch are read once; kBatch is 1 where 32 choices for each
 // of a CTA's warps are all (1024 choices: 3.5 us against 4.4 with 8). 131072 choices of 256 experts: 11.8 us with 16 CTAs, 19 with 8; 40 with
-// one load at a time and a match for the peers. What is left at that size is the second pass, 6 of the 11.8 us: the votes that find a choice's peers, and
-// one store to a place of its own for every choice, which 16 SMs have to make.
+// one load at a time and a match for the peers. What is left at that size is the second pass, 6 of the 11.8 us: some 150 instructions for 32 choices, half
+// of them the votes that find a choice's peers, and one store to a place of its own for every choice, which 16 SMs have to make. (Four clusters that
+// count all choices each and share the second pass: 12.4 us; all votes of a batch at once, unrolled: 14.2.)
 template <typename T, uint32_t kBatch>
 __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a) {
     extern __shared__ uint32_t smem[];
@@ -158,13 +159,15 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a
     }
     __syncthreads();
     const uint32_t bits = 32 - __clz(a.experts);
-    for (uint32_t i0 = first; i0 < last; i0 += 32 * kBatch) {
-        if (last - first > 32 * kBatch) load_experts<T>(a, i0 + lane, last, expert);
+    // (every warp takes the same turns, with no choices in those behind its last: 32768 choices 6.7 us, and 8.0 where each ended at its own)
+    for (uint32_t at = 0; at < a.segment; at += 32 * kBatch) {
+        if (a.segment > 32 * kBatch) load_experts<T>(a, first + at + lane, last, expert);
         #pragma unroll
         for (uint32_t k = 0; k < kBatch; ++k) held[k * kSortThreads + tid] = (uint16_t)expert[k];
+        const uint32_t turns = min(kBatch, (a.segment - at) / 32);
         #pragma unroll 1
-        for (uint32_t k = 0; k < kBatch && i0 + k * 32 < last; ++k) {
-            const uint32_t i = i0 + k * 32 + lane, e = held[k * kSortThreads + tid], peers = same_expert(e, bits);
+        for (uint32_t k = 0; k < turns; ++k) {
+            const uint32_t i = first + at + k * 32 + lane, e = held[k * kSortThreads + tid], peers = same_expert(e, bits);
             uint32_t row = 0xffffffffu;
             if (e < a.experts) {
                 row = bases[e] + mine[e] + __popc(peers & ((1u << lane) - 1u));
