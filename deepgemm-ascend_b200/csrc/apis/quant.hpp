@@ -101,7 +101,7 @@ inline void register_quant_apis(py::module_& m) {
         return quantise_fp8(x, x.size(1) / 2, true, topk_weights, psum, clamp_value, expert_alignment);
     }, py::arg("x"), py::arg("topk_weights") = std::nullopt, py::arg("psum_num_tokens_per_expert") = std::nullopt,
        py::arg("clamp_value") = std::nullopt, py::arg("expert_alignment") = 128);
-    m.def("cast_to_fp4", &cast_to_fp4, py::arg("x"), py::arg("psum_num_tokens_per_expert") = std::nullopt, py::arg("expert_alignment") = 128,
+    m.def("cast_to_fp4", &cast_to_fp4, py::arg("x"), py::arg("psum_num_tokens_per_expert") = std::nullopt, py::arg("expert_alignment") = kMkAlignment,
           py::arg("mn_major") = false);
     m.def("cast_from_fp4", &cast_from_fp4, py::arg("x"), py::arg("out_dtype") = torch::kBFloat16, py::arg("mn_major") = false);
     m.def("cast_to_fp8", [](const torch::Tensor& x, const std::optional<torch::Tensor>& psum, int64_t expert_alignment) {

@@ -14,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib as L
-from ._api import _C, _ceil_div, _host_assert, _stream_ptr
+from ._api import MK_ALIGNMENT, _C, _ceil_div, _host_assert, _stream_ptr
 
 
 def _launch(x, hidden, swiglu, topk_weights, psum, clamp_value, expert_alignment):
@@ -61,7 +61,7 @@ def _empty_scales(shape, device):
     return torch.empty_strided(shape, (rows * cols, 1, rows)[-len(shape):], dtype=torch.int16, device=device)
 
 
-def cast_to_fp4(x: torch.Tensor, psum_num_tokens_per_expert: Optional[torch.Tensor] = None, expert_alignment: int = 128, mn_major: bool = False):
+def cast_to_fp4(x: torch.Tensor, psum_num_tokens_per_expert: Optional[torch.Tensor] = None, expert_alignment: int = MK_ALIGNMENT, mn_major: bool = False):
     """x [rows, cols] or [groups, rows, cols] BF16 or FP32 -> (packed E2M1 int8 [.., rows, cols / 2], packed UE8M0 scales), one scale per
     32 values along K, in the layout that the GEMMs read:
 
@@ -72,7 +72,8 @@ def cast_to_fp4(x: torch.Tensor, psum_num_tokens_per_expert: Optional[torch.Tens
 
     The scale is the smallest power of two with which the block's largest magnitude is at most 6 (2^-126 or more); values are rounded to the
     nearest code, halves to the even one. A block that holds an infinity or a NaN gets the scale NaN. Rows in the padding of a psum layout
-    are not written; with mn_major they count as zeros and are written as zeros (`expert_alignment` is a multiple of 64 then)."""
+    are not written; with mn_major they count as zeros and are written as zeros. `expert_alignment` is that of the layout, the one of `moe_sort` and
+    the grouped GEMMs if it is not given: a multiple of 32, or of 64 with mn_major."""
     _host_assert(x.is_cuda and x.dim() in (2, 3) and x.stride(-1) == 1 and x.dtype in (torch.bfloat16, torch.float32),
                  'x must be a row-major 2-D or 3-D BF16 or FP32 tensor on a CUDA device')
     groups, rows, cols = x.size(0) if x.dim() == 3 else 1, x.size(-2), x.size(-1)
