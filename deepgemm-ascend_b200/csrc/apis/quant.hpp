@@ -46,6 +46,8 @@ inline TensorPair cast_to_fp4(const torch::Tensor& x, const std::optional<torch:
     if (psum.has_value()) {
         host_assert(psum->scalar_type() == torch::kInt32 && psum->dim() == 1 && psum->is_contiguous() && psum->device() == x.device(),
                     "psum_num_tokens_per_expert must be a contiguous int32 vector on the device of x");
+        // (an empty tensor has no address, and the C ABI takes a null pointer for no layout)
+        host_assert(psum->numel() > 0, "psum_num_tokens_per_expert must hold an expert");
         host_assert(x.dim() == 2, "a psum layout needs a 2-D x");
         host_assert(expert_alignment > 0 && expert_alignment <= INT32_MAX && expert_alignment % (mn_major ? 64 : 32) == 0,
                     "expert_alignment must be a positive multiple of 32 (64 when mn_major)");

@@ -83,6 +83,7 @@ def cast_to_fp4(x: torch.Tensor, psum_num_tokens_per_expert: Optional[torch.Tens
     if psum is not None:
         _host_assert(psum.dtype == torch.int32 and psum.dim() == 1 and psum.is_contiguous() and psum.device == x.device,
                      'psum_num_tokens_per_expert must be a contiguous int32 vector on the device of x')
+        _host_assert(psum.numel() > 0, 'psum_num_tokens_per_expert must hold an expert')
         _host_assert(x.dim() == 2, 'a psum layout needs a 2-D x')
         _host_assert(0 < expert_alignment < 2 ** 31 and expert_alignment % (64 if mn_major else 32) == 0,
                      'expert_alignment must be a positive multiple of 32 (64 when mn_major)')

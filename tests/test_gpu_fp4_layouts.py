@@ -78,3 +78,14 @@ def test_the_weight_gradient_in_fp4_as_it_is_documented(host):
     total = oracle.align(psum[-1], 256)
     ref = oracle.k_grouped_psum_ref(*(oracle.cast_fp4_ref(t, -2, valid)[2].float()[:total] for t in (dy, x)), psum, torch.float32)
     assert_close(d, ref, 'weight gradient')
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('host', quant_hosts)
+@pytest.mark.parametrize('mn_major', [False, True])
+def test_a_layout_without_experts_is_refused(host, mn_major):
+    """It is not the same as no layout, for which all rows count."""
+    none = torch.empty(0, dtype=torch.int32, device='cuda')
+    for rows in (64, 0):
+        with pytest.raises(RuntimeError, match='must hold an expert'):
+            host.cast_to_fp4(torch.ones(rows, 64, device='cuda'), none, mn_major=mn_major)
