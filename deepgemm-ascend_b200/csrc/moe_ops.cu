@@ -112,8 +112,9 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a
     }
     uint32_t before = 0;
     if (ctas > 1) {
-        cluster_arrive();
-        cluster_wait();
+        // (all three barriers follow branches that a number of experts or choices can end inside a warp)
+        cluster_arrive_diverged();
+        cluster_wait_diverged();
         if (tid < a.experts) {
             // (all on their way at once: one after the other, sixteen of them took 2 us)
             const uint32_t at = smem_u32(totals + tid);
@@ -130,7 +131,7 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a
                 total += c[r];
             }
         }
-        cluster_arrive();
+        cluster_arrive_diverged();
     }
     // exclusive sum over the experts' sizes
     const uint32_t size = tid >= a.experts ? 0u : a.max_m ? a.max_m : (total + a.alignment - 1) / a.alignment * a.alignment;
@@ -180,7 +181,7 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a
             if (row < a.rows) a.row_choices[row] = (int32_t)i;
         }
     }
-    if (ctas > 1) cluster_wait();                       // the others have read this CTA's totals
+    if (ctas > 1) cluster_wait_diverged();              // the others have read this CTA's totals
 }
 
 // -------------------------------------------------------------------------------------------------- rows and layouts

@@ -45,6 +45,13 @@ __device__ __forceinline__ void cluster_arrive() {
 __device__ __forceinline__ void cluster_wait() {
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The same where the threads of a warp may come one by one (the aligned forms want the whole warp at the instruction).
+__device__ __forceinline__ void cluster_arrive_diverged() {
+    asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait_diverged() {
+    asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
 // Address of the same shared-memory offset in CTA `rank` of this cluster.
 __device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
     uint32_t r;

@@ -129,3 +129,13 @@ def test_dispatch_to_fp8_of_many_tokens_in_one_launch(tokens, topk, hidden):
         got, got_sf = host.moe_dispatch_to_fp8(x, plan, out=(data.view(torch.float8_e4m3fn), scales))
         assert torch.equal(data[live], codes.view(torch.uint8)[choice[live] // topk]) and torch.equal(got_sf[live], sf[choice[live] // topk])
         assert (data[~live] == 0x11).all() and (got_sf[~live] == 0x2222).all()
+
+
+def test_any_number_of_experts_over_a_cluster():
+    """Numbers of experts that end inside a warp, on the paths with barriers between the CTAs."""
+    gen = torch.Generator().manual_seed(1)
+    for experts in (1, 2, 7, 31, 33, 100, 161, 511, 1000, 1023):
+        idx = torch.randint(-1, experts, (6001, 3), generator=gen)
+        for max_m in (None, 50):
+            plan, ref = deep_gemm.moe_sort(idx.cuda(), experts, max_m=max_m), oracle.moe_sort_ref(idx, experts, 256, max_m)
+            assert all(torch.equal(a.cpu(), b) for a, b in zip(plan, ref)), (experts, max_m)
