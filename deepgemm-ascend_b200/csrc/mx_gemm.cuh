@@ -194,12 +194,13 @@ struct Scheduler {
     // m-blocks are counted in units of (128 * kCtaGroup) rows.
     uint32_t cur_kb_begin = 0, cur_kb_end = 0;
 
+    // (not through the read-only path: the kernel in front may be the one that makes the layout, and this one is resident by then)
     __device__ __forceinline__ void load_group() {
         if (p.gemm_type == kKGroupedPsum) {
             // scheduler.hpp:163-180: group g owns the K range [align(psum[g-1],256), psum[g]); every group spans the
             // whole M x N grid, an empty group has no tiles (its D is zeroed by a separate kernel).
-            const uint32_t start = cur_group == 0 ? 0u : ((uint32_t)__ldg(p.grouped_layout + cur_group - 1) + 255u) / 256u * 256u;
-            const uint32_t end = (uint32_t)__ldg(p.grouped_layout + cur_group);
+            const uint32_t start = cur_group == 0 ? 0u : (ld_global_u32(p.grouped_layout + cur_group - 1) + 255u) / 256u * 256u;
+            const uint32_t end = ld_global_u32(p.grouped_layout + cur_group);
             cur_row0 = 0;
             cur_kb_begin = start / p.stage_k;
             cur_kb_end = end > start ? (end + p.stage_k - 1) / p.stage_k : cur_kb_begin;
@@ -207,14 +208,14 @@ struct Scheduler {
         } else if (p.gemm_type == kMGroupedPsum) {
             // scheduler.hpp:147-162: group g owns rows [align(psum[g-1],256), psum[g]) and the
             // kernel computes whole 256-row blocks of it.
-            const uint32_t start = cur_group == 0 ? 0u : ((uint32_t)__ldg(p.grouped_layout + cur_group - 1) + 255u) / 256u * 256u;
-            const uint32_t end = (uint32_t)__ldg(p.grouped_layout + cur_group);
+            const uint32_t start = cur_group == 0 ? 0u : (ld_global_u32(p.grouped_layout + cur_group - 1) + 255u) / 256u * 256u;
+            const uint32_t end = ld_global_u32(p.grouped_layout + cur_group);
             const uint32_t rows = end > start ? end - start : 0u;
             cur_row0 = start;
             cur_blocks = (rows + 255u) / 256u * (256u / (kBlockM * kCtaGroup));
         } else {
             // masked: the group's valid row count comes from the device array
-            const uint32_t rows = min((uint32_t)max(__ldg(p.grouped_layout + cur_group), 0), p.m);
+            const uint32_t rows = min((uint32_t)max((int32_t)ld_global_u32(p.grouped_layout + cur_group), 0), p.m);
             cur_row0 = 0;
             cur_rows = rows;
             cur_blocks = (rows + kBlockM * kCtaGroup - 1) / (kBlockM * kCtaGroup);
