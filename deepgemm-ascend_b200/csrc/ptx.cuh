@@ -94,6 +94,12 @@ __device__ __forceinline__ uint32_t ld_global_u32(const void* p) {
     asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
     return v;
 }
+// The same from L2, whatever L1 holds.
+__device__ __forceinline__ uint32_t ld_relaxed_u32(const void* p) {
+    uint32_t v;
+    asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
 __device__ __forceinline__ uint16_t ld_global_u16(const void* p) {
     uint16_t v;
     asm volatile("ld.global.u16 %0, [%1];" : "=h"(v) : "l"(p));

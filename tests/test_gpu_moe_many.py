@@ -139,3 +139,37 @@ def test_any_number_of_experts_over_a_cluster():
         for max_m in (None, 50):
             plan, ref = deep_gemm.moe_sort(idx.cuda(), experts, max_m=max_m), oracle.moe_sort_ref(idx, experts, 256, max_m)
             assert all(torch.equal(a.cpu(), b) for a, b in zip(plan, ref)), (experts, max_m)
+
+
+def test_a_captured_run_of_many_tokens_on_other_choices():
+    """Replays write the same memory: what a kernel may find there before the one in front of it is done is the plan of the run before."""
+    tokens, topk, experts, h = 2300, 6, 40, 2048
+    gen = torch.Generator().manual_seed(4)
+    choices = lambda: torch.where(torch.rand(tokens, topk, generator=gen) < 0.7, torch.randint(0, experts, (tokens, topk), generator=gen), -1)  # noqa: E731
+    assert deep_gemm._lib.lib().dg_moe_dispatch_fp8_scratch_bytes(tokens, h) > 0
+    idx, x = choices().cuda(), torch.randn(tokens, h, device='cuda').bfloat16()
+
+    def way():
+        plan = deep_gemm.moe_sort(idx, experts)
+        q, sf = deep_gemm.moe_dispatch_to_fp8(x, plan)
+        y = deep_gemm.moe_dispatch(x, plan)
+        return (*plan, q.view(torch.uint8), sf, y, deep_gemm.moe_combine(y, plan))
+
+    way()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = way()
+    for seed in range(8):
+        idx.copy_(choices())
+        x.copy_(torch.randn(tokens, h))
+        graph.replay()
+        codes, sf = deep_gemm.cast_to_fp8(x)
+        choice = held[2].long()
+        live = choice >= 0
+        of = choice[live] // topk
+        for a, b in zip(held[:3], oracle.moe_sort_ref(idx.cpu(), experts)):
+            assert torch.equal(a.cpu(), b), seed
+        assert torch.equal(held[3][live], codes.view(torch.uint8)[of]) and torch.equal(held[4][live], sf[of]) and torch.equal(held[5][live], x[of]), seed
+        ref = x.double() * (idx >= 0).sum(1, keepdim=True)
+        size = ref.abs()
+        assert ((held[6].double() - ref).abs() <= (topk + 1) * E * size + HALF[torch.bfloat16] * (size + (topk + 1) * E * size)).all(), seed
