@@ -86,10 +86,7 @@ __device__ __forceinline__ void e2m1_to_bf16(uint32_t q, uint32_t (&w)[4]) {
         w[2 * h + 1] = __byte_perm(low, high, 0x7362);
     }
 }
-// A power of two from its exponent byte, as FP32 or BF16 bits: 2^-127 is a subnormal number, 255 is NaN.
-__device__ __forceinline__ float ue8m0_value(uint32_t e) {
-    return e == 0u ? __uint_as_float(0x00400000u) : e == 255u ? __uint_as_float(0x7fffffffu) : __uint_as_float(e << 23);
-}
+// A power of two from its exponent byte, as BF16 bits: 2^-127 is a subnormal number, 255 is NaN.
 __device__ __forceinline__ uint32_t ue8m0_bf16(uint32_t e) { return e == 0u ? 0x0040u : e == 255u ? 0x7fffu : e << 7; }
 // Two products of BF16 values. (One factor is a power of two here: exact but where the result is subnormal.)
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
