@@ -73,7 +73,8 @@ inline MoePlan moe_sort(const torch::Tensor& topk_idx, int64_t num_experts, int6
     const int64_t rows = slots ? num_experts * slots : (int64_t)dg_moe_num_rows((uint32_t)topk_idx.numel(), (uint32_t)num_experts, (uint32_t)expert_alignment);
     host_assert(rows <= INT32_MAX, "the layout has too many rows");
     const c10::cuda::CUDAGuard guard(topk_idx.device());
-    // one allocation for the three (about a microsecond of host time each); every part starts on 16 bytes
+    // one allocation for the three (about a microsecond of host time each; to torch they are no views, but keeping one keeps all); every part
+    // starts on 16 bytes
     const int64_t part[3] = {num_experts, topk_idx.numel(), rows};
     int64_t offset = 0;
     const auto buffer = empty_on({align_up(part[0], 4) + align_up(part[1], 4) + part[2]}, torch::kInt32, topk_idx);

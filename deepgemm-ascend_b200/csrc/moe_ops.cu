@@ -69,8 +69,8 @@ __device__ __forceinline__ uint32_t same_expert(uint32_t e, uint32_t bits) {
 // Every warp owns a run of choices and a row of counters of its own: it counts (in any order, a count does not depend on it), the counters
 // become offsets (over the warps of the CTA, the CTAs of the cluster, and the experts with their alignment), and it walks its run a
 // second time to hand out rows. Within 32 choices the order is that of the lanes. Runs that fit kBatch are read once; kBatch is 1 where 32 choices for each
-// of a CTA's warps are all (1024 choices: 3.5 us against 4.4 with 8). 131072 choices of 256 experts: 11.8 us with 16 CTAs, 19 with 8; 40 with
-// one load at a time and a match for the peers. What is left at that size is the second pass, 6 of the 11.8 us: some 150 instructions for 32 choices, half
+// of a CTA's warps are all (1024 choices: 3.5 us against 4.4 with 8). 131072 choices of 256 experts: 11.6 us with 16 CTAs, 19 with 8; 40 with
+// one load at a time and a match for the peers. What is left at that size is the second pass, 6 of the 11.6 us: some 150 instructions for 32 choices, half
 // of them the votes that find a choice's peers, and one store to a place of its own for every choice, which 16 SMs have to make. (Four clusters that
 // count all choices each and share the second pass: 12.4 us; all votes of a batch at once, unrolled: 14.2.)
 template <typename T, uint32_t kBatch>
@@ -160,7 +160,7 @@ __global__ void __launch_bounds__(kSortThreads) moe_sort_kernel(const SortArgs a
     }
     __syncthreads();
     const uint32_t bits = 32 - __clz(a.experts);
-    // (every warp takes the same turns, with no choices in those behind its last: 32768 choices 6.7 us, and 8.0 where each ended at its own)
+    // (every warp takes the same turns, with no choices in those behind its last: 32768 choices 6.5 us, and 8.0 where each ended at its own)
     for (uint32_t at = 0; at < a.segment; at += 32 * kBatch) {
         if (a.segment > 32 * kBatch) load_experts<T>(a, first + at + lane, last, expert);
         #pragma unroll
@@ -460,8 +460,8 @@ __device__ __forceinline__ void store_pieces(const CombineArgs& a, uint32_t toke
 
 // A warp takes 32 x turns pieces of 16 bytes of a token's result (turns is 1, or kCombineTurns where there are tokens enough): eight pieces of rows
 // are on their way at once, of eight rows or of fewer and more turns. 8192 tokens x 7168 of 8 rows each: 164 us, 6.4 TB/s; 16384 tokens of
-// which a rank has one row of eight: 186 us with one turn, 86 with four. Seven CTAs of 128 threads: with eight (64 registers) 167 and
-// 86 us, with five of 256 threads 171 and 97.
+// which a rank has one row of eight: 186 us with one turn, 86 with four. Seven CTAs of 128 threads, which leaves 72 registers, one too few (4 bytes
+// of a thread are in local memory): with eight (64 registers) 167 and 86 us, with five of 256 threads 171 and 97.
 constexpr uint32_t kCombineTurns = 4, kCombineThreads = 128;
 template <typename T>
 __global__ void __launch_bounds__(kCombineThreads, 7) moe_combine_kernel(const CombineArgs a) {

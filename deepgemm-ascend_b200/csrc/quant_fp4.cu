@@ -141,7 +141,9 @@ __global__ void __launch_bounds__(kFp4Threads) quant_fp4_kernel(const Fp4Args a)
 // that a row of the warp's tile is a whole 128-byte line of BF16 and the maximum down a column takes two shuffles. The codes go through
 // shared memory and out as lines of 128 bytes (written by the lanes as they are, a row of a warp's tile is one sector of 32 bytes, and
 // the number of stores bounds the kernel: 114 us against 110 for 8 x 4096 x 7168 BF16); its rows are 40 words apart, which keeps the four rows of a
-// store in banks of their own. That size now: 90 us, 6.6 TB/s, since whole tiles check no bounds and BF16 goes two at a time.
+// store in banks of their own. That size now: 90 us, 6.6 TB/s, since whole tiles check no bounds and BF16 goes two at a time. FP32 holds 64 words
+// of a tile in each lane, 96 registers, so two CTAs are on an SM where BF16 has five; with twice the bytes on their way in each that is enough: 8 x 4096 x 7168
+// 150 us, 7.1 TB/s (84 % of DRAM's cycles), 4096 x 7168 22.4 us, 2112 x 7168 13.3 (12.1 when K-major).
 constexpr uint32_t kFp4StageWords = 40;
 template <typename T>
 __global__ void __launch_bounds__(kFp4Threads) quant_fp4_mn_kernel(const Fp4Args a) {

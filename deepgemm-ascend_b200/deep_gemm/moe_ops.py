@@ -5,12 +5,18 @@
 
     layout        int32 [experts]      what the m-grouped GEMMs take as `grouped_layout` (psum layout) or `masked_m` (with `max_m`)
     token_rows    int32 [tokens, k]    the row of every choice; -1 where it has none (an expert outside [0, experts), such as the -1
-                                       of another rank's, or one that has more than `max_m` choices in front of it)
+                                       of another rank's, or one that has `max_m` choices in front of it already)
     row_choices   int32 [rows], or [experts, max_m]   the choice t * k + j that a row holds, -1 where it holds none
 
 The other functions take the plan as it is. `rows` is the most that any choices can need (the number that they do need is known on the
 device only); rows that hold no choice are neither read nor written, except for the zeros that `zero_padding` asks for. The order
 inside an expert is that of the choices: nothing depends on timing. All tensors are on one device, whose current stream is used.
+
+Experts are counted from 0: a rank that holds those from `first` on sorts `topk_idx - first`. With `max_m` nothing but the -1 in `token_rows` of a
+choice for one of the experts here says that it was dropped; `layout` ends at `max_m`. The plan's tensors may share one allocation (they do in the
+compiled host layer), so keeping one may keep all three. Groups start on multiples of 256 rows, which is the default of everything here and of `cast_to_fp4`;
+`cast_to_fp8` and `swiglu_apply_weight_to_fp8` have the reference's 128 and want expert_alignment=256 for such a layout (with 128 every row with a choice
+is right, but rows of the padding are read and written too).
 
     plan = moe_sort(topk_idx, experts)
     a = moe_dispatch_to_fp8(x, plan)
@@ -188,7 +194,7 @@ def moe_combine_grad(grad_out: torch.Tensor, rows: torch.Tensor, plan, topk_weig
                      zero_padding: bool = False, expert_alignment: int = MK_ALIGNMENT):
     """Gradients of `moe_combine(rows, plan, topk_weights)` for grad_out [tokens, hidden]: (grad_rows like rows, grad_weights float32
     [tokens, k]). A choice without a row has the gradient 0. `zero_padding` as in `moe_dispatch`. `out`: where grad_rows goes; it may be
-    `rows` itself and must not overlap it otherwise."""
+    `rows` itself and must not overlap it otherwise, nor grad_out."""
     _check_tokens(grad_out, 'grad_out must be a row-major 2-D BF16 or FP32 tensor on a CUDA device')
     p = _Rows(plan, grad_out, grad_out.size(0))
     hidden = grad_out.size(1)

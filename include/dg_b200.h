@@ -325,7 +325,7 @@ int dg_dequant_fp4_launch(const void* codes, uint64_t code_stride, uint64_t code
  * choice a row holds, and must agree with token_rows. NULL works for any size, slower for many tokens.
  * dg_moe_combine_launch: out[t] = sum over j of topk_weights[t, j] (1 when NULL) x rows[token_rows[t, j]], summed in FP32.
  * dg_moe_combine_grad_launch: its gradients, grad_rows[token_rows[t, j]] = topk_weights[t, j] x grad_out[t] and grad_weights[t, j] =
- * <rows[token_rows[t, j]], grad_out[t]> (0 for a choice without a row); grad_rows may be `rows` itself. Strides in elements. */
+ * <rows[token_rows[t, j]], grad_out[t]> (0 for a choice without a row); grad_rows may be `rows` itself and overlaps nothing else. Strides in elements. */
 uint64_t dg_moe_num_rows(uint32_t choices, uint32_t num_experts, uint32_t alignment);
 int dg_moe_sort_launch(const void* topk_idx, int idx_is_int64, uint32_t tokens, uint32_t topk, uint32_t num_experts, uint32_t alignment,
                        uint32_t max_m, int32_t* layout, int32_t* token_rows, int32_t* row_choices, uint64_t num_rows, void* stream);
