@@ -61,6 +61,60 @@ inline void check_weights(const torch::Tensor& w, const MoeRows& plan) {
                 "topk_weights must be a contiguous float32 tensor with one weight per choice, on the device of the rows");
 }
 
+inline void check_router(const torch::Tensor& logits, int64_t topk, const std::string& scoring) {
+    host_assert(logits.is_cuda() && logits.dim() == 2 && bf16_or_fp32(logits) && (logits.stride(1) == 1 || logits.size(1) == 1),
+                "logits must be a row-major 2-D BF16 or FP32 tensor on a CUDA device");
+    host_assert(scoring == "softmax" || scoring == "sigmoid", "scoring must be 'softmax' or 'sigmoid'");
+    const int64_t experts = logits.size(1);
+    host_assert(experts > 0 && experts <= 1024, "the number of experts must be between 1 and 1024");
+    host_assert(topk > 0 && topk <= std::min<int64_t>(32, experts), "topk must be between 1 and 32, and at most the number of experts");
+    host_assert(logits.size(0) <= INT32_MAX, "there are too many tokens");
+}
+
+inline TensorPair moe_route(const torch::Tensor& logits, int64_t topk, const std::string& scoring, const std::optional<torch::Tensor>& bias, int64_t num_groups,
+                            int64_t topk_groups, int64_t group_best, bool renormalize, double scale) {
+    check_router(logits, topk, scoring);
+    const int64_t tokens = logits.size(0), experts = logits.size(1);
+    if (bias.has_value())
+        host_assert(bias->scalar_type() == torch::kFloat32 && bias->is_contiguous() && bias->dim() == 1 && bias->size(0) == experts && bias->device() == logits.device(),
+                    "bias must be a contiguous float32 vector with one value per expert, on the device of logits");
+    host_assert(num_groups > 0 && num_groups <= 32 && experts % num_groups == 0, "num_groups must be between 1 and 32 and divide the number of experts");
+    host_assert(topk_groups > 0 && topk_groups <= num_groups, "topk_groups must be between 1 and num_groups");
+    host_assert(group_best == 1 || group_best == 2, "group_best must be 1 or 2");
+    host_assert(topk <= experts / num_groups * topk_groups, "the groups that are taken hold fewer experts than topk");
+    const c10::cuda::CUDAGuard guard(logits.device());
+    auto idx = empty_on({tokens, topk}, torch::kInt32, logits), weights = empty_on({tokens, topk}, torch::kFloat32, logits);
+    if (tokens != 0)
+        check(dg_moe_route_launch(logits.data_ptr(), logits.scalar_type() == torch::kFloat32, (uint64_t)stride_of_rows(logits), (uint32_t)tokens, (uint32_t)experts,
+                                  (uint32_t)topk, scoring == "sigmoid", bias.has_value() ? static_cast<const float*>(bias->data_ptr()) : nullptr, (uint32_t)num_groups,
+                                  (uint32_t)topk_groups, (uint32_t)group_best, renormalize, (float)scale, static_cast<int32_t*>(idx.data_ptr()),
+                                  static_cast<float*>(weights.data_ptr()), stream_of(logits)));
+    return {idx, weights};
+}
+
+inline torch::Tensor moe_route_grad(const torch::Tensor& grad_weights, const torch::Tensor& logits, const torch::Tensor& topk_idx, const std::string& scoring,
+                                    bool renormalize, double scale, const std::optional<torch::Tensor>& out_in) {
+    host_assert(topk_idx.dim() == 2 && (topk_idx.scalar_type() == torch::kInt32 || topk_idx.scalar_type() == torch::kInt64) && topk_idx.is_contiguous() &&
+                topk_idx.device() == logits.device() && topk_idx.size(0) == logits.size(0),
+                "topk_idx must be a contiguous int32 or int64 [tokens, topk] tensor on the device of logits");
+    check_router(logits, topk_idx.size(1), scoring);
+    host_assert(grad_weights.scalar_type() == torch::kFloat32 && grad_weights.is_contiguous() && grad_weights.device() == logits.device() &&
+                grad_weights.sizes() == topk_idx.sizes(), "grad_weights must be a contiguous float32 tensor with one value per choice, on the device of logits");
+    const int64_t tokens = logits.size(0), experts = logits.size(1);
+    const c10::cuda::CUDAGuard guard(logits.device());
+    if (out_in.has_value())
+        host_assert(out_in->scalar_type() == logits.scalar_type() && out_in->device() == logits.device() && out_in->sizes() == logits.sizes() &&
+                    (out_in->stride(1) == 1 || experts == 1) && stride_of_rows(out_in.value()) >= experts,
+                    "out must be row-major, of the type, the shape and the device of logits");
+    const auto out = out_in.has_value() ? out_in.value() : empty_on({tokens, experts}, logits.scalar_type(), logits);
+    if (tokens != 0)
+        check(dg_moe_route_grad_launch(static_cast<const float*>(grad_weights.data_ptr()), logits.data_ptr(), logits.scalar_type() == torch::kFloat32,
+                                       (uint64_t)stride_of_rows(logits), (uint32_t)tokens, (uint32_t)experts, topk_idx.data_ptr(),
+                                       topk_idx.scalar_type() == torch::kInt64, (uint32_t)topk_idx.size(1), scoring == "sigmoid", renormalize, (float)scale,
+                                       out.data_ptr(), (uint64_t)stride_of_rows(out), stream_of(logits)));
+    return out;
+}
+
 inline MoePlan moe_sort(const torch::Tensor& topk_idx, int64_t num_experts, int64_t expert_alignment, const std::optional<int64_t>& max_m) {
     host_assert(topk_idx.is_cuda() && topk_idx.dim() == 2 && topk_idx.is_contiguous() &&
                 (topk_idx.scalar_type() == torch::kInt64 || topk_idx.scalar_type() == torch::kInt32),
@@ -186,6 +240,10 @@ inline TensorPair moe_combine_grad(const torch::Tensor& grad_out, const torch::T
 }
 
 inline void register_moe_apis(py::module_& m) {
+    m.def("moe_route", &moe_route, py::arg("logits"), py::arg("topk"), py::arg("scoring") = "softmax", py::arg("bias") = std::nullopt, py::arg("num_groups") = 1,
+          py::arg("topk_groups") = 1, py::arg("group_best") = 2, py::arg("renormalize") = false, py::arg("scale") = 1.0);
+    m.def("moe_route_grad", &moe_route_grad, py::arg("grad_weights"), py::arg("logits"), py::arg("topk_idx"), py::arg("scoring") = "softmax",
+          py::arg("renormalize") = false, py::arg("scale") = 1.0, py::arg("out") = std::nullopt);
     m.def("moe_sort", &moe_sort, py::arg("topk_idx"), py::arg("num_experts"), py::arg("expert_alignment") = kMkAlignment, py::arg("max_m") = std::nullopt);
     m.def("moe_dispatch", &moe_dispatch, py::arg("x"), py::arg("plan"), py::arg("out") = std::nullopt, py::arg("zero_padding") = false,
           py::arg("expert_alignment") = kMkAlignment);

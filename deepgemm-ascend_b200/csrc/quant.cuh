@@ -29,10 +29,11 @@ __device__ __forceinline__ GroupEnd group_end_of(const int32_t* psum, uint32_t n
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
-// ---- E4M3: scale = max(amax, 1e-4) * (1/448) rounded up to a power of two; exponent byte from the bit pattern
-__device__ __forceinline__ uint32_t e4m3_scale_byte(float amax) {
-    const uint32_t bits = __float_as_uint(fmaxf(amax, 1e-4f) * (1.0f / 448.0f));
-    return ((bits - 1u) >> 23) + 1u;
+// ---- E4M3: scale = max(amax, floor) * (1/448) rounded up to a power of two, 2^-126 or more; exponent byte from the bit pattern (255 = NaN
+// for an infinity)
+__device__ __forceinline__ uint32_t e4m3_scale_byte(float amax, float floor = 1e-4f) {
+    const uint32_t bits = __float_as_uint(fmaxf(amax, floor) * (1.0f / 448.0f));
+    return max((bits + 0x7fffffu) >> 23, 1u);
 }
 // Eight values times the inverse of a scale of exponent byte `e`, rounded to E4M3.
 __device__ __forceinline__ uint2 e4m3_pack8(const float (&v)[8], uint32_t e) {
@@ -46,6 +47,19 @@ __device__ __forceinline__ uint2 e4m3_pack8(const float (&v)[8], uint32_t e) {
     }
     return make_uint2(q[0], q[1]);
 }
+
+// Four E4M3 codes as FP32, exactly.
+__device__ __forceinline__ void e4m3_unpack4(uint32_t q, float (&v)[4]) {
+    #pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(q >> (16 * h)), __NV_E4M3);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&r));
+        v[2 * h] = f.x;
+        v[2 * h + 1] = f.y;
+    }
+}
+// A power of two from its exponent byte (0: 2^-127, a subnormal number; 255: NaN).
+__device__ __forceinline__ float ue8m0_float(uint32_t e) { return __uint_as_float(e == 0u ? 0x00400000u : e == 255u ? 0x7fc00000u : e << 23); }
 
 // ---- E2M1: scale = the smallest power of two s with amax <= 6 s, from the bits of amax without a product that could round:
 // 6 s = 1.5 x 2^(e + 2), so the exponent goes up by one where the mantissa is above 1.5. There is no floor under amax (small

@@ -1,0 +1,253 @@
+// E4M3 operands whose contraction runs down the rows (both sides of a weight gradient, the weights of a gradient of the activations), made from BF16 or
+// from E4M3 rows with scales along them (what a forward pass has kept in 8 bits), and the way back to BF16 or FP32.
+//
+// Mathematics: over 32 rows of a column, scale = 2^ceil(log2(max(amax, floor) / 448)) as in quant.cuh, codes = x / scale rounded to E4M3. x is exact
+// in FP32 in either form (four significant bits times a power of two), so the rounding to E4M3 is the only one. A block that holds an
+// infinity or a NaN gets the scale byte of NaN.
+//
+// HBM-bound: 2 (or 1 + 1/32) bytes read and 1 + 1/32 written per value.
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/dg_b200.h"
+#include "host_common.h"
+#include "ptx.cuh"
+#include "quant.cuh"
+
+namespace dg {
+
+constexpr uint32_t kMnThreads = 256, kMnCols = 256, kMnRows = 64;
+
+struct MnArgs {
+    const uint8_t* x; uint64_t x_stride, x_group_stride;                  // bytes: BF16, or E4M3 with scales along the rows
+    const uint8_t* x_sf; uint64_t x_sf_stride, x_sf_group_stride;         // int16 [ceil(cols / 64)][rows] seen as bytes
+    uint8_t* out; uint64_t out_stride, out_group_stride;                  // bytes
+    uint8_t* sf; uint64_t sf_stride, sf_group_stride;                     // int16 [ceil(rows / 64)][cols] seen as bytes
+    const int32_t* psum; uint32_t num_experts, alignment;
+    uint32_t rows, cols, tiles_c;
+    float floor;
+};
+
+// One CTA = 64 rows x 256 columns, a warp 32 rows x 64 columns: lane = (every fourth row, eight columns), so that the maximum down a column takes
+// two shuffles, and a row of the warp's tile is a line of 128 bytes of BF16 or two whole sectors of codes. The 64 columns are one column of the
+// scales of an 8-bit input, whose 32 rows are one read of 64 bytes.
+template <bool kFromFp8>
+__global__ void __launch_bounds__(kMnThreads) quant_fp8_mn_kernel(const MnArgs a) {
+    __shared__ __align__(8) uint8_t sf_smem[2][kMnCols];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint64_t group = blockIdx.z;
+    const uint32_t row_base = blockIdx.x / a.tiles_c * kMnRows, c0 = blockIdx.x % a.tiles_c * kMnCols;
+    const uint32_t half = warp / 4, tc = warp % 4 * 64 + lane % 8 * 8, c = c0 + tc;
+    const uint32_t warp_row = row_base + half * 32, r0 = warp_row + lane / 8;
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint32_t write_end = min(a.rows, row_base + kMnRows);
+    uint32_t row_end = write_end;
+    if (a.psum != nullptr) {
+        // (groups start on multiples of 64 rows: a tile lies in one) Rows of the padding count as zeros and are written as zeros
+        const GroupEnd end = group_end_of(a.psum, a.num_experts, a.alignment, row_base, lane);
+        if (end.whole <= row_base) return;                // behind the last group (uniform over the CTA)
+        row_end = min(row_end, end.valid);
+    }
+    float v[8][8];
+    const uint8_t* x = a.x + group * a.x_group_stride + (uint64_t)r0 * a.x_stride + (uint64_t)c * (kFromFp8 ? 1 : 2);
+    if constexpr (kFromFp8) {
+        uint32_t pair = 0;
+        if (c0 + warp % 4 * 64 < a.cols && warp_row + lane < row_end)
+            pair = ld_global_u16(a.x_sf + group * a.x_sf_group_stride + (uint64_t)((c0 + warp % 4 * 64) / 64) * a.x_sf_stride + (uint64_t)(warp_row + lane) * 2);
+        uint2 q[8];
+        #pragma unroll
+        for (uint32_t i = 0; i < 8; ++i, x += 4 * a.x_stride) {
+            q[i] = make_uint2(0u, 0u);
+            if (r0 + i * 4 < row_end && c < a.cols) q[i] = ld_stream_v2(x);
+        }
+        #pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t e = __shfl_sync(0xffffffffu, pair, i * 4 + lane / 8) >> (lane % 8 / 4 * 8) & 0xffu;
+            // (a row that does not count has no scale either)
+            const float scale = ue8m0_float(r0 + i * 4 < row_end ? e : 127u);
+            float lo[4], hi[4];
+            e4m3_unpack4(q[i].x, lo);
+            e4m3_unpack4(q[i].y, hi);
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) { v[i][j] = lo[j] * scale; v[i][4 + j] = hi[j] * scale; }
+        }
+    } else {
+        uint4 q[8];
+        #pragma unroll
+        for (uint32_t i = 0; i < 8; ++i, x += 4 * a.x_stride) {
+            q[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (r0 + i * 4 < row_end && c < a.cols) q[i] = ld_stream_v4(x);
+        }
+        #pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) { v[i][2 * j] = bf16_lo(w[j]); v[i][2 * j + 1] = bf16_hi(w[j]); }
+        }
+    }
+    // (as whole numbers: infinities and NaN come out on top)
+    uint32_t m[8] = {}, e[8];
+    #pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) m[j] = max(m[j], __float_as_uint(v[i][j]) & 0x7fffffffu);
+    uint32_t bytes[2] = {};
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
+        m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+        e[j] = m[j] >= 0x7f800000u ? 255u : e4m3_scale_byte(__uint_as_float(m[j]), a.floor);
+        bytes[j / 4] |= e[j] << (j % 4 * 8);
+    }
+    // (blocks behind the last row are zero)
+    if (lane < 8) *reinterpret_cast<uint2*>(&sf_smem[half][tc]) = warp_row < a.rows ? make_uint2(bytes[0], bytes[1]) : make_uint2(0u, 0u);
+    uint8_t* out = a.out + group * a.out_group_stride + (uint64_t)r0 * a.out_stride + c;
+    #pragma unroll
+    for (uint32_t i = 0; i < 8; ++i, out += 4 * a.out_stride) {
+        float s[8];
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = v[i][j] * __uint_as_float((254u - min(e[j], 254u)) << 23);
+        if (r0 + i * 4 < write_end && c < a.cols) *reinterpret_cast<uint2*>(out) = e4m3_pack8(s, 127u);
+    }
+    __syncthreads();
+    if (c0 + threadIdx.x < a.cols)
+        *reinterpret_cast<uint16_t*>(a.sf + group * a.sf_group_stride + (uint64_t)(row_base / 64) * a.sf_stride + (uint64_t)(c0 + threadIdx.x) * 2) =
+            (uint16_t)(sf_smem[0][threadIdx.x] | ((uint32_t)sf_smem[1][threadIdx.x] << 8));
+}
+
+// The way back: code x 2^(byte - 127), rounded once to BF16 or FP32 (which changes nothing but where those have subnormals). One CTA = 32 rows x 256
+// columns, a warp four rows, a lane eight columns. The scales of K-major rows come in runs down the rows, through shared memory; those of an MN-major
+// tile lie along the columns.
+template <typename T, bool kMnMajor>
+__global__ void __launch_bounds__(kMnThreads) dequant_fp8_kernel(const MnArgs a) {
+    constexpr uint32_t kWarpRows = 4, kTileRows = 32;
+    __shared__ __align__(8) uint8_t sf_smem[kTileRows][kMnCols / 32];
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint64_t group = blockIdx.z;
+    const uint32_t row_base = blockIdx.x / a.tiles_c * kTileRows, c0 = blockIdx.x % a.tiles_c * kMnCols;
+    const uint32_t c = c0 + lane * 8, r0 = row_base + warp * kWarpRows;
+    griddep_wait();
+    griddep_launch_dependents();
+    const uint8_t* x = a.x + group * a.x_group_stride + (uint64_t)r0 * a.x_stride + c;
+    uint2 q[kWarpRows];
+    #pragma unroll
+    for (uint32_t i = 0; i < kWarpRows; ++i, x += a.x_stride) {
+        q[i] = make_uint2(0u, 0u);
+        if (r0 + i < a.rows && c < a.cols) q[i] = ld_stream_v2(x);
+    }
+    const uint8_t* sf = a.x_sf + group * a.x_sf_group_stride;
+    float scale[8] = {};
+    if constexpr (kMnMajor) {
+        if (c < a.cols) {
+            #pragma unroll
+            for (int j = 0; j < 8; ++j)
+                scale[j] = ue8m0_float(ld_global_u16(sf + (uint64_t)(r0 / 64) * a.x_sf_stride + (uint64_t)(c + j) * 2) >> (r0 / 32 % 2 * 8) & 0xffu);
+        }
+    } else {
+        const uint32_t col = threadIdx.x / kTileRows, r = threadIdx.x % kTileRows;
+        if (col < kMnCols / 64 && c0 + col * 64 < a.cols && row_base + r < a.rows)
+            *reinterpret_cast<uint16_t*>(&sf_smem[r][col * 2]) = ld_global_u16(sf + (uint64_t)(c0 / 64 + col) * a.x_sf_stride + (uint64_t)(row_base + r) * 2);
+        __syncthreads();
+    }
+    uint8_t* out = a.out + group * a.out_group_stride + (uint64_t)r0 * a.out_stride + (uint64_t)c * sizeof(T);
+    #pragma unroll
+    for (uint32_t i = 0; i < kWarpRows; ++i, out += a.out_stride) {
+        if (r0 + i >= a.rows || c >= a.cols) continue;
+        if constexpr (!kMnMajor) {
+            const float s = ue8m0_float(sf_smem[warp * kWarpRows + i][lane / 4]);
+            #pragma unroll
+            for (int j = 0; j < 8; ++j) scale[j] = s;
+        }
+        float v[8];
+        #pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float four[4];
+            e4m3_unpack4(h ? q[i].y : q[i].x, four);
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) v[4 * h + j] = four[j] * scale[4 * h + j];
+        }
+        if constexpr (sizeof(T) == 2) {
+            uint32_t w[4];
+            #pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+                w[j] = *reinterpret_cast<const uint32_t*>(&p);
+            }
+            *reinterpret_cast<uint4*>(out) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else {
+            // (one store of 32 bytes: as two, each leaves half of every sector to the other)
+            asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(out), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]),
+                         "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]) : "memory");
+        }
+    }
+}
+
+}  // namespace dg
+
+using namespace dg;
+
+static int mn_checks(uint32_t rows, uint32_t cols, const void* x, const void* x_sf, bool needs_sf, const void* out, const void* sf, bool makes_sf) {
+    DG_CHECK_ARG(x != nullptr && out != nullptr && (!needs_sf || x_sf != nullptr) && (!makes_sf || sf != nullptr), "fp8: null pointer");
+    DG_CHECK_ARG(cols % 32 == 0, "fp8: the row length must be a multiple of 32");
+    DG_CHECK_ARG(rows <= 0x7fffffffu && cols <= 0x7fffffffu, "fp8: too many values");
+    return DG_OK;
+}
+
+// One launch for as many matrices as a grid holds.
+static int launch_mn(const void* fn, MnArgs a, uint32_t tile_rows, uint32_t groups, void* stream) {
+    constexpr uint32_t kMostGroups = 65535;
+    a.tiles_c = (a.cols + kMnCols - 1) / kMnCols;
+    const uint64_t tiles = (uint64_t)((a.rows + tile_rows - 1) / tile_rows) * a.tiles_c;
+    DG_CHECK_ARG(tiles <= 0x7fffffffull, "fp8: too many values");
+    void* params[] = {&a};
+    for (uint32_t g = 0; g < groups; g += kMostGroups) {
+        const dim3 grid((uint32_t)tiles, 1, groups - g < kMostGroups ? groups - g : kMostGroups);
+        if (int rc = launch_overlapped(fn, grid, dim3(kMnThreads), params, static_cast<cudaStream_t>(stream))) return rc;
+        a.x += kMostGroups * a.x_group_stride; a.x_sf += kMostGroups * a.x_sf_group_stride;
+        a.out += kMostGroups * a.out_group_stride; a.sf += kMostGroups * a.sf_group_stride;
+    }
+    return DG_OK;
+}
+
+extern "C" int dg_quant_fp8_mn_launch(const void* x, uint64_t x_stride, uint64_t x_group_stride, const int16_t* x_sf, uint64_t x_sf_stride, uint64_t x_sf_group_stride,
+                                      uint32_t groups, uint32_t rows, uint32_t cols, const int32_t* psum, uint32_t num_experts, uint32_t alignment, float min_amax,
+                                      void* out, uint64_t out_stride, uint64_t out_group_stride, int16_t* sf, uint64_t sf_stride, uint64_t sf_group_stride, void* stream) {
+    if (groups == 0 || rows == 0 || cols == 0) return DG_OK;
+    const bool from_fp8 = x_sf != nullptr;
+    const uint64_t es = from_fp8 ? 1 : 2;
+    if (int rc = mn_checks(rows, cols, x, x_sf, false, out, sf, true)) return rc;
+    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(x) | x_stride * es | x_group_stride * es) % (from_fp8 ? 8 : 16) == 0, "fp8: input rows must start on %d-byte boundaries", from_fp8 ? 8 : 16);
+    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(out) | out_stride | out_group_stride) % 8 == 0, "fp8: output rows must start on 8-byte boundaries");
+    DG_CHECK_ARG(sf_stride >= cols && (!from_fp8 || x_sf_stride >= rows), "fp8: scale stride smaller than the columns (rows of a K-major input)");
+    DG_CHECK_ARG(psum == nullptr || (groups == 1 && num_experts > 0 && alignment > 0 && alignment % 64 == 0),
+                 "fp8: a psum layout needs one matrix, experts, and an alignment that is a multiple of 64");
+    DG_CHECK_ARG(min_amax >= 0.0f && min_amax <= 3.0e38f, "fp8: min_amax must be a finite number that is not negative");
+    MnArgs a{};
+    a.x = static_cast<const uint8_t*>(x); a.x_stride = x_stride * es; a.x_group_stride = x_group_stride * es;
+    a.x_sf = reinterpret_cast<const uint8_t*>(x_sf); a.x_sf_stride = x_sf_stride * 2; a.x_sf_group_stride = x_sf_group_stride * 2;
+    a.out = static_cast<uint8_t*>(out); a.out_stride = out_stride; a.out_group_stride = out_group_stride;
+    a.sf = reinterpret_cast<uint8_t*>(sf); a.sf_stride = sf_stride * 2; a.sf_group_stride = sf_group_stride * 2;
+    a.psum = psum; a.num_experts = psum ? num_experts : 0; a.alignment = alignment;
+    a.rows = rows; a.cols = cols; a.floor = min_amax;
+    return launch_mn(from_fp8 ? (const void*)quant_fp8_mn_kernel<true> : (const void*)quant_fp8_mn_kernel<false>, a, kMnRows, groups, stream);
+}
+
+extern "C" int dg_dequant_fp8_launch(const void* codes, uint64_t code_stride, uint64_t code_group_stride, const int16_t* sf, uint64_t sf_stride, uint64_t sf_group_stride,
+                                     uint32_t groups, uint32_t rows, uint32_t cols, int mn_major, void* out, int out_is_fp32, uint64_t out_stride,
+                                     uint64_t out_group_stride, void* stream) {
+    if (groups == 0 || rows == 0 || cols == 0) return DG_OK;
+    const uint64_t es = out_is_fp32 ? 4 : 2;
+    if (int rc = mn_checks(rows, cols, codes, sf, true, out, nullptr, false)) return rc;
+    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(codes) | code_stride | code_group_stride) % 8 == 0, "fp8: rows of codes must start on 8-byte boundaries");
+    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(out) | out_stride * es | out_group_stride * es) % (8 * es) == 0, "fp8: output rows must start on %d-byte boundaries", (int)(8 * es));
+    DG_CHECK_ARG(sf_stride >= (mn_major ? cols : rows), "fp8: scale stride smaller than the rows (columns when MN-major)");
+    MnArgs a{};
+    a.x = static_cast<const uint8_t*>(codes); a.x_stride = code_stride; a.x_group_stride = code_group_stride;
+    a.x_sf = reinterpret_cast<const uint8_t*>(sf); a.x_sf_stride = sf_stride * 2; a.x_sf_group_stride = sf_group_stride * 2;
+    a.out = static_cast<uint8_t*>(out); a.out_stride = out_stride * es; a.out_group_stride = out_group_stride * es;
+    a.rows = rows; a.cols = cols;
+    const void* fn = mn_major ? (out_is_fp32 ? (const void*)dequant_fp8_kernel<float, true> : (const void*)dequant_fp8_kernel<__nv_bfloat16, true>)
+                              : (out_is_fp32 ? (const void*)dequant_fp8_kernel<float, false> : (const void*)dequant_fp8_kernel<__nv_bfloat16, false>);
+    return launch_mn(fn, a, 32, groups, stream);
+}

@@ -9,7 +9,8 @@
 // inverse scale rounded to E4M3 (:250-252), packed scales transposed per group of 32 tokens (:104-125), tokens in
 // the padding of a psum layout skipped (:263-268).
 //
-// HBM-bound: 4 H bytes read and H + H/32 bytes written per token (2 H + H + H/32 without SwiGLU).
+// HBM-bound: 4 H bytes read and H + H/32 bytes written per token (2 H + H + H/32 without SwiGLU). With a checkpoint the input itself is written in 8 bits
+// too, as the plain cast would write it: 2 H + H/16 bytes instead of the 6 H that a cast of its own would move.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -32,17 +33,35 @@ struct QuantArgs {
     const float* weights;                               // [tokens] or nullptr
     const int32_t* psum; uint32_t num_experts, alignment;
     uint32_t tokens, hidden;
-    float clamp; uint32_t has_clamp, swiglu;
+    float clamp, floor; uint32_t has_clamp;
+    uint8_t* kept; uint64_t kept_stride;                // [tokens, 2 * hidden] E4M3
+    uint8_t* kept_sf; uint64_t kept_sf_col_stride;      // int16 [hidden/32][kept_sf_col_stride] seen as bytes
 };
+
+// The eight BF16 values of a lane in the plain cast's 8 bits; answers the exponent byte of the block, which four lanes share.
+__device__ __forceinline__ uint32_t cast_piece(const uint4& q, float floor, uint2& codes) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    float v[8], amax = 0.f;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) { v[j * 2] = bf16_lo(w[j]); v[j * 2 + 1] = bf16_hi(w[j]); }
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[j]));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t e = e4m3_scale_byte(amax, floor);
+    codes = e4m3_pack8(v, e);
+    return e;
+}
 
 // One CTA = 32 tokens x 256 channels. A warp takes four tokens and issues the loads of all of them (4 or 8 x 16 bytes per
 // lane) before it uses the first. Cutting the channels as well as the tokens is what gives a decoding step its parallelism:
 // a CTA that ran through the whole row left 64 tokens x 7168 channels to two CTAs. Bound by HBM for many tokens, by one
 // round trip to memory and the launch for few. Measured back to back: 64 x 7168 25.8 -> 1.7 us, 4096 x 7168 31 -> 12.6 us
 // (7.1 TB/s), 68495 x 7168 237 -> 214 us (6.9 TB/s); SwiGLU 4096 x 2048 15.0 -> 7.9 us, 68495 x 2048 118 -> 106 us.
-template <bool kSwiglu>
+template <bool kSwiglu, bool kKeep>
 __global__ void __launch_bounds__(kQuantThreads) quant_fp8_kernel(const QuantArgs a) {
     __shared__ __align__(8) uint8_t sf_smem[kTokenGroup][kTileChannels / 32];
+    __shared__ __align__(8) uint8_t kept_smem[kKeep ? 2 : 1][kKeep ? kTokenGroup : 1][kTileChannels / 32];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t tiles_c = (a.hidden + kTileChannels - 1) / kTileChannels;
     const uint32_t tg = blockIdx.x / tiles_c, c0 = (blockIdx.x - tg * tiles_c) * kTileChannels;
@@ -100,9 +119,22 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp8_kernel(const QuantArg
         for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[j]));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const uint32_t e = e4m3_scale_byte(amax);
+        const uint32_t e = e4m3_scale_byte(amax, a.floor);
         if (t0 + i < valid_end && c < a.hidden)
             *reinterpret_cast<uint2*>(a.out + (uint64_t)(t0 + i) * a.out_stride + c) = e4m3_pack8(v, e);
+        if constexpr (kKeep) {
+            uint2 codes[2];
+            const uint32_t el = cast_piece(left[i], a.floor, codes[0]), er = cast_piece(right[i], a.floor, codes[1]);
+            if (t0 + i < valid_end && c < a.hidden) {
+                uint8_t* row = a.kept + (uint64_t)(t0 + i) * a.kept_stride + c;
+                *reinterpret_cast<uint2*>(row) = codes[0];
+                *reinterpret_cast<uint2*>(row + a.hidden) = codes[1];
+            }
+            if ((lane & 3u) == 0) {
+                kept_smem[0][warp * kWarpTokens + i][lane / 4] = (uint8_t)el;
+                kept_smem[1][warp * kWarpTokens + i][lane / 4] = (uint8_t)er;
+            }
+        }
         // (the second block of a last, half-used scale column is zero)
         if ((lane & 3u) == 0) sf_smem[warp * kWarpTokens + i][lane / 4] = c < a.hidden ? (uint8_t)e : (uint8_t)0;
     }
@@ -112,6 +144,13 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp8_kernel(const QuantArg
     if (col < kTileChannels / 64 && c0 + col * 64 < a.hidden && tl < valid_end - token_base) {
         const uint16_t pair = *reinterpret_cast<const uint16_t*>(&sf_smem[tl][col * 2]);
         *reinterpret_cast<uint16_t*>(a.out_sf + ((uint64_t)(c0 / 64 + col) * a.sf_col_stride + token_base + tl) * 2) = pair;
+        if constexpr (kKeep) {
+            // (hidden is a multiple of 64: no column holds blocks of both halves)
+            #pragma unroll
+            for (uint32_t half = 0; half < 2; ++half)
+                *reinterpret_cast<uint16_t*>(a.kept_sf + ((uint64_t)((half * a.hidden + c0) / 64 + col) * a.kept_sf_col_stride + token_base + tl) * 2) =
+                    *reinterpret_cast<const uint16_t*>(&kept_smem[half][tl][col * 2]);
+        }
     }
 }
 
@@ -119,32 +158,63 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp8_kernel(const QuantArg
 
 using namespace dg;
 
-extern "C" int dg_quant_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t hidden, int swiglu,
-                                   const float* topk_weights, const int32_t* psum, uint32_t num_experts, uint32_t alignment,
-                                   int has_clamp, float clamp_value, void* out, uint64_t out_stride,
-                                   int16_t* out_sf, uint64_t sf_col_stride, void* stream) {
-    DG_CHECK_ARG(x != nullptr && out != nullptr && out_sf != nullptr, "quant_fp8: null pointer");
-    DG_CHECK_ARG(hidden > 0 && hidden % 32 == 0, "quant_fp8: hidden must be a multiple of 32");
-    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(x) & 15) == 0 && x_stride % 8 == 0,
+static int launch_quant_fp8(QuantArgs a, const void* fn, void* stream) {
+    DG_CHECK_ARG(a.x != nullptr && a.out != nullptr && a.out_sf != nullptr, "quant_fp8: null pointer");
+    DG_CHECK_ARG(a.hidden > 0 && a.hidden % 32 == 0, "quant_fp8: hidden must be a multiple of 32");
+    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.x_stride % 8 == 0,
                  "quant_fp8: input rows must start on 16-byte boundaries");
-    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(out) & 7) == 0 && out_stride % 8 == 0,
+    DG_CHECK_ARG((reinterpret_cast<uintptr_t>(a.out) & 7) == 0 && a.out_stride % 8 == 0,
                  "quant_fp8: output rows must start on 8-byte boundaries");
-    DG_CHECK_ARG(!swiglu || hidden % 8 == 0, "quant_fp8: hidden must be a multiple of 8");
-    DG_CHECK_ARG(sf_col_stride >= tokens, "quant_fp8: scale column stride smaller than the token count");
-    DG_CHECK_ARG(psum == nullptr || (num_experts > 0 && alignment > 0 && alignment % kTokenGroup == 0),
+    DG_CHECK_ARG(a.sf_col_stride >= a.tokens, "quant_fp8: scale column stride smaller than the token count");
+    DG_CHECK_ARG(a.psum == nullptr || (a.num_experts > 0 && a.alignment > 0 && a.alignment % kTokenGroup == 0),
                  "quant_fp8: a psum layout needs experts and an alignment that is a multiple of 32");
-    if (tokens == 0) return DG_OK;
+    if (a.tokens == 0) return DG_OK;
+    if (a.psum == nullptr) a.num_experts = 0;
+    const uint64_t tiles = (uint64_t)((a.tokens + kTokenGroup - 1) / kTokenGroup) * ((a.hidden + kTileChannels - 1) / kTileChannels);
+    DG_CHECK_ARG(tiles <= 0x7fffffffull, "quant_fp8: too many tokens");
+    void* params[] = {&a};
+    return launch_overlapped(fn, dim3((uint32_t)tiles), dim3(kQuantThreads), params, static_cast<cudaStream_t>(stream));
+}
+
+static QuantArgs quant_args(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t hidden, const float* topk_weights, const int32_t* psum, uint32_t num_experts,
+                            uint32_t alignment, int has_clamp, float clamp_value, float floor, void* out, uint64_t out_stride, int16_t* out_sf, uint64_t sf_col_stride) {
     QuantArgs a{};
     a.x = static_cast<const __nv_bfloat16*>(x); a.x_stride = x_stride;
     a.out = static_cast<uint8_t*>(out); a.out_stride = out_stride;
     a.out_sf = reinterpret_cast<uint8_t*>(out_sf); a.sf_col_stride = sf_col_stride;
-    a.weights = topk_weights; a.psum = psum; a.num_experts = psum ? num_experts : 0; a.alignment = alignment;
+    a.weights = topk_weights; a.psum = psum; a.num_experts = num_experts; a.alignment = alignment;
     a.tokens = tokens; a.hidden = hidden;
-    a.clamp = clamp_value; a.has_clamp = has_clamp ? 1u : 0u; a.swiglu = swiglu ? 1u : 0u;
-    const uint64_t tiles = (uint64_t)((tokens + kTokenGroup - 1) / kTokenGroup) * ((hidden + kTileChannels - 1) / kTileChannels);
-    DG_CHECK_ARG(tiles <= 0x7fffffffull, "quant_fp8: too many tokens");
-    const void* fn = swiglu ? (const void*)quant_fp8_kernel<true> : (const void*)quant_fp8_kernel<false>;
-    void* params[] = {&a};
-    if (int rc = launch_overlapped(fn, dim3((uint32_t)tiles), dim3(kQuantThreads), params, static_cast<cudaStream_t>(stream))) return rc;
-    return DG_OK;
+    a.clamp = clamp_value; a.has_clamp = has_clamp ? 1u : 0u; a.floor = floor;
+    return a;
+}
+
+extern "C" int dg_quant_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t hidden, int swiglu,
+                                   const float* topk_weights, const int32_t* psum, uint32_t num_experts, uint32_t alignment,
+                                   int has_clamp, float clamp_value, void* out, uint64_t out_stride,
+                                   int16_t* out_sf, uint64_t sf_col_stride, void* stream) {
+    const QuantArgs a = quant_args(x, x_stride, tokens, hidden, topk_weights, psum, num_experts, alignment, has_clamp, clamp_value, 1e-4f, out, out_stride, out_sf, sf_col_stride);
+    return launch_quant_fp8(a, swiglu ? (const void*)quant_fp8_kernel<true, false> : (const void*)quant_fp8_kernel<false, false>, stream);
+}
+
+extern "C" int dg_cast_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t hidden, const int32_t* psum, uint32_t num_experts, uint32_t alignment,
+                                  float min_amax, void* out, uint64_t out_stride, int16_t* out_sf, uint64_t sf_col_stride, void* stream) {
+    DG_CHECK_ARG(min_amax >= 0.0f && min_amax <= 3.0e38f, "cast_fp8: min_amax must be a finite number that is not negative");
+    const QuantArgs a = quant_args(x, x_stride, tokens, hidden, nullptr, psum, num_experts, alignment, 0, 0.0f, min_amax, out, out_stride, out_sf, sf_col_stride);
+    return launch_quant_fp8(a, (const void*)quant_fp8_kernel<false, false>, stream);
+}
+
+extern "C" int dg_swiglu_checkpoint_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t hidden, const float* topk_weights, const int32_t* psum,
+                                           uint32_t num_experts, uint32_t alignment, int has_clamp, float clamp_value, void* out, uint64_t out_stride,
+                                           int16_t* out_sf, uint64_t sf_col_stride, void* kept, uint64_t kept_stride, int16_t* kept_sf, uint64_t kept_sf_col_stride,
+                                           void* stream) {
+    QuantArgs a = quant_args(x, x_stride, tokens, hidden, topk_weights, psum, num_experts, alignment, has_clamp, clamp_value, 1e-4f, out, out_stride, out_sf, sf_col_stride);
+    if (tokens != 0) {
+        DG_CHECK_ARG(kept != nullptr && kept_sf != nullptr, "swiglu_checkpoint: null pointer");
+        DG_CHECK_ARG(hidden % 64 == 0, "swiglu_checkpoint: hidden must be a multiple of 64");
+        DG_CHECK_ARG((reinterpret_cast<uintptr_t>(kept) | kept_stride) % 8 == 0, "swiglu_checkpoint: rows of the checkpoint must start on 8-byte boundaries");
+        DG_CHECK_ARG(kept_sf_col_stride >= tokens, "swiglu_checkpoint: scale column stride smaller than the token count");
+    }
+    a.kept = static_cast<uint8_t*>(kept); a.kept_stride = kept_stride;
+    a.kept_sf = reinterpret_cast<uint8_t*>(kept_sf); a.kept_sf_col_stride = kept_sf_col_stride;
+    return launch_quant_fp8(a, (const void*)quant_fp8_kernel<true, true>, stream);
 }

@@ -46,8 +46,26 @@ for _name in _HOT_PATH_NAMES:
 del _name
 
 from . import epilogue, moe_ops, quant_ops, testing  # noqa: E402,F401
-from .quant_ops import cast_from_fp4, cast_to_fp4, cast_to_fp8, swiglu_apply_weight_to_fp8  # noqa: F401
-from .moe_ops import moe_combine, moe_combine_grad, moe_dispatch, moe_dispatch_to_fp8, moe_sort  # noqa: F401
+from .quant_ops import (  # noqa: F401
+    cast_from_fp4,
+    cast_from_fp8,
+    cast_to_fp4,
+    cast_to_fp8,
+    rms_norm_grad,
+    rms_norm_to_fp8,
+    swiglu_apply_weight_grad,
+    swiglu_apply_weight_to_fp8,
+    swiglu_apply_weight_to_fp8_with_checkpoint,
+)
+from .moe_ops import (  # noqa: F401
+    moe_combine,
+    moe_combine_grad,
+    moe_dispatch,
+    moe_dispatch_to_fp8,
+    moe_route,
+    moe_route_grad,
+    moe_sort,
+)
 from .locality_domain import (  # noqa: F401
     destroy_localizer,
     get_num_locality_domains,

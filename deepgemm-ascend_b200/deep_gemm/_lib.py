@@ -93,6 +93,33 @@ _PROTOTYPES = {
     'dg_dequant_fp4_launch': (C.c_int, [
         C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
         C.c_void_p, C.c_int, C.c_uint64, C.c_uint64, C.c_void_p]),
+    'dg_cast_fp8_launch': (C.c_int, [
+        C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32, C.c_uint32, C.c_float, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]),
+    'dg_swiglu_checkpoint_launch': (C.c_int, [
+        C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_int, C.c_float, C.c_void_p, C.c_uint64,
+        C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]),
+    'dg_swiglu_grad_launch': (C.c_int, [
+        C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32,
+        C.c_uint32, C.c_int, C.c_float, C.c_void_p, C.c_uint64, C.c_void_p, C.c_int, C.c_void_p]),
+    'dg_quant_fp8_mn_launch': (C.c_int, [
+        C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32,
+        C.c_uint32, C.c_float, C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p]),
+    'dg_dequant_fp8_launch': (C.c_int, [
+        C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int, C.c_void_p, C.c_int,
+        C.c_uint64, C.c_uint64, C.c_void_p]),
+    'dg_rms_norm_fp8_launch': (C.c_int, [
+        C.c_void_p, C.c_int, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_int, C.c_float, C.c_uint32, C.c_uint32,
+        C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p]),
+    'dg_rms_norm_grad_scratch_bytes': (C.c_uint64, [C.c_uint32, C.c_uint32]),
+    'dg_rms_norm_grad_launch': (C.c_int, [
+        C.c_void_p, C.c_int, C.c_uint64, C.c_void_p, C.c_int, C.c_uint64, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint32,
+        C.c_uint32, C.c_void_p, C.c_uint64, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),
+    'dg_moe_route_launch': (C.c_int, [
+        C.c_void_p, C.c_int, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int, C.c_void_p, C.c_uint32, C.c_uint32, C.c_uint32, C.c_int,
+        C.c_float, C.c_void_p, C.c_void_p, C.c_void_p]),
+    'dg_moe_route_grad_launch': (C.c_int, [
+        C.c_void_p, C.c_void_p, C.c_int, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_int, C.c_uint32, C.c_int, C.c_int, C.c_float, C.c_void_p,
+        C.c_uint64, C.c_void_p]),
     'dg_moe_num_rows': (C.c_uint64, [C.c_uint32, C.c_uint32, C.c_uint32]),
     'dg_moe_sort_launch': (C.c_int, [
         C.c_void_p, C.c_int, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64, C.c_void_p]),

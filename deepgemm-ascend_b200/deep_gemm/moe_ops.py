@@ -1,4 +1,4 @@
-"""From the router's choices to the rows of a grouped layout and back: the steps in front of and behind the m-grouped GEMMs.
+"""From a router's scores to the rows of a grouped layout and back: the steps in front of and behind the m-grouped GEMMs.
 
 `moe_sort` orders the choices of a batch (the result of a top-k over the router's scores) by expert and answers a plan,
 `(layout, token_rows, row_choices)`:
@@ -18,10 +18,13 @@ compiled host layer), so keeping one may keep all three. Groups start on multipl
 `cast_to_fp8` and `swiglu_apply_weight_to_fp8` have the reference's 128 and want expert_alignment=256 for such a layout (with 128 every row with a choice
 is right, but rows of the padding are read and written too).
 
+    topk_idx, topk_weights = moe_route(logits, topk, 'sigmoid', bias=bias, num_groups=8, topk_groups=4, renormalize=True)
     plan = moe_sort(topk_idx, experts)
     a = moe_dispatch_to_fp8(x, plan)
     m_grouped_fp8_gemm_nt_contiguous(a, w, y, plan[0], recipe=(1, 1, 32))
     out = moe_combine(y, plan, topk_weights)
+
+`moe_route` makes the choices from the router's logits, and `moe_route_grad` leads the gradient of their weights back to those.
 
 Gradients: of `moe_combine` with weights, `moe_combine_grad`; without weights, `moe_dispatch`; of `moe_dispatch`, `moe_combine` without
 weights. None of these has a counterpart in the reference, whose fused MoE does both steps inside its kernel.
@@ -91,6 +94,73 @@ def _check_alignment(expert_alignment):
 def _check_weights(w, plan):
     _host_assert(w.dtype == torch.float32 and w.is_contiguous() and w.device == plan.token_rows.device and w.shape == plan.token_rows.shape,
                  'topk_weights must be a contiguous float32 tensor with one weight per choice, on the device of the rows')
+
+
+def _check_router(logits, topk, scoring):
+    _host_assert(logits.is_cuda and logits.dim() == 2 and _is_float(logits) and (logits.stride(1) == 1 or logits.size(1) == 1),
+                 'logits must be a row-major 2-D BF16 or FP32 tensor on a CUDA device')
+    _host_assert(scoring in ('softmax', 'sigmoid'), "scoring must be 'softmax' or 'sigmoid'")
+    experts = logits.size(1)
+    _host_assert(0 < experts <= 1024, 'the number of experts must be between 1 and 1024')
+    _host_assert(0 < topk <= min(32, experts), 'topk must be between 1 and 32, and at most the number of experts')
+    _host_assert(logits.size(0) <= _INT_MAX, 'there are too many tokens')
+
+
+def moe_route(logits: torch.Tensor, topk: int, scoring: str = 'softmax', bias: Optional[torch.Tensor] = None, num_groups: int = 1, topk_groups: int = 1,
+              group_best: int = 2, renormalize: bool = False, scale: float = 1.0):
+    """logits [tokens, experts] BF16 or FP32 -> (topk_idx int32 [tokens, topk], topk_weights float32 [tokens, topk]), the largest choice first:
+
+        s = softmax(logits) or sigmoid(logits)           what the weights are made of
+        c = s + bias                                     what chooses (bias float32 [experts]; None: 0)
+
+    With groups (num_groups of the same number of neighbouring experts) the score of a group is the sum of its `group_best` (1 or 2) largest c, and
+    only the experts of the `topk_groups` best groups can be chosen. The weights are s of the chosen, divided by their sum (1e-20 or more)
+    with `renormalize`, times `scale`. c is compared in 64 bits, ties go to the lowest index (the lowest group), NaN counts as the largest, as in torch.topk.
+    An expert whose logit or bias is -inf is never chosen; where fewer than topk are left, -1 with the weight 0 takes their place: `moe_sort`
+    gives it no row, so a padded token is one whose logits are all -inf. At most 1024 experts, 32 groups, 32 choices."""
+    _check_router(logits, topk, scoring)
+    tokens, experts = logits.shape
+    if bias is not None:
+        _host_assert(bias.dtype == torch.float32 and bias.is_contiguous() and tuple(bias.shape) == (experts,) and bias.device == logits.device,
+                     'bias must be a contiguous float32 vector with one value per expert, on the device of logits')
+    _host_assert(0 < num_groups <= 32 and experts % num_groups == 0, 'num_groups must be between 1 and 32 and divide the number of experts')
+    _host_assert(0 < topk_groups <= num_groups, 'topk_groups must be between 1 and num_groups')
+    _host_assert(group_best in (1, 2), 'group_best must be 1 or 2')
+    _host_assert(topk <= experts // num_groups * topk_groups, 'the groups that are taken hold fewer experts than topk')
+    with torch.cuda.device(logits.device):
+        idx = torch.empty((tokens, topk), dtype=torch.int32, device=logits.device)
+        weights = torch.empty((tokens, topk), dtype=torch.float32, device=logits.device)
+        if tokens:
+            L.check(L.lib().dg_moe_route_launch(
+                logits.data_ptr(), int(logits.dtype == torch.float32), _row_stride(logits), tokens, experts, topk, int(scoring == 'sigmoid'),
+                bias.data_ptr() if bias is not None else None, num_groups, topk_groups, group_best, int(renormalize), float(scale),
+                idx.data_ptr(), weights.data_ptr(), _stream_ptr(logits.device)))
+    return idx, weights
+
+
+def moe_route_grad(grad_weights: torch.Tensor, logits: torch.Tensor, topk_idx: torch.Tensor, scoring: str = 'softmax', renormalize: bool = False,
+                   scale: float = 1.0, out: Optional[torch.Tensor] = None):
+    """The gradient of the weights of `moe_route` with respect to the logits, for grad_weights float32 [tokens, topk] and the choices topk_idx (int32 or
+    int64): grad_logits like logits. The choice itself has no gradient (nor have bias and groups); a choice of -1 counts for nothing, whatever its
+    grad_weights; equal choices add up. `out`: where grad_logits goes; it may be `logits` itself."""
+    _host_assert(topk_idx.dim() == 2 and topk_idx.dtype in (torch.int32, torch.int64) and topk_idx.is_contiguous() and topk_idx.device == logits.device and
+                 topk_idx.size(0) == logits.size(0), 'topk_idx must be a contiguous int32 or int64 [tokens, topk] tensor on the device of logits')
+    _check_router(logits, topk_idx.size(1), scoring)
+    _host_assert(grad_weights.dtype == torch.float32 and grad_weights.is_contiguous() and grad_weights.device == logits.device and grad_weights.shape == topk_idx.shape,
+                 'grad_weights must be a contiguous float32 tensor with one value per choice, on the device of logits')
+    tokens, experts = logits.shape
+    with torch.cuda.device(logits.device):
+        if out is not None:
+            _host_assert(out.dtype == logits.dtype and out.device == logits.device and out.shape == logits.shape and (out.stride(1) == 1 or experts == 1) and
+                         _row_stride(out) >= experts, 'out must be row-major, of the type, the shape and the device of logits')
+        else:
+            out = torch.empty((tokens, experts), dtype=logits.dtype, device=logits.device)
+        if tokens:
+            L.check(L.lib().dg_moe_route_grad_launch(
+                grad_weights.data_ptr(), logits.data_ptr(), int(logits.dtype == torch.float32), _row_stride(logits), tokens, experts, topk_idx.data_ptr(),
+                int(topk_idx.dtype == torch.int64), topk_idx.size(1), int(scoring == 'sigmoid'), int(renormalize), float(scale), out.data_ptr(), _row_stride(out),
+                _stream_ptr(logits.device)))
+    return out
 
 
 def moe_sort(topk_idx: torch.Tensor, num_experts: int, expert_alignment: int = MK_ALIGNMENT, max_m: Optional[int] = None):
@@ -222,4 +292,5 @@ def moe_combine_grad(grad_out: torch.Tensor, rows: torch.Tensor, plan, topk_weig
 # The compiled host layer has the same functions (csrc/apis/moe.hpp).
 if _C is not None:
     moe_sort, moe_dispatch, moe_dispatch_to_fp8 = _C.moe_sort, _C.moe_dispatch, _C.moe_dispatch_to_fp8
+    moe_route, moe_route_grad = _C.moe_route, _C.moe_route_grad
     moe_combine, moe_combine_grad = _C.moe_combine, _C.moe_combine_grad

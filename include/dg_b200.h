@@ -287,6 +287,57 @@ int dg_quant_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint3
                         int has_clamp, float clamp_value, void* out, uint64_t out_stride,
                         int16_t* out_sf, uint64_t sf_col_stride, void* stream);
 
+/* The same without SwiGLU and with the least amax that a scale is made for: scale = 2^ceil(log2(max(amax, min_amax) / 448)), at least 2^-126
+ * (dg_quant_fp8_launch has the reference's 1e-4, which small gradients do not reach). */
+int dg_cast_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t hidden, const int32_t* psum, uint32_t num_experts,
+                       uint32_t alignment, float min_amax, void* out, uint64_t out_stride, int16_t* out_sf, uint64_t sf_col_stride, void* stream);
+
+/* dg_quant_fp8_launch with swiglu, and the input x [tokens, 2 * hidden] itself in 8 bits as the cast without it makes them: what the
+ * backward pass keeps. hidden % 64 == 0; rows of `kept` 8-byte aligned, its scales int16 [hidden / 32][kept_sf_col_stride]. */
+int dg_swiglu_checkpoint_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t hidden, const float* topk_weights,
+                                const int32_t* psum, uint32_t num_experts, uint32_t alignment, int has_clamp, float clamp_value,
+                                void* out, uint64_t out_stride, int16_t* out_sf, uint64_t sf_col_stride,
+                                void* kept, uint64_t kept_stride, int16_t* kept_sf, uint64_t kept_sf_col_stride, void* stream);
+
+/* Its gradient. grad_out BF16 [tokens, hidden]; x [tokens, 2 * hidden] BF16 (x_sf NULL), or E4M3 with the scales that
+ * dg_swiglu_checkpoint_launch writes; grad_x BF16 [tokens, 2 * hidden]; grad_weights float [tokens] or NULL (0 for rows without a value). Where the
+ * clamp cuts off, the gradient is 0. Rows of the psum layout's padding, and behind its last group, are not read; `zero_padding` writes zeros to
+ * the former. grad_x may not overlap anything else. hidden % 64 == 0; rows 16-byte aligned (8 for E4M3). */
+int dg_swiglu_grad_launch(const void* grad_out, uint64_t grad_stride, const void* x, uint64_t x_stride, const int16_t* x_sf,
+                          uint64_t x_sf_col_stride, uint32_t tokens, uint32_t hidden, const float* topk_weights, const int32_t* psum,
+                          uint32_t num_experts, uint32_t alignment, int has_clamp, float clamp_value, void* grad_x, uint64_t grad_x_stride,
+                          float* grad_weights, int zero_padding, void* stream);
+
+/* E4M3 operands whose contraction runs down the rows (MN-major), from BF16 (x_sf NULL) or from E4M3 rows with scales along them, x_sf int16
+ * [ceil(cols / 64)][x_sf_stride]. sf[g * sf_group_stride + r * sf_stride + col], r = K64 row, ceil(rows / 64) of them. Scales as in
+ * dg_cast_fp8_launch; a block that holds an infinity or a NaN gets the byte 255. `psum`: as in dg_quant_fp4_launch with mn_major. Strides of BF16 in
+ * elements, of codes in bytes, of scales in int16 elements. cols % 32 == 0; rows of BF16 16-byte aligned, of codes 8-byte aligned.
+ * dg_dequant_fp8_launch is the way back for either major: code x 2^(byte - 127) in BF16 or FP32 (rows aligned to eight values). */
+int dg_quant_fp8_mn_launch(const void* x, uint64_t x_stride, uint64_t x_group_stride, const int16_t* x_sf, uint64_t x_sf_stride,
+                           uint64_t x_sf_group_stride, uint32_t groups, uint32_t rows, uint32_t cols, const int32_t* psum, uint32_t num_experts,
+                           uint32_t alignment, float min_amax, void* out, uint64_t out_stride, uint64_t out_group_stride,
+                           int16_t* sf, uint64_t sf_stride, uint64_t sf_group_stride, void* stream);
+int dg_dequant_fp8_launch(const void* codes, uint64_t code_stride, uint64_t code_group_stride, const int16_t* sf, uint64_t sf_stride,
+                          uint64_t sf_group_stride, uint32_t groups, uint32_t rows, uint32_t cols, int mn_major,
+                          void* out, int out_is_fp32, uint64_t out_stride, uint64_t out_group_stride, void* stream);
+
+/* The norm in front of a block-scaled product; no reference counterpart. h = x + residual, rounded to their type (BF16 or FP32; without a
+ * residual h is x and is not written); rstd[t] = 1 / sqrt(mean(h^2) + eps), the sum in 64 bits; y = (h * rstd) * weight (BF16 or FP32) in FP32. out / out_sf: y as
+ * dg_quant_fp8_launch writes it; rows: y in BF16, or NULL. h may be x or residual itself. Strides in elements.
+ * dg_rms_norm_grad_launch: grad_x = rstd (u - n mean(u n)) + grad_h (NULL: 0), u = grad_out * weight, n = h * rstd, in the type of h; grad_weight float
+ * [hidden] = sum over the tokens of grad_out n. grad_out is BF16, or FP32 beside an FP32 h; grad_x may be grad_h, h or (of its type) grad_out itself.
+ * `scratch`: dg_rms_norm_grad_scratch_bytes of device memory that the call may use until it has run.
+ * hidden % 32 == 0, at most 32768; rows and the weight 16-byte aligned (out: 8). */
+int dg_rms_norm_fp8_launch(const void* x, int is_fp32, uint64_t x_stride, const void* residual, uint64_t residual_stride, void* h,
+                           uint64_t h_stride, const void* weight, int weight_is_fp32, float eps, uint32_t tokens, uint32_t hidden,
+                           void* out, uint64_t out_stride, int16_t* out_sf, uint64_t sf_col_stride, void* rows, uint64_t rows_stride,
+                           float* rstd, void* stream);
+uint64_t dg_rms_norm_grad_scratch_bytes(uint32_t tokens, uint32_t hidden);
+int dg_rms_norm_grad_launch(const void* grad_out, int grad_is_fp32, uint64_t grad_stride, const void* h, int is_fp32, uint64_t h_stride,
+                            const void* weight, int weight_is_fp32, const float* rstd, const void* grad_h, uint64_t grad_h_stride,
+                            uint32_t tokens, uint32_t hidden, void* grad_x, uint64_t grad_x_stride, float* grad_weight,
+                            void* scratch, uint64_t scratch_bytes, void* stream);
+
 /* BF16 or FP32 values <-> packed E2M1 (two codes per byte along the row, low nibble first) plus UE8M0 scales, one per 32 values along
  * K, in the layout the GEMM reads. No reference counterpart (tests/generators.py:34-95 quantises on the host). `groups` matrices of
  * [rows, cols]; strides of values in elements, of codes in bytes, of scales in int16 elements. cols % 32 == 0; rows of values
@@ -304,6 +355,21 @@ int dg_quant_fp4_launch(const void* x, int x_is_fp32, uint64_t x_stride, uint64_
 int dg_dequant_fp4_launch(const void* codes, uint64_t code_stride, uint64_t code_group_stride, const int16_t* sf, uint64_t sf_stride,
                           uint64_t sf_group_stride, uint32_t groups, uint32_t rows, uint32_t cols, int mn_major,
                           void* out, int out_is_fp32, uint64_t out_stride, uint64_t out_group_stride, void* stream);
+
+/* A router's scores -> the experts of every token and their weights; no reference counterpart. logits [tokens, experts] FP32 or BF16, `stride`
+ * elements between rows. score s = 1 / (1 + e^-l) (sigmoid) or softmax(l); c = s + bias[e] (NULL: 0). With num_groups > 1 the experts lie in groups of
+ * experts / num_groups, whose scores are the sums of their group_best (1 or 2) largest c, and the topk_groups best groups stay. The topk largest c
+ * are chosen (compared in 64 bits; NaN is the largest; ties to the lowest index), the largest first; weights[t, j] = s, divided by max(1e-20, the
+ * sum of the token's) with `renormalize`, times `scale`. Logits and biases of -inf are never chosen: -1 with the weight 0 takes their place.
+ * At most 1024 experts, 32 groups, 32 choices.
+ * dg_moe_route_grad_launch: the gradient of the weights with respect to the logits for given choices (those outside [0, experts) count for nothing,
+ * equal ones add up), in the type of the logits. Bias and groups have no part in it. grad_logits may be the logits themselves. */
+int dg_moe_route_launch(const void* logits, int is_fp32, uint64_t stride, uint32_t tokens, uint32_t experts, uint32_t topk, int sigmoid,
+                        const float* bias, uint32_t num_groups, uint32_t topk_groups, uint32_t group_best, int renormalize, float scale,
+                        int32_t* topk_idx, float* topk_weights, void* stream);
+int dg_moe_route_grad_launch(const float* grad_weights, const void* logits, int is_fp32, uint64_t stride, uint32_t tokens, uint32_t experts,
+                             const void* topk_idx, int idx_is_int64, uint32_t topk, int sigmoid, int renormalize, float scale,
+                             void* grad_logits, uint64_t grad_stride, void* stream);
 
 /* From the router's choices to the rows of a grouped layout and back; no reference counterpart (its fused MoE does both inside).
  * Choice t * topk + j is the j-th expert of token t; experts outside [0, num_experts) (another rank's, -1) have no row.

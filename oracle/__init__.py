@@ -33,6 +33,15 @@ from .mxgemm import (  # noqa: F401
     quantize_e4m3,
     stochastic_round_bf16,
 )
+from .layers import (  # noqa: F401
+    cast_fp8_ref,
+    moe_route_grad_ref,
+    moe_route_ref,
+    pack_scales,
+    rms_norm_grad_ref,
+    rms_norm_ref,
+    swiglu_grad_ref,
+)
 from .moe import moe_combine_grad_ref, moe_combine_ref, moe_padding, moe_rows, moe_sort_ref  # noqa: F401
 from .quant import cast_fp4_ref, swiglu_quant_ref  # noqa: F401
 from .sf_layout import (  # noqa: F401

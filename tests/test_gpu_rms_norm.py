@@ -1,0 +1,238 @@
+"""The norm in front of a product and its gradient against 64 bits on the CPU (oracle/layers.py).
+
+Tolerances, e = 2^-24, u = half a step of the result's type (BF16 2^-8, FP32 e). Forward: h is one FP32 addition and one rounding, which torch does
+alike: the same bits. rstd is a number of 64 bits rounded once: within e (1 + 2^-20). y = (h rstd) weight in FP32, one rounding each: bit for bit what
+torch makes of the returned rstd, and its 8 bits are bit for bit those of the oracle's quantiser. Gradient: a mean over H terms passes every
+term through at most H / 32 + 80 additions whatever the split, and a term (g w) (h rstd) has three roundings; dx then takes five more. dweight passes a
+term (one product, one fused multiply-add) through at most tokens + 300 additions."""
+
+import pytest
+import torch
+
+import deep_gemm
+import oracle
+from both_hosts import python_layer, quant_hosts
+from helpers import seed_all
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float32: E}
+BF16, FP32 = torch.bfloat16, torch.float32
+
+
+def _check_forward(x, weight, residual=None, eps=1e-6, host=deep_gemm, **kw):
+    (q, sf), rows, h, rstd = host.rms_norm_to_fp8(x.cuda(), weight.cuda(), residual=None if residual is None else residual.cuda(), eps=eps, with_rows=True, **kw)
+    want_h = x if residual is None else (x.float() + residual.float()).to(x.dtype)
+    assert h.dtype == x.dtype and torch.equal(h.cpu(), want_h)
+    rstd = rstd.cpu()
+    want, _ = oracle.rms_norm_ref(want_h, weight, eps)
+    assert rstd.dtype == FP32 and ((rstd.double() - want).abs() <= E * (1 + 2.0 ** -20) * want).all()
+    y = want_h.float() * rstd[:, None] * weight.float()
+    assert rows.dtype == BF16 and torch.equal(rows.cpu(), y.bfloat16())
+    codes, byte, _ = oracle.cast_fp8_ref(y, 1)
+    assert q.dtype == torch.float8_e4m3fn and torch.equal(q.view(torch.uint8).cpu(), codes)
+    assert sf.dtype == torch.int16 and (sf.stride(0) == 1 or x.size(0) <= 1) and torch.equal(sf.cpu(), oracle.pack_scales(byte, 1))
+    return (q, sf), rows, h, rstd
+
+
+SHAPES = [(1, 32), (1, 7168), (2, 96), (3, 2048), (37, 1120), (5, 8192), (150, 288), (299, 4096), (3, 16384), (2, 32768), (301, 64)]
+
+
+@pytest.mark.parametrize('host', quant_hosts)
+@pytest.mark.parametrize('tokens,hidden', SHAPES)
+@pytest.mark.parametrize('dtype', [BF16, FP32])
+def test_forward(host, tokens, hidden, dtype):
+    seed_all(hidden)
+    x, residual = torch.randn(tokens, hidden).to(dtype), (torch.randn(tokens, hidden) * 3).to(dtype)
+    for weight in (torch.randn(hidden), (1 + 0.1 * torch.randn(hidden)).bfloat16()):
+        _check_forward(x, weight, None, host=host)
+        _check_forward(x, weight, residual, 1e-5, host)
+
+
+def test_small_large_and_empty_rows():
+    seed_all(1)
+    x = torch.randn(7, 512)
+    x[0] = 0
+    x[1] *= 1e-20
+    x[2] *= 1e18
+    x[3, 1:] = 0
+    _check_forward(x, torch.ones(512))
+    _check_forward(x.bfloat16(), torch.ones(512), eps=1e-12)
+    _check_forward(x, torch.zeros(512))
+    for host in quant_hosts:
+        (q, sf), rows, h, rstd = host.rms_norm_to_fp8(torch.zeros(0, 64, device='cuda'), torch.ones(64, device='cuda'), with_rows=True)
+        assert q.shape == (0, 64) and sf.shape == (0, 1) and rows.shape == h.shape == (0, 64) and rstd.shape == (0,)
+        (q, sf), rows, h, rstd = host.rms_norm_to_fp8(torch.ones(2, 64, device='cuda'), torch.ones(64, device='cuda'))
+        assert rows is None
+
+
+def test_rows_do_not_depend_on_their_number():
+    seed_all(2)
+    x, r, w = torch.randn(1000, 7168, device='cuda').bfloat16(), torch.randn(1000, 7168, device='cuda').bfloat16(), torch.randn(7168, device='cuda')
+    (q, sf), rows, h, rstd = deep_gemm.rms_norm_to_fp8(x, w, residual=r, with_rows=True)
+    for first, last in ((0, 1), (5, 8), (500, 700), (1, 1000)):
+        (q1, sf1), rows1, h1, rstd1 = deep_gemm.rms_norm_to_fp8(x[first:last], w, residual=r[first:last], with_rows=True)
+        assert torch.equal(q1.view(torch.uint8), q[first:last].view(torch.uint8)) and torch.equal(sf1, sf[first:last])
+        assert torch.equal(rows1, rows[first:last]) and torch.equal(h1, h[first:last]) and torch.equal(rstd1, rstd[first:last])
+
+
+def test_in_place_and_strides():
+    seed_all(3)
+    for dtype in (BF16, FP32):
+        for tokens in (3, 400):
+            wide = torch.randn(tokens, 3088, device='cuda').to(dtype)
+            x, r, w = wide[:, 8:1032], wide[:, 1040:2064], torch.randn(1024, device='cuda')
+            want = deep_gemm.rms_norm_to_fp8(x.contiguous(), w, residual=r.contiguous(), with_rows=True)
+            for target in ('new', 'residual', 'x'):
+                both = wide.clone()
+                x, r = both[:, 8:1032], both[:, 1040:2064]
+                out = {'new': both[:, 2064:], 'residual': r, 'x': x}[target]
+                got = deep_gemm.rms_norm_to_fp8(x, w, residual=r, with_rows=True, out_h=out)
+                assert got[2].data_ptr() == out.data_ptr() and torch.equal(got[2], want[2]) and torch.equal(got[1], want[1]) and torch.equal(got[3], want[3])
+                assert torch.equal(got[0][0].view(torch.uint8), want[0][0].view(torch.uint8)) and torch.equal(got[0][1], want[0][1])
+                assert torch.equal(both[:, :8], wide[:, :8])
+    one = torch.randn(1, 512, device='cuda')
+    got = deep_gemm.rms_norm_to_fp8(torch.randn(1, 512, device='cuda').expand(9, 512) * 0 + one, torch.ones(512, device='cuda'), residual=one.expand(9, 512))
+    assert torch.equal(got[2], (2 * one).expand(9, 512))
+
+
+def test_not_finite():
+    x = torch.randn(3, 256)
+    x[1, 40], x[2, 3] = float('nan'), float('inf')
+    (q, sf), rows, h, rstd = deep_gemm.rms_norm_to_fp8(x.cuda(), torch.ones(256, device='cuda'), with_rows=True)
+    _, alone, _, _ = deep_gemm.rms_norm_to_fp8(x[:1].cuda(), torch.ones(256, device='cuda'), with_rows=True)
+    assert torch.equal(rows[:1], alone) and rows[1].isnan().all() and rstd[2] == 0 and rows[2, 3].isnan() and (rows[2, 4:] == 0).all()
+
+
+# --------------------------------------------------------------------------------------------------------------- gradient
+def _check_grad(g, h, weight, rstd, grad_h=None, host=deep_gemm, **kw):
+    cuda = lambda t: None if t is None else t.cuda()  # noqa: E731
+    dx, dw = host.rms_norm_grad(cuda(g), cuda(h), cuda(weight), cuda(rstd), grad_h=cuda(grad_h), **kw)
+    tokens, hidden = h.shape
+    assert dx.dtype == h.dtype and dx.shape == h.shape and dw.dtype == FP32 and dw.shape == (hidden,)
+    ref = oracle.rms_norm_grad_ref(g, h, weight, rstd, grad_h)
+    r = rstd.double()[:, None]
+    mean_err = (hidden / 32 + 85) * E * ref['mean_size']
+    err = r * (3 * E * ref['u'] + ref['n'] * (mean_err + 4 * E * (ref['mean'] + mean_err))) + 4 * E * r * (ref['u'] + ref['n'] * ref['mean'])
+    err = err + E * (0 if grad_h is None else grad_h.double().abs())
+    err = err + HALF[h.dtype] * (ref['dx'].abs() + err) + 2.0 ** -140
+    assert ((dx.cpu().double() - ref['dx']).abs() <= err).all()
+    assert ((dw.cpu().double() - ref['dw']).abs() <= (tokens + 303) * E * ref['dw_size'] + 2.0 ** -140).all()
+    return dx, dw
+
+
+@pytest.mark.parametrize('host', quant_hosts)
+@pytest.mark.parametrize('tokens,hidden', SHAPES + [(700, 1024), (1531, 2048)])
+@pytest.mark.parametrize('dtype,grad_dtype', [(BF16, BF16), (FP32, BF16), (FP32, FP32)])
+def test_gradient(host, tokens, hidden, dtype, grad_dtype):
+    seed_all(tokens)
+    h, g, more = torch.randn(tokens, hidden).to(dtype), torch.randn(tokens, hidden).to(grad_dtype), torch.randn(tokens, hidden).to(dtype)
+    weight = torch.randn(hidden) if tokens % 2 else torch.randn(hidden).bfloat16()
+    rstd = oracle.rms_norm_ref(h, weight, 1e-6)[0].float()
+    first = _check_grad(g, h, weight, rstd, None, host)
+    again = host.rms_norm_grad(g.cuda(), h.cuda(), weight.cuda(), rstd.cuda())
+    assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+    _check_grad(g, h, weight, rstd, more, host)
+
+
+def test_gradient_in_place_and_strides():
+    seed_all(5)
+    for dtype in (BF16, FP32):
+        for tokens in (2, 600):
+            wide = torch.randn(tokens, 4096, device='cuda').to(dtype)
+            views = lambda t: (t[:, 8:1032], t[:, 1032:2056], t[:, 2064:3088])  # noqa: E731
+            g, h, more = views(wide)
+            w, rstd = torch.randn(1024, device='cuda'), torch.rand(tokens, device='cuda') + 0.5
+            want = deep_gemm.rms_norm_grad(g.contiguous(), h.contiguous(), w, rstd, grad_h=more.contiguous())
+            for target in range(3):
+                both = wide.clone()
+                g, h, more = views(both)
+                got = deep_gemm.rms_norm_grad(g, h, w, rstd, grad_h=more, out=(g, h, more)[target])
+                assert got[0].data_ptr() == (g, h, more)[target].data_ptr() and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+                assert torch.equal(both[:, 3088:], wide[:, 3088:]) and torch.equal(both[:, :8], wide[:, :8])
+
+
+def test_gradient_of_no_tokens():
+    for host in quant_hosts:
+        dx, dw = host.rms_norm_grad(torch.zeros(0, 64, device='cuda'), torch.zeros(0, 64, device='cuda'), torch.ones(64, device='cuda'), torch.zeros(0, device='cuda'))
+        assert dx.shape == (0, 64) and (dw == 0).all()
+
+
+def test_gradient_against_differences():
+    seed_all(6)
+    h, w, g, eps = torch.randn(3, 64, dtype=torch.float64), torch.randn(64, dtype=torch.float64), torch.randn(3, 64), 1e-3
+    rstd = oracle.rms_norm_ref(h, w, eps)[0].float()
+    dx, dw = deep_gemm.rms_norm_grad(g.cuda(), h.float().cuda(), w.float().cuda(), rstd.cuda())
+    loss = lambda h, w: float((oracle.rms_norm_ref(h, w, eps)[1] * g.double()).sum())  # noqa: E731
+    # (a central difference in 64 bits, 1e-9; inputs rounded to FP32 and the kernel's sums, 1e-5 of values around 1 to 10)
+    for t, c in ((0, 0), (1, 33), (2, 63)):
+        step = torch.zeros_like(h)
+        step[t, c] = 1e-5
+        assert abs((loss(h + step, w) - loss(h - step, w)) / 2e-5 - float(dx[t, c])) < 1e-4
+        assert abs((loss(h, w + step[t]) - loss(h, w - step[t])) / 2e-5 - float(dw[c])) < 1e-4
+
+
+def test_refusals():
+    x, w, r = torch.zeros(4, 64, device='cuda'), torch.ones(64, device='cuda'), torch.ones(4, device='cuda')
+    for host in quant_hosts:
+        for args, kw, match in (((x.half(), w), {}, 'x must be'), ((x.t(), w), {}, 'x must be'), ((x[:, :48], w[:48]), {}, 'multiple of 32'),
+                                ((torch.zeros(2, 32800, device='cuda'), torch.zeros(32800, device='cuda')), {}, 'at most 32768'),
+                                ((x, w[:32]), {}, 'weight must be'), ((x, w.half()), {}, 'weight must be'), ((x, w.cpu()), {}, 'weight must be'),
+                                ((x, w), dict(residual=x.bfloat16()), 'residual must be'), ((x, w), dict(residual=x[:3]), 'residual must be'),
+                                ((x, w), dict(residual=x, out_h=x[:3]), 'out_h must be'), ((x, w), dict(out_h=x), 'out_h needs'),
+                                ((x, w), dict(residual=x, out_h=x[:1].expand(4, 64)), 'out_h must be'),
+                                ((torch.zeros(4, 66, device='cuda')[:, 2:], w), {}, '16-byte')):
+            with pytest.raises(RuntimeError, match=match):
+                host.rms_norm_to_fp8(*args, **kw)
+        b = x.bfloat16()
+        for args, kw, match in (((x, b, w, r), {}, 'grad_out must be'), ((x[:3], x, w, r), {}, 'grad_out must be'), ((x, x, w, r[:3]), {}, 'rstd must be'),
+                                ((x, x, w, r.double()), {}, 'rstd must be'), ((x, x, w, r), dict(grad_h=b), 'grad_h must be'), ((x, x, w, r), dict(out=b), 'out must be'),
+                                ((x, x, w, r), dict(out=x[:1].expand(4, 64)), 'out must be'), ((x, x, w[:32], r), {}, 'weight must be')):
+            with pytest.raises(RuntimeError, match=match):
+                host.rms_norm_grad(*args, **kw)
+
+
+def test_rows_behind_32_bits():
+    tokens, hidden, stride = 70000, 32, 40960
+    base = torch.zeros(tokens * stride, dtype=BF16, device='cuda')
+    x = base.as_strided((tokens, hidden), (stride, 1))
+    x.copy_(torch.randn(tokens, hidden))
+    w = torch.randn(hidden, device='cuda')
+    (q, sf), _, h, rstd = deep_gemm.rms_norm_to_fp8(x, w)
+    (q2, sf2), _, _, rstd2 = deep_gemm.rms_norm_to_fp8(x.contiguous(), w)
+    assert torch.equal(q.view(torch.uint8), q2.view(torch.uint8)) and torch.equal(sf, sf2) and torch.equal(rstd, rstd2)
+    g = torch.randn(tokens, hidden, device='cuda').bfloat16()
+    a, b = deep_gemm.rms_norm_grad(g, x, w, rstd), deep_gemm.rms_norm_grad(g, x.contiguous(), w, rstd)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_two_streams_at_once_a_captured_run_and_both_hosts():
+    seed_all(8)
+    layer = python_layer('quant_ops')
+    sets = [tuple(torch.randn(500, 1024, device='cuda').bfloat16() for _ in range(3)) for _ in range(2)]
+    w = torch.randn(1024, device='cuda')
+
+    def way(s, host=deep_gemm):
+        (q, sf), rows, h, rstd = host.rms_norm_to_fp8(s[0], w, residual=s[1], with_rows=True)
+        return (q.view(torch.uint8), sf, rows, h, rstd, *host.rms_norm_grad(s[2], h, w, rstd, grad_h=s[1]))
+    want = [way(s) for s in sets]
+    assert all(torch.equal(a, b) for a, b in zip(want[0], way(sets[0], layer)))
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [None, None]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i] = way(sets[i])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = way(sets[0])
+    for t in sets[0]:
+        t.copy_(torch.randn_like(t))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(held, way(sets[0])))
