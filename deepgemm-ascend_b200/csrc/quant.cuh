@@ -29,6 +29,19 @@ __device__ __forceinline__ GroupEnd group_end_of(const int32_t* psum, uint32_t n
 __device__ __forceinline__ float bf16_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
+// 2^x and 1 / x within 2 ulp, subnormal results as zeros.
+__device__ __forceinline__ float fast_exp2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float fast_reciprocal(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+constexpr float kLog2E = 1.4426950408889634f;
+
 // ---- E4M3: scale = max(amax, floor) * (1/448) rounded up to a power of two, 2^-126 or more; exponent byte from the bit pattern (255 = NaN
 // for an infinity)
 __device__ __forceinline__ uint32_t e4m3_scale_byte(float amax, float floor = 1e-4f) {
