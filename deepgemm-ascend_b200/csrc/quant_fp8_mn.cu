@@ -28,11 +28,120 @@ struct MnArgs {
     float floor;
 };
 
+// Eight values in each of a lane's eight rows -> codes and scale bytes, through FP32.
+__device__ __forceinline__ void quantise_down(const float (&v)[8][8], float floor, uint32_t (&e)[8], uint2 (&codes)[8]) {
+    #pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        // (as whole numbers: infinities and NaN come out on top)
+        uint32_t m = 0;
+        #pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i][j]) & 0x7fffffffu);
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 8));
+        m = max(m, __shfl_xor_sync(0xffffffffu, m, 16));
+        e[j] = m >= 0x7f800000u ? 255u : e4m3_scale_byte(__uint_as_float(m), floor);
+    }
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float s[8];
+        #pragma unroll
+        for (int j = 0; j < 8; ++j) s[j] = v[i][j] * __uint_as_float((254u - min(e[j], 254u)) << 23);
+        codes[i] = e4m3_pack8(s, 127u);
+    }
+}
+
+// BF16 rows, two values at a time: magnitudes are compared as whole numbers, products with the inverse scales are exact.
+__device__ __forceinline__ void quantise_down_bf16(const uint4 (&q)[8], float floor, uint32_t (&e)[8], uint2 (&codes)[8]) {
+    uint32_t m[4] = {}, f[4];
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) m[j] = __vmaxu2(m[j], w[j] & 0x7fff7fffu);
+    }
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        m[j] = __vmaxu2(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
+        m[j] = __vmaxu2(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+        const float lo = bf16_lo(m[j]), hi = bf16_hi(m[j]);
+        e[2 * j] = (m[j] & 0xffffu) >= 0x7f80u ? 255u : e4m3_scale_byte(lo, floor);
+        e[2 * j + 1] = m[j] >= 0x7f800000u ? 255u : e4m3_scale_byte(hi, floor);
+        f[j] = (254u - min(e[2 * j], 254u)) << 7 | (254u - min(e[2 * j + 1], 254u)) << 23;
+    }
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+        float s[8];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t p = mul_bf16x2(w[j], f[j]);
+            s[2 * j] = bf16_lo(p);
+            s[2 * j + 1] = bf16_hi(p);
+        }
+        codes[i] = e4m3_pack8(s, 127u);
+    }
+}
+
+// E4M3 rows with scale bytes b (of this lane's block) through FP16, two values at a time, relative to the largest byte of the warp's rows: the codes are FP16
+// numbers and their factors powers of two. Exact while no factor is below 2^-15 and the columns' inverse scales lie in 2^-15 .. 2^15; answers whether
+// that is so (the same in all lanes), which it is where the magnitudes of a tile's rows and columns lie within a few thousand.
+__device__ __forceinline__ bool quantise_down_fp8(const uint2 (&q)[8], const uint32_t (&b)[8], float floor, uint32_t (&e)[8], uint2 (&codes)[8]) {
+    uint32_t top = 0, low = 255;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) { top = max(top, b[i]); low = min(low, b[i]); }
+    top = __reduce_max_sync(0xffffffffu, top);
+    low = __reduce_min_sync(0xffffffffu, low);
+    if (top == 255u || low == 0u || top - low > 15u) return false;
+    uint32_t h[8][4], m[4] = {}, f[4];
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        // 2^(b - top) in both halves (2^-15 is a subnormal number of FP16)
+        const uint32_t d = top - b[i], factor = (d == 15u ? 0x0200u : (15u - d) << 10) * 0x10001u;
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((j < 2 ? q[i].x : q[i].y) >> (16 * (j % 2))), __NV_E4M3);
+            const __half2 p = __hmul2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&factor));
+            h[i][j] = *reinterpret_cast<const uint32_t*>(&p);
+            m[j] = __vmaxu2(m[j], h[i][j] & 0x7fff7fffu);
+        }
+    }
+    bool fits = true;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        m[j] = __vmaxu2(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
+        m[j] = __vmaxu2(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+        const float2 largest = __half22float2(*reinterpret_cast<const __half2*>(&m[j]));
+        f[j] = 0;
+        #pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float v = k ? largest.y : largest.x;
+            e[2 * j + k] = e4m3_scale_byte(v * __uint_as_float(top << 23), floor);
+            // 2^(top - e); a column of zeros is one under any factor
+            const int32_t x = v == 0.0f ? 0 : (int32_t)top - (int32_t)e[2 * j + k];
+            fits &= x >= -15 && x <= 15 && v == v;
+            f[j] |= (x == -15 ? 0x0200u : (uint32_t)(15 + x) << 10) << (16 * k);
+        }
+    }
+    if (!__all_sync(0xffffffffu, fits)) return false;
+    #pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        uint32_t w[2];
+        #pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const __half2 lo = __hmul2(*reinterpret_cast<const __half2*>(&h[i][2 * k]), *reinterpret_cast<const __half2*>(&f[2 * k]));
+            const __half2 hi = __hmul2(*reinterpret_cast<const __half2*>(&h[i][2 * k + 1]), *reinterpret_cast<const __half2*>(&f[2 * k + 1]));
+            w[k] = (uint32_t)__nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(lo), __NV_SATFINITE, __NV_E4M3) |
+                   (uint32_t)__nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(hi), __NV_SATFINITE, __NV_E4M3) << 16;
+        }
+        codes[i] = make_uint2(w[0], w[1]);
+    }
+    return true;
+}
+
 // One CTA = 64 rows x 256 columns, a warp 32 rows x 64 columns: lane = (every fourth row, eight columns), so that the maximum down a column takes
 // two shuffles, and a row of the warp's tile is a line of 128 bytes of BF16 or two whole sectors of codes. The 64 columns are one column of the
 // scales of an 8-bit input, whose 32 rows are one read of 64 bytes.
 template <bool kFromFp8>
-__global__ void __launch_bounds__(kMnThreads) quant_fp8_mn_kernel(const MnArgs a) {
+__global__ void __launch_bounds__(kMnThreads, 3) quant_fp8_mn_kernel(const MnArgs a) {
     __shared__ __align__(8) uint8_t sf_smem[2][kMnCols];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint64_t group = blockIdx.z;
@@ -49,28 +158,39 @@ __global__ void __launch_bounds__(kMnThreads) quant_fp8_mn_kernel(const MnArgs a
         if (end.whole <= row_base) return;                // behind the last group (uniform over the CTA)
         row_end = min(row_end, end.valid);
     }
-    float v[8][8];
     const uint8_t* x = a.x + group * a.x_group_stride + (uint64_t)r0 * a.x_stride + (uint64_t)c * (kFromFp8 ? 1 : 2);
+    uint2 codes[8];
+    uint32_t e[8];
     if constexpr (kFromFp8) {
-        uint32_t pair = 0;
+        // (rows that do not count hold zeros and have no scale: one that does lends them its own)
+        uint32_t pair = 0x7f7fu;
         if (c0 + warp % 4 * 64 < a.cols && warp_row + lane < row_end)
             pair = ld_global_u16(a.x_sf + group * a.x_sf_group_stride + (uint64_t)((c0 + warp % 4 * 64) / 64) * a.x_sf_stride + (uint64_t)(warp_row + lane) * 2);
         uint2 q[8];
+        uint32_t b[8];
         #pragma unroll
         for (uint32_t i = 0; i < 8; ++i, x += 4 * a.x_stride) {
             q[i] = make_uint2(0u, 0u);
             if (r0 + i * 4 < row_end && c < a.cols) q[i] = ld_stream_v2(x);
         }
+        const uint32_t first = __shfl_sync(0xffffffffu, pair, 0);
+        if (warp_row + lane >= row_end) pair = first;
+        // (nor has the second half of a last, half-used column)
+        const uint32_t shift = c < a.cols ? lane % 8 / 4 * 8 : 0;
         #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-            const uint32_t e = __shfl_sync(0xffffffffu, pair, i * 4 + lane / 8) >> (lane % 8 / 4 * 8) & 0xffu;
-            // (a row that does not count has no scale either)
-            const float scale = ue8m0_float(r0 + i * 4 < row_end ? e : 127u);
-            float lo[4], hi[4];
-            e4m3_unpack4(q[i].x, lo);
-            e4m3_unpack4(q[i].y, hi);
+        for (uint32_t i = 0; i < 8; ++i) b[i] = __shfl_sync(0xffffffffu, pair, i * 4 + lane / 8) >> shift & 0xffu;
+        if (!quantise_down_fp8(q, b, a.floor, e, codes)) {
+            float v[8][8];
             #pragma unroll
-            for (int j = 0; j < 4; ++j) { v[i][j] = lo[j] * scale; v[i][4 + j] = hi[j] * scale; }
+            for (uint32_t i = 0; i < 8; ++i) {
+                const float scale = ue8m0_float(r0 + i * 4 < row_end ? b[i] : 127u);
+                float lo[4], hi[4];
+                e4m3_unpack4(q[i].x, lo);
+                e4m3_unpack4(q[i].y, hi);
+                #pragma unroll
+                for (int j = 0; j < 4; ++j) { v[i][j] = lo[j] * scale; v[i][4 + j] = hi[j] * scale; }
+            }
+            quantise_down(v, a.floor, e, codes);
         }
     } else {
         uint4 q[8];
@@ -79,37 +199,16 @@ __global__ void __launch_bounds__(kMnThreads) quant_fp8_mn_kernel(const MnArgs a
             q[i] = make_uint4(0u, 0u, 0u, 0u);
             if (r0 + i * 4 < row_end && c < a.cols) q[i] = ld_stream_v4(x);
         }
-        #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-            const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) { v[i][2 * j] = bf16_lo(w[j]); v[i][2 * j + 1] = bf16_hi(w[j]); }
-        }
-    }
-    // (as whole numbers: infinities and NaN come out on top)
-    uint32_t m[8] = {}, e[8];
-    #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i)
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) m[j] = max(m[j], __float_as_uint(v[i][j]) & 0x7fffffffu);
-    uint32_t bytes[2] = {};
-    #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
-        m[j] = max(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
-        e[j] = m[j] >= 0x7f800000u ? 255u : e4m3_scale_byte(__uint_as_float(m[j]), a.floor);
-        bytes[j / 4] |= e[j] << (j % 4 * 8);
+        quantise_down_bf16(q, a.floor, e, codes);
     }
     // (blocks behind the last row are zero)
-    if (lane < 8) *reinterpret_cast<uint2*>(&sf_smem[half][tc]) = warp_row < a.rows ? make_uint2(bytes[0], bytes[1]) : make_uint2(0u, 0u);
+    if (lane < 8)
+        *reinterpret_cast<uint2*>(&sf_smem[half][tc]) = warp_row < a.rows ? make_uint2(e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24, e[4] | e[5] << 8 | e[6] << 16 | e[7] << 24)
+                                                                          : make_uint2(0u, 0u);
     uint8_t* out = a.out + group * a.out_group_stride + (uint64_t)r0 * a.out_stride + c;
     #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i, out += 4 * a.out_stride) {
-        float s[8];
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = v[i][j] * __uint_as_float((254u - min(e[j], 254u)) << 23);
-        if (r0 + i * 4 < write_end && c < a.cols) *reinterpret_cast<uint2*>(out) = e4m3_pack8(s, 127u);
-    }
+    for (uint32_t i = 0; i < 8; ++i, out += 4 * a.out_stride)
+        if (r0 + i * 4 < write_end && c < a.cols) *reinterpret_cast<uint2*>(out) = codes[i];
     __syncthreads();
     if (c0 + threadIdx.x < a.cols)
         *reinterpret_cast<uint16_t*>(a.sf + group * a.sf_group_stride + (uint64_t)(row_base / 64) * a.sf_stride + (uint64_t)(c0 + threadIdx.x) * 2) =
