@@ -5,13 +5,13 @@
 // lowest index; the weights are s, divided by their sum where that is asked for, times `scale`. An expert whose logit or bias is
 // -inf is never chosen; where fewer than k are left the rest of the choices is -1 with the weight 0.
 //
-// Who is chosen is decided by c in 64 bits. FP32 scores come first: their error is bounded (score_error), and only where two of those that
-// decide lie closer together than that, the warp does the token again with 64-bit scores. Without a bias the scores' order is that of the
-// logits, which decide by themselves then.
+// Who is chosen is decided by c in 64 bits. A whole number that stands for c within a bound comes first (quick_choice): 21 to 23 bits of its distance from
+// the token's largest, above the expert's index, so that a choice is one maximum over the warp (redux) and a lane's next candidate one fused add-and-maximum
+// for each expert it holds. Only where two of those that decide lie closer together than the bound, the warp does the token again with 64-bit
+// scores (exact_choice). Without a bias the order of the scores is that of the logits, which stand for them then.
 //
 // One warp a token, nothing shared between warps. A group of experts lies in 32 / num_groups lanes (rounded down to a power of two), so that a
-// lane holds experts of one group only and a group that is not taken is dropped by its lanes. A choice is a maximum over the lanes and a
-// minimum over the places that hold it: one instruction each for a whole warp (redux).
+// lane holds experts of one group only and a group that is not taken is dropped by its lanes.
 #include <cuda_runtime.h>
 #include <math_constants.h>
 #include <stdint.h>
@@ -33,8 +33,9 @@ struct RouteArgs {
     void* idx; float* weights;                                // [tokens, topk]
     const float* grad_weights;
     uint8_t* grad_logits; uint64_t grad_stride;
-    uint32_t tokens, experts, topk, groups, group_size, topk_groups, lanes_log2;
+    uint32_t tokens, experts, topk, groups, group_size, topk_groups, lanes_log2, index_bits;
     uint32_t fp32, idx64, sigmoid, renormalize, best_two, by_logits;
+    uint32_t aligned;                                         // four neighbours can be read (and written) at once
     float scale;
 };
 
@@ -55,21 +56,33 @@ __device__ __forceinline__ float logit_at(const RouteArgs& a, const uint8_t* row
 }
 __device__ __forceinline__ float bias_at(const RouteArgs& a, uint32_t e) { return a.bias ? __uint_as_float(ld_global_u32(a.bias + e)) : 0.0f; }
 
-// The experts of a lane, and their logits (-inf behind the last).
-struct Share { uint32_t first, step, end; };
-template <uint32_t kItems>
-__device__ __forceinline__ void load_logits(const RouteArgs& a, const uint8_t* row, const Share& of, float (&l)[kItems]) {
-    if (a.fp32) {
+// The experts of a lane, below `end`: runs of kVec neighbours, `step` apart, from `first` on; and their logits (-inf behind the last). Runs of four, all whole, wherever
+// the number of experts allows it, whether they can be read at once or not: a token's sums do not depend on where it lies.
+template <uint32_t kVec> struct Share {
+    uint32_t first, step, end;
+    __device__ __forceinline__ uint32_t at(uint32_t i) const { return first + i / kVec * step + i % kVec; }
+};
+template <uint32_t kVec, uint32_t kItems>
+__device__ __forceinline__ void load_logits(const RouteArgs& a, const uint8_t* row, const Share<kVec>& of, float (&l)[kItems]) {
+    #pragma unroll
+    for (uint32_t i = 0; i < kItems; i += kVec) {
+        const uint32_t e = of.at(i);
         #pragma unroll
-        for (uint32_t i = 0; i < kItems; ++i) {
-            const uint32_t e = of.first + i * of.step;
-            l[i] = e < of.end ? __uint_as_float(ld_global_u32(row + (uint64_t)e * 4)) : -CUDART_INF_F;
-        }
-    } else {
-        #pragma unroll
-        for (uint32_t i = 0; i < kItems; ++i) {
-            const uint32_t e = of.first + i * of.step;
-            l[i] = e < of.end ? __uint_as_float((uint32_t)ld_global_u16(row + (uint64_t)e * 2) << 16) : -CUDART_INF_F;
+        for (uint32_t j = 0; j < kVec; ++j) l[i + j] = -CUDART_INF_F;
+        if (e >= of.end) continue;
+        if (kVec == 4 && a.aligned) {
+            if (a.fp32) {
+                const uint4 q = ld_stream_v4(row + (uint64_t)e * 4);
+                l[i] = __uint_as_float(q.x);
+                if constexpr (kVec == 4) { l[i + 1] = __uint_as_float(q.y); l[i + 2] = __uint_as_float(q.z); l[i + 3] = __uint_as_float(q.w); }
+            } else {
+                const uint2 q = ld_stream_v2(row + (uint64_t)e * 2);
+                l[i] = bf16_lo(q.x);
+                if constexpr (kVec == 4) { l[i + 1] = bf16_hi(q.x); l[i + 2] = bf16_lo(q.y); l[i + 3] = bf16_hi(q.y); }
+            }
+        } else {
+            #pragma unroll
+            for (uint32_t j = 0; j < kVec; ++j) l[i + j] = logit_at(a, row, e + j);
         }
     }
 }
@@ -83,7 +96,7 @@ __device__ __forceinline__ Softmax softmax_of(const float (&l)[kItems]) {
     for (uint32_t i = 0; i < kItems; ++i) m.top = fmaxf(m.top, l[i]);
     m.top = warp_max(m.top);
     #pragma unroll
-    for (uint32_t i = 0; i < kItems; ++i) m.sum += expf(l[i] - m.top);
+    for (uint32_t i = 0; i < kItems; ++i) m.sum += fast_exp2((l[i] - m.top) * kLog2E);
     m.sum = warp_sum(m.sum);
     // (a NaN beside masked experts stays one)
     if (m.top == -CUDART_INF_F) {
@@ -100,154 +113,215 @@ __device__ __forceinline__ float sigmoid_of(float l) {
     return __fdiv_rn(l < 0.0f ? z : 1.0f, 1.0f + z);
 }
 __device__ __forceinline__ float score_of(bool sigmoid, const Softmax& m, float l) { return sigmoid ? sigmoid_of(l) : __fdiv_rn(expf(l - m.top), m.sum); }
-// How far an FP32 score c = s + b can be from the exact one; `largest`: the largest s. Sigmoid: the exponential within 2 ulp (2^-22), half an ulp
-// for the addition and for the division: s within 2^-21 of its value. Softmax: rounding l - top moves s by less than x e^-x 2^-24 < 2^-25 of the
-// largest; the exponential 2 ulp; at most 64 + 5 additions of the sum, 2^-17.8; the division: under 2^-17 of the largest in all. The addition of b is
-// within 2^-24 of c, its sum with another score of the group (whose errors the caller doubles) too.
-__device__ __forceinline__ float score_error(bool sigmoid, float largest, float c) { return (sigmoid ? 0x1p-21f : 0x1p-17f) * largest + 0x1p-23f * fabsf(c); }
+__device__ __forceinline__ float redux_max(float v) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+}
+__device__ __forceinline__ float redux_min(float v) {
+    float m;
+    asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+}
 
-// Whole numbers in the order of the values: NaN above everything (as in torch.topk), 0 for what cannot be chosen.
-template <typename T> struct Key;
-template <> struct Key<float> {
-    using type = uint32_t;
-    static __device__ __forceinline__ type of(float v) {
-        if (v != v) return 0xffffffffu;
-        const uint32_t b = __float_as_uint(v + 0.0f);                     // (-0 is 0)
-        return b & 0x80000000u ? ~b : b | 0x80000000u;
-    }
-    static __device__ __forceinline__ float back(type k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
-    static __device__ __forceinline__ type largest(type k) { return __reduce_max_sync(kAll, k); }
-};
-template <> struct Key<double> {
-    using type = uint64_t;
-    static __device__ __forceinline__ type of(double v) {
-        if (v != v) return ~0ull;
-        const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
-        return b >> 63 ? ~b : b | 1ull << 63;
-    }
-    static __device__ __forceinline__ type largest(type k) {
-        const uint32_t high = __reduce_max_sync(kAll, (uint32_t)(k >> 32));
-        return (uint64_t)high << 32 | __reduce_max_sync(kAll, (uint32_t)(k >> 32) == high ? (uint32_t)k : 0u);
-    }
-};
-
-// The choice of a token with scores of type T: the expert of choice `lane` (-1: none). Answers whether FP32 scores leave it open.
-template <typename T, uint32_t kItems>
-__device__ __forceinline__ bool choose(const RouteArgs& a, const uint8_t* row, const Share& of, const float (&l)[kItems], const Softmax& m, uint32_t lane,
-                                       int32_t& chosen) {
-    using K = typename Key<T>::type;
-    constexpr bool kFast = sizeof(T) == 4;
+// The choice of a token, the expert of choice `lane` in `chosen` (-1: none), by whole numbers that stand for c; answers whether that decides it.
+//
+// How far the c here can be from the exact one (score_error). Sigmoid: the fast exponential moves e^-l by (2 + 1.2 |l|) 2^-23 of it, so s by at most
+// s (1 - s) (2 + 1.2 |l|) 2^-23 < 2^-23, the addition and the reciprocal by less than 3 x 2^-23 of s: 2^-21 in all. Softmax: l - top times log2(e) is within
+// 2^-23 of its value x, the exponential 2 ulp more, which moves s by x e^-x 2^-23 + 2^-22 < 2^-21.5 of the largest; the sum likewise, and by
+// at most 64 + 5 additions, 2^-17.8: under 2^-17 of the largest in all. The addition of b is within 2^-24 of c, and so is the sum of two scores.
+template <uint32_t kVec, uint32_t kItems>
+__device__ __forceinline__ bool quick_choice(const RouteArgs& a, const uint8_t* row, const Share<kVec>& of, const float (&l)[kItems], const Softmax& m, uint32_t lane,
+                                             int32_t& chosen) {
     const bool sigmoid = a.sigmoid != 0, with_scores = !a.by_logits || (a.groups > 1 && a.best_two);
-    T total = 1;
-    if constexpr (!kFast) {
-        if (!sigmoid && with_scores) {
-            total = 0;
-            #pragma unroll 1
-            for (uint32_t i = 0; i < kItems; ++i) {
-                const uint32_t e = of.first + i * of.step;
-                if (e < of.end) total += exp((double)logit_at(a, row, e) - (double)m.top);
-            }
-            total = warp_sum(total);
-        }
-    }
-    K key[kItems];
-    T best = -CUDART_INF, second = -CUDART_INF;               // of the group's values in this lane
-    bool nan = false;
-    float largest = 0.0f;
+    const float inverse = __frcp_rn(m.sum);
+    float c[kItems], order[kItems], largest = 0.0f;
+    bool open = false;
     #pragma unroll
     for (uint32_t i = 0; i < kItems; ++i) {
-        const uint32_t e = of.first + i * of.step;
-        key[i] = 0;
-        if (e >= of.end || l[i] == -CUDART_INF_F) continue;
-        const float b = bias_at(a, e);
-        if (b == -CUDART_INF_F) continue;
-        T c = (T)l[i];
+        const uint32_t e = of.at(i);
+        c[i] = l[i];
         if (with_scores) {
-            T s;
-            if constexpr (kFast) s = score_of(sigmoid, m, l[i]);
-            else s = sigmoid ? 1.0 / (1.0 + exp(-(double)l[i])) : exp((double)l[i] - (double)m.top) / total;
-            largest = fmaxf(largest, (float)s);
-            c = s + (T)b;
+            float s;
+            if (sigmoid) s = fast_reciprocal(1.0f + fast_exp2(-kLog2E * l[i]));
+            else s = fast_exp2((l[i] - m.top) * kLog2E) * inverse;
+            largest = fmaxf(largest, s);
+            const float b = a.bias && e < of.end ? bias_at(a, e) : 0.0f;
+            // (-inf where the expert cannot be chosen, whichever of the two says so)
+            c[i] = l[i] == -CUDART_INF_F ? -CUDART_INF_F : s + b;
         }
-        key[i] = Key<T>::of(a.by_logits ? (T)l[i] : c);
+        open |= c[i] != c[i];
+        order[i] = a.by_logits ? l[i] : c[i];
+    }
+    const float relative = sigmoid ? 0x1p-21f : 0x1p-17f;
+    const float error = with_scores ? relative * (sigmoid ? 1.0f : redux_max(largest)) : 0.0f;
+    if (a.groups > 1) {
+        const uint32_t lanes = 1u << a.lanes_log2, group = lane >> a.lanes_log2;
+        float best = -CUDART_INF_F, second = -CUDART_INF_F;   // of the group's values
+        #pragma unroll
+        for (uint32_t i = 0; i < kItems; ++i) {
+            second = fmaxf(second, fminf(best, c[i]));
+            best = fmaxf(best, c[i]);
+        }
+        for (uint32_t o = lanes / 2; o > 0; o >>= 1) {
+            const float b = __shfl_xor_sync(kAll, best, o), s = __shfl_xor_sync(kAll, second, o);
+            second = fmaxf(fmaxf(second, s), fminf(best, b));
+            best = fmaxf(best, b);
+        }
+        // (a group with a single expert that can be chosen counts that one alone)
+        const float score = a.best_two && second > -CUDART_INF_F ? best + second : best;
+        // The groups in their order, ties to the lowest: all lanes of a group hold its score.
+        float left = group < a.groups ? score : -CUDART_INF_F, last = 0.0f;
+        bool taken = false;
+        for (uint32_t k = 0; k < a.topk_groups; ++k) {
+            last = redux_max(left);
+            const uint32_t first = __ffs(__ballot_sync(kAll, left == last)) - 1;
+            if (last == -CUDART_INF_F) break;
+            if (group == first >> a.lanes_log2) { taken = true; left = -CUDART_INF_F; }
+        }
+        const float next = redux_max(left);
+        // (equal scores made of logits alone are equal)
+        if (with_scores) open |= next > -CUDART_INF_F && last - next <= 4.0f * error + 0x1p-21f * fabsf(last);
+        if (!taken) {
+            #pragma unroll
+            for (uint32_t i = 0; i < kItems; ++i) order[i] = -CUDART_INF_F;
+        }
+    }
+    // Distances from the largest, in `units` of their range, which ends 2 (32 among logits) below it: what lies further down is not told apart.
+    float top = -CUDART_INF_F, bottom = CUDART_INF_F;
+    #pragma unroll
+    for (uint32_t i = 0; i < kItems; ++i) {
+        top = fmaxf(top, order[i]);
+        if (order[i] > -CUDART_INF_F) bottom = fminf(bottom, order[i]);
+    }
+    top = redux_max(top);
+    bottom = redux_min(bottom);
+    const float range = fminf(top - bottom, a.by_logits ? 32.0f : 2.0f);
+    // (16 units are left free at both ends for what per_unit, rounded, is off by)
+    const uint32_t units = (1u << (31 - a.index_bits < 23 ? 31 - a.index_bits : 23)) - 32;
+    const float per_unit = range > 0.0f ? __fdividef((float)units, range) : 1.0f;
+    open |= top == CUDART_INF_F || per_unit > 0x1p100f;
+    uint32_t key[kItems], mine = 0;
+    #pragma unroll
+    for (uint32_t i = 0; i < kItems; ++i) {
+        // (a float in 2^23 .. 2^24 holds the whole number in its low bits)
+        const float field = fmaf(-fminf(top - order[i], range), per_unit, 8388608.0f + (float)(units + 16));
+        key[i] = order[i] > -CUDART_INF_F ? (__float_as_uint(field) & 0x7fffffu) << a.index_bits | (kMostExperts - 1 - of.at(i)) & ((1u << a.index_bits) - 1) : 0u;
+        mine = max(mine, key[i]);
+    }
+    uint32_t held = 0;
+    for (uint32_t k = 0; k < a.topk; ++k) {
+        const uint32_t m1 = __reduce_max_sync(kAll, mine);
+        if (lane == k) held = m1;
+        // the largest below it: key - m1 wraps around, and the nearest below has the largest difference
+        uint32_t next = 0x80000000u;
+        #pragma unroll
+        for (uint32_t i = 0; i < kItems; ++i) next = __viaddmax_u32(key[i], 0u - m1, next);
+        if (mine == m1) mine = next == 0x80000000u ? 0u : next + m1;
+    }
+    const uint32_t mask = (1u << a.index_bits) - 1;
+    chosen = held != 0 ? (int32_t)((kMostExperts - 1 - held) & mask) : -1;
+    // Are neighbours of the order apart by more than their errors, or equal because their logits and biases are? The last choice's neighbour is the one that
+    // was not taken; where these two are equal, its own neighbour might stand between them.
+    const uint32_t behind = __reduce_max_sync(kAll, mine);
+    uint32_t after = __shfl_down_sync(kAll, held, 1);
+    if (lane == a.topk - 1) after = behind;
+    const float bound = 2.0f * (error + 0x1p-22f * (fabsf(top) + range)) * per_unit + 3.0f;
+    const auto near = [&](uint32_t k, uint32_t below) { return below != 0 && (float)((k >> a.index_bits) - (below >> a.index_bits)) <= bound; };
+    bool equal = false;
+    if (near(held, after)) {
+        const uint32_t e = (kMostExperts - 1 - after) & mask;
+        equal = logit_at(a, row, (uint32_t)chosen) == logit_at(a, row, e) && bias_at(a, (uint32_t)chosen) == bias_at(a, e);
+        open |= !equal;
+    }
+    if (__any_sync(kAll, equal && lane == a.topk - 1)) {
+        uint32_t next = 0;
+        #pragma unroll
+        for (uint32_t i = 0; i < kItems; ++i) next = max(next, key[i] < behind ? key[i] : 0u);
+        open |= near(behind, __reduce_max_sync(kAll, next));
+    }
+    return !__any_sync(kAll, open);
+}
+
+// The same with scores of 64 bits. In the order of whole numbers: NaN above everything (as in torch.topk), 0 for what cannot be chosen.
+__device__ __forceinline__ uint64_t key_of(double v) {
+    if (v != v) return ~0ull;
+    const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);           // (-0 is 0)
+    return b >> 63 ? ~b : b | 1ull << 63;
+}
+__device__ __forceinline__ uint64_t largest_key(uint64_t k) {
+    const uint32_t high = __reduce_max_sync(kAll, (uint32_t)(k >> 32));
+    return (uint64_t)high << 32 | __reduce_max_sync(kAll, (uint32_t)(k >> 32) == high ? (uint32_t)k : 0u);
+}
+// (out of line: few tokens come here, and its registers would be everybody's)
+template <uint32_t kVec, uint32_t kItems>
+__device__ __noinline__ int32_t exact_choice(const RouteArgs& a, const uint8_t* row, const Share<kVec> of, float softmax_top, uint32_t lane) {
+    const bool sigmoid = a.sigmoid != 0;
+    double total = 1;
+    if (!sigmoid) {
+        total = 0;
+        #pragma unroll 1
+        for (uint32_t i = 0; i < kItems; ++i)
+            if (of.at(i) < of.end) total += exp((double)logit_at(a, row, of.at(i)) - (double)softmax_top);
+        total = warp_sum(total);
+    }
+    uint64_t key[kItems];
+    double best = -CUDART_INF, second = -CUDART_INF;
+    bool nan = false;
+    #pragma unroll
+    for (uint32_t i = 0; i < kItems; ++i) {
+        const uint32_t e = of.at(i);
+        key[i] = 0;
+        if (e >= of.end) continue;
+        const double l = logit_at(a, row, e), b = bias_at(a, e);
+        if (l == -CUDART_INF || b == -CUDART_INF) continue;
+        double c = l;
+        if (!a.by_logits || a.best_two) c = (sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - (double)softmax_top) / total) + b;
+        key[i] = key_of(a.by_logits ? l : c);
         nan |= c != c;
         if (c > best) { second = best; best = c; }
         else if (c > second) second = c;
     }
-    bool open = false;
-    if (kFast && with_scores) largest = warp_max(largest);
     if (a.groups > 1) {
         const uint32_t lanes = 1u << a.lanes_log2, group = lane >> a.lanes_log2;
         for (uint32_t o = lanes / 2; o > 0; o >>= 1) {
-            const T b = __shfl_xor_sync(kAll, best, o), s = __shfl_xor_sync(kAll, second, o);
+            const double b = __shfl_xor_sync(kAll, best, o), s = __shfl_xor_sync(kAll, second, o);
             nan |= __shfl_xor_sync(kAll, (int)nan, o) != 0;
-            const T lower = best < b ? best : b;
+            const double lower = best < b ? best : b;
             best = best < b ? b : best;
             second = second < s ? s : second;
             second = second < lower ? lower : second;
         }
-        // (a group with a single expert that can be chosen counts that one alone)
-        T score = a.best_two && second > (T)-CUDART_INF ? best + second : best;
-        if (nan) score = (T)CUDART_NAN;
-        const K mine = Key<T>::of(score);
-        uint32_t ahead = 0, near = 0;
+        const uint64_t mine = key_of(nan ? CUDART_NAN : a.best_two && second > -CUDART_INF ? best + second : best);
+        uint32_t ahead = 0;
         for (uint32_t g = 0; g < a.groups; ++g) {
-            const T other = __shfl_sync(kAll, score, g << a.lanes_log2);
-            const K k = Key<T>::of(other);
+            const uint64_t k = __shfl_sync(kAll, mine, g << a.lanes_log2);
             ahead += k > mine || (k == mine && g < group);
-            if constexpr (kFast)
-                if (with_scores && fabsf(other - score) <= 4.0f * score_error(sigmoid, largest, score)) near |= 1u << g;
         }
-        const bool taken = group < a.groups && ahead < a.topk_groups;
-        const uint32_t all_taken = __ballot_sync(kAll, taken);
-        if (group >= a.groups) near = 0;
-        for (; near != 0; near &= near - 1) open |= taken != ((all_taken >> ((__ffs(near) - 1) << a.lanes_log2) & 1u) != 0);
-        if (!taken) {
+        if (group >= a.groups || ahead >= a.topk_groups) {
             #pragma unroll
             for (uint32_t i = 0; i < kItems; ++i) key[i] = 0;
         }
     }
-    // One choice after the other; one more says whether the last of them is certain.
-    K mine = 0;
-    uint32_t place = 0;
-    const auto find = [&]() {
-        mine = 0;
+    int32_t chosen = -1;
+    for (uint32_t k = 0; k < a.topk; ++k) {
+        uint64_t mine = 0;
+        uint32_t place = 0;
         #pragma unroll
         for (uint32_t i = 0; i < kItems; ++i)
-            if (key[i] > mine) { mine = key[i]; place = of.first + i * of.step; }
-    };
-    find();
-    chosen = -1;
-    const bool check = kFast && !a.by_logits;
-    K before = 0;
-    uint32_t expert_before = 0;
-    for (uint32_t k = 0; k < a.topk + (check ? 1u : 0u); ++k) {
-        const K top = Key<T>::largest(mine);
+            if (key[i] > mine) { mine = key[i]; place = of.at(i); }
+        const uint64_t top = largest_key(mine);
         if (top == 0) break;
         const uint32_t e = __reduce_min_sync(kAll, mine == top ? place : 0xffffffffu);
-        if (lane == k && k < a.topk) chosen = (int32_t)e;
-        if constexpr (kFast) {
-            if (check && k > 0) {
-                const float here = Key<T>::back(top), there = Key<T>::back(before);
-                // (equal logits and biases make a tie in any number of bits)
-                if (there - here <= 2.0f * score_error(sigmoid, largest, fmaxf(fabsf(here), fabsf(there))) &&
-                    (logit_at(a, row, e) != logit_at(a, row, expert_before) || bias_at(a, e) != bias_at(a, expert_before))) open = true;
-            }
-            before = top;
-            expert_before = e;
-        }
-        if (mine == top && place == e) {
-            #pragma unroll
-            for (uint32_t i = 0; i < kItems; ++i)
-                if (of.first + i * of.step == e) key[i] = 0;
-            find();
-        }
-        __syncwarp();
+        if (lane == k) chosen = (int32_t)e;
+        #pragma unroll
+        for (uint32_t i = 0; i < kItems; ++i)
+            if (of.at(i) == e) key[i] = 0;
     }
-    return __any_sync(kAll, open);
+    return chosen;
 }
 
-template <uint32_t kItems>
+template <uint32_t kVec, uint32_t kItems>
 __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const RouteArgs a) {
     const uint32_t lane = threadIdx.x % 32, token = blockIdx.x * (kRouteThreads / 32) + threadIdx.x / 32;
     griddep_wait();
@@ -255,14 +329,14 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const RouteArg
     if (token >= a.tokens) return;
     const uint8_t* row = a.logits + (uint64_t)token * a.stride;
     const uint32_t group = lane >> a.lanes_log2;
-    Share of{group * a.group_size + (lane & ((1u << a.lanes_log2) - 1)), 1u << a.lanes_log2, (group + 1) * a.group_size};
+    Share<kVec> of{group * a.group_size + (lane & ((1u << a.lanes_log2) - 1)) * kVec, kVec << a.lanes_log2, (group + 1) * a.group_size};
     if (group >= a.groups) of.first = of.end = 0;
     float l[kItems];
     load_logits(a, row, of, l);
     Softmax m{0.0f, 1.0f};
     if (!a.sigmoid) m = softmax_of(l);
     int32_t chosen;
-    if (choose<float>(a, row, of, l, m, lane, chosen)) choose<double>(a, row, of, l, m, lane, chosen);
+    if (!quick_choice(a, row, of, l, m, lane, chosen)) chosen = exact_choice<kVec, kItems>(a, row, of, m.top, lane);
     float w = 0.0f;
     if (chosen >= 0) w = score_of(a.sigmoid != 0, m, logit_at(a, row, (uint32_t)chosen));
     if (a.renormalize) w = __fdiv_rn(w, fmaxf(warp_sum(w), kLeastSum));
@@ -273,58 +347,85 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const RouteArg
 }
 
 // The gradient: with A_j from choice j (below), dl_e = sum over the choices of e of A_j, and for a softmax that is not renormalised
-// - p_e sum(g p) on every expert. Choices of the same expert add up in their order. Bound by HBM for many tokens: the logits are read once and
-// their gradient is written once.
-template <uint32_t kItems>
+// - p_e sum(g p) on every expert. A lane writes the latter (or zeros) for its experts, and then lane j what its choice adds up to, over the same: equal
+// choices add up in their order. Bound by HBM for many tokens: the logits are read once and their gradient is written once.
+template <uint32_t kVec, uint32_t kItems>
 __global__ void __launch_bounds__(kRouteThreads) moe_route_grad_kernel(const RouteArgs a) {
     const uint32_t lane = threadIdx.x % 32, token = blockIdx.x * (kRouteThreads / 32) + threadIdx.x / 32;
     griddep_wait();
     griddep_launch_dependents();
     if (token >= a.tokens) return;
     const uint8_t* row = a.logits + (uint64_t)token * a.stride;
-    const Share of{lane, 32, a.experts};
+    const Share<kVec> of{lane * kVec, 32 * kVec, a.experts};
+    const bool sigmoid = a.sigmoid != 0, everywhere = !sigmoid && !a.renormalize;
     float l[kItems];
-    load_logits(a, row, of, l);
-    int64_t idx = -1;
-    float g = 0.0f;
+    if (!sigmoid) load_logits(a, row, of, l);
+    int32_t idx = -1;
+    float g = 0.0f, mine = 0.0f;
     if (lane < a.topk) {
         const uint64_t at = (uint64_t)token * a.topk + lane;
-        idx = a.idx64 ? *(static_cast<const volatile int64_t*>(a.idx) + at) : (int64_t)(int32_t)ld_global_u32(static_cast<const int32_t*>(a.idx) + at);
-        if (idx < 0 || idx >= a.experts) idx = -1;
-        if (idx >= 0) g = __uint_as_float(ld_global_u32(a.grad_weights + at)) * a.scale;
+        const int64_t e = a.idx64 ? *(static_cast<const volatile int64_t*>(a.idx) + at) : (int64_t)(int32_t)ld_global_u32(static_cast<const int32_t*>(a.idx) + at);
+        g = __uint_as_float(ld_global_u32(a.grad_weights + at)) * a.scale;
+        if (e >= 0 && e < a.experts) {
+            idx = (int32_t)e;
+            mine = logit_at(a, row, (uint32_t)idx);
+        }
     }
-    const bool sigmoid = a.sigmoid != 0;
+    if (idx < 0) g = 0.0f;
     Softmax m{0.0f, 1.0f};
     if (!sigmoid) m = softmax_of(l);
-    const float mine = idx >= 0 ? logit_at(a, row, (uint32_t)idx) : 0.0f;
     const float s = idx >= 0 ? score_of(sigmoid, m, mine) : 0.0f;
     // the slope of log s (for a softmax the other part of it is the sum over all experts): 1 - s would lose its bits where s is near 1
     const float slope = sigmoid ? sigmoid_of(-mine) : 1.0f;
     float from_choice, from_all = 0.0f;
     if (a.renormalize) {
-        const float sum = warp_sum(s), q = __fdiv_rn(s, fmaxf(sum, kLeastSum)), dot = warp_sum(idx >= 0 ? g * q : 0.0f);
+        const float sum = warp_sum(s), q = __fdiv_rn(s, fmaxf(sum, kLeastSum)), dot = warp_sum(g * q);
         from_choice = q * (sum > kLeastSum ? g - dot : g) * slope;
     } else {
         from_choice = g * s * slope;
-        if (!sigmoid) from_all = warp_sum(idx >= 0 ? g * s : 0.0f);
-    }
-    float d[kItems];
-    #pragma unroll
-    for (uint32_t i = 0; i < kItems; ++i) d[i] = sigmoid || a.renormalize ? 0.0f : -from_all * score_of(false, m, l[i]);
-    for (uint32_t j = 0; j < a.topk; ++j) {
-        const int32_t e = __shfl_sync(kAll, (int32_t)idx, j);
-        const float add = __shfl_sync(kAll, from_choice, j);
-        #pragma unroll
-        for (uint32_t i = 0; i < kItems; ++i)
-            if ((int32_t)(lane + i * 32) == e) d[i] += add;
+        if (!sigmoid) from_all = warp_sum(g * s);
     }
     uint8_t* out = a.grad_logits + (uint64_t)token * a.grad_stride;
+    // (the logits may lie where their gradient goes)
+    __syncwarp();
+    const float each = everywhere ? -from_all * __frcp_rn(m.sum) : 0.0f;
     #pragma unroll
-    for (uint32_t i = 0; i < kItems; ++i) {
-        const uint32_t e = lane + i * 32;
-        if (e >= a.experts) continue;
-        if (a.fp32) reinterpret_cast<float*>(out)[e] = d[i];
-        else reinterpret_cast<__nv_bfloat16*>(out)[e] = __float2bfloat16_rn(d[i]);
+    for (uint32_t i = 0; i < kItems; i += kVec) {
+        const uint32_t e = of.at(i);
+        if (e >= of.end) continue;
+        float d[kVec];
+        #pragma unroll
+        for (uint32_t j = 0; j < kVec; ++j) d[j] = everywhere ? each * fast_exp2((l[i + j] - m.top) * kLog2E) : 0.0f;
+        if (kVec == 4 && a.aligned) {
+            if (a.fp32) {
+                *reinterpret_cast<float4*>(out + (uint64_t)e * 4) = make_float4(d[0], d[kVec / 4], d[kVec / 2], d[kVec - 1]);
+            } else {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(d[0], d[kVec / 4]), hi = __floats2bfloat162_rn(d[kVec / 2], d[kVec - 1]);
+                *reinterpret_cast<uint2*>(out + (uint64_t)e * 2) = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            }
+        } else {
+            #pragma unroll
+            for (uint32_t j = 0; j < kVec; ++j) {
+                if (a.fp32) reinterpret_cast<float*>(out)[e + j] = d[j];
+                else reinterpret_cast<__nv_bfloat16*>(out)[e + j] = __float2bfloat16_rn(d[j]);
+            }
+        }
+    }
+    const uint32_t same = __match_any_sync(kAll, idx);
+    float sum = from_choice;
+    if (__any_sync(kAll, idx >= 0 && (same & (same - 1)) != 0)) {
+        sum = 0.0f;
+        for (uint32_t j = 0; j < a.topk; ++j) {
+            const float add = __shfl_sync(kAll, from_choice, j);
+            if (same >> j & 1u) sum += add;
+        }
+    }
+    // (behind the stores of the other lanes)
+    __syncwarp();
+    if (idx >= 0 && (same & ((1u << lane) - 1)) == 0) {
+        const float d = (everywhere ? -from_all * s : 0.0f) + sum;
+        if (a.fp32) reinterpret_cast<float*>(out)[idx] = d;
+        else reinterpret_cast<__nv_bfloat16*>(out)[idx] = __float2bfloat16_rn(d);
     }
 }
 
@@ -332,13 +433,14 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_grad_kernel(const Rou
 
 using namespace dg;
 
-template <template <uint32_t> class Pick> static const void* for_items(uint32_t items) {
-    return items <= 1 ? Pick<1>::fn() : items <= 2 ? Pick<2>::fn() : items <= 4 ? Pick<4>::fn() : items <= 8 ? Pick<8>::fn() : items <= 16 ? Pick<16>::fn()
-           : items <= 32 ? Pick<32>::fn() : Pick<64>::fn();
+// The instantiation for as many experts as a lane holds. (At most 60 of a forward pass, at least 17 lanes having experts, and 32 of a backward one.)
+template <template <uint32_t, uint32_t> class Pick> static const void* for_items(bool vec, uint32_t items) {
+    if (vec) return items <= 4 ? Pick<4, 4>::fn() : items <= 8 ? Pick<4, 8>::fn() : items <= 16 ? Pick<4, 16>::fn() : items <= 32 ? Pick<4, 32>::fn() : Pick<4, 64>::fn();
+    return items <= 2 ? Pick<1, 2>::fn() : items <= 4 ? Pick<1, 4>::fn() : items <= 8 ? Pick<1, 8>::fn() : items <= 16 ? Pick<1, 16>::fn()
+           : items <= 32 ? Pick<1, 32>::fn() : Pick<1, 64>::fn();
 }
-template <uint32_t kItems> struct Forward { static const void* fn() { return (const void*)moe_route_kernel<kItems>; } };
-// (a lane holds every 32nd of at most 1024 experts)
-template <uint32_t kItems> struct Backward { static const void* fn() { return (const void*)moe_route_grad_kernel<(kItems < 32 ? kItems : 32)>; } };
+template <uint32_t kVec, uint32_t kItems> struct Forward { static const void* fn() { return (const void*)moe_route_kernel<kVec, kItems>; } };
+template <uint32_t kVec, uint32_t kItems> struct Backward { static const void* fn() { return (const void*)moe_route_grad_kernel<kVec, (kItems < 32 ? kItems : 32)>; } };
 
 static int route_args(RouteArgs& a, const void* logits, int is_fp32, uint64_t stride, uint32_t tokens, uint32_t experts, uint32_t topk, int sigmoid,
                       int renormalize, float scale) {
@@ -372,9 +474,12 @@ extern "C" int dg_moe_route_launch(const void* logits, int is_fp32, uint64_t str
     a.groups = num_groups; a.group_size = experts / num_groups; a.topk_groups = topk_groups;
     a.best_two = group_best == 2; a.by_logits = bias == nullptr;
     while ((2u << a.lanes_log2) * num_groups <= 32) ++a.lanes_log2;
-    const uint32_t items = (a.group_size + (1u << a.lanes_log2) - 1) >> a.lanes_log2;
+    while ((1u << a.index_bits) < experts) ++a.index_bits;
+    const bool vec = a.group_size % 4 == 0;
+    a.aligned = vec && (reinterpret_cast<uintptr_t>(logits) | a.stride) % (is_fp32 ? 16 : 8) == 0;
+    const uint32_t run = vec ? 4 : 1, items = (a.group_size + (run << a.lanes_log2) - 1) / (run << a.lanes_log2) * run;
     void* params[] = {&a};
-    return launch_overlapped(for_items<Forward>(items), dim3((tokens + kRouteThreads / 32 - 1) / (kRouteThreads / 32)), dim3(kRouteThreads), params,
+    return launch_overlapped(for_items<Forward>(vec, items), dim3((tokens + kRouteThreads / 32 - 1) / (kRouteThreads / 32)), dim3(kRouteThreads), params,
                              static_cast<cudaStream_t>(stream));
 }
 
@@ -388,7 +493,9 @@ extern "C" int dg_moe_route_grad_launch(const float* grad_weights, const void* l
     DG_CHECK_ARG(reinterpret_cast<uintptr_t>(grad_logits) % (is_fp32 ? 4 : 2) == 0, "moe_route_grad: grad_logits must be an aligned pointer");
     a.grad_weights = grad_weights; a.idx = const_cast<void*>(topk_idx); a.idx64 = idx_is_int64 ? 1u : 0u;
     a.grad_logits = static_cast<uint8_t*>(grad_logits); a.grad_stride = grad_stride * (is_fp32 ? 4 : 2);
+    const bool vec = experts % 4 == 0;
+    a.aligned = vec && (reinterpret_cast<uintptr_t>(logits) | a.stride | reinterpret_cast<uintptr_t>(grad_logits) | a.grad_stride) % (is_fp32 ? 16 : 8) == 0;
     void* params[] = {&a};
-    return launch_overlapped(for_items<Backward>((experts + 31) / 32), dim3((tokens + kRouteThreads / 32 - 1) / (kRouteThreads / 32)), dim3(kRouteThreads), params,
+    return launch_overlapped(for_items<Backward>(vec, vec ? (experts + 127) / 128 * 4 : (experts + 31) / 32), dim3((tokens + kRouteThreads / 32 - 1) / (kRouteThreads / 32)), dim3(kRouteThreads), params,
                              static_cast<cudaStream_t>(stream));
 }
