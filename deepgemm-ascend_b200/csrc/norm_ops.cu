@@ -107,75 +107,78 @@ struct NormArgs {
     float* rstd;
     uint32_t tokens, hidden;
     float eps;
+    double inverse_hidden;
 };
 
-// A CTA takes kRows tokens at a time (all loads are issued before the first is used), a thread kPieces x 8 channels of each.
-template <typename T, uint32_t kRows, uint32_t kPieces>
-__global__ void __launch_bounds__(1024) rms_norm_fp8_kernel(const NormArgs a) {
-    __shared__ double partial[32 * kRows];
-    const uint32_t lane = threadIdx.x % 32, token = blockIdx.x * kRows;
+// 1 / sqrt(m) as the nearest FP32 number (but for one in 10^8): two steps of Newton's method in 64 bits behind the FP32 instruction, where FP32 holds m.
+__device__ __forceinline__ float rsqrt_of(double m) {
+    if (m > 0x1p-120 && m < 0x1p120) {
+        double y = (double)rsqrtf((float)m);
+        y = y * fma(-0.5 * m * y, y, 1.5);
+        y = y * fma(-0.5 * m * y, y, 1.5);
+        return (float)y;
+    }
+    return (float)(1.0 / sqrt(m));
+}
+
+// A CTA walks tokens at a distance of the grid, a thread kPieces x 8 channels of each. With kAhead the next token is asked for before the sum over
+// the CTA: what keeps HBM busy over the barrier.
+template <typename T, uint32_t kPieces, bool kAhead>
+__global__ void __launch_bounds__(kPieces == 1 ? 1024 : 512, kPieces == 2 ? 2 : 1) rms_norm_fp8_kernel(const NormArgs a) {
+    __shared__ double partial[2][32];
+    const uint32_t lane = threadIdx.x % 32;
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t rows = min(kRows, a.tokens - token);
-    Piece<T> held[kRows][kPieces];
-    #pragma unroll
-    for (uint32_t r = 0; r < kRows; ++r)
+    Piece<T> x[kPieces], more[kPieces];
+    const auto load = [&](uint64_t token) {
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
             const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
-            held[r][i].clear();
-            if (r < rows && c < a.hidden) held[r][i].load(a.x + (uint64_t)(token + r) * a.x_stride + (uint64_t)c * sizeof(T));
+            if (c >= a.hidden) continue;
+            x[i].load(a.x + token * a.x_stride + (uint64_t)c * sizeof(T));
+            if (a.residual) more[i].load(a.residual + token * a.residual_stride + (uint64_t)c * sizeof(T));
         }
-    double sum[kRows];
+    };
     #pragma unroll
-    for (uint32_t r = 0; r < kRows; ++r) {
-        sum[r] = 0.0;
-        Piece<T> more[kPieces];
-        if (a.residual) {
-            #pragma unroll
-            for (uint32_t i = 0; i < kPieces; ++i) {
-                const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
-                more[i].clear();
-                if (r < rows && c < a.hidden) more[i].load(a.residual + (uint64_t)(token + r) * a.residual_stride + (uint64_t)c * sizeof(T));
-            }
-        }
+    for (uint32_t i = 0; i < kPieces; ++i) { x[i].clear(); more[i].clear(); }
+    if (kAhead) load(blockIdx.x);
+    uint32_t turn = 0;
+    for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x, turn ^= 1) {
+        if (!kAhead) load(token);
+        Piece<T> h[kPieces];
+        double sum[1] = {0.0};
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
             const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
             float v[8];
+            h[i] = x[i];
             if (a.residual) {
                 float u[8];
-                held[r][i].get(v);
+                x[i].get(v);
                 more[i].get(u);
                 #pragma unroll
                 for (int j = 0; j < 8; ++j) v[j] += u[j];
-                held[r][i].set(v);
-                if (r < rows && c < a.hidden) held[r][i].store(a.h + (uint64_t)(token + r) * a.h_stride + (uint64_t)c * sizeof(T));
+                h[i].set(v);
+                if (c < a.hidden) h[i].store(a.h + token * a.h_stride + (uint64_t)c * sizeof(T));
             }
-            held[r][i].get(v);
+            h[i].get(v);
             #pragma unroll
-            for (int j = 0; j < 8; ++j) sum[r] = fma((double)v[j], (double)v[j], sum[r]);
+            for (int j = 0; j < 8; ++j) sum[0] = fma((double)v[j], (double)v[j], sum[0]);
         }
-    }
-    cta_sums<double, kRows>(sum, partial);
-    float rstd[kRows];
-    #pragma unroll
-    for (uint32_t r = 0; r < kRows; ++r) {
-        rstd[r] = (float)(1.0 / sqrt(sum[r] / a.hidden + (double)a.eps));
-        if (threadIdx.x == 0 && r < rows) a.rstd[token + r] = rstd[r];
-    }
-    #pragma unroll
-    for (uint32_t i = 0; i < kPieces; ++i) {
-        const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
-        float w[8] = {};
-        if (c < a.hidden) weight_at(a.weight, a.weight_fp32, c, w);
+        if (kAhead && token + gridDim.x < a.tokens) load(token + gridDim.x);
+        // (two sets of shared memory: a warp that is a turn ahead does not write to what another still reads)
+        cta_sums<double, 1>(sum, partial[turn]);
+        const float rstd = rsqrt_of(fma(sum[0], a.inverse_hidden, (double)a.eps));
+        if (threadIdx.x == 0) a.rstd[token] = rstd;
         #pragma unroll
-        for (uint32_t r = 0; r < kRows; ++r) {
-            float v[8], amax = 0.0f;
-            held[r][i].get(v);
+        for (uint32_t i = 0; i < kPieces; ++i) {
+            const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
+            float w[8] = {}, v[8], amax = 0.0f;
+            if (c < a.hidden) weight_at(a.weight, a.weight_fp32, c, w);
+            h[i].get(v);
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                v[j] = __fmul_rn(__fmul_rn(v[j], rstd[r]), w[j]);
+                v[j] = __fmul_rn(__fmul_rn(v[j], rstd), w[j]);
                 amax = fmaxf(amax, fabsf(v[j]));
             }
             amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 1));
@@ -183,14 +186,14 @@ __global__ void __launch_bounds__(1024) rms_norm_fp8_kernel(const NormArgs a) {
             const uint32_t e = e4m3_scale_byte(amax);
             // (the second block of a last, half-used scale column is zero)
             const uint32_t next = __shfl_down_sync(kAll, c < a.hidden ? e : 0u, 4);
-            if (r >= rows || c >= a.hidden) continue;
-            *reinterpret_cast<uint2*>(a.out + (uint64_t)(token + r) * a.out_stride + c) = e4m3_pack8(v, e);
+            if (c >= a.hidden) continue;
+            *reinterpret_cast<uint2*>(a.out + token * a.out_stride + c) = e4m3_pack8(v, e);
             if (a.rows) {
                 Piece<__nv_bfloat16> y;
                 y.set(v);
-                y.store(a.rows + (uint64_t)(token + r) * a.rows_stride + (uint64_t)c * 2);
+                y.store(a.rows + token * a.rows_stride + (uint64_t)c * 2);
             }
-            if (lane % 8 == 0) *reinterpret_cast<uint16_t*>(a.sf + (uint64_t)(c / 64) * a.sf_col_stride + (uint64_t)(token + r) * 2) = (uint16_t)(e | next << 8);
+            if (lane % 8 == 0) *reinterpret_cast<uint16_t*>(a.sf + (uint64_t)(c / 64) * a.sf_col_stride + token * 2) = (uint16_t)(e | next << 8);
         }
     }
 }
@@ -206,14 +209,32 @@ struct NormGradArgs {
     uint8_t* dx; uint64_t dx_stride;
     float* partial;                                                      // [gridDim.x][hidden]
     uint32_t tokens, hidden;
+    float inverse_hidden;
 };
 
-template <typename T, typename G, uint32_t kPieces>
-__global__ void __launch_bounds__(1024) rms_norm_grad_kernel(const NormGradArgs a) {
+template <typename T, typename G, uint32_t kPieces, bool kAhead>
+__global__ void __launch_bounds__(kPieces == 1 ? 1024 : 512, kPieces == 2 ? 2 : 1) rms_norm_grad_kernel(const NormGradArgs a) {
     __shared__ float sums[2][32];
     griddep_wait();
     griddep_launch_dependents();
     float w[kPieces][8], dw[kPieces][8];
+    Piece<T> h[kPieces], more[kPieces];
+    Piece<G> g[kPieces];
+    float rstd = 0.0f;
+    const auto load = [&](uint64_t token) {
+        #pragma unroll
+        for (uint32_t i = 0; i < kPieces; ++i) {
+            const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
+            if (c >= a.hidden) continue;
+            h[i].load(a.h + token * a.h_stride + (uint64_t)c * sizeof(T));
+            g[i].load(a.g + token * a.g_stride + (uint64_t)c * sizeof(G));
+            if (a.grad_h) more[i].load(a.grad_h + token * a.grad_h_stride + (uint64_t)c * sizeof(T));
+        }
+        rstd = __uint_as_float(ld_global_u32(a.rstd + token));
+    };
+    #pragma unroll
+    for (uint32_t i = 0; i < kPieces; ++i) { h[i].clear(); g[i].clear(); more[i].clear(); }
+    if (kAhead) load(blockIdx.x);
     #pragma unroll
     for (uint32_t i = 0; i < kPieces; ++i) {
         const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
@@ -223,44 +244,37 @@ __global__ void __launch_bounds__(1024) rms_norm_grad_kernel(const NormGradArgs 
     }
     uint32_t turn = 0;
     for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x, turn ^= 1) {
-        Piece<T> h[kPieces], more[kPieces];
-        Piece<G> g[kPieces];
-        #pragma unroll
-        for (uint32_t i = 0; i < kPieces; ++i) {
-            const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
-            h[i].clear(); g[i].clear(); more[i].clear();
-            if (c >= a.hidden) continue;
-            h[i].load(a.h + token * a.h_stride + (uint64_t)c * sizeof(T));
-            g[i].load(a.g + token * a.g_stride + (uint64_t)c * sizeof(G));
-            if (a.grad_h) more[i].load(a.grad_h + token * a.grad_h_stride + (uint64_t)c * sizeof(T));
-        }
-        const float rstd = __uint_as_float(ld_global_u32(a.rstd + token));
+        if (!kAhead) load(token);
+        Piece<T> h0[kPieces], more0[kPieces];
+        Piece<G> g0[kPieces];
+        const float r = rstd;
         float dot[1] = {0.0f};
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
+            h0[i] = h[i]; more0[i] = more[i]; g0[i] = g[i];
             float n[8], u[8];
-            h[i].get(n);
-            g[i].get(u);
+            h0[i].get(n);
+            g0[i].get(u);
             #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                n[j] *= rstd;
+                n[j] *= r;
                 dw[i][j] = fmaf(u[j], n[j], dw[i][j]);
                 dot[0] = fmaf(u[j] * w[i][j], n[j], dot[0]);
             }
         }
-        // (two sets of shared memory: a warp that is a turn ahead does not write to what another still reads)
+        if (kAhead && token + gridDim.x < a.tokens) load(token + gridDim.x);
         cta_sums<float, 1>(dot, sums[turn]);
-        const float mean = dot[0] / (float)a.hidden;
+        const float mean = dot[0] * a.inverse_hidden;
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
             const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
             if (c >= a.hidden) continue;
             float n[8], u[8], d[8];
-            h[i].get(n);
-            g[i].get(u);
-            more[i].get(d);
+            h0[i].get(n);
+            g0[i].get(u);
+            more0[i].get(d);
             #pragma unroll
-            for (int j = 0; j < 8; ++j) d[j] += rstd * (u[j] * w[i][j] - n[j] * rstd * mean);
+            for (int j = 0; j < 8; ++j) d[j] += r * (u[j] * w[i][j] - n[j] * r * mean);
             Piece<T> out;
             out.set(d);
             out.store(a.dx + token * a.dx_stride + (uint64_t)c * sizeof(T));
@@ -276,25 +290,37 @@ __global__ void __launch_bounds__(1024) rms_norm_grad_kernel(const NormGradArgs 
     }
 }
 
-constexpr uint32_t kSumThreads = 256, kSumChannels = 32;
+// 32 channels a CTA, a warp every 32nd of the parts.
+constexpr uint32_t kSumThreads = 1024, kSumChannels = 32;
 __global__ void __launch_bounds__(kSumThreads) rms_norm_grad_sum_kernel(const float* partial, float* dw, uint32_t parts, uint32_t hidden) {
-    __shared__ float sums[kSumThreads / kSumChannels][kSumChannels];
-    const uint32_t channel = threadIdx.x % kSumChannels, c = blockIdx.x * kSumChannels + channel, first = threadIdx.x / kSumChannels;
+    __shared__ float sums[32][kSumChannels];
+    const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32, c = blockIdx.x * kSumChannels + lane;
     griddep_wait();
     griddep_launch_dependents();
     float sum = 0.0f;
-    for (uint32_t p = first; p < parts; p += kSumThreads / kSumChannels) sum += __uint_as_float(ld_global_u32(partial + (uint64_t)p * hidden + c));
-    sums[first][channel] = sum;
+    #pragma unroll 4
+    for (uint32_t p = warp; p < parts; p += 32) sum += __uint_as_float(ld_global_u32(partial + (uint64_t)p * hidden + c));
+    sums[warp][lane] = sum;
     __syncthreads();
-    if (first != 0) return;
+    if (warp != 0) return;
     #pragma unroll
-    for (uint32_t i = 1; i < kSumThreads / kSumChannels; ++i) sum += sums[i][channel];
+    for (uint32_t i = 1; i < 32; ++i) sum += sums[i][lane];
     dw[c] = sum;
 }
 
 // Threads of a CTA whose threads take `pieces` pieces of a row each.
 static uint32_t norm_threads(uint32_t hidden, uint32_t pieces) { return ((hidden / 8 + pieces - 1) / pieces + 31) / 32 * 32; }
-static uint32_t norm_grad_parts(uint32_t tokens) { return tokens < 148 * 2 ? tokens : 148 * 2; }
+// CTAs on the 148 SMs: with up to two pieces a thread has 64 registers, beyond that 128.
+static uint32_t norm_ctas(uint32_t tokens, uint32_t hidden, uint32_t pieces) {
+    const uint32_t most = 148 * (pieces <= 2 ? 1024 / norm_threads(hidden, pieces) : 1);
+    return tokens < most ? tokens : most;
+}
+// Pieces of a row for a thread: one while the row fits `most` threads, then two where there are such kernels, four, eight.
+static uint32_t norm_pieces(uint32_t hidden, uint32_t most, bool two) {
+    if (norm_threads(hidden, 1) <= most) return 1;
+    return two && norm_threads(hidden, 2) <= 512 ? 2 : norm_threads(hidden, 4) <= 512 ? 4 : 8;
+}
+static uint32_t norm_grad_parts(uint32_t tokens, uint32_t hidden) { return norm_ctas(tokens, hidden, norm_pieces(hidden, 1024, false)); }
 
 }  // namespace dg
 
@@ -308,9 +334,10 @@ static int norm_checks(uint32_t tokens, uint32_t hidden) {
 static bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<uintptr_t>(p) | stride_bytes) % 16 == 0; }
 
 template <typename T>
-static const void* norm_kernel(uint32_t rows, uint32_t pieces) {
-    if (rows == 1) return pieces == 1 ? (const void*)rms_norm_fp8_kernel<T, 1, 1> : pieces == 2 ? (const void*)rms_norm_fp8_kernel<T, 1, 2> : (const void*)rms_norm_fp8_kernel<T, 1, 4>;
-    return pieces == 1 ? (const void*)rms_norm_fp8_kernel<T, 2, 1> : pieces == 2 ? (const void*)rms_norm_fp8_kernel<T, 2, 2> : (const void*)rms_norm_fp8_kernel<T, 2, 4>;
+static const void* norm_kernel(uint32_t pieces) {
+    if constexpr (sizeof(T) == 2)
+        if (pieces == 2) return (const void*)rms_norm_fp8_kernel<T, 2, true>;
+    return pieces == 1 ? (const void*)rms_norm_fp8_kernel<T, 1, true> : pieces == 4 ? (const void*)rms_norm_fp8_kernel<T, 4, false> : (const void*)rms_norm_fp8_kernel<T, 8, false>;
 }
 
 extern "C" int dg_rms_norm_fp8_launch(const void* x, int is_fp32, uint64_t x_stride, const void* residual, uint64_t residual_stride, void* h, uint64_t h_stride,
@@ -334,19 +361,20 @@ extern "C" int dg_rms_norm_fp8_launch(const void* x, int is_fp32, uint64_t x_str
     a.out = static_cast<uint8_t*>(out); a.out_stride = out_stride;
     a.sf = reinterpret_cast<uint8_t*>(out_sf); a.sf_col_stride = sf_col_stride * 2;
     a.rstd = rstd; a.tokens = tokens; a.hidden = hidden; a.eps = eps;
-    const uint32_t rows_each = tokens <= 148 ? 1 : 2;
-    uint32_t pieces = tokens <= 148 ? 1 : 2;
-    while (norm_threads(hidden, pieces) > 1024) pieces *= 2;
-    const void* fn = is_fp32 ? norm_kernel<float>(rows_each, pieces) : norm_kernel<__nv_bfloat16>(rows_each, pieces);
+    a.inverse_hidden = 1.0 / hidden;
+    // Few tokens: as many threads as a row has pieces; many of BF16: at most 512, so that two CTAs are on an SM. (FP32 has twice the bytes in each.)
+    const uint32_t pieces = norm_pieces(hidden, is_fp32 || tokens <= 148 ? 1024 : 512, !is_fp32);
     void* params[] = {&a};
-    return launch_overlapped(fn, dim3((tokens + rows_each - 1) / rows_each), dim3(norm_threads(hidden, pieces)), params, static_cast<cudaStream_t>(stream));
+    return launch_overlapped(is_fp32 ? norm_kernel<float>(pieces) : norm_kernel<__nv_bfloat16>(pieces), dim3(norm_ctas(tokens, hidden, pieces)),
+                             dim3(norm_threads(hidden, pieces)), params, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" uint64_t dg_rms_norm_grad_scratch_bytes(uint32_t tokens, uint32_t hidden) { return (uint64_t)norm_grad_parts(tokens) * hidden * 4; }
+extern "C" uint64_t dg_rms_norm_grad_scratch_bytes(uint32_t tokens, uint32_t hidden) { return hidden ? (uint64_t)norm_grad_parts(tokens, hidden) * hidden * 4 : 0; }
 
 template <typename T, typename G>
 static const void* norm_grad_kernel(uint32_t pieces) {
-    return pieces == 1 ? (const void*)rms_norm_grad_kernel<T, G, 1> : pieces == 2 ? (const void*)rms_norm_grad_kernel<T, G, 2> : (const void*)rms_norm_grad_kernel<T, G, 4>;
+    return pieces == 1 ? (const void*)rms_norm_grad_kernel<T, G, 1, true> : pieces == 4 ? (const void*)rms_norm_grad_kernel<T, G, 4, false>
+                                                                                        : (const void*)rms_norm_grad_kernel<T, G, 8, false>;
 }
 
 extern "C" int dg_rms_norm_grad_launch(const void* grad_out, int grad_is_fp32, uint64_t grad_stride, const void* h, int is_fp32, uint64_t h_stride, const void* weight,
@@ -373,8 +401,9 @@ extern "C" int dg_rms_norm_grad_launch(const void* grad_out, int grad_is_fp32, u
     a.dx = static_cast<uint8_t*>(grad_x); a.dx_stride = grad_x_stride * es;
     a.partial = static_cast<float*>(scratch);
     a.tokens = tokens; a.hidden = hidden;
-    uint32_t pieces = 1, parts = norm_grad_parts(tokens);
-    while (norm_threads(hidden, pieces) > 1024) pieces *= 2;
+    a.inverse_hidden = 1.0f / (float)hidden;
+    const uint32_t pieces = norm_pieces(hidden, 1024, false);
+    uint32_t parts = norm_grad_parts(tokens, hidden);
     const void* fn = !is_fp32 ? norm_grad_kernel<__nv_bfloat16, __nv_bfloat16>(pieces) : grad_is_fp32 ? norm_grad_kernel<float, float>(pieces)
                                                                                                       : norm_grad_kernel<float, __nv_bfloat16>(pieces);
     void* params[] = {&a};

@@ -72,7 +72,7 @@ __device__ __forceinline__ void e4m3_unpack4(uint32_t q, float (&v)[4]) {
     }
 }
 // A power of two from its exponent byte (0: 2^-127, a subnormal number; 255: NaN).
-__device__ __forceinline__ float ue8m0_float(uint32_t e) { return __uint_as_float(e == 0u ? 0x00400000u : e == 255u ? 0x7fc00000u : e << 23); }
+__device__ __forceinline__ float ue8m0_float(uint32_t e) { return __uint_as_float(max(e << 23, 0x00400000u) | (((e + 1u) << 14) & 0x00400000u)); }
 
 // ---- E2M1: scale = the smallest power of two s with amax <= 6 s, from the bits of amax without a product that could round:
 // 6 s = 1.5 x 2^(e + 2), so the exponent goes up by one where the mantissa is above 1.5. There is no floor under amax (small

@@ -4,7 +4,7 @@
 // r = min(max(x_r, -clamp), clamp), p = 1 / (1 + e^-l):
 //     dx_l = g w r p (1 + l (1 - p)) where x_l <= clamp (else 0)      dx_r = g w l p where |x_r| <= clamp (else 0)
 //     dw = sum over the row of g l p r
-// all in FP32 (the fast exponential and reciprocal: p within a few ulp, 0 under 2^-126), dx rounded once to BF16.
+// all in FP32 (the fast exponential and reciprocal: p within a few ulp, and not below 2^-126), dx rounded once to BF16.
 //
 // HBM-bound: 2 H + 2 H + H / 16 bytes read (6 H from BF16) and 4 H written per row; the arithmetic, about 25 instructions a channel, is two thirds of
 // that time, so a warp asks for its next 256 channels before it works on those it has.
@@ -128,9 +128,8 @@ __global__ void __launch_bounds__(kGradThreads, 4) swiglu_grad_kernel(const Swig
                     if (outside_l) l[j] = a.clamp;
                     if (outside_r) r[j] = copysignf(a.clamp, r[j]);
                 }
-                // (by e^-|l|: the reciprocal of a number beyond 2^126 would be 0, and 1 - p would lose its bits where p is near 1)
-                const float z = fast_exp2(-kLog2E * fabsf(l[j])), near = fast_reciprocal(1.0f + z), far = z * near;
-                const float p = l[j] < 0.0f ? far : near, rest = l[j] < 0.0f ? near : far, silu = l[j] * p;
+                // (the reciprocal of a number beyond 2^126 would be 0, and its product with that an invalid one; 1 - p would lose its bits where p is near 1)
+                const float z = fast_exp2(fminf(-kLog2E * l[j], 126.0f)), p = fast_reciprocal(1.0f + z), rest = z * p, silu = l[j] * p;
                 const float gs = g[j] * silu, gr = g[j] * r[j] * weight;
                 dw = fmaf(gs, r[j], dw);
                 l[j] = outside_l ? 0.0f : gr * fmaf(silu, rest, p);

@@ -3,8 +3,8 @@ expert layer's training step with all of them.
 
 Tolerances, e = 2^-24. Everything that does not depend on the exponential is compared bit for bit. Gradient of SwiGLU, p = 1 / (1 + e^-l): the fast
 exponential is within (2 + 1.173 |l|) ulp, the reciprocal within 2 ulp: p within d p, d = (2 (2 + 1.2 |l|) + 8) e. dx_r = g w l p: d and four roundings.
-dx_l = g w r (p + l p (1 - p)): the terms move by d p and 3 d |l| p (1 - p carries d p too), and a few roundings. The exponential gives 0 for what is
-under the least normal number: p moves by at most t = 2^-126 beyond that, dx_r by t |g w l| and dx_l by t |g w r| (1 + |l|). dx is rounded to BF16 once, 2^-8 of the value.
+dx_l = g w r (p + l p (1 - p)): the terms move by d p and 3 d |l| p (1 - p carries d p too), and a few roundings. p stays at the least
+normal number where it is below: it moves by at most t = 2^-126 beyond that, dx_r by t |g w l| and dx_l by t |g w r| (1 + |l|). dx is rounded to BF16 once, 2^-8 of the value.
 dw: a sum whose terms pass at most H / 32 + 60 additions."""
 
 import pytest
