@@ -143,12 +143,14 @@ inline std::pair<torch::Tensor, std::optional<torch::Tensor>> swiglu_grad(const 
     const auto out = out_in.has_value() ? out_in.value() : empty_on({tokens, 2 * hidden}, torch::kBFloat16, x);
     std::optional<torch::Tensor> grad_weights;
     if (topk_weights.has_value()) grad_weights = empty_on(topk_weights->sizes(), torch::kFloat32, x);
+    const uint64_t nbytes = topk_weights.has_value() ? dg_swiglu_grad_scratch_bytes((uint32_t)tokens, (uint32_t)hidden) : 0;
+    const auto scratch = nbytes ? empty_on({(int64_t)nbytes}, torch::kUInt8, x) : torch::Tensor();
     if (x.numel() != 0)
         check(dg_swiglu_grad_launch(grad_out.data_ptr(), (uint64_t)distance_of_rows(grad_out), x.data_ptr(), (uint64_t)distance_of_rows(x), in.sf_ptr(),
                                     in.is_pair ? scale_stride(in.sf) : 0, (uint32_t)tokens, (uint32_t)hidden, float_ptr(topk_weights), int_ptr(psum), experts_of(psum),
                                     (uint32_t)expert_alignment, clamp_value.has_value() ? 1 : 0, (float)clamp_value.value_or(0.0), out.data_ptr(),
                                     (uint64_t)distance_of_rows(out), grad_weights.has_value() ? static_cast<float*>(grad_weights->data_ptr()) : nullptr, zero_padding,
-                                    stream_of(x)));
+                                    nbytes ? scratch.data_ptr() : nullptr, nbytes, stream_of(x)));
     else if (grad_weights.has_value())
         grad_weights->zero_();
     return {out, grad_weights};
@@ -215,7 +217,7 @@ inline torch::Tensor cast_from_fp8(const TensorPair& x, const torch::Dtype& out_
 }
 
 inline void check_norm(const torch::Tensor& x, const torch::Tensor& weight) {
-    host_assert(x.size(1) > 0 && x.size(1) % 32 == 0 && x.size(1) <= 32768, "the row length must be a multiple of 32, at most 32768");
+    host_assert(x.size(1) > 0 && x.size(1) % 32 == 0 && x.size(1) <= 16384, "the row length must be a multiple of 32, at most 16384");
     host_assert(x.size(0) <= INT32_MAX, "there are too many tokens");
     host_assert(weight.device() == x.device() && is_bf16_or_fp32(weight) && weight.dim() == 1 && weight.size(0) == x.size(1) && weight.is_contiguous(),
                 "weight must be a contiguous BF16 or FP32 vector of the row length, on the device of the rows");

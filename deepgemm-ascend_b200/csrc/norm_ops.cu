@@ -17,7 +17,7 @@
 
 namespace dg {
 
-constexpr uint32_t kAll = 0xffffffffu, kMostHidden = 32768;
+constexpr uint32_t kAll = 0xffffffffu, kMostHidden = 16384;
 
 // Eight channels of a lane as they lie in memory.
 template <typename T> struct Piece;
@@ -25,16 +25,18 @@ template <> struct Piece<__nv_bfloat16> {
     uint4 q;
     __device__ __forceinline__ void load(const uint8_t* p) { q = ld_stream_v4(p); }
     __device__ __forceinline__ void clear() { q = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
+    __device__ __forceinline__ void get(Pair (&v)[4]) const {
         const uint32_t w[4] = {q.x, q.y, q.z, q.w};
         #pragma unroll
-        for (int j = 0; j < 4; ++j) { v[2 * j] = bf16_lo(w[j]); v[2 * j + 1] = bf16_hi(w[j]); }
+        for (int j = 0; j < 4; ++j) v[j] = Pair(bf16_lo(w[j]), bf16_hi(w[j]));
     }
-    __device__ __forceinline__ void set(const float (&v)[8]) {
+    __device__ __forceinline__ void set(const Pair (&v)[4]) {
         uint32_t w[4];
         #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
+            float lo, hi;
+            v[j].get(lo, hi);
+            const __nv_bfloat162 p = __floats2bfloat162_rn(lo, hi);
             w[j] = *reinterpret_cast<const uint32_t*>(&p);
         }
         q = make_uint4(w[0], w[1], w[2], w[3]);
@@ -45,56 +47,47 @@ template <> struct Piece<float> {
     uint4 q, r;
     __device__ __forceinline__ void load(const uint8_t* p) { q = ld_stream_v4(p); r = ld_stream_v4(p + 16); }
     __device__ __forceinline__ void clear() { q = r = make_uint4(0u, 0u, 0u, 0u); }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        const uint32_t w[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+    __device__ __forceinline__ void get(Pair (&v)[4]) const {
+        v[0] = Pair(__uint_as_float(q.x), __uint_as_float(q.y)); v[1] = Pair(__uint_as_float(q.z), __uint_as_float(q.w));
+        v[2] = Pair(__uint_as_float(r.x), __uint_as_float(r.y)); v[3] = Pair(__uint_as_float(r.z), __uint_as_float(r.w));
     }
-    __device__ __forceinline__ void set(const float (&v)[8]) {
-        q = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
-        r = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+    __device__ __forceinline__ void set(const Pair (&v)[4]) {
+        float f[8];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) v[j].get(f[2 * j], f[2 * j + 1]);
+        q = make_uint4(__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3]));
+        r = make_uint4(__float_as_uint(f[4]), __float_as_uint(f[5]), __float_as_uint(f[6]), __float_as_uint(f[7]));
     }
     __device__ __forceinline__ void store(uint8_t* p) const {
         *reinterpret_cast<uint4*>(p) = q;
         *reinterpret_cast<uint4*>(p + 16) = r;
     }
 };
-__device__ __forceinline__ void weight_at(const void* weight, uint32_t fp32, uint32_t c, float (&v)[8]) {
+__device__ __forceinline__ void weight_at(const void* weight, uint32_t fp32, uint32_t c, Pair (&v)[4]) {
     if (fp32) {
-        const uint4 q = ld_global_v4(static_cast<const float*>(weight) + c), r = ld_global_v4(static_cast<const float*>(weight) + c + 4);
-        const uint32_t w[8] = {q.x, q.y, q.z, q.w, r.x, r.y, r.z, r.w};
-        #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(w[j]);
+        Piece<float> p;
+        p.q = ld_global_v4(static_cast<const float*>(weight) + c);
+        p.r = ld_global_v4(static_cast<const float*>(weight) + c + 4);
+        p.get(v);
     } else {
-        const uint4 q = ld_global_v4(static_cast<const __nv_bfloat16*>(weight) + c);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) { v[2 * j] = bf16_lo(w[j]); v[2 * j + 1] = bf16_hi(w[j]); }
+        Piece<__nv_bfloat16> p;
+        p.q = ld_global_v4(static_cast<const __nv_bfloat16*>(weight) + c);
+        p.get(v);
     }
 }
 
-// Sums of kRows values over the CTA, in every thread. `partial`: [warps][kRows] of shared memory that nobody reads any more.
-template <typename S, uint32_t kRows>
-__device__ __forceinline__ void cta_sums(S (&v)[kRows], S* partial) {
-    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32, warps = blockDim.x / 32;
+// The sum over a group of `warps` warps, of which `first` is the first, in all its threads. `partial`: a place for each warp of the CTA that nobody reads any more.
+template <typename S>
+__device__ __forceinline__ S group_sum(S v, S* partial, uint32_t first, uint32_t warps, uint32_t barrier) {
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     #pragma unroll
-    for (uint32_t r = 0; r < kRows; ++r)
-        #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) v[r] += __shfl_xor_sync(kAll, v[r], o);
-    if (lane < kRows) {
-        S mine = v[0];
-        #pragma unroll
-        for (uint32_t r = 1; r < kRows; ++r) mine = lane == r ? v[r] : mine;
-        partial[warp * kRows + lane] = mine;
-    }
-    __syncthreads();
-    // lane = (a warp, a row); the rows' sums end up in lanes 0 .. kRows - 1
-    S sum = 0;
-    for (uint32_t at = lane; at < warps * kRows; at += 32) sum += partial[at];
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+    if (lane == 0) partial[warp] = v;
+    named_bar_sync(barrier, warps * 32);
+    v = lane < warps ? partial[first + lane] : (S)0;
     #pragma unroll
-    for (uint32_t o = 16; o >= kRows; o >>= 1) sum += __shfl_xor_sync(kAll, sum, o);
-    #pragma unroll
-    for (uint32_t r = 0; r < kRows; ++r) v[r] = __shfl_sync(kAll, sum, r);
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+    return v;
 }
 
 struct NormArgs {
@@ -123,8 +116,8 @@ __device__ __forceinline__ float rsqrt_of(double m) {
 
 // A CTA walks tokens at a distance of the grid, a thread kPieces x 8 channels of each. With kAhead the next token is asked for before the sum over
 // the CTA: what keeps HBM busy over the barrier.
-template <typename T, uint32_t kPieces, bool kAhead>
-__global__ void __launch_bounds__(kPieces == 1 ? 1024 : 512, kPieces == 2 ? 2 : 1) rms_norm_fp8_kernel(const NormArgs a) {
+template <typename T, uint32_t kPieces, uint32_t kThreads, uint32_t kCtas, bool kAhead>
+__global__ void __launch_bounds__(kThreads, kCtas) rms_norm_fp8_kernel(const NormArgs a) {
     __shared__ double partial[2][32];
     const uint32_t lane = threadIdx.x % 32;
     griddep_wait();
@@ -146,40 +139,47 @@ __global__ void __launch_bounds__(kPieces == 1 ? 1024 : 512, kPieces == 2 ? 2 : 
     for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x, turn ^= 1) {
         if (!kAhead) load(token);
         Piece<T> h[kPieces];
-        double sum[1] = {0.0};
+        double sum = 0.0;
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
             const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
-            float v[8];
+            Pair v[4];
             h[i] = x[i];
             if (a.residual) {
-                float u[8];
+                Pair u[4];
                 x[i].get(v);
                 more[i].get(u);
                 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] += u[j];
+                for (int j = 0; j < 4; ++j) v[j] = v[j] + u[j];
                 h[i].set(v);
                 if (c < a.hidden) h[i].store(a.h + token * a.h_stride + (uint64_t)c * sizeof(T));
             }
             h[i].get(v);
             #pragma unroll
-            for (int j = 0; j < 8; ++j) sum[0] = fma((double)v[j], (double)v[j], sum[0]);
+            for (int j = 0; j < 4; ++j) {
+                float lo, hi;
+                v[j].get(lo, hi);
+                sum = fma((double)lo, (double)lo, sum);
+                sum = fma((double)hi, (double)hi, sum);
+            }
         }
         if (kAhead && token + gridDim.x < a.tokens) load(token + gridDim.x);
         // (two sets of shared memory: a warp that is a turn ahead does not write to what another still reads)
-        cta_sums<double, 1>(sum, partial[turn]);
-        const float rstd = rsqrt_of(fma(sum[0], a.inverse_hidden, (double)a.eps));
+        sum = group_sum(sum, partial[turn], 0, blockDim.x / 32, 1);
+        const float rstd = rsqrt_of(fma(sum, a.inverse_hidden, (double)a.eps));
         if (threadIdx.x == 0) a.rstd[token] = rstd;
+        const Pair scale(rstd);
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
             const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
-            float w[8] = {}, v[8], amax = 0.0f;
+            Pair w[4] = {}, v[4];
             if (c < a.hidden) weight_at(a.weight, a.weight_fp32, c, w);
             h[i].get(v);
+            float amax = 0.0f;
             #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                v[j] = __fmul_rn(__fmul_rn(v[j], rstd), w[j]);
-                amax = fmaxf(amax, fabsf(v[j]));
+            for (int j = 0; j < 4; ++j) {
+                v[j] = v[j] * scale * w[j];
+                amax = larger_magnitude(amax, v[j]);
             }
             amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 2));
@@ -198,9 +198,12 @@ __global__ void __launch_bounds__(kPieces == 1 ? 1024 : 512, kPieces == 2 ? 2 : 
     }
 }
 
-// The gradient. With n = h * rstd, u = g * weight: dx = rstd (u - n mean(u n)) + grad_h, dweight = sum over the tokens of g n. A CTA walks tokens at a
-// distance of the grid, holds its channels' part of dweight in registers (FP32) and writes it to `partial` at the end, which a second
-// kernel sums in the order of the CTAs: nothing depends on timing.
+// The gradient. With n = h * rstd, u = g * weight: dx = rstd (u - n mean(u n)) + grad_h, dweight = sum over the tokens of g n. A group of a CTA's warps takes
+// a token, and walks tokens at a distance of all groups; a thread holds its channels' part of dweight in registers (FP32), the groups of a CTA add theirs up,
+// and a second kernel sums the CTAs' in their order: nothing depends on timing.
+//
+// HBM-bound, and what bounds the walk is the way from a token's loads over its barrier to its stores: with kAhead the next token is asked for in front of the
+// barrier.
 struct NormGradArgs {
     const uint8_t* g; uint64_t g_stride;                                 // BF16 or FP32 as `h` is, or BF16 beside FP32
     const uint8_t *h, *grad_h; uint64_t h_stride, grad_h_stride;         // bytes between rows; grad_h or nullptr
@@ -209,22 +212,25 @@ struct NormGradArgs {
     uint8_t* dx; uint64_t dx_stride;
     float* partial;                                                      // [gridDim.x][hidden]
     uint32_t tokens, hidden;
+    uint32_t groups, threads;                                            // of a CTA; of a group
     float inverse_hidden;
 };
 
-template <typename T, typename G, uint32_t kPieces, bool kAhead>
-__global__ void __launch_bounds__(kPieces == 1 ? 1024 : 512, kPieces == 2 ? 2 : 1) rms_norm_grad_kernel(const NormGradArgs a) {
+template <typename T, typename G, uint32_t kPieces, uint32_t kThreads, bool kAhead>
+__global__ void __launch_bounds__(kThreads) rms_norm_grad_kernel(const NormGradArgs a) {
+    extern __shared__ __align__(16) uint8_t others[];
     __shared__ float sums[2][32];
+    const uint32_t group = threadIdx.x / a.threads, t = threadIdx.x - group * a.threads, warps = a.threads / 32;
+    const uint64_t stride = (uint64_t)gridDim.x * a.groups, first = (uint64_t)blockIdx.x * a.groups + group;
     griddep_wait();
     griddep_launch_dependents();
-    float w[kPieces][8], dw[kPieces][8];
     Piece<T> h[kPieces], more[kPieces];
     Piece<G> g[kPieces];
     float rstd = 0.0f;
     const auto load = [&](uint64_t token) {
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
-            const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
+            const uint32_t c = (i * a.threads + t) * 8;
             if (c >= a.hidden) continue;
             h[i].load(a.h + token * a.h_stride + (uint64_t)c * sizeof(T));
             g[i].load(a.g + token * a.g_stride + (uint64_t)c * sizeof(G));
@@ -232,61 +238,89 @@ __global__ void __launch_bounds__(kPieces == 1 ? 1024 : 512, kPieces == 2 ? 2 : 
         }
         rstd = __uint_as_float(ld_global_u32(a.rstd + token));
     };
-    #pragma unroll
-    for (uint32_t i = 0; i < kPieces; ++i) { h[i].clear(); g[i].clear(); more[i].clear(); }
-    if (kAhead) load(blockIdx.x);
+    Pair sum_w[kPieces][4];
     #pragma unroll
     for (uint32_t i = 0; i < kPieces; ++i) {
-        const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
+        h[i].clear(); g[i].clear(); more[i].clear();
         #pragma unroll
-        for (int j = 0; j < 8; ++j) w[i][j] = dw[i][j] = 0.0f;
-        if (c < a.hidden) weight_at(a.weight, a.weight_fp32, c, w[i]);
+        for (int j = 0; j < 4; ++j) sum_w[i][j] = Pair(0.0f);
     }
+    if (kAhead && first < a.tokens) load(first);
     uint32_t turn = 0;
-    for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x, turn ^= 1) {
+    for (uint64_t token = first; token < a.tokens; token += stride, turn ^= 1) {
         if (!kAhead) load(token);
         Piece<T> h0[kPieces], more0[kPieces];
         Piece<G> g0[kPieces];
         const float r = rstd;
-        float dot[1] = {0.0f};
+        const Pair scale(r);
+        // sum(u n) = rstd sum(u h)
+        Pair dots(0.0f);
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
+            const uint32_t c = (i * a.threads + t) * 8;
             h0[i] = h[i]; more0[i] = more[i]; g0[i] = g[i];
-            float n[8], u[8];
+            Pair n[4], u[4], w[4] = {};
+            if (c < a.hidden) weight_at(a.weight, a.weight_fp32, c, w);
             h0[i].get(n);
             g0[i].get(u);
             #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                n[j] *= r;
-                dw[i][j] = fmaf(u[j], n[j], dw[i][j]);
-                dot[0] = fmaf(u[j] * w[i][j], n[j], dot[0]);
+            for (int j = 0; j < 4; ++j) {
+                dots = fma2(u[j] * w[j], n[j], dots);
+                sum_w[i][j] = fma2(u[j], n[j] * scale, sum_w[i][j]);
             }
         }
-        if (kAhead && token + gridDim.x < a.tokens) load(token + gridDim.x);
-        cta_sums<float, 1>(dot, sums[turn]);
-        const float mean = dot[0] * a.inverse_hidden;
+        if (kAhead && token + stride < a.tokens) load(token + stride);
+        float dot, other;
+        dots.get(dot, other);
+        // (two sets of sums: a warp that is a turn ahead does not write to what another still reads)
+        dot = group_sum(dot + other, sums[turn], group * warps, warps, group + 1);
+        // dx = rstd u - h (rstd^3 mean(u h)) + grad_h
+        const Pair slope(-(r * r * (r * (dot * a.inverse_hidden))));
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
-            const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
+            const uint32_t c = (i * a.threads + t) * 8;
             if (c >= a.hidden) continue;
-            float n[8], u[8], d[8];
+            Pair n[4], u[4], d[4], w[4];
+            weight_at(a.weight, a.weight_fp32, c, w);
             h0[i].get(n);
             g0[i].get(u);
             more0[i].get(d);
             #pragma unroll
-            for (int j = 0; j < 8; ++j) d[j] += r * (u[j] * w[i][j] - n[j] * r * mean);
-            Piece<T> out;
-            out.set(d);
-            out.store(a.dx + token * a.dx_stride + (uint64_t)c * sizeof(T));
+            for (int j = 0; j < 4; ++j) d[j] = fma2(n[j], slope, fma2(scale, u[j] * w[j], d[j]));
+            h0[i].set(d);
+            h0[i].store(a.dx + token * a.dx_stride + (uint64_t)c * sizeof(T));
         }
+    }
+    float dw[kPieces][8];
+    #pragma unroll
+    for (uint32_t i = 0; i < kPieces; ++i)
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) sum_w[i][j].get(dw[i][2 * j], dw[i][2 * j + 1]);
+    if (a.groups > 1) {
+        float4* const to = reinterpret_cast<float4*>(others);
+        #pragma unroll
+        for (uint32_t i = 0; i < kPieces; ++i)
+            #pragma unroll
+            for (uint32_t k = 0; k < 2; ++k)
+                if (group > 0) to[((group - 1) * 2 * kPieces + 2 * i + k) * a.threads + t] = make_float4(dw[i][4 * k], dw[i][4 * k + 1], dw[i][4 * k + 2], dw[i][4 * k + 3]);
+        __syncthreads();
+        if (group > 0) return;
+        for (uint32_t o = 0; o + 1 < a.groups; ++o)
+            #pragma unroll
+            for (uint32_t i = 0; i < kPieces; ++i)
+                #pragma unroll
+                for (uint32_t k = 0; k < 2; ++k) {
+                    const float4 v = to[(o * 2 * kPieces + 2 * i + k) * a.threads + t];
+                    dw[i][4 * k] += v.x; dw[i][4 * k + 1] += v.y; dw[i][4 * k + 2] += v.z; dw[i][4 * k + 3] += v.w;
+                }
     }
     #pragma unroll
     for (uint32_t i = 0; i < kPieces; ++i) {
-        const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
+        const uint32_t c = (i * a.threads + t) * 8;
         if (c >= a.hidden) continue;
-        Piece<float> out;
-        out.set(dw[i]);
-        out.store(reinterpret_cast<uint8_t*>(a.partial + (uint64_t)blockIdx.x * a.hidden + c));
+        float4* const out = reinterpret_cast<float4*>(a.partial + (uint64_t)blockIdx.x * a.hidden + c);
+        out[0] = make_float4(dw[i][0], dw[i][1], dw[i][2], dw[i][3]);
+        out[1] = make_float4(dw[i][4], dw[i][5], dw[i][6], dw[i][7]);
     }
 }
 
@@ -310,17 +344,21 @@ __global__ void __launch_bounds__(kSumThreads) rms_norm_grad_sum_kernel(const fl
 
 // Threads of a CTA whose threads take `pieces` pieces of a row each.
 static uint32_t norm_threads(uint32_t hidden, uint32_t pieces) { return ((hidden / 8 + pieces - 1) / pieces + 31) / 32 * 32; }
-// CTAs on the 148 SMs: with up to two pieces a thread has 64 registers, beyond that 128.
-static uint32_t norm_ctas(uint32_t tokens, uint32_t hidden, uint32_t pieces) {
-    const uint32_t most = 148 * (pieces <= 2 ? 1024 / norm_threads(hidden, pieces) : 1);
-    return tokens < most ? tokens : most;
+
+// How the gradient's kernel is laid over the SMs, one CTA each: one piece of a row a thread where that takes at most 896 threads (512 of FP32), in as many groups
+// as fit, else four; as many CTAs as finish together.
+struct NormGradShape { uint32_t pieces, threads, groups, parts; };
+static NormGradShape norm_grad_shape(uint32_t tokens, uint32_t hidden, bool fp32) {
+    const uint32_t most = fp32 ? 512 : 896;
+    NormGradShape s{};
+    s.pieces = norm_threads(hidden, 1) <= most ? 1 : 4;
+    s.threads = norm_threads(hidden, s.pieces);
+    s.groups = s.pieces == 4 ? 1 : most / s.threads < 8 ? most / s.threads : 8;
+    while (s.groups > 1 && (s.groups - 1) * 148 >= tokens) --s.groups;
+    const uint32_t wanted = (tokens + s.groups - 1) / s.groups, turns = (wanted + 147) / 148;
+    s.parts = turns ? (wanted + turns - 1) / turns : 0;
+    return s;
 }
-// Pieces of a row for a thread: one while the row fits `most` threads, then two where there are such kernels, four, eight.
-static uint32_t norm_pieces(uint32_t hidden, uint32_t most, bool two) {
-    if (norm_threads(hidden, 1) <= most) return 1;
-    return two && norm_threads(hidden, 2) <= 512 ? 2 : norm_threads(hidden, 4) <= 512 ? 4 : 8;
-}
-static uint32_t norm_grad_parts(uint32_t tokens, uint32_t hidden) { return norm_ctas(tokens, hidden, norm_pieces(hidden, 1024, false)); }
 
 }  // namespace dg
 
@@ -332,13 +370,6 @@ static int norm_checks(uint32_t tokens, uint32_t hidden) {
     return DG_OK;
 }
 static bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<uintptr_t>(p) | stride_bytes) % 16 == 0; }
-
-template <typename T>
-static const void* norm_kernel(uint32_t pieces) {
-    if constexpr (sizeof(T) == 2)
-        if (pieces == 2) return (const void*)rms_norm_fp8_kernel<T, 2, true>;
-    return pieces == 1 ? (const void*)rms_norm_fp8_kernel<T, 1, true> : pieces == 4 ? (const void*)rms_norm_fp8_kernel<T, 4, false> : (const void*)rms_norm_fp8_kernel<T, 8, false>;
-}
 
 extern "C" int dg_rms_norm_fp8_launch(const void* x, int is_fp32, uint64_t x_stride, const void* residual, uint64_t residual_stride, void* h, uint64_t h_stride,
                                       const void* weight, int weight_is_fp32, float eps, uint32_t tokens, uint32_t hidden, void* out, uint64_t out_stride,
@@ -362,19 +393,34 @@ extern "C" int dg_rms_norm_fp8_launch(const void* x, int is_fp32, uint64_t x_str
     a.sf = reinterpret_cast<uint8_t*>(out_sf); a.sf_col_stride = sf_col_stride * 2;
     a.rstd = rstd; a.tokens = tokens; a.hidden = hidden; a.eps = eps;
     a.inverse_hidden = 1.0 / hidden;
-    // Few tokens: as many threads as a row has pieces; many of BF16: at most 512, so that two CTAs are on an SM. (FP32 has twice the bytes in each.)
-    const uint32_t pieces = norm_pieces(hidden, is_fp32 || tokens <= 148 ? 1024 : 512, !is_fp32);
+    // Few tokens: as many threads as a row has pieces. Many of BF16: half as many, and two CTAs on an SM. (FP32 has twice the bytes in each.)
+    const void* fn;
+    uint32_t pieces = 1, resident = 1;
+    if (norm_threads(hidden, 1) <= (is_fp32 || tokens <= 148 ? 1024 : 448)) {
+        resident = 896 / norm_threads(hidden, pieces);
+        fn = is_fp32 ? (const void*)rms_norm_fp8_kernel<float, 1, 1024, 1, true> : (const void*)rms_norm_fp8_kernel<__nv_bfloat16, 1, 1024, 1, true>;
+    } else if (!is_fp32 && norm_threads(hidden, 2) <= 448) {
+        pieces = 2;
+        resident = 896 / norm_threads(hidden, pieces);
+        fn = (const void*)rms_norm_fp8_kernel<__nv_bfloat16, 2, 448, 2, true>;
+    } else {
+        pieces = 4;
+        fn = is_fp32 ? (const void*)rms_norm_fp8_kernel<float, 4, 512, 1, false> : (const void*)rms_norm_fp8_kernel<__nv_bfloat16, 4, 512, 1, true>;
+    }
+    resident = resident < 1 ? 1 : resident > 16 ? 16 : resident;
     void* params[] = {&a};
-    return launch_overlapped(is_fp32 ? norm_kernel<float>(pieces) : norm_kernel<__nv_bfloat16>(pieces), dim3(norm_ctas(tokens, hidden, pieces)),
-                             dim3(norm_threads(hidden, pieces)), params, static_cast<cudaStream_t>(stream));
+    return launch_overlapped(fn, dim3(tokens < 148 * resident ? tokens : 148 * resident), dim3(norm_threads(hidden, pieces)), params, static_cast<cudaStream_t>(stream));
 }
 
-extern "C" uint64_t dg_rms_norm_grad_scratch_bytes(uint32_t tokens, uint32_t hidden) { return hidden ? (uint64_t)norm_grad_parts(tokens, hidden) * hidden * 4 : 0; }
+extern "C" uint64_t dg_rms_norm_grad_scratch_bytes(uint32_t tokens, uint32_t hidden) {
+    if (hidden == 0) return 0;
+    const uint32_t bf16 = norm_grad_shape(tokens, hidden, false).parts, fp32 = norm_grad_shape(tokens, hidden, true).parts;
+    return (uint64_t)(bf16 > fp32 ? bf16 : fp32) * hidden * 4;
+}
 
 template <typename T, typename G>
 static const void* norm_grad_kernel(uint32_t pieces) {
-    return pieces == 1 ? (const void*)rms_norm_grad_kernel<T, G, 1, true> : pieces == 4 ? (const void*)rms_norm_grad_kernel<T, G, 4, false>
-                                                                                        : (const void*)rms_norm_grad_kernel<T, G, 8, false>;
+    return pieces == 1 ? (const void*)rms_norm_grad_kernel<T, G, 1, sizeof(T) == 4 ? 512 : 896, true> : (const void*)rms_norm_grad_kernel<T, G, 4, 512, false>;
 }
 
 extern "C" int dg_rms_norm_grad_launch(const void* grad_out, int grad_is_fp32, uint64_t grad_stride, const void* h, int is_fp32, uint64_t h_stride, const void* weight,
@@ -402,12 +448,14 @@ extern "C" int dg_rms_norm_grad_launch(const void* grad_out, int grad_is_fp32, u
     a.partial = static_cast<float*>(scratch);
     a.tokens = tokens; a.hidden = hidden;
     a.inverse_hidden = 1.0f / (float)hidden;
-    const uint32_t pieces = norm_pieces(hidden, 1024, false);
-    uint32_t parts = norm_grad_parts(tokens, hidden);
-    const void* fn = !is_fp32 ? norm_grad_kernel<__nv_bfloat16, __nv_bfloat16>(pieces) : grad_is_fp32 ? norm_grad_kernel<float, float>(pieces)
-                                                                                                      : norm_grad_kernel<float, __nv_bfloat16>(pieces);
+    const NormGradShape shape = norm_grad_shape(tokens, hidden, is_fp32);
+    a.groups = shape.groups; a.threads = shape.threads;
+    uint32_t parts = shape.parts;
+    const void* fn = !is_fp32 ? norm_grad_kernel<__nv_bfloat16, __nv_bfloat16>(shape.pieces) : grad_is_fp32 ? norm_grad_kernel<float, float>(shape.pieces)
+                                                                                             : norm_grad_kernel<float, __nv_bfloat16>(shape.pieces);
     void* params[] = {&a};
-    if (int rc = launch_overlapped(fn, dim3(parts), dim3(norm_threads(hidden, pieces)), params, static_cast<cudaStream_t>(stream))) return rc;
+    if (int rc = launch_overlapped(fn, dim3(parts), dim3(shape.groups * shape.threads), params, static_cast<cudaStream_t>(stream),
+                                   (shape.groups - 1) * shape.threads * shape.pieces * 32)) return rc;
     const float* from = a.partial;
     void* sum_params[] = {&from, &grad_weight, &parts, &hidden};
     return launch_overlapped((const void*)rms_norm_grad_sum_kernel, dim3(hidden / kSumChannels), dim3(kSumThreads), sum_params, static_cast<cudaStream_t>(stream));

@@ -40,6 +40,36 @@ __device__ __forceinline__ float fast_reciprocal(float x) {
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+// Two FP32 numbers in one instruction.
+struct Pair {
+    uint64_t v;
+    Pair() = default;
+    __device__ __forceinline__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ explicit Pair(float a) : Pair(a, a) {}
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ Pair operator*(const Pair& a, const Pair& b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Pair operator+(const Pair& a, const Pair& b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Pair fma2(const Pair& a, const Pair& b, const Pair& c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+// The largest of m and both magnitudes (a NaN does not count).
+__device__ __forceinline__ float larger_magnitude(float m, const Pair& p) {
+    float a, b, d;
+    p.get(a, b);
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(m), "f"(fabsf(a)), "f"(fabsf(b)));
+    return d;
+}
 constexpr float kLog2E = 1.4426950408889634f;
 
 // ---- E4M3: scale = max(amax, floor) * (1/448) rounded up to a power of two, 2^-126 or more; exponent byte from the bit pattern (255 = NaN
@@ -61,6 +91,17 @@ __device__ __forceinline__ uint2 e4m3_pack8(const float (&v)[8], uint32_t e) {
     return make_uint2(q[0], q[1]);
 }
 
+__device__ __forceinline__ uint2 e4m3_pack8(const Pair (&v)[4], uint32_t e) {
+    const Pair inv(__uint_as_float((254u - e) << 23));
+    uint32_t q[4];
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float2 f;
+        (v[j] * inv).get(f.x, f.y);
+        q[j] = (uint32_t)__nv_cvt_float2_to_fp8x2(f, __NV_SATFINITE, __NV_E4M3);
+    }
+    return make_uint2(q[0] | q[1] << 16, q[2] | q[3] << 16);
+}
 // Four E4M3 codes as FP32, exactly.
 __device__ __forceinline__ void e4m3_unpack4(uint32_t q, float (&v)[4]) {
     #pragma unroll

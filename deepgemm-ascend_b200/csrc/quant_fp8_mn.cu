@@ -8,6 +8,9 @@
 // HBM-bound: 2 (or 1 + 1/32) bytes read and 1 + 1/32 written per value.
 #include <cuda_runtime.h>
 #include <stdint.h>
+#include <string.h>
+
+#include <type_traits>
 
 #include "../../include/dg_b200.h"
 #include "host_common.h"
@@ -16,7 +19,8 @@
 
 namespace dg {
 
-constexpr uint32_t kMnThreads = 256, kMnCols = 256, kMnRows = 64;
+constexpr uint32_t kMnThreads = 128, kMnCols = 128, kMnRows = 64;      // a CTA of the quantiser: a thread a column of its scales
+constexpr uint32_t kBackThreads = 256, kBackCols = 256, kBackRows = 32; // and of the way back
 
 struct MnArgs {
     const uint8_t* x; uint64_t x_stride, x_group_stride;                  // bytes: BF16, or E4M3 with scales along the rows
@@ -25,11 +29,12 @@ struct MnArgs {
     uint8_t* sf; uint64_t sf_stride, sf_group_stride;                     // int16 [ceil(rows / 64)][cols] seen as bytes
     const int32_t* psum; uint32_t num_experts, alignment;
     uint32_t rows, cols, tiles_c;
-    float floor;
+    float floor; uint32_t least;                                          // the least amax, and the scale byte of it
 };
 
 // Eight values in each of a lane's eight rows -> codes and scale bytes, through FP32.
-__device__ __forceinline__ void quantise_down(const float (&v)[8][8], float floor, uint32_t (&e)[8], uint2 (&codes)[8]) {
+__device__ __forceinline__ void quantise_down(const float (&v)[8][8], float floor, uint32_t (&bytes)[2], uint2 (&codes)[8]) {
+    uint32_t e[8];
     #pragma unroll
     for (int j = 0; j < 8; ++j) {
         // (as whole numbers: infinities and NaN come out on top)
@@ -47,11 +52,13 @@ __device__ __forceinline__ void quantise_down(const float (&v)[8][8], float floo
         for (int j = 0; j < 8; ++j) s[j] = v[i][j] * __uint_as_float((254u - min(e[j], 254u)) << 23);
         codes[i] = e4m3_pack8(s, 127u);
     }
+    bytes[0] = e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24;
+    bytes[1] = e[4] | e[5] << 8 | e[6] << 16 | e[7] << 24;
 }
 
 // BF16 rows, two values at a time: magnitudes are compared as whole numbers, products with the inverse scales are exact.
-__device__ __forceinline__ void quantise_down_bf16(const uint4 (&q)[8], float floor, uint32_t (&e)[8], uint2 (&codes)[8]) {
-    uint32_t m[4] = {}, f[4];
+__device__ __forceinline__ void quantise_down_bf16(const uint4 (&q)[8], float floor, uint32_t (&bytes)[2], uint2 (&codes)[8]) {
+    uint32_t m[4] = {}, f[4], e[8];
     #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
@@ -79,107 +86,131 @@ __device__ __forceinline__ void quantise_down_bf16(const uint4 (&q)[8], float fl
         }
         codes[i] = e4m3_pack8(s, 127u);
     }
+    bytes[0] = e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24;
+    bytes[1] = e[4] | e[5] << 8 | e[6] << 16 | e[7] << 24;
 }
 
-// E4M3 rows with scale bytes b (of this lane's block) through FP16, two values at a time, relative to the largest byte of the warp's rows: the codes are FP16
-// numbers and their factors powers of two. Exact while no factor is below 2^-15 and the columns' inverse scales lie in 2^-15 .. 2^15; answers whether
-// that is so (the same in all lanes), which it is where the magnitudes of a tile's rows and columns lie within a few thousand.
-__device__ __forceinline__ bool quantise_down_fp8(const uint2 (&q)[8], const uint32_t (&b)[8], float floor, uint32_t (&e)[8], uint2 (&codes)[8]) {
-    uint32_t top = 0, low = 255;
+__device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
+    const __half2 p = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+// The larger magnitude of each half, NaN if one is.
+__device__ __forceinline__ uint32_t larger_f16x2(uint32_t m, uint32_t v) {
+    const __half2 p = __hmax2_nan(*reinterpret_cast<const __half2*>(&m), __habs2(*reinterpret_cast<const __half2*>(&v)));
+    return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t e4m3_to_f16x2(uint32_t pair) {
+    const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)pair, __NV_E4M3);
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ uint32_t f16x2_to_e4m3(uint32_t v) {
+    return (uint32_t)__nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&v), __NV_SATFINITE, __NV_E4M3);
+}
+
+// E4M3 rows with scale bytes b (of this lane's block) through FP16, two values at a time, relative to the largest byte of the warp's rows, `top`: the codes are
+// FP16 numbers h, the rows' factors 2^(b - top) and the columns' 2^(top - e) powers of two. Exact while the former are 2^-15 or more and the latter lie in
+// 2^-14 .. 2^15; answers whether that is so (the same in all lanes), which it is where the magnitudes of a tile's rows and columns lie within a
+// few thousand. The scale bytes of two columns at a time: amax <= 448 s = 1.75 x 2^8 s, so with amax = 1.m x 2^x (m of ten bits) s is 2^(x - 8), or twice that
+// where m is above 0.75, which is an addition to the bits that carries; `least` is the byte of the least amax.
+__device__ __forceinline__ bool quantise_down_fp8(const uint2 (&q)[8], const uint32_t (&b)[8], uint32_t least, uint32_t (&bytes)[2], uint2 (&codes)[8]) {
+    uint32_t top = b[0], low = b[0];
     #pragma unroll
-    for (int i = 0; i < 8; ++i) { top = max(top, b[i]); low = min(low, b[i]); }
+    for (int i = 1; i < 8; ++i) { top = max(top, b[i]); low = min(low, b[i]); }
     top = __reduce_max_sync(0xffffffffu, top);
     low = __reduce_min_sync(0xffffffffu, low);
     if (top == 255u || low == 0u || top - low > 15u) return false;
     uint32_t h[8][4], m[4] = {}, f[4];
     #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        // 2^(b - top) in both halves (2^-15 is a subnormal number of FP16)
-        const uint32_t d = top - b[i], factor = (d == 15u ? 0x0200u : (15u - d) << 10) * 0x10001u;
+        // (2^-15 is a subnormal number of FP16)
+        const uint32_t d = top - b[i], factor = max((15u - d) << 10, 0x0200u) * 0x10001u;
         #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((j < 2 ? q[i].x : q[i].y) >> (16 * (j % 2))), __NV_E4M3);
-            const __half2 p = __hmul2(*reinterpret_cast<const __half2*>(&r), *reinterpret_cast<const __half2*>(&factor));
-            h[i][j] = *reinterpret_cast<const uint32_t*>(&p);
-            m[j] = __vmaxu2(m[j], h[i][j] & 0x7fff7fffu);
+            h[i][j] = mul_f16x2(e4m3_to_f16x2((j < 2 ? q[i].x : q[i].y) >> (16 * (j % 2))), factor);
+            m[j] = larger_f16x2(m[j], h[i][j]);
         }
     }
     bool fits = true;
+    const uint32_t offset = ((top - 23u) & 0xffffu) * 0x10001u, floor = least * 0x10001u;
     #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        m[j] = __vmaxu2(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
-        m[j] = __vmaxu2(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
-        const float2 largest = __half22float2(*reinterpret_cast<const __half2*>(&m[j]));
-        f[j] = 0;
-        #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const float v = k ? largest.y : largest.x;
-            e[2 * j + k] = e4m3_scale_byte(v * __uint_as_float(top << 23), floor);
-            // 2^(top - e); a column of zeros is one under any factor
-            const int32_t x = v == 0.0f ? 0 : (int32_t)top - (int32_t)e[2 * j + k];
-            fits &= x >= -15 && x <= 15 && v == v;
-            f[j] |= (x == -15 ? 0x0200u : (uint32_t)(15 + x) << 10) << (16 * k);
-        }
+        m[j] = larger_f16x2(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
+        m[j] = larger_f16x2(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
+        // (the exponent field is x + 15; a subnormal m stands for no more than top - 22, which `least` covers or the factor shows)
+        const uint32_t some = __vcmpgtu2(m[j], 0u), e = (__vmaxs2(__vadd2(((m[j] + 0x00ff00ffu) >> 10) & 0x003f003fu, offset), floor) & some) | (floor & ~some);
+        const uint32_t x = __vsub2(top * 0x10001u, e), x_in = __vmins2(__vmaxs2(x, 0xfff2fff2u), 0x000f000fu);
+        // (a column of zeros is one under any factor; a NaN is above all codes)
+        fits &= ((x ^ x_in) & some) == 0u && __vmaxu2(m[j], 0x5f005f00u) == 0x5f005f00u;
+        f[j] = __vadd2(x_in, 0x000f000fu) << 10;
+        const uint32_t two = __byte_perm(e, 0u, 0x4420);
+        if (j % 2 == 0) bytes[j / 2] = two & 0xffffu;
+        else bytes[j / 2] |= two << 16;
     }
     if (!__all_sync(0xffffffffu, fits)) return false;
     #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        uint32_t w[2];
-        #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const __half2 lo = __hmul2(*reinterpret_cast<const __half2*>(&h[i][2 * k]), *reinterpret_cast<const __half2*>(&f[2 * k]));
-            const __half2 hi = __hmul2(*reinterpret_cast<const __half2*>(&h[i][2 * k + 1]), *reinterpret_cast<const __half2*>(&f[2 * k + 1]));
-            w[k] = (uint32_t)__nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(lo), __NV_SATFINITE, __NV_E4M3) |
-                   (uint32_t)__nv_cvt_halfraw2_to_fp8x2(static_cast<__half2_raw>(hi), __NV_SATFINITE, __NV_E4M3) << 16;
-        }
-        codes[i] = make_uint2(w[0], w[1]);
-    }
+    for (int i = 0; i < 8; ++i)
+        codes[i] = make_uint2(f16x2_to_e4m3(mul_f16x2(h[i][0], f[0])) | f16x2_to_e4m3(mul_f16x2(h[i][1], f[1])) << 16,
+                              f16x2_to_e4m3(mul_f16x2(h[i][2], f[2])) | f16x2_to_e4m3(mul_f16x2(h[i][3], f[3])) << 16);
     return true;
 }
 
-// One CTA = 64 rows x 256 columns, a warp 32 rows x 64 columns: lane = (every fourth row, eight columns), so that the maximum down a column takes
+__device__ __forceinline__ void load_raw(uint2& q, const uint8_t* p) { q = ld_stream_v2(p); }
+__device__ __forceinline__ void load_raw(uint4& q, const uint8_t* p) { q = ld_stream_v4(p); }
+
+// One CTA = 64 rows x 128 columns, a warp 32 rows x 64 columns: lane = (every fourth row, eight columns), so that the maximum down a column takes
 // two shuffles, and a row of the warp's tile is a line of 128 bytes of BF16 or two whole sectors of codes. The 64 columns are one column of the
 // scales of an 8-bit input, whose 32 rows are one read of 64 bytes.
 template <bool kFromFp8>
-__global__ void __launch_bounds__(kMnThreads, 3) quant_fp8_mn_kernel(const MnArgs a) {
+__global__ void __launch_bounds__(kMnThreads, 8) quant_fp8_mn_kernel(const MnArgs a) {
     __shared__ __align__(8) uint8_t sf_smem[2][kMnCols];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint64_t group = blockIdx.z;
     const uint32_t row_base = blockIdx.x / a.tiles_c * kMnRows, c0 = blockIdx.x % a.tiles_c * kMnCols;
-    const uint32_t half = warp / 4, tc = warp % 4 * 64 + lane % 8 * 8, c = c0 + tc;
-    const uint32_t warp_row = row_base + half * 32, r0 = warp_row + lane / 8;
+    const uint32_t half = warp / (kMnCols / 64), tc = warp % (kMnCols / 64) * 64 + lane % 8 * 8, c = c0 + tc;
+    const uint32_t warp_col = c0 + tc / 64 * 64, warp_row = row_base + half * 32, r0 = warp_row + lane / 8;
     griddep_wait();
     griddep_launch_dependents();
     const uint32_t write_end = min(a.rows, row_base + kMnRows);
+    const uint8_t* x = a.x + group * a.x_group_stride + (uint64_t)r0 * a.x_stride + (uint64_t)c * (kFromFp8 ? 1 : 2);
+    // (the same for the whole CTA: no bounds inside) What lies there is asked for before it is known which rows count.
+    const bool inside = row_base + kMnRows <= a.rows && c0 + kMnCols <= a.cols;
+    using Raw = typename std::conditional<kFromFp8, uint2, uint4>::type;
+    Raw q[8];
+    uint32_t pair = 0x7f7fu;                                  // scales of this lane's row of the tile
+    if (inside) {
+        #pragma unroll
+        for (uint32_t i = 0; i < 8; ++i, x += 4 * a.x_stride) load_raw(q[i], x);
+    } else {
+        #pragma unroll
+        for (uint32_t i = 0; i < 8; ++i, x += 4 * a.x_stride) {
+            q[i] = Raw{};
+            if (r0 + i * 4 < a.rows && c < a.cols) load_raw(q[i], x);
+        }
+    }
+    if (kFromFp8 && warp_col < a.cols && warp_row + lane < a.rows)
+        pair = ld_global_u16(a.x_sf + group * a.x_sf_group_stride + (uint64_t)(warp_col / 64) * a.x_sf_stride + (uint64_t)(warp_row + lane) * 2);
     uint32_t row_end = write_end;
     if (a.psum != nullptr) {
         // (groups start on multiples of 64 rows: a tile lies in one) Rows of the padding count as zeros and are written as zeros
         const GroupEnd end = group_end_of(a.psum, a.num_experts, a.alignment, row_base, lane);
         if (end.whole <= row_base) return;                // behind the last group (uniform over the CTA)
         row_end = min(row_end, end.valid);
+        if (row_end < write_end) {
+            #pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                if (r0 + i * 4 >= row_end) q[i] = Raw{};
+        }
     }
-    const uint8_t* x = a.x + group * a.x_group_stride + (uint64_t)r0 * a.x_stride + (uint64_t)c * (kFromFp8 ? 1 : 2);
     uint2 codes[8];
-    uint32_t e[8];
+    uint32_t bytes[2];
     if constexpr (kFromFp8) {
-        // (rows that do not count hold zeros and have no scale: one that does lends them its own)
-        uint32_t pair = 0x7f7fu;
-        if (c0 + warp % 4 * 64 < a.cols && warp_row + lane < row_end)
-            pair = ld_global_u16(a.x_sf + group * a.x_sf_group_stride + (uint64_t)((c0 + warp % 4 * 64) / 64) * a.x_sf_stride + (uint64_t)(warp_row + lane) * 2);
-        uint2 q[8];
+        // (rows that do not count are zeros and have no scale: the first row lends them its own; nor has the second half of a last, half-used column)
+        const uint32_t lent = __shfl_sync(0xffffffffu, pair, 0), shift = c < a.cols ? lane % 8 / 4 * 8 : 0;
+        if (warp_row + lane >= row_end) pair = warp_row < row_end ? lent : 0x7f7fu;
         uint32_t b[8];
         #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i, x += 4 * a.x_stride) {
-            q[i] = make_uint2(0u, 0u);
-            if (r0 + i * 4 < row_end && c < a.cols) q[i] = ld_stream_v2(x);
-        }
-        const uint32_t first = __shfl_sync(0xffffffffu, pair, 0);
-        if (warp_row + lane >= row_end) pair = first;
-        // (nor has the second half of a last, half-used column)
-        const uint32_t shift = c < a.cols ? lane % 8 / 4 * 8 : 0;
-        #pragma unroll
         for (uint32_t i = 0; i < 8; ++i) b[i] = __shfl_sync(0xffffffffu, pair, i * 4 + lane / 8) >> shift & 0xffu;
-        if (!quantise_down_fp8(q, b, a.floor, e, codes)) {
+        if (!quantise_down_fp8(q, b, a.least, bytes, codes)) {
             float v[8][8];
             #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
@@ -190,25 +221,22 @@ __global__ void __launch_bounds__(kMnThreads, 3) quant_fp8_mn_kernel(const MnArg
                 #pragma unroll
                 for (int j = 0; j < 4; ++j) { v[i][j] = lo[j] * scale; v[i][4 + j] = hi[j] * scale; }
             }
-            quantise_down(v, a.floor, e, codes);
+            quantise_down(v, a.floor, bytes, codes);
         }
     } else {
-        uint4 q[8];
-        #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i, x += 4 * a.x_stride) {
-            q[i] = make_uint4(0u, 0u, 0u, 0u);
-            if (r0 + i * 4 < row_end && c < a.cols) q[i] = ld_stream_v4(x);
-        }
-        quantise_down_bf16(q, a.floor, e, codes);
+        quantise_down_bf16(q, a.floor, bytes, codes);
     }
     // (blocks behind the last row are zero)
-    if (lane < 8)
-        *reinterpret_cast<uint2*>(&sf_smem[half][tc]) = warp_row < a.rows ? make_uint2(e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24, e[4] | e[5] << 8 | e[6] << 16 | e[7] << 24)
-                                                                          : make_uint2(0u, 0u);
+    if (lane < 8) *reinterpret_cast<uint2*>(&sf_smem[half][tc]) = warp_row < a.rows ? make_uint2(bytes[0], bytes[1]) : make_uint2(0u, 0u);
     uint8_t* out = a.out + group * a.out_group_stride + (uint64_t)r0 * a.out_stride + c;
-    #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i, out += 4 * a.out_stride)
-        if (r0 + i * 4 < write_end && c < a.cols) *reinterpret_cast<uint2*>(out) = codes[i];
+    if (inside) {
+        #pragma unroll
+        for (uint32_t i = 0; i < 8; ++i, out += 4 * a.out_stride) *reinterpret_cast<uint2*>(out) = codes[i];
+    } else {
+        #pragma unroll
+        for (uint32_t i = 0; i < 8; ++i, out += 4 * a.out_stride)
+            if (r0 + i * 4 < write_end && c < a.cols) *reinterpret_cast<uint2*>(out) = codes[i];
+    }
     __syncthreads();
     if (c0 + threadIdx.x < a.cols)
         *reinterpret_cast<uint16_t*>(a.sf + group * a.sf_group_stride + (uint64_t)(row_base / 64) * a.sf_stride + (uint64_t)(c0 + threadIdx.x) * 2) =
@@ -219,12 +247,12 @@ __global__ void __launch_bounds__(kMnThreads, 3) quant_fp8_mn_kernel(const MnArg
 // columns, a warp four rows, a lane eight columns. The scales of K-major rows come in runs down the rows, through shared memory; those of an MN-major
 // tile lie along the columns.
 template <typename T, bool kMnMajor>
-__global__ void __launch_bounds__(kMnThreads) dequant_fp8_kernel(const MnArgs a) {
-    constexpr uint32_t kWarpRows = 4, kTileRows = 32;
-    __shared__ __align__(8) uint8_t sf_smem[kTileRows][kMnCols / 32];
+__global__ void __launch_bounds__(kBackThreads) dequant_fp8_kernel(const MnArgs a) {
+    constexpr uint32_t kTileRows = kBackRows, kWarpRows = kTileRows / (kBackThreads / 32);
+    __shared__ __align__(8) uint8_t sf_smem[kTileRows][kBackCols / 32];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint64_t group = blockIdx.z;
-    const uint32_t row_base = blockIdx.x / a.tiles_c * kTileRows, c0 = blockIdx.x % a.tiles_c * kMnCols;
+    const uint32_t row_base = blockIdx.x / a.tiles_c * kTileRows, c0 = blockIdx.x % a.tiles_c * kBackCols;
     const uint32_t c = c0 + lane * 8, r0 = row_base + warp * kWarpRows;
     griddep_wait();
     griddep_launch_dependents();
@@ -245,7 +273,7 @@ __global__ void __launch_bounds__(kMnThreads) dequant_fp8_kernel(const MnArgs a)
         }
     } else {
         const uint32_t col = threadIdx.x / kTileRows, r = threadIdx.x % kTileRows;
-        if (col < kMnCols / 64 && c0 + col * 64 < a.cols && row_base + r < a.rows)
+        if (col < kBackCols / 64 && c0 + col * 64 < a.cols && row_base + r < a.rows)
             *reinterpret_cast<uint16_t*>(&sf_smem[r][col * 2]) = ld_global_u16(sf + (uint64_t)(c0 / 64 + col) * a.x_sf_stride + (uint64_t)(row_base + r) * 2);
         __syncthreads();
     }
@@ -294,19 +322,28 @@ static int mn_checks(uint32_t rows, uint32_t cols, const void* x, const void* x_
 }
 
 // One launch for as many matrices as a grid holds.
-static int launch_mn(const void* fn, MnArgs a, uint32_t tile_rows, uint32_t groups, void* stream) {
+static int launch_mn(const void* fn, MnArgs a, uint32_t tile_rows, uint32_t tile_cols, uint32_t threads, uint32_t groups, void* stream) {
     constexpr uint32_t kMostGroups = 65535;
-    a.tiles_c = (a.cols + kMnCols - 1) / kMnCols;
+    a.tiles_c = (a.cols + tile_cols - 1) / tile_cols;
     const uint64_t tiles = (uint64_t)((a.rows + tile_rows - 1) / tile_rows) * a.tiles_c;
     DG_CHECK_ARG(tiles <= 0x7fffffffull, "fp8: too many values");
     void* params[] = {&a};
     for (uint32_t g = 0; g < groups; g += kMostGroups) {
         const dim3 grid((uint32_t)tiles, 1, groups - g < kMostGroups ? groups - g : kMostGroups);
-        if (int rc = launch_overlapped(fn, grid, dim3(kMnThreads), params, static_cast<cudaStream_t>(stream))) return rc;
+        if (int rc = launch_overlapped(fn, grid, dim3(threads), params, static_cast<cudaStream_t>(stream))) return rc;
         a.x += kMostGroups * a.x_group_stride; a.x_sf += kMostGroups * a.x_sf_group_stride;
         a.out += kMostGroups * a.out_group_stride; a.sf += kMostGroups * a.sf_group_stride;
     }
     return DG_OK;
+}
+
+// The scale byte of a block whose largest magnitude is `amax`, as on the device.
+static uint32_t least_byte(float amax) {
+    const float scaled = amax * (1.0f / 448.0f);
+    uint32_t bits;
+    memcpy(&bits, &scaled, 4);
+    const uint32_t e = (bits + 0x7fffffu) >> 23;
+    return e < 1u ? 1u : e;
 }
 
 extern "C" int dg_quant_fp8_mn_launch(const void* x, uint64_t x_stride, uint64_t x_group_stride, const int16_t* x_sf, uint64_t x_sf_stride, uint64_t x_sf_group_stride,
@@ -328,8 +365,8 @@ extern "C" int dg_quant_fp8_mn_launch(const void* x, uint64_t x_stride, uint64_t
     a.out = static_cast<uint8_t*>(out); a.out_stride = out_stride; a.out_group_stride = out_group_stride;
     a.sf = reinterpret_cast<uint8_t*>(sf); a.sf_stride = sf_stride * 2; a.sf_group_stride = sf_group_stride * 2;
     a.psum = psum; a.num_experts = psum ? num_experts : 0; a.alignment = alignment;
-    a.rows = rows; a.cols = cols; a.floor = min_amax;
-    return launch_mn(from_fp8 ? (const void*)quant_fp8_mn_kernel<true> : (const void*)quant_fp8_mn_kernel<false>, a, kMnRows, groups, stream);
+    a.rows = rows; a.cols = cols; a.floor = min_amax; a.least = least_byte(min_amax);
+    return launch_mn(from_fp8 ? (const void*)quant_fp8_mn_kernel<true> : (const void*)quant_fp8_mn_kernel<false>, a, kMnRows, kMnCols, kMnThreads, groups, stream);
 }
 
 extern "C" int dg_dequant_fp8_launch(const void* codes, uint64_t code_stride, uint64_t code_group_stride, const int16_t* sf, uint64_t sf_stride, uint64_t sf_group_stride,
@@ -348,5 +385,5 @@ extern "C" int dg_dequant_fp8_launch(const void* codes, uint64_t code_stride, ui
     a.rows = rows; a.cols = cols;
     const void* fn = mn_major ? (out_is_fp32 ? (const void*)dequant_fp8_kernel<float, true> : (const void*)dequant_fp8_kernel<__nv_bfloat16, true>)
                               : (out_is_fp32 ? (const void*)dequant_fp8_kernel<float, false> : (const void*)dequant_fp8_kernel<__nv_bfloat16, false>);
-    return launch_mn(fn, a, 32, groups, stream);
+    return launch_mn(fn, a, kBackRows, kBackCols, kBackThreads, groups, stream);
 }

@@ -38,30 +38,14 @@ struct QuantArgs {
     uint8_t* kept_sf; uint64_t kept_sf_col_stride;      // int16 [hidden/32][kept_sf_col_stride] seen as bytes
 };
 
-// The eight BF16 values of a lane in the plain cast's 8 bits; answers the exponent byte of the block, which four lanes share.
-__device__ __forceinline__ uint32_t cast_piece(const uint4& q, float floor, uint2& codes) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    float v[8], amax = 0.f;
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) { v[j * 2] = bf16_lo(w[j]); v[j * 2 + 1] = bf16_hi(w[j]); }
-    #pragma unroll
-    for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(v[j]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const uint32_t e = e4m3_scale_byte(amax, floor);
-    codes = e4m3_pack8(v, e);
-    return e;
-}
-
 // One CTA = 32 tokens x 256 channels. A warp takes four tokens and issues the loads of all of them (4 or 8 x 16 bytes per
 // lane) before it uses the first. Cutting the channels as well as the tokens is what gives a decoding step its parallelism:
 // a CTA that ran through the whole row left 64 tokens x 7168 channels to two CTAs. Bound by HBM for many tokens, by one
 // round trip to memory and the launch for few. Measured back to back: 64 x 7168 25.8 -> 1.7 us, 4096 x 7168 31 -> 12.6 us
 // (7.1 TB/s), 68495 x 7168 237 -> 214 us (6.9 TB/s); SwiGLU 4096 x 2048 15.0 -> 7.9 us, 68495 x 2048 118 -> 106 us.
-template <bool kSwiglu, bool kKeep>
+template <bool kSwiglu>
 __global__ void __launch_bounds__(kQuantThreads) quant_fp8_kernel(const QuantArgs a) {
     __shared__ __align__(8) uint8_t sf_smem[kTokenGroup][kTileChannels / 32];
-    __shared__ __align__(8) uint8_t kept_smem[kKeep ? 2 : 1][kKeep ? kTokenGroup : 1][kTileChannels / 32];
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t tiles_c = (a.hidden + kTileChannels - 1) / kTileChannels;
     const uint32_t tg = blockIdx.x / tiles_c, c0 = (blockIdx.x - tg * tiles_c) * kTileChannels;
@@ -122,19 +106,6 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp8_kernel(const QuantArg
         const uint32_t e = e4m3_scale_byte(amax, a.floor);
         if (t0 + i < valid_end && c < a.hidden)
             *reinterpret_cast<uint2*>(a.out + (uint64_t)(t0 + i) * a.out_stride + c) = e4m3_pack8(v, e);
-        if constexpr (kKeep) {
-            uint2 codes[2];
-            const uint32_t el = cast_piece(left[i], a.floor, codes[0]), er = cast_piece(right[i], a.floor, codes[1]);
-            if (t0 + i < valid_end && c < a.hidden) {
-                uint8_t* row = a.kept + (uint64_t)(t0 + i) * a.kept_stride + c;
-                *reinterpret_cast<uint2*>(row) = codes[0];
-                *reinterpret_cast<uint2*>(row + a.hidden) = codes[1];
-            }
-            if ((lane & 3u) == 0) {
-                kept_smem[0][warp * kWarpTokens + i][lane / 4] = (uint8_t)el;
-                kept_smem[1][warp * kWarpTokens + i][lane / 4] = (uint8_t)er;
-            }
-        }
         // (the second block of a last, half-used scale column is zero)
         if ((lane & 3u) == 0) sf_smem[warp * kWarpTokens + i][lane / 4] = c < a.hidden ? (uint8_t)e : (uint8_t)0;
     }
@@ -144,12 +115,100 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp8_kernel(const QuantArg
     if (col < kTileChannels / 64 && c0 + col * 64 < a.hidden && tl < valid_end - token_base) {
         const uint16_t pair = *reinterpret_cast<const uint16_t*>(&sf_smem[tl][col * 2]);
         *reinterpret_cast<uint16_t*>(a.out_sf + ((uint64_t)(c0 / 64 + col) * a.sf_col_stride + token_base + tl) * 2) = pair;
-        if constexpr (kKeep) {
-            // (hidden is a multiple of 64: no column holds blocks of both halves)
+    }
+}
+
+// SwiGLU with a checkpoint. A warp takes four tokens x 256 channels and shares nothing with others, so that small CTAs come and go by themselves: the scales of a
+// block's four tokens are collected by shuffles and written in one store of eight bytes where the column starts on a boundary of that.
+constexpr uint32_t kKeepThreads = 128, kKeepTokens = kWarpTokens * kKeepThreads / 32;
+__device__ __forceinline__ uint32_t cast_piece(const Pair (&v)[4], float floor, uint2& codes) {
+    float amax = 0.f;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) amax = larger_magnitude(amax, v[j]);
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const uint32_t e = e4m3_scale_byte(amax, floor);
+    codes = e4m3_pack8(v, e);
+    return e;
+}
+__global__ void __launch_bounds__(kKeepThreads, 8) swiglu_checkpoint_kernel(const QuantArgs a) {
+    const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t tiles_c = (a.hidden + kTileChannels - 1) / kTileChannels;
+    const uint32_t tg = blockIdx.x / tiles_c, c = (blockIdx.x - tg * tiles_c) * kTileChannels + lane * 8;
+    const uint32_t token_base = tg * kKeepTokens, t0 = token_base + warp * kWarpTokens;
+    griddep_wait();
+    griddep_launch_dependents();
+    // (asked for before it is known which rows hold a value)
+    uint4 left[kWarpTokens], right[kWarpTokens];
+    float weight[kWarpTokens];
+    const bool inside = c < a.hidden;
+    const __nv_bfloat16* row = a.x + (uint64_t)t0 * a.x_stride + c;
+    #pragma unroll
+    for (uint32_t i = 0; i < kWarpTokens; ++i, row += a.x_stride) {
+        left[i] = right[i] = make_uint4(0u, 0u, 0u, 0u);
+        weight[i] = 1.0f;
+        if (t0 + i >= a.tokens) continue;
+        if (inside) {
+            left[i] = ld_stream_v4(row);
+            right[i] = ld_stream_v4(row + a.hidden);
+        }
+        if (a.weights) weight[i] = __uint_as_float(ld_global_u32(a.weights + t0 + i));
+    }
+    uint32_t valid_end = min(a.tokens, token_base + kKeepTokens);
+    if (a.psum != nullptr) valid_end = min(valid_end, group_end_of(a.psum, a.num_experts, a.alignment, token_base, lane).valid);
+    if (t0 >= valid_end) return;                          // (the same for the whole warp)
+    uint32_t bytes[3] = {};                               // scales of the result, of the left half, of the right one: a byte a token
+    #pragma unroll
+    for (uint32_t i = 0; i < kWarpTokens; ++i) {
+        const uint32_t lw[4] = {left[i].x, left[i].y, left[i].z, left[i].w}, rw[4] = {right[i].x, right[i].y, right[i].z, right[i].w};
+        // The numbers of the kernel above, two at a time: with its instructions one by one the arithmetic takes longer than the bytes (65536 x 2048 rows 182
+        // against 161 us).
+        Pair l[4], r[4], y[4];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            l[j] = Pair(bf16_lo(lw[j]), bf16_hi(lw[j]));
+            r[j] = Pair(bf16_lo(rw[j]), bf16_hi(rw[j]));
+        }
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            Pair xl = l[j], xr = r[j];
+            float v0, v1;
+            if (a.has_clamp) {
+                xl.get(v0, v1);
+                xl = Pair(fminf(v0, a.clamp), fminf(v1, a.clamp));
+                xr.get(v0, v1);
+                xr = Pair(fmaxf(fminf(v0, a.clamp), -a.clamp), fmaxf(fminf(v1, a.clamp), -a.clamp));
+            }
+            (xl * Pair(-kLog2E)).get(v0, v1);
+            (Pair(fast_exp2(v0), fast_exp2(v1)) + Pair(1.0f)).get(v0, v1);
+            y[j] = xl * Pair(fast_reciprocal(v0), fast_reciprocal(v1)) * xr;
+            if (a.weights) y[j] = y[j] * Pair(weight[i]);
+        }
+        uint2 codes[3];
+        bytes[0] |= cast_piece(y, a.floor, codes[0]) << (8 * i);
+        bytes[1] |= cast_piece(l, a.floor, codes[1]) << (8 * i);
+        bytes[2] |= cast_piece(r, a.floor, codes[2]) << (8 * i);
+        if (t0 + i < valid_end && inside) {
+            *reinterpret_cast<uint2*>(a.out + (uint64_t)(t0 + i) * a.out_stride + c) = codes[0];
+            uint8_t* to = a.kept + (uint64_t)(t0 + i) * a.kept_stride + c;
+            *reinterpret_cast<uint2*>(to) = codes[1];
+            *reinterpret_cast<uint2*>(to + a.hidden) = codes[2];
+        }
+    }
+    // Lane 0 of eight has the even block's bytes, lane 4 the odd one's. (hidden is a multiple of 64: no column is half used or holds blocks of both halves)
+    #pragma unroll
+    for (uint32_t k = 0; k < 3; ++k) {
+        const uint32_t odd = __shfl_down_sync(0xffffffffu, bytes[k], 4);
+        if (lane % 8 != 0 || !inside) continue;
+        const uint64_t stride = k == 0 ? a.sf_col_stride : a.kept_sf_col_stride;
+        uint8_t* to = (k == 0 ? a.out_sf : a.kept_sf) + ((uint64_t)((k == 2 ? a.hidden + c : c) / 64) * stride + t0) * 2;
+        const uint2 pairs = make_uint2(__byte_perm(bytes[k], odd, 0x5140), __byte_perm(bytes[k], odd, 0x7362));
+        if (t0 + kWarpTokens <= valid_end && reinterpret_cast<uintptr_t>(to) % 8 == 0) {
+            *reinterpret_cast<uint2*>(to) = pairs;
+        } else {
             #pragma unroll
-            for (uint32_t half = 0; half < 2; ++half)
-                *reinterpret_cast<uint16_t*>(a.kept_sf + ((uint64_t)((half * a.hidden + c0) / 64 + col) * a.kept_sf_col_stride + token_base + tl) * 2) =
-                    *reinterpret_cast<const uint16_t*>(&kept_smem[half][tl][col * 2]);
+            for (uint32_t i = 0; i < kWarpTokens; ++i)
+                if (t0 + i < valid_end) reinterpret_cast<uint16_t*>(to)[i] = (uint16_t)((i < 2 ? pairs.x : pairs.y) >> (16 * (i % 2)));
         }
     }
 }
@@ -158,7 +217,7 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp8_kernel(const QuantArg
 
 using namespace dg;
 
-static int launch_quant_fp8(QuantArgs a, const void* fn, void* stream) {
+static int launch_quant_fp8(QuantArgs a, const void* fn, uint32_t tile_tokens, uint32_t threads, void* stream) {
     DG_CHECK_ARG(a.x != nullptr && a.out != nullptr && a.out_sf != nullptr, "quant_fp8: null pointer");
     DG_CHECK_ARG(a.hidden > 0 && a.hidden % 32 == 0, "quant_fp8: hidden must be a multiple of 32");
     DG_CHECK_ARG((reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && a.x_stride % 8 == 0,
@@ -170,10 +229,10 @@ static int launch_quant_fp8(QuantArgs a, const void* fn, void* stream) {
                  "quant_fp8: a psum layout needs experts and an alignment that is a multiple of 32");
     if (a.tokens == 0) return DG_OK;
     if (a.psum == nullptr) a.num_experts = 0;
-    const uint64_t tiles = (uint64_t)((a.tokens + kTokenGroup - 1) / kTokenGroup) * ((a.hidden + kTileChannels - 1) / kTileChannels);
+    const uint64_t tiles = (((uint64_t)a.tokens + tile_tokens - 1) / tile_tokens) * ((a.hidden + kTileChannels - 1) / kTileChannels);
     DG_CHECK_ARG(tiles <= 0x7fffffffull, "quant_fp8: too many tokens");
     void* params[] = {&a};
-    return launch_overlapped(fn, dim3((uint32_t)tiles), dim3(kQuantThreads), params, static_cast<cudaStream_t>(stream));
+    return launch_overlapped(fn, dim3((uint32_t)tiles), dim3(threads), params, static_cast<cudaStream_t>(stream));
 }
 
 static QuantArgs quant_args(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t hidden, const float* topk_weights, const int32_t* psum, uint32_t num_experts,
@@ -193,14 +252,14 @@ extern "C" int dg_quant_fp8_launch(const void* x, uint64_t x_stride, uint32_t to
                                    int has_clamp, float clamp_value, void* out, uint64_t out_stride,
                                    int16_t* out_sf, uint64_t sf_col_stride, void* stream) {
     const QuantArgs a = quant_args(x, x_stride, tokens, hidden, topk_weights, psum, num_experts, alignment, has_clamp, clamp_value, 1e-4f, out, out_stride, out_sf, sf_col_stride);
-    return launch_quant_fp8(a, swiglu ? (const void*)quant_fp8_kernel<true, false> : (const void*)quant_fp8_kernel<false, false>, stream);
+    return launch_quant_fp8(a, swiglu ? (const void*)quant_fp8_kernel<true> : (const void*)quant_fp8_kernel<false>, kTokenGroup, kQuantThreads, stream);
 }
 
 extern "C" int dg_cast_fp8_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t hidden, const int32_t* psum, uint32_t num_experts, uint32_t alignment,
                                   float min_amax, void* out, uint64_t out_stride, int16_t* out_sf, uint64_t sf_col_stride, void* stream) {
     DG_CHECK_ARG(min_amax >= 0.0f && min_amax <= 3.0e38f, "cast_fp8: min_amax must be a finite number that is not negative");
     const QuantArgs a = quant_args(x, x_stride, tokens, hidden, nullptr, psum, num_experts, alignment, 0, 0.0f, min_amax, out, out_stride, out_sf, sf_col_stride);
-    return launch_quant_fp8(a, (const void*)quant_fp8_kernel<false, false>, stream);
+    return launch_quant_fp8(a, (const void*)quant_fp8_kernel<false>, kTokenGroup, kQuantThreads, stream);
 }
 
 extern "C" int dg_swiglu_checkpoint_launch(const void* x, uint64_t x_stride, uint32_t tokens, uint32_t hidden, const float* topk_weights, const int32_t* psum,
@@ -216,5 +275,5 @@ extern "C" int dg_swiglu_checkpoint_launch(const void* x, uint64_t x_stride, uin
     }
     a.kept = static_cast<uint8_t*>(kept); a.kept_stride = kept_stride;
     a.kept_sf = reinterpret_cast<uint8_t*>(kept_sf); a.kept_sf_col_stride = kept_sf_col_stride;
-    return launch_quant_fp8(a, (const void*)quant_fp8_kernel<true, true>, stream);
+    return launch_quant_fp8(a, (const void*)swiglu_checkpoint_kernel, kKeepTokens, kKeepThreads, stream);
 }

@@ -18,162 +18,209 @@
 
 namespace dg {
 
-constexpr uint32_t kGradThreads = 256, kGradTokens = kGradThreads / 32, kGradTile = 256, kMostCtas = 8;
-constexpr uint32_t kFewGroups = 148 * 4;                    // groups of rows that give every SM its CTAs
+constexpr uint32_t kGradThreads = 128, kWarpTokens = 4, kGradTokens = kWarpTokens * kGradThreads / 32, kGradTile = 256;
 
 struct SwigluGradArgs {
     const uint8_t* g; uint64_t g_stride;                      // BF16 [tokens, hidden], bytes between rows
     const uint8_t* x; uint64_t x_stride;                      // BF16 or E4M3 [tokens, 2 * hidden]
     const uint8_t* x_sf; uint64_t x_sf_stride;                // int16 [hidden / 32][x_sf_stride / 2] seen as bytes
     uint8_t* dx; uint64_t dx_stride;                          // BF16 [tokens, 2 * hidden]
-    const float* weights; float* grad_weights;                // [tokens] or nullptr
+    const float* weights;                                     // [tokens] or nullptr
+    float* partial;                                           // [tiles][tokens]: sums for dw, or nullptr
     const int32_t* psum; uint32_t num_experts, alignment;
-    uint32_t tokens, hidden, ctas, zero_padding;
+    uint32_t tokens, hidden, tiles, zero_padding;
     float clamp;
 };
 
-__device__ __forceinline__ uint4 pack_bf16(const float (&v)[8]) {
-    uint32_t w[4];
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
-        w[j] = *reinterpret_cast<const uint32_t*>(&p);
+// Where a lane's channels of a row lie.
+template <bool kFromFp8> struct Cursor {
+    const uint8_t *g, *l, *r, *sf;
+    uint64_t sf_right;
+    uint32_t shift;
+    __device__ __forceinline__ Cursor(const SwigluGradArgs& a, uint64_t token, uint32_t c) : shift(c / 32 % 2 * 8) {
+        g = a.g + token * a.g_stride + (uint64_t)c * 2;
+        l = a.x + token * a.x_stride + (uint64_t)c * (kFromFp8 ? 1 : 2);
+        r = l + (uint64_t)a.hidden * (kFromFp8 ? 1 : 2);
+        sf = a.x_sf + (uint64_t)(c / 64) * a.x_sf_stride + token * 2;
+        sf_right = (uint64_t)(a.hidden / 64) * a.x_sf_stride;
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
-}
-__device__ __forceinline__ void unpack_bf16(const uint4& q, float (&v)[8]) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-    #pragma unroll
-    for (int j = 0; j < 4; ++j) { v[2 * j] = bf16_lo(w[j]); v[2 * j + 1] = bf16_hi(w[j]); }
-}
-
+    __device__ __forceinline__ void next_row(const SwigluGradArgs& a) {
+        g += a.g_stride;
+        l += a.x_stride;
+        r += a.x_stride;
+        sf += 2;
+    }
+};
 // Eight channels of a row as they lie in memory: the gradient, and both halves of the input in BF16, or in codes with their scales.
 template <bool kFromFp8> struct Tile8;
 template <> struct Tile8<false> {
     uint4 g, l, r;
-    __device__ __forceinline__ void load(const SwigluGradArgs& a, uint64_t token, uint32_t c) {
-        g = ld_stream_v4(a.g + token * a.g_stride + (uint64_t)c * 2);
-        const uint8_t* x = a.x + token * a.x_stride + (uint64_t)c * 2;
-        l = ld_stream_v4(x);
-        r = ld_stream_v4(x + (uint64_t)a.hidden * 2);
+    __device__ __forceinline__ void load(const Cursor<false>& at) {
+        g = ld_stream_v4(at.g);
+        l = ld_stream_v4(at.l);
+        r = ld_stream_v4(at.r);
     }
-    __device__ __forceinline__ void get(float (&lv)[8], float (&rv)[8]) const { unpack_bf16(l, lv); unpack_bf16(r, rv); }
+    __device__ __forceinline__ void get(uint32_t, Pair (&lv)[4], Pair (&rv)[4]) const {
+        const uint32_t lw[4] = {l.x, l.y, l.z, l.w}, rw[4] = {r.x, r.y, r.z, r.w};
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) { lv[j] = Pair(bf16_lo(lw[j]), bf16_hi(lw[j])); rv[j] = Pair(bf16_lo(rw[j]), bf16_hi(rw[j])); }
+    }
 };
 template <> struct Tile8<true> {
     uint4 g;
     uint2 l, r;
-    uint16_t el, er;
-    uint32_t shift;
-    __device__ __forceinline__ void load(const SwigluGradArgs& a, uint64_t token, uint32_t c) {
-        g = ld_stream_v4(a.g + token * a.g_stride + (uint64_t)c * 2);
-        const uint8_t *x = a.x + token * a.x_stride + c, *sf = a.x_sf + (uint64_t)(c / 64) * a.x_sf_stride + token * 2;
-        l = ld_stream_v2(x);
-        r = ld_stream_v2(x + a.hidden);
-        // (the rows of the other warps have theirs in the same sectors: these stay in L1)
-        el = ld_global_u16(sf);
-        er = ld_global_u16(sf + (uint64_t)(a.hidden / 64) * a.x_sf_stride);
-        shift = c / 32 % 2 * 8;
+    uint32_t e;
+    __device__ __forceinline__ void load(const Cursor<true>& at) {
+        g = ld_stream_v4(at.g);
+        l = ld_stream_v2(at.l);
+        r = ld_stream_v2(at.r);
+        // (the other rows of the tile have theirs in the same sectors: these stay in L1)
+        e = ld_global_u16(at.sf) | (uint32_t)ld_global_u16(at.sf + at.sf_right) << 16;
     }
-    static __device__ __forceinline__ void values(const uint2& q, float scale, float (&v)[8]) {
-        float lo[4], hi[4];
-        e4m3_unpack4(q.x, lo);
-        e4m3_unpack4(q.y, hi);
+    static __device__ __forceinline__ void values(const uint2& q, float scale, Pair (&v)[4]) {
+        float four[4];
+        const Pair s(scale);
         #pragma unroll
-        for (int j = 0; j < 4; ++j) { v[j] = lo[j] * scale; v[4 + j] = hi[j] * scale; }
+        for (int h = 0; h < 2; ++h) {
+            e4m3_unpack4(h ? q.y : q.x, four);
+            v[2 * h] = Pair(four[0], four[1]) * s;
+            v[2 * h + 1] = Pair(four[2], four[3]) * s;
+        }
     }
-    __device__ __forceinline__ void get(float (&lv)[8], float (&rv)[8]) const {
-        values(l, ue8m0_float((uint32_t)el >> shift & 0xffu), lv);
-        values(r, ue8m0_float((uint32_t)er >> shift & 0xffu), rv);
+    __device__ __forceinline__ void get(uint32_t shift, Pair (&lv)[4], Pair (&rv)[4]) const {
+        values(l, ue8m0_float(e >> shift & 0xffu), lv);
+        values(r, ue8m0_float(e >> (shift + 16) & 0xffu), rv);
     }
 };
 
-// A warp takes a row. Where there are few rows, the channels are shared by a cluster of CTAs, and their sums for dw meet in the first CTA's
-// shared memory, added in the order of the CTAs.
+// One CTA = 16 rows x 256 channels, a warp four rows, a lane eight channels of each: everything a warp reads is asked for at once, and small CTAs that come and go
+// overlap better than a loop over the channels does (65536 x 2048 from 8 bits: a warp a row with one to three tiles on their way 209 to 226 us; four rows a
+// warp at 80 registers 206, at 64 registers 198 and in CTAs of 128 threads 192; two rows a warp 215). The sums of a row's tiles go to `partial`
+// and are added up in the order of the tiles by a second kernel.
 template <bool kFromFp8, bool kClamp>
-__global__ void __launch_bounds__(kGradThreads, 4) swiglu_grad_kernel(const SwigluGradArgs a) {
-    __shared__ float sums[kMostCtas][kGradTokens];
+__global__ void __launch_bounds__(kGradThreads, 8) swiglu_grad_kernel(const SwigluGradArgs a) {
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-    const uint32_t part = a.ctas > 1 ? blockIdx.x % a.ctas : 0, token_base = (a.ctas > 1 ? blockIdx.x / a.ctas : blockIdx.x) * kGradTokens, token = token_base + warp;
-    // (the other CTAs write to this one's shared memory, which has to be there)
-    const bool in_cluster = a.grad_weights != nullptr && a.ctas > 1;
-    if (in_cluster) cluster_arrive();
+    const uint32_t token_base = blockIdx.x / a.tiles * kGradTokens, tile = blockIdx.x % a.tiles, c = tile * kGradTile + lane * 8, t0 = token_base + warp * kWarpTokens;
     griddep_wait();
     griddep_launch_dependents();
-    const uint32_t step = a.ctas * kGradTile;
-    uint32_t c = part * kGradTile + lane * 8;
-    // (asked for before it is known whether the row holds a value)
-    Tile8<kFromFp8> now{}, next{};
-    if (token < a.tokens && c < a.hidden) now.load(a, token, c);
-    const float weight = a.weights && token < a.tokens ? __uint_as_float(ld_stream_u32(a.weights + token)) : 1.0f;
-    bool valid = token < a.tokens, zero = false;
+    // (asked for before it is known which rows hold a value)
+    Tile8<kFromFp8> tiles[kWarpTokens]{};
+    float weight[kWarpTokens];
+    const bool inside = c < a.hidden;
+    Cursor<kFromFp8> at(a, t0, c);
+    #pragma unroll
+    for (uint32_t i = 0; i < kWarpTokens; ++i, at.next_row(a)) {
+        weight[i] = 1.0f;
+        if (t0 + i >= a.tokens) continue;
+        if (inside) tiles[i].load(at);
+        if (a.weights) weight[i] = __uint_as_float(ld_global_u32(a.weights + t0 + i));
+    }
+    uint32_t valid_end = min(a.tokens, token_base + kGradTokens), zero_end = 0;
     if (a.psum != nullptr) {
         const GroupEnd end = group_end_of(a.psum, a.num_experts, a.alignment, token_base, lane);
-        zero = valid && a.zero_padding && token >= end.valid && token < end.whole;
-        valid = token < min(a.tokens, end.valid);
+        zero_end = a.zero_padding ? min(valid_end, end.whole) : 0;
+        valid_end = min(valid_end, end.valid);
     }
-    float dw = 0.0f;
-    if (valid) {
-        for (; c < a.hidden; c += step) {
-            if (c + step < a.hidden) next.load(a, token, c + step);
-            float g[8], l[8], r[8];
-            unpack_bf16(now.g, g);
-            now.get(l, r);
-            #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                bool outside_l = false, outside_r = false;
-                if constexpr (kClamp) {
-                    // (a NaN is on no side of the clamp, and stays one)
-                    outside_l = l[j] > a.clamp;
-                    outside_r = fabsf(r[j]) > a.clamp;
-                    if (outside_l) l[j] = a.clamp;
-                    if (outside_r) r[j] = copysignf(a.clamp, r[j]);
-                }
-                // (the reciprocal of a number beyond 2^126 would be 0, and its product with that an invalid one; 1 - p would lose its bits where p is near 1)
-                const float z = fast_exp2(fminf(-kLog2E * l[j], 126.0f)), p = fast_reciprocal(1.0f + z), rest = z * p, silu = l[j] * p;
-                const float gs = g[j] * silu, gr = g[j] * r[j] * weight;
-                dw = fmaf(gs, r[j], dw);
-                l[j] = outside_l ? 0.0f : gr * fmaf(silu, rest, p);
-                r[j] = outside_r ? 0.0f : gs * weight;
-            }
-            uint8_t* to = a.dx + (uint64_t)token * a.dx_stride + (uint64_t)c * 2;
-            *reinterpret_cast<uint4*>(to) = pack_bf16(l);
-            *reinterpret_cast<uint4*>(to + (uint64_t)a.hidden * 2) = pack_bf16(r);
-            now = next;
-        }
-    } else if (zero) {
-        for (; c < a.hidden; c += step) {
-            uint8_t* to = a.dx + (uint64_t)token * a.dx_stride + (uint64_t)c * 2;
-            *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(to + (uint64_t)a.hidden * 2) = make_uint4(0u, 0u, 0u, 0u);
-        }
-    }
-    if (a.grad_weights == nullptr) return;                    // (the same for all CTAs)
-    __syncwarp();
+    uint8_t* to = a.dx + (uint64_t)t0 * a.dx_stride + (uint64_t)c * 2;
+    const uint64_t to_right = (uint64_t)a.hidden * 2;
+    const Pair one(1.0f), exponent(-kLog2E);
+    float dw[kWarpTokens];
     #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) dw += __shfl_xor_sync(0xffffffffu, dw, o);
-    // (rows that hold no value have the gradient 0: nothing was added)
-    if (!in_cluster) {
-        if (lane == 0 && token < a.tokens) a.grad_weights[token] = dw;
-        return;
+    for (uint32_t t = 0; t < kWarpTokens; ++t, to += a.dx_stride) {
+        dw[t] = 0.0f;
+        if (t0 + t >= valid_end) {
+            if (t0 + t < zero_end && inside) *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(to + to_right) = make_uint4(0u, 0u, 0u, 0u);
+            continue;
+        }
+        const uint32_t gw[4] = {tiles[t].g.x, tiles[t].g.y, tiles[t].g.z, tiles[t].g.w};
+        const Pair weights(weight[t]);
+        Pair l[4], r[4], sum(0.0f);
+        tiles[t].get(at.shift, l, r);
+        uint32_t dl[4], dr[4];
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            bool outside_l[2] = {}, outside_r[2] = {};
+            if constexpr (kClamp) {
+                // (a NaN is on no side of the clamp, and stays one)
+                float lv[2], rv[2];
+                l[j].get(lv[0], lv[1]);
+                r[j].get(rv[0], rv[1]);
+                #pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    outside_l[i] = lv[i] > a.clamp;
+                    outside_r[i] = fabsf(rv[i]) > a.clamp;
+                    if (outside_l[i]) lv[i] = a.clamp;
+                    if (outside_r[i]) rv[i] = copysignf(a.clamp, rv[i]);
+                }
+                l[j] = Pair(lv[0], lv[1]);
+                r[j] = Pair(rv[0], rv[1]);
+            }
+            // (the reciprocal of a number beyond 2^126 would be 0, and its product with that an invalid one; 1 - p would lose its bits where p is near 1)
+            float x0, x1;
+            (l[j] * exponent).get(x0, x1);
+            const Pair z(fast_exp2(fminf(x0, 126.0f)), fast_exp2(fminf(x1, 126.0f)));
+            (z + one).get(x0, x1);
+            const Pair p(fast_reciprocal(x0), fast_reciprocal(x1)), rest = z * p, silu = l[j] * p, g(bf16_lo(gw[j]), bf16_hi(gw[j]));
+            const Pair gs = g * silu, gr = g * r[j];
+            sum = fma2(gs, r[j], sum);
+            float v[4];
+            (gr * weights * fma2(silu, rest, p)).get(v[0], v[1]);
+            (gs * weights).get(v[2], v[3]);
+            if constexpr (kClamp) {
+                #pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (outside_l[i]) v[i] = 0.0f;
+                    if (outside_r[i]) v[2 + i] = 0.0f;
+                }
+            }
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(v[0], v[1]), hi = __floats2bfloat162_rn(v[2], v[3]);
+            dl[j] = *reinterpret_cast<const uint32_t*>(&lo);
+            dr[j] = *reinterpret_cast<const uint32_t*>(&hi);
+        }
+        if (inside) {
+            *reinterpret_cast<uint4*>(to) = make_uint4(dl[0], dl[1], dl[2], dl[3]);
+            *reinterpret_cast<uint4*>(to + to_right) = make_uint4(dr[0], dr[1], dr[2], dr[3]);
+        }
+        float other;
+        sum.get(dw[t], other);
+        dw[t] += other;
     }
-    cluster_wait();
-    if (lane == 0) asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(mapa_shared(smem_u32(&sums[part][warp]), 0)), "f"(dw) : "memory");
-    __syncwarp();
-    cluster_arrive();
-    cluster_wait();
-    if (part == 0 && threadIdx.x < kGradTokens && token_base + threadIdx.x < a.tokens) {
-        float sum = 0.0f;
-        for (uint32_t i = 0; i < a.ctas; ++i) sum += sums[i][threadIdx.x];
-        a.grad_weights[token_base + threadIdx.x] = sum;
+    if (a.partial == nullptr) return;
+    // (lanes behind the last channel hold zeros; rows without a value have the gradient 0)
+    #pragma unroll
+    for (uint32_t t = 0; t < kWarpTokens; ++t) {
+        #pragma unroll
+        for (int o = 16; o > 0; o >>= 1) dw[t] += __shfl_xor_sync(0xffffffffu, dw[t], o);
+        if (lane == t && t0 + t < a.tokens) a.partial[(uint64_t)tile * a.tokens + t0 + t] = dw[t];
     }
+}
+
+constexpr uint32_t kSumThreads = 256;
+__global__ void __launch_bounds__(kSumThreads) swiglu_grad_sum_kernel(const float* partial, float* out, uint32_t tiles, uint32_t tokens) {
+    const uint32_t token = blockIdx.x * kSumThreads + threadIdx.x;
+    griddep_wait();
+    griddep_launch_dependents();
+    if (token >= tokens) return;
+    float sum = 0.0f;
+    #pragma unroll 8
+    for (uint32_t i = 0; i < tiles; ++i) sum += __uint_as_float(ld_global_u32(partial + (uint64_t)i * tokens + token));
+    out[token] = sum;
 }
 
 }  // namespace dg
 
 using namespace dg;
 
+// Sums of the tiles, where there is more than one.
+extern "C" uint64_t dg_swiglu_grad_scratch_bytes(uint32_t tokens, uint32_t hidden) {
+    const uint32_t tiles = (hidden + kGradTile - 1) / kGradTile;
+    return tiles > 1 ? (uint64_t)tiles * tokens * 4 : 0;
+}
+
 extern "C" int dg_swiglu_grad_launch(const void* grad_out, uint64_t grad_stride, const void* x, uint64_t x_stride, const int16_t* x_sf, uint64_t x_sf_col_stride,
                                      uint32_t tokens, uint32_t hidden, const float* topk_weights, const int32_t* psum, uint32_t num_experts, uint32_t alignment,
-                                     int has_clamp, float clamp_value, void* grad_x, uint64_t grad_x_stride, float* grad_weights, int zero_padding, void* stream) {
+                                     int has_clamp, float clamp_value, void* grad_x, uint64_t grad_x_stride, float* grad_weights, int zero_padding, void* scratch, uint64_t scratch_bytes,
+                                     void* stream) {
     if (tokens == 0) return DG_OK;
     const bool from_fp8 = x_sf != nullptr;
     const uint64_t es = from_fp8 ? 1 : 2;
@@ -192,15 +239,23 @@ extern "C" int dg_swiglu_grad_launch(const void* grad_out, uint64_t grad_stride,
     a.x = static_cast<const uint8_t*>(x); a.x_stride = x_stride * es;
     a.x_sf = reinterpret_cast<const uint8_t*>(x_sf); a.x_sf_stride = x_sf_col_stride * 2;
     a.dx = static_cast<uint8_t*>(grad_x); a.dx_stride = grad_x_stride * 2;
-    a.weights = topk_weights; a.grad_weights = grad_weights;
+    a.weights = topk_weights;
     a.psum = psum; a.num_experts = psum ? num_experts : 0; a.alignment = alignment;
     a.tokens = tokens; a.hidden = hidden; a.zero_padding = zero_padding ? 1u : 0u;
     a.clamp = clamp_value;
-    const uint32_t tiles = (hidden + kGradTile - 1) / kGradTile, groups = (tokens + kGradTokens - 1) / kGradTokens;
-    a.ctas = 1;
-    while (a.ctas < kMostCtas && a.ctas < tiles && groups * a.ctas < kFewGroups) a.ctas *= 2;
+    a.tiles = (hidden + kGradTile - 1) / kGradTile;
+    const uint64_t grid = (uint64_t)((tokens + kGradTokens - 1) / kGradTokens) * a.tiles;
+    DG_CHECK_ARG(grid <= 0x7fffffffull, "swiglu_grad: too many tokens");
+    const bool sums = grad_weights != nullptr && a.tiles > 1;
+    DG_CHECK_ARG(!sums || (scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 4 == 0 && scratch_bytes >= dg_swiglu_grad_scratch_bytes(tokens, hidden)),
+                 "swiglu_grad: scratch is too small");
+    a.partial = sums ? static_cast<float*>(scratch) : grad_weights;
     void* params[] = {&a};
     const void* fn = has_clamp ? (from_fp8 ? (const void*)swiglu_grad_kernel<true, true> : (const void*)swiglu_grad_kernel<false, true>)
                                : (from_fp8 ? (const void*)swiglu_grad_kernel<true, false> : (const void*)swiglu_grad_kernel<false, false>);
-    return launch_overlapped(fn, dim3(groups * a.ctas), dim3(kGradThreads), params, static_cast<cudaStream_t>(stream), 0, grad_weights ? a.ctas : 1);
+    if (int rc = launch_overlapped(fn, dim3((uint32_t)grid), dim3(kGradThreads), params, static_cast<cudaStream_t>(stream))) return rc;
+    if (!sums) return DG_OK;
+    const float* from = a.partial;
+    void* sum_params[] = {&from, &grad_weights, &a.tiles, &tokens};
+    return launch_overlapped((const void*)swiglu_grad_sum_kernel, dim3((tokens + kSumThreads - 1) / kSumThreads), dim3(kSumThreads), sum_params, static_cast<cudaStream_t>(stream));
 }

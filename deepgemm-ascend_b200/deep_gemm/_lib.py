@@ -98,9 +98,10 @@ _PROTOTYPES = {
     'dg_swiglu_checkpoint_launch': (C.c_int, [
         C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint32, C.c_int, C.c_float, C.c_void_p, C.c_uint64,
         C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]),
+    'dg_swiglu_grad_scratch_bytes': (C.c_uint64, [C.c_uint32, C.c_uint32]),
     'dg_swiglu_grad_launch': (C.c_int, [
         C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p, C.c_void_p, C.c_uint32,
-        C.c_uint32, C.c_int, C.c_float, C.c_void_p, C.c_uint64, C.c_void_p, C.c_int, C.c_void_p]),
+        C.c_uint32, C.c_int, C.c_float, C.c_void_p, C.c_uint64, C.c_void_p, C.c_int, C.c_void_p, C.c_uint64, C.c_void_p]),
     'dg_quant_fp8_mn_launch': (C.c_int, [
         C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64, C.c_uint32, C.c_uint32, C.c_uint32, C.c_void_p, C.c_uint32,
         C.c_uint32, C.c_float, C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p]),

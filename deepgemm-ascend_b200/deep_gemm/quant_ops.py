@@ -174,11 +174,14 @@ def swiglu_apply_weight_grad(grad_out: torch.Tensor, x, topk_weights: Optional[t
         else:
             out = torch.empty((tokens, 2 * hidden), dtype=torch.bfloat16, device=x.device)
         grad_weights = torch.empty_like(topk_weights) if topk_weights is not None else None
+        nbytes = L.lib().dg_swiglu_grad_scratch_bytes(tokens, hidden) if topk_weights is not None else 0
+        scratch = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         if x.numel():
             L.check(L.lib().dg_swiglu_grad_launch(
                 grad_out.data_ptr(), _row_stride(grad_out), x.data_ptr(), _row_stride(x), _ptr(sf), _scale_stride(sf) if is_pair else 0, tokens, hidden,
                 _ptr(topk_weights), _ptr(psum), psum.numel() if psum is not None else 0, int(expert_alignment), int(clamp_value is not None),
-                float(clamp_value or 0.0), out.data_ptr(), _row_stride(out), _ptr(grad_weights), int(zero_padding), _stream_ptr(x.device)))
+                float(clamp_value or 0.0), out.data_ptr(), _row_stride(out), _ptr(grad_weights), int(zero_padding), _ptr(scratch), nbytes,
+                _stream_ptr(x.device)))
         elif grad_weights is not None:
             grad_weights.zero_()
     return out, grad_weights
@@ -267,7 +270,7 @@ def rms_norm_to_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[to
         y = h * rstd * weight        (out, out_sf): y as `cast_to_fp8` quantises it, but from FP32; rows: y in BF16 `with_rows`, else None
 
     weight: BF16 or FP32 [hidden]. The sum of squares is held in 64 bits: a token's results do not depend on how many others there are. `out_h`:
-    where h goes with a residual, which may be `residual` or x itself. hidden is a multiple of 32, at most 32768; rows start on 16-byte boundaries."""
+    where h goes with a residual, which may be `residual` or x itself. hidden is a multiple of 32, at most 16384; rows start on 16-byte boundaries."""
     _host_assert(x.is_cuda and x.dim() == 2 and x.stride(1) == 1 and _is_float(x), 'x must be a row-major 2-D BF16 or FP32 tensor on a CUDA device')
     tokens, hidden = x.shape
     _check_norm(x, weight, tokens, hidden)
@@ -291,7 +294,7 @@ def rms_norm_to_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[to
 
 
 def _check_norm(x, weight, tokens, hidden):
-    _host_assert(hidden > 0 and hidden % 32 == 0 and hidden <= 32768, 'the row length must be a multiple of 32, at most 32768')
+    _host_assert(hidden > 0 and hidden % 32 == 0 and hidden <= 16384, 'the row length must be a multiple of 32, at most 16384')
     _host_assert(tokens <= _INT_MAX, 'there are too many tokens')
     _host_assert(weight.device == x.device and _is_float(weight) and weight.dim() == 1 and weight.size(0) == hidden and weight.is_contiguous(),
                  'weight must be a contiguous BF16 or FP32 vector of the row length, on the device of the rows')

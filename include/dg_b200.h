@@ -302,11 +302,13 @@ int dg_swiglu_checkpoint_launch(const void* x, uint64_t x_stride, uint32_t token
 /* Its gradient. grad_out BF16 [tokens, hidden]; x [tokens, 2 * hidden] BF16 (x_sf NULL), or E4M3 with the scales that
  * dg_swiglu_checkpoint_launch writes; grad_x BF16 [tokens, 2 * hidden]; grad_weights float [tokens] or NULL (0 for rows without a value). Where the
  * clamp cuts off, the gradient is 0. Rows of the psum layout's padding, and behind its last group, are not read; `zero_padding` writes zeros to
- * the former. grad_x may not overlap anything else. hidden % 64 == 0; rows 16-byte aligned (8 for E4M3). */
+ * the former. grad_x may not overlap anything else. `scratch`: with grad_weights, dg_swiglu_grad_scratch_bytes (0 for short rows) of device memory that
+ * the call may use until it has run. hidden % 64 == 0; rows 16-byte aligned (8 for E4M3). */
+uint64_t dg_swiglu_grad_scratch_bytes(uint32_t tokens, uint32_t hidden);
 int dg_swiglu_grad_launch(const void* grad_out, uint64_t grad_stride, const void* x, uint64_t x_stride, const int16_t* x_sf,
                           uint64_t x_sf_col_stride, uint32_t tokens, uint32_t hidden, const float* topk_weights, const int32_t* psum,
                           uint32_t num_experts, uint32_t alignment, int has_clamp, float clamp_value, void* grad_x, uint64_t grad_x_stride,
-                          float* grad_weights, int zero_padding, void* stream);
+                          float* grad_weights, int zero_padding, void* scratch, uint64_t scratch_bytes, void* stream);
 
 /* E4M3 operands whose contraction runs down the rows (MN-major), from BF16 (x_sf NULL) or from E4M3 rows with scales along them, x_sf int16
  * [ceil(cols / 64)][x_sf_stride]. sf[g * sf_group_stride + r * sf_stride + col], r = K64 row, ceil(rows / 64) of them. Scales as in
@@ -327,7 +329,7 @@ int dg_dequant_fp8_launch(const void* codes, uint64_t code_stride, uint64_t code
  * dg_rms_norm_grad_launch: grad_x = rstd (u - n mean(u n)) + grad_h (NULL: 0), u = grad_out * weight, n = h * rstd, in the type of h; grad_weight float
  * [hidden] = sum over the tokens of grad_out n. grad_out is BF16, or FP32 beside an FP32 h; grad_x may be grad_h, h or (of its type) grad_out itself.
  * `scratch`: dg_rms_norm_grad_scratch_bytes of device memory that the call may use until it has run.
- * hidden % 32 == 0, at most 32768; rows and the weight 16-byte aligned (out: 8). */
+ * hidden % 32 == 0, at most 16384; rows and the weight 16-byte aligned (out: 8). */
 int dg_rms_norm_fp8_launch(const void* x, int is_fp32, uint64_t x_stride, const void* residual, uint64_t residual_stride, void* h,
                            uint64_t h_stride, const void* weight, int weight_is_fp32, float eps, uint32_t tokens, uint32_t hidden,
                            void* out, uint64_t out_stride, int16_t* out_sf, uint64_t sf_col_stride, void* rows, uint64_t rows_stride,

@@ -73,7 +73,7 @@ def test_the_c_abi_refuses_norms_it_cannot_run():
         x, 0, stride, res, 64, h, 64, w, 0, 1e-6, 8, hidden, out, 64, p, sf_stride, rows, 64, p, None)
     _refused(norm(hidden=48), 'multiple of 32')
     _refused(norm(hidden=0), 'multiple of 32')
-    _refused(norm(hidden=32768 + 32), 'at most 32768')
+    _refused(norm(hidden=16384 + 32), 'at most 16384')
     _refused(norm(x=None), 'null pointer')
     _refused(norm(res=p, h=None), 'null pointer')
     for bad in (dict(x=p + 8), dict(res=p + 2), dict(h=p + 4), dict(w=p + 8), dict(rows=p + 8), dict(stride=68)):
@@ -84,7 +84,7 @@ def test_the_c_abi_refuses_norms_it_cannot_run():
         g, g32, 64, p, h32, 64, p, 0, p, None, 0, 8, hidden, dx, 64, p, scratch, nbytes, None)
     _refused(grad(g=None), 'null pointer')
     _refused(grad(g32=1), 'FP32 gradient beside BF16 rows')
-    _refused(grad(hidden=32800), 'at most 32768')
+    _refused(grad(hidden=16416), 'at most 16384')
     _refused(grad(nbytes=lib.dg_rms_norm_grad_scratch_bytes(8, 64) - 1), 'scratch is too small')
     _refused(grad(scratch=None), 'null pointer')
     _refused(grad(dx=p + 8), '16-byte')
@@ -100,8 +100,8 @@ def test_the_c_abi_refuses_8_bit_rows_it_cannot_read():
     _refused(keep(stride=7), 'scale column stride')
     _refused(keep(psum=p, align=48), 'multiple of 32')
     _refused(keep(psum=p, experts=0), 'multiple of 32')
-    grad = lambda hidden=128, x=p, sf=p, stride=8, w=None, dw=None, dx=p, psum=None, align=128: lib.dg_swiglu_grad_launch(  # noqa: E731
-        p, 128, x, 256, sf, stride, 8, hidden, w, psum, 1, align, 0, 0.0, dx, 256, dw, 0, None)
+    grad = lambda hidden=128, x=p, sf=p, stride=8, w=None, dw=None, dx=p, psum=None, align=128, scratch=None, nbytes=0: lib.dg_swiglu_grad_launch(  # noqa: E731
+        p, 128, x, 256, sf, stride, 8, hidden, w, psum, 1, align, 0, 0.0, dx, 256, dw, 0, scratch, nbytes, None)
     _refused(grad(hidden=96), 'multiple of 64')
     _refused(grad(x=None), 'null pointer')
     _refused(grad(x=p + 4), 'boundaries')
@@ -110,6 +110,8 @@ def test_the_c_abi_refuses_8_bit_rows_it_cannot_read():
     _refused(grad(stride=7), 'scale column stride')
     _refused(grad(dw=p), 'weights that are not there')
     _refused(grad(psum=p, align=33), 'multiple of 32')
+    _refused(grad(hidden=512, w=p, dw=p), 'scratch is too small')
+    _refused(grad(hidden=512, w=p, dw=p, scratch=p, nbytes=lib.dg_swiglu_grad_scratch_bytes(8, 512) - 1), 'scratch is too small')
     mn = lambda cols=64, x=p, sf=None, sf_stride=8, out=p, stride=64, psum=None, align=64, groups=1, floor=1e-4: lib.dg_quant_fp8_mn_launch(  # noqa: E731
         x, 64, 0, sf, sf_stride, 0, groups, 8, cols, psum, 1, align, floor, out, 64, 0, p, stride, 0, None)
     _refused(mn(cols=48), 'multiple of 32')
@@ -140,7 +142,7 @@ def test_nothing_to_do_is_no_error():
     assert lib.dg_moe_route_launch(None, 1, 64, 0, 64, 4, 0, None, 1, 1, 2, 0, 1.0, None, None, None) == L.DG_OK
     assert lib.dg_moe_route_grad_launch(None, None, 1, 64, 0, 64, None, 0, 4, 0, 0, 1.0, None, 64, None) == L.DG_OK
     assert lib.dg_rms_norm_fp8_launch(None, 0, 64, None, 0, None, 0, None, 0, 1e-6, 0, 64, None, 64, None, 0, None, 0, None, None) == L.DG_OK
-    assert lib.dg_swiglu_grad_launch(None, 0, None, 0, None, 0, 0, 128, None, None, 0, 128, 0, 0.0, None, 0, None, 0, None) == L.DG_OK
+    assert lib.dg_swiglu_grad_launch(None, 0, None, 0, None, 0, 0, 128, None, None, 0, 128, 0, 0.0, None, 0, None, 0, None, 0, None) == L.DG_OK
     assert lib.dg_quant_fp8_mn_launch(None, 0, 0, None, 0, 0, 1, 0, 64, None, 0, 0, 0.0, None, 0, 0, None, 0, 0, None) == L.DG_OK
     assert lib.dg_dequant_fp8_launch(None, 0, 0, None, 0, 0, 1, 0, 64, 0, None, 0, 0, 0, None) == L.DG_OK
     assert lib.dg_rms_norm_grad_scratch_bytes(0, 64) == 0
