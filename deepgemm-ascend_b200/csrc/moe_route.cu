@@ -35,7 +35,7 @@ struct RouteArgs {
     uint8_t* grad_logits; uint64_t grad_stride;
     uint32_t tokens, experts, topk, groups, group_size, topk_groups, lanes_log2, index_bits;
     uint32_t fp32, idx64, sigmoid, renormalize, best_two, by_logits;
-    uint32_t aligned;                                         // four neighbours can be read (and written) at once
+    uint32_t aligned, bias_aligned;                           // four neighbours can be read (and written) at once
     float scale;
 };
 
@@ -124,48 +124,84 @@ __device__ __forceinline__ float redux_min(float v) {
     return m;
 }
 
-// The choice of a token, the expert of choice `lane` in `chosen` (-1: none), by whole numbers that stand for c; answers whether that decides it.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// (NaN if one of them is)
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// The choice of a token, the expert of choice `lane` in `chosen` (-1: none), by whole numbers that stand for c; answers whether that decides it. kScores: scores
+// are looked at (there is a bias, or groups are compared by sums); else the logits are c.
 //
-// How far the c here can be from the exact one (score_error). Sigmoid: the fast exponential moves e^-l by (2 + 1.2 |l|) 2^-23 of it, so s by at most
+// How far the c here can be from the exact one. Sigmoid: the fast exponential moves e^-l by (2 + 1.2 |l|) 2^-23 of it, so s by at most
 // s (1 - s) (2 + 1.2 |l|) 2^-23 < 2^-23, the addition and the reciprocal by less than 3 x 2^-23 of s: 2^-21 in all. Softmax: l - top times log2(e) is within
 // 2^-23 of its value x, the exponential 2 ulp more, which moves s by x e^-x 2^-23 + 2^-22 < 2^-21.5 of the largest; the sum likewise, and by
 // at most 64 + 5 additions, 2^-17.8: under 2^-17 of the largest in all. The addition of b is within 2^-24 of c, and so is the sum of two scores.
-template <uint32_t kVec, uint32_t kItems>
+template <uint32_t kVec, uint32_t kItems, bool kScores>
 __device__ __forceinline__ bool quick_choice(const RouteArgs& a, const uint8_t* row, const Share<kVec>& of, const float (&l)[kItems], const Softmax& m, uint32_t lane,
                                              int32_t& chosen) {
-    const bool sigmoid = a.sigmoid != 0, with_scores = !a.by_logits || (a.groups > 1 && a.best_two);
-    const float inverse = __frcp_rn(m.sum);
-    float c[kItems], order[kItems], largest = 0.0f;
+    float c[kItems], error = 0.0f;
     bool open = false;
-    #pragma unroll
-    for (uint32_t i = 0; i < kItems; ++i) {
-        const uint32_t e = of.at(i);
-        c[i] = l[i];
-        if (with_scores) {
-            float s;
-            if (sigmoid) s = fast_reciprocal(1.0f + fast_exp2(-kLog2E * l[i]));
-            else s = fast_exp2((l[i] - m.top) * kLog2E) * inverse;
-            largest = fmaxf(largest, s);
-            const float b = a.bias && e < of.end ? bias_at(a, e) : 0.0f;
-            // (-inf where the expert cannot be chosen, whichever of the two says so)
-            c[i] = l[i] == -CUDART_INF_F ? -CUDART_INF_F : s + b;
+    if constexpr (kScores) {
+        float b[kItems] = {};
+        if (a.bias) {
+            #pragma unroll
+            for (uint32_t i = 0; i < kItems; i += kVec) {
+                const uint32_t e = of.at(i);
+                if (e >= of.end) continue;
+                if (kVec == 4 && a.bias_aligned) {
+                    const uint4 q = ld_global_v4(a.bias + e);
+                    b[i] = __uint_as_float(q.x);
+                    if constexpr (kVec == 4) { b[i + 1] = __uint_as_float(q.y); b[i + 2] = __uint_as_float(q.z); b[i + 3] = __uint_as_float(q.w); }
+                } else {
+                    #pragma unroll
+                    for (uint32_t j = 0; j < kVec; ++j) b[i + j] = __uint_as_float(ld_global_u32(a.bias + e + j));
+                }
+            }
         }
-        open |= c[i] != c[i];
-        order[i] = a.by_logits ? l[i] : c[i];
+        if (a.sigmoid) {
+            error = 0x1p-21f;
+            #pragma unroll
+            for (uint32_t i = 0; i < kItems; ++i) c[i] = fast_reciprocal(1.0f + fast_exp2(-kLog2E * l[i]));
+        } else {
+            const float inverse = fast_reciprocal(m.sum);
+            float largest = 0.0f;
+            #pragma unroll
+            for (uint32_t i = 0; i < kItems; ++i) {
+                c[i] = fast_exp2((l[i] - m.top) * kLog2E) * inverse;
+                largest = fmaxf(largest, c[i]);
+            }
+            error = 0x1p-17f * redux_max(largest);
+        }
+        // (-inf where the expert cannot be chosen, whichever of the two says so)
+        #pragma unroll
+        for (uint32_t i = 0; i < kItems; ++i) c[i] = l[i] == -CUDART_INF_F ? -CUDART_INF_F : c[i] + b[i];
+    } else {
+        #pragma unroll
+        for (uint32_t i = 0; i < kItems; ++i) c[i] = l[i];
     }
-    const float relative = sigmoid ? 0x1p-21f : 0x1p-17f;
-    const float error = with_scores ? relative * (sigmoid ? 1.0f : redux_max(largest)) : 0.0f;
+    float top;
     if (a.groups > 1) {
         const uint32_t lanes = 1u << a.lanes_log2, group = lane >> a.lanes_log2;
-        float best = -CUDART_INF_F, second = -CUDART_INF_F;   // of the group's values
+        // the two largest of the group's values, in pairs
+        float best = fmaxf(c[0], c[1]), second = fminf(c[0], c[1]), nan = max3_nan(c[0], c[1], c[1]);
         #pragma unroll
-        for (uint32_t i = 0; i < kItems; ++i) {
-            second = fmaxf(second, fminf(best, c[i]));
-            best = fmaxf(best, c[i]);
+        for (uint32_t i = 2; i < kItems; i += 2) {
+            const float high = fmaxf(c[i], c[i + 1]), low = fminf(c[i], c[i + 1]);
+            second = max3(second, low, fminf(best, high));
+            best = fmaxf(best, high);
+            nan = max3_nan(nan, c[i], c[i + 1]);
         }
+        open |= nan != nan;
         for (uint32_t o = lanes / 2; o > 0; o >>= 1) {
             const float b = __shfl_xor_sync(kAll, best, o), s = __shfl_xor_sync(kAll, second, o);
-            second = fmaxf(fmaxf(second, s), fminf(best, b));
+            second = max3(second, s, fminf(best, b));
             best = fmaxf(best, b);
         }
         // (a group with a single expert that can be chosen counts that one alone)
@@ -175,41 +211,52 @@ __device__ __forceinline__ bool quick_choice(const RouteArgs& a, const uint8_t* 
         bool taken = false;
         for (uint32_t k = 0; k < a.topk_groups; ++k) {
             last = redux_max(left);
-            const uint32_t first = __ffs(__ballot_sync(kAll, left == last)) - 1;
             if (last == -CUDART_INF_F) break;
+            const uint32_t first = __ffs(__ballot_sync(kAll, left == last)) - 1;
             if (group == first >> a.lanes_log2) { taken = true; left = -CUDART_INF_F; }
         }
         const float next = redux_max(left);
-        // (equal scores made of logits alone are equal)
-        if (with_scores) open |= next > -CUDART_INF_F && last - next <= 4.0f * error + 0x1p-21f * fabsf(last);
+        // (scores that are logits are exact)
+        if (kScores) open |= next > -CUDART_INF_F && last - next <= 4.0f * error + 0x1p-21f * fabsf(last);
         if (!taken) {
             #pragma unroll
-            for (uint32_t i = 0; i < kItems; ++i) order[i] = -CUDART_INF_F;
+            for (uint32_t i = 0; i < kItems; ++i) c[i] = -CUDART_INF_F;
         }
     }
-    // Distances from the largest, in `units` of their range, which ends 2 (32 among logits) below it: what lies further down is not told apart.
-    float top = -CUDART_INF_F, bottom = CUDART_INF_F;
-    #pragma unroll
-    for (uint32_t i = 0; i < kItems; ++i) {
-        top = fmaxf(top, order[i]);
-        if (order[i] > -CUDART_INF_F) bottom = fminf(bottom, order[i]);
+    if (kScores && a.by_logits) {
+        error = 0.0f;
+        #pragma unroll
+        for (uint32_t i = 0; i < kItems; ++i) c[i] = c[i] == -CUDART_INF_F ? -CUDART_INF_F : l[i];
     }
+    // Distances from the largest in units of a range that ends 2 below it (of logits: at the smallest, or 32 below): what lies further down is not told apart.
+    top = max3_nan(c[0], c[1], c[1]);
+    #pragma unroll
+    for (uint32_t i = 2; i < kItems; i += 2) top = max3_nan(top, c[i], c[i + 1]);
+    open |= top != top;
     top = redux_max(top);
-    bottom = redux_min(bottom);
-    const float range = fminf(top - bottom, a.by_logits ? 32.0f : 2.0f);
-    // (16 units are left free at both ends for what per_unit, rounded, is off by)
     const uint32_t units = (1u << (31 - a.index_bits < 23 ? 31 - a.index_bits : 23)) - 32;
-    const float per_unit = range > 0.0f ? __fdividef((float)units, range) : 1.0f;
-    open |= top == CUDART_INF_F || per_unit > 0x1p100f;
+    float range = 2.0f;
+    if (!kScores || a.by_logits) {
+        float bottom = CUDART_INF_F;
+        #pragma unroll
+        for (uint32_t i = 0; i < kItems; ++i)
+            if (c[i] > -CUDART_INF_F) bottom = fminf(bottom, c[i]);
+        range = fmaxf(fminf(top - redux_min(bottom), 32.0f), 0x1p-60f);
+    }
+    chosen = -1;
+    if (top == -CUDART_INF_F) return !__any_sync(kAll, open);    // (nothing can be chosen, unless by NaN)
+    open |= top == CUDART_INF_F;
+    const float per_unit = __fdividef((float)units, range), offset = (float)(units + 16);
+    const uint32_t mask = (1u << a.index_bits) - 1, code = mask - of.first;
     uint32_t key[kItems], mine = 0;
     #pragma unroll
     for (uint32_t i = 0; i < kItems; ++i) {
-        // (a float in 2^23 .. 2^24 holds the whole number in its low bits)
-        const float field = fmaf(-fminf(top - order[i], range), per_unit, 8388608.0f + (float)(units + 16));
-        key[i] = order[i] > -CUDART_INF_F ? (__float_as_uint(field) & 0x7fffffu) << a.index_bits | (kMostExperts - 1 - of.at(i)) & ((1u << a.index_bits) - 1) : 0u;
+        // (the conversion gives 0 for what is below the range, -inf and NaN)
+        const uint32_t field = __float2uint_rn(fmaf(c[i] - top, per_unit, offset));
+        key[i] = (field << a.index_bits) + (code - (of.at(i) - of.first)) % (mask + 1);
         mine = max(mine, key[i]);
     }
-    uint32_t held = 0;
+    uint32_t held = 0xffffffffu;
     for (uint32_t k = 0; k < a.topk; ++k) {
         const uint32_t m1 = __reduce_max_sync(kAll, mine);
         if (lane == k) held = m1;
@@ -219,19 +266,23 @@ __device__ __forceinline__ bool quick_choice(const RouteArgs& a, const uint8_t* 
         for (uint32_t i = 0; i < kItems; ++i) next = __viaddmax_u32(key[i], 0u - m1, next);
         if (mine == m1) mine = next == 0x80000000u ? 0u : next + m1;
     }
-    const uint32_t mask = (1u << a.index_bits) - 1;
-    chosen = held != 0 ? (int32_t)((kMostExperts - 1 - held) & mask) : -1;
+    chosen = lane < a.topk ? (int32_t)(mask - (held & mask)) : -1;
+    // (below the range, or nothing that can be chosen)
+    open |= held >> a.index_bits == 0;
     // Are neighbours of the order apart by more than their errors, or equal because their logits and biases are? The last choice's neighbour is the one that
     // was not taken; where these two are equal, its own neighbour might stand between them.
     const uint32_t behind = __reduce_max_sync(kAll, mine);
     uint32_t after = __shfl_down_sync(kAll, held, 1);
     if (lane == a.topk - 1) after = behind;
     const float bound = 2.0f * (error + 0x1p-22f * (fabsf(top) + range)) * per_unit + 3.0f;
-    const auto near = [&](uint32_t k, uint32_t below) { return below != 0 && (float)((k >> a.index_bits) - (below >> a.index_bits)) <= bound; };
+    const auto near = [&](uint32_t k, uint32_t below) { return (float)((k >> a.index_bits) - (below >> a.index_bits)) <= bound; };
     bool equal = false;
-    if (near(held, after)) {
-        const uint32_t e = (kMostExperts - 1 - after) & mask;
-        equal = logit_at(a, row, (uint32_t)chosen) == logit_at(a, row, e) && bias_at(a, (uint32_t)chosen) == bias_at(a, e);
+    if (lane < a.topk && near(held, after)) {
+        // (only keys above 0 units stand for an expert)
+        if (held >> a.index_bits != 0 && after >> a.index_bits != 0) {
+            const uint32_t e = mask - (after & mask);
+            equal = logit_at(a, row, (uint32_t)chosen) == logit_at(a, row, e) && bias_at(a, (uint32_t)chosen) == bias_at(a, e);
+        }
         open |= !equal;
     }
     if (__any_sync(kAll, equal && lane == a.topk - 1)) {
@@ -321,7 +372,7 @@ __device__ __noinline__ int32_t exact_choice(const RouteArgs& a, const uint8_t* 
     return chosen;
 }
 
-template <uint32_t kVec, uint32_t kItems>
+template <uint32_t kVec, uint32_t kItems, bool kScores>
 __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const RouteArgs a) {
     const uint32_t lane = threadIdx.x % 32, token = blockIdx.x * (kRouteThreads / 32) + threadIdx.x / 32;
     griddep_wait();
@@ -336,7 +387,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const RouteArg
     Softmax m{0.0f, 1.0f};
     if (!a.sigmoid) m = softmax_of(l);
     int32_t chosen;
-    if (!quick_choice(a, row, of, l, m, lane, chosen)) chosen = exact_choice<kVec, kItems>(a, row, of, m.top, lane);
+    if (!quick_choice<kVec, kItems, kScores>(a, row, of, l, m, lane, chosen)) chosen = exact_choice<kVec, kItems>(a, row, of, m.top, lane);
     float w = 0.0f;
     if (chosen >= 0) w = score_of(a.sigmoid != 0, m, logit_at(a, row, (uint32_t)chosen));
     if (a.renormalize) w = __fdiv_rn(w, fmaxf(warp_sum(w), kLeastSum));
@@ -439,7 +490,8 @@ template <template <uint32_t, uint32_t> class Pick> static const void* for_items
     return items <= 2 ? Pick<1, 2>::fn() : items <= 4 ? Pick<1, 4>::fn() : items <= 8 ? Pick<1, 8>::fn() : items <= 16 ? Pick<1, 16>::fn()
            : items <= 32 ? Pick<1, 32>::fn() : Pick<1, 64>::fn();
 }
-template <uint32_t kVec, uint32_t kItems> struct Forward { static const void* fn() { return (const void*)moe_route_kernel<kVec, kItems>; } };
+template <uint32_t kVec, uint32_t kItems> struct ByScores { static const void* fn() { return (const void*)moe_route_kernel<kVec, kItems, true>; } };
+template <uint32_t kVec, uint32_t kItems> struct ByLogits { static const void* fn() { return (const void*)moe_route_kernel<kVec, kItems, false>; } };
 template <uint32_t kVec, uint32_t kItems> struct Backward { static const void* fn() { return (const void*)moe_route_grad_kernel<kVec, (kItems < 32 ? kItems : 32)>; } };
 
 static int route_args(RouteArgs& a, const void* logits, int is_fp32, uint64_t stride, uint32_t tokens, uint32_t experts, uint32_t topk, int sigmoid,
@@ -477,9 +529,11 @@ extern "C" int dg_moe_route_launch(const void* logits, int is_fp32, uint64_t str
     while ((1u << a.index_bits) < experts) ++a.index_bits;
     const bool vec = a.group_size % 4 == 0;
     a.aligned = vec && (reinterpret_cast<uintptr_t>(logits) | a.stride) % (is_fp32 ? 16 : 8) == 0;
+    a.bias_aligned = reinterpret_cast<uintptr_t>(bias) % 16 == 0;
     const uint32_t run = vec ? 4 : 1, items = (a.group_size + (run << a.lanes_log2) - 1) / (run << a.lanes_log2) * run;
     void* params[] = {&a};
-    return launch_overlapped(for_items<Forward>(vec, items), dim3((tokens + kRouteThreads / 32 - 1) / (kRouteThreads / 32)), dim3(kRouteThreads), params,
+    const bool scores = !a.by_logits || (num_groups > 1 && a.best_two);
+    return launch_overlapped(scores ? for_items<ByScores>(vec, items) : for_items<ByLogits>(vec, items), dim3((tokens + kRouteThreads / 32 - 1) / (kRouteThreads / 32)), dim3(kRouteThreads), params,
                              static_cast<cudaStream_t>(stream));
 }
 

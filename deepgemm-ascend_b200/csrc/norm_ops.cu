@@ -246,6 +246,12 @@ __global__ void __launch_bounds__(kThreads) rms_norm_grad_kernel(const NormGradA
         for (int j = 0; j < 4; ++j) sum_w[i][j] = Pair(0.0f);
     }
     if (kAhead && first < a.tokens) load(first);
+    Pair w[4] = {};                                           // (those of several pieces come from L1 each time)
+    const auto weights = [&](uint32_t i) {
+        const uint32_t c = (i * a.threads + t) * 8;
+        if (c < a.hidden) weight_at(a.weight, a.weight_fp32, c, w);
+    };
+    if constexpr (kPieces == 1) weights(0);
     uint32_t turn = 0;
     for (uint64_t token = first; token < a.tokens; token += stride, turn ^= 1) {
         if (!kAhead) load(token);
@@ -257,10 +263,9 @@ __global__ void __launch_bounds__(kThreads) rms_norm_grad_kernel(const NormGradA
         Pair dots(0.0f);
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
-            const uint32_t c = (i * a.threads + t) * 8;
             h0[i] = h[i]; more0[i] = more[i]; g0[i] = g[i];
-            Pair n[4], u[4], w[4] = {};
-            if (c < a.hidden) weight_at(a.weight, a.weight_fp32, c, w);
+            Pair n[4], u[4];
+            if constexpr (kPieces > 1) weights(i);
             h0[i].get(n);
             g0[i].get(u);
             #pragma unroll
@@ -276,12 +281,15 @@ __global__ void __launch_bounds__(kThreads) rms_norm_grad_kernel(const NormGradA
         dot = group_sum(dot + other, sums[turn], group * warps, warps, group + 1);
         // dx = rstd u - h (rstd^3 mean(u h)) + grad_h
         const Pair slope(-(r * r * (r * (dot * a.inverse_hidden))));
+        // (what several pieces would hold over the barrier is read again: it lies in L2)
+        if constexpr (!kAhead) load(token);
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
             const uint32_t c = (i * a.threads + t) * 8;
             if (c >= a.hidden) continue;
-            Pair n[4], u[4], d[4], w[4];
-            weight_at(a.weight, a.weight_fp32, c, w);
+            Pair n[4], u[4], d[4];
+            if constexpr (kPieces > 1) weights(i);
+            if constexpr (!kAhead) { h0[i] = h[i]; g0[i] = g[i]; more0[i] = more[i]; }
             h0[i].get(n);
             g0[i].get(u);
             more0[i].get(d);
