@@ -136,15 +136,18 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
     return d;
 }
 
-// The choice of a token, the expert of choice `lane` in `chosen` (-1: none), by whole numbers that stand for c; answers whether that decides it. kScores: scores
-// are looked at (there is a bias, or groups are compared by sums); else the logits are c.
+// The choice of a token, the expert of choice `lane` in `chosen` (-1: none; the one behind the last in lane topk), by whole numbers that stand for c; answers
+// whether that decides it, or leaves open the order of these only, or who they are. kScores: scores are looked at (there is a bias, or groups are
+// compared by sums); else the logits are c.
 //
-// How far the c here can be from the exact one. Sigmoid: the fast exponential moves e^-l by (2 + 1.2 |l|) 2^-23 of it, so s by at most
-// s (1 - s) (2 + 1.2 |l|) 2^-23 < 2^-23, the addition and the reciprocal by less than 3 x 2^-23 of s: 2^-21 in all. Softmax: l - top times log2(e) is within
+// How far the c here can be from the exact one. Sigmoid: the product with log2(e) is rounded by 2^-24 of it and the exponential is within 2^-22 of its
+// value, which moves s by s (1 - s) (|l| + 4) 2^-24 < 1.3 x 2^-24; the addition and the reciprocal by 2^-24 and 2^-23 of s: 4.3 x 2^-24 in all. Softmax: l - top times log2(e) is within
 // 2^-23 of its value x, the exponential 2 ulp more, which moves s by x e^-x 2^-23 + 2^-22 < 2^-21.5 of the largest; the sum likewise, and by
-// at most 64 + 5 additions, 2^-17.8: under 2^-17 of the largest in all. The addition of b is within 2^-24 of c, and so is the sum of two scores.
+// at most 64 + 5 additions, 2^-17.8: under 2^-17 of the largest in all. The addition of b and the difference from the largest are within 2^-24 of their
+// values, and so is the sum of two scores.
+enum class Choice { kDecided, kOrderOpen, kOpen };
 template <uint32_t kVec, uint32_t kItems, bool kScores>
-__device__ __forceinline__ bool quick_choice(const RouteArgs& a, const uint8_t* row, const Share<kVec>& of, const float (&l)[kItems], const Softmax& m, uint32_t lane,
+__device__ __forceinline__ Choice quick_choice(const RouteArgs& a, const uint8_t* row, const Share<kVec>& of, const float (&l)[kItems], const Softmax& m, uint32_t lane,
                                              int32_t& chosen) {
     float c[kItems], error = 0.0f;
     bool open = false;
@@ -166,7 +169,7 @@ __device__ __forceinline__ bool quick_choice(const RouteArgs& a, const uint8_t* 
             }
         }
         if (a.sigmoid) {
-            error = 0x1p-21f;
+            error = 0x1.2p-22f;
             #pragma unroll
             for (uint32_t i = 0; i < kItems; ++i) c[i] = fast_reciprocal(1.0f + fast_exp2(-kLog2E * l[i]));
         } else {
@@ -244,7 +247,7 @@ __device__ __forceinline__ bool quick_choice(const RouteArgs& a, const uint8_t* 
         range = fmaxf(fminf(top - redux_min(bottom), 32.0f), 0x1p-60f);
     }
     chosen = -1;
-    if (top == -CUDART_INF_F) return !__any_sync(kAll, open);    // (nothing can be chosen, unless by NaN)
+    if (top == -CUDART_INF_F) return __any_sync(kAll, open) ? Choice::kOpen : Choice::kDecided;    // (nothing can be chosen, unless by NaN)
     open |= top == CUDART_INF_F;
     const float per_unit = __fdividef((float)units, range), offset = (float)(units + 16);
     const uint32_t mask = (1u << a.index_bits) - 1, code = mask - of.first;
@@ -253,7 +256,7 @@ __device__ __forceinline__ bool quick_choice(const RouteArgs& a, const uint8_t* 
     for (uint32_t i = 0; i < kItems; ++i) {
         // (the conversion gives 0 for what is below the range, -inf and NaN)
         const uint32_t field = __float2uint_rn(fmaf(c[i] - top, per_unit, offset));
-        key[i] = (field << a.index_bits) + (code - (of.at(i) - of.first)) % (mask + 1);
+        key[i] = (field << a.index_bits) + ((code - (of.at(i) - of.first)) & mask);
         mine = max(mine, key[i]);
     }
     uint32_t held = 0xffffffffu;
@@ -266,32 +269,57 @@ __device__ __forceinline__ bool quick_choice(const RouteArgs& a, const uint8_t* 
         for (uint32_t i = 0; i < kItems; ++i) next = __viaddmax_u32(key[i], 0u - m1, next);
         if (mine == m1) mine = next == 0x80000000u ? 0u : next + m1;
     }
-    chosen = lane < a.topk ? (int32_t)(mask - (held & mask)) : -1;
-    // (below the range, or nothing that can be chosen)
-    open |= held >> a.index_bits == 0;
-    // Are neighbours of the order apart by more than their errors, or equal because their logits and biases are? The last choice's neighbour is the one that
-    // was not taken; where these two are equal, its own neighbour might stand between them.
     const uint32_t behind = __reduce_max_sync(kAll, mine);
+    if (lane == a.topk) held = behind;
+    chosen = lane <= a.topk && held >> a.index_bits != 0 ? (int32_t)(mask - (held & mask)) : -1;
+    // (below the range, or nothing that can be chosen)
+    if (lane < a.topk) open |= held >> a.index_bits == 0;
+    // Are neighbours of the order apart by more than their errors, or equal because their logits and biases are? The last choice's neighbour is the one that
+    // was not taken; where these two are equal or their order is open, its own neighbour might stand between them.
     uint32_t after = __shfl_down_sync(kAll, held, 1);
     if (lane == a.topk - 1) after = behind;
-    const float bound = 2.0f * (error + 0x1p-22f * (fabsf(top) + range)) * per_unit + 3.0f;
+    const float bound = 2.0f * (error + 0x1p-23f * (fabsf(top) + range)) * per_unit + 3.0f;
     const auto near = [&](uint32_t k, uint32_t below) { return (float)((k >> a.index_bits) - (below >> a.index_bits)) <= bound; };
-    bool equal = false;
+    bool equal = false, order_open = false;
     if (lane < a.topk && near(held, after)) {
         // (only keys above 0 units stand for an expert)
         if (held >> a.index_bits != 0 && after >> a.index_bits != 0) {
             const uint32_t e = mask - (after & mask);
             equal = logit_at(a, row, (uint32_t)chosen) == logit_at(a, row, e) && bias_at(a, (uint32_t)chosen) == bias_at(a, e);
+            order_open = !equal;
+        } else {
+            open = true;
         }
-        open |= !equal;
     }
-    if (__any_sync(kAll, equal && lane == a.topk - 1)) {
+    if (__any_sync(kAll, order_open || (equal && lane == a.topk - 1))) {
         uint32_t next = 0;
         #pragma unroll
         for (uint32_t i = 0; i < kItems; ++i) next = max(next, key[i] < behind ? key[i] : 0u);
         open |= near(behind, __reduce_max_sync(kAll, next));
     }
-    return !__any_sync(kAll, open);
+    return __any_sync(kAll, open) ? Choice::kOpen : __any_sync(kAll, order_open) ? Choice::kOrderOpen : Choice::kDecided;
+}
+
+// The order of the choices and the one behind them, where that alone is open: lane j <= topk knows one of them, and its score in 64 bits (a sigmoid's, which
+// needs no sum over the others) takes its place.
+__device__ __noinline__ int32_t exact_order(const RouteArgs& a, const uint8_t* row, int32_t mine, uint32_t lane) {
+    double c = -CUDART_INF;
+    if (mine >= 0) {
+        const double l = logit_at(a, row, (uint32_t)mine);
+        c = a.by_logits ? l : 1.0 / (1.0 + exp(-l)) + bias_at(a, (uint32_t)mine);
+    }
+    uint32_t place = 0;
+    for (uint32_t k = 0; k <= a.topk; ++k) {
+        const double other = __shfl_sync(kAll, c, k);
+        const int32_t e = __shfl_sync(kAll, mine, k);
+        place += other > c || (other == c && e < mine);
+    }
+    int32_t chosen = -1;
+    for (uint32_t k = 0; k <= a.topk; ++k) {
+        const int32_t e = __shfl_sync(kAll, mine, k);
+        if (__shfl_sync(kAll, place, k) == lane) chosen = e;
+    }
+    return chosen;
 }
 
 // The same with scores of 64 bits. In the order of whole numbers: NaN above everything (as in torch.topk), 0 for what cannot be chosen.
@@ -387,7 +415,14 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const RouteArg
     Softmax m{0.0f, 1.0f};
     if (!a.sigmoid) m = softmax_of(l);
     int32_t chosen;
-    if (!quick_choice<kVec, kItems, kScores>(a, row, of, l, m, lane, chosen)) chosen = exact_choice<kVec, kItems>(a, row, of, m.top, lane);
+    Choice state = quick_choice<kVec, kItems, kScores>(a, row, of, l, m, lane, chosen);
+    // (a softmax's scores want its sum in 64 bits, and the 33 of 32 choices more lanes)
+    if (state == Choice::kOrderOpen) {
+        if ((a.sigmoid || a.by_logits) && a.topk < 32) chosen = exact_order(a, row, chosen, lane);
+        else state = Choice::kOpen;
+    }
+    if (state == Choice::kOpen) chosen = exact_choice<kVec, kItems>(a, row, of, m.top, lane);
+    if (lane >= a.topk) chosen = -1;
     float w = 0.0f;
     if (chosen >= 0) w = score_of(a.sigmoid != 0, m, logit_at(a, row, (uint32_t)chosen));
     if (a.renormalize) w = __fdiv_rn(w, fmaxf(warp_sum(w), kLeastSum));

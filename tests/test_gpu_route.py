@@ -70,6 +70,10 @@ def test_choices_that_32_bits_leave_open():
             for bias in (None, torch.zeros(128), torch.full((128,), 0.25), torch.randn(4).repeat(32) * 1e-7, 8 + torch.randn(128) * 1e-6):
                 for best in (1, 2):
                     _check(logits, 8, scoring, bias=bias, num_groups=groups, topk_groups=taken, group_best=best)
+        # all that there are, and all but one; as many as lanes
+        for bias in (None, torch.zeros(128), torch.randn(4).repeat(32) * 1e-7):
+            for n in (8, 9, 32, 33):
+                _check(logits[:, :n].contiguous(), min(n, 8 if n < 10 else 32), scoring, bias=None if bias is None else bias[:n].contiguous())
         # a bias that makes up for the scores' differences
         logits = torch.randn(1, 64).expand(40, 64) + torch.randn(40, 1)
         scores = torch.sigmoid(logits) if scoring == 'sigmoid' else torch.softmax(logits, 1)
