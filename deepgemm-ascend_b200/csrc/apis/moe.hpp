@@ -83,7 +83,8 @@ inline TensorPair moe_route(const torch::Tensor& logits, int64_t topk, const std
     host_assert(group_best == 1 || group_best == 2, "group_best must be 1 or 2");
     host_assert(topk <= experts / num_groups * topk_groups, "the groups that are taken hold fewer experts than topk");
     const c10::cuda::CUDAGuard guard(logits.device());
-    auto idx = empty_on({tokens, topk}, torch::kInt32, logits), weights = empty_on({tokens, topk}, torch::kFloat32, logits);
+    SharedAllocation both(2 * SharedAllocation::room(tokens * topk * 4), logits);
+    const auto idx = both.take({tokens, topk}, {topk, 1}, torch::kInt32), weights = both.take({tokens, topk}, {topk, 1}, torch::kFloat32);
     if (tokens != 0)
         check(dg_moe_route_launch(logits.data_ptr(), logits.scalar_type() == torch::kFloat32, (uint64_t)stride_of_rows(logits), (uint32_t)tokens, (uint32_t)experts,
                                   (uint32_t)topk, scoring == "sigmoid", bias.has_value() ? static_cast<const float*>(bias->data_ptr()) : nullptr, (uint32_t)num_groups,

@@ -239,7 +239,10 @@ inline std::tuple<TensorPair, std::optional<torch::Tensor>, torch::Tensor, torch
     host_assert(!out_h.has_value() || residual.has_value(), "out_h needs a residual");
     const int64_t tokens = x.size(0), hidden = x.size(1);
     const c10::cuda::CUDAGuard guard(x.device());
-    auto q = empty_on({tokens, hidden}, torch::kFloat8_e4m3fn, x), sf = empty_scales({tokens, ceil_div(hidden, 64)}, x), rstd = empty_on({tokens}, torch::kFloat32, x);
+    const int64_t cols = ceil_div(hidden, 64);
+    SharedAllocation small(SharedAllocation::room(tokens * cols * 2) + SharedAllocation::room(tokens * 4), x);
+    const auto q = empty_on({tokens, hidden}, torch::kFloat8_e4m3fn, x);
+    const auto sf = small.take({tokens, cols}, {1, std::max<int64_t>(tokens, 1)}, torch::kInt16), rstd = small.take({tokens}, {1}, torch::kFloat32);
     std::optional<torch::Tensor> rows;
     if (with_rows) rows = empty_on({tokens, hidden}, torch::kBFloat16, x);
     auto h = !residual.has_value() ? x : out_h.has_value() ? out_h.value() : empty_on({tokens, hidden}, x.scalar_type(), x);

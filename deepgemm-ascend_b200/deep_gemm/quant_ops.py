@@ -270,7 +270,8 @@ def rms_norm_to_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[to
         y = h * rstd * weight        (out, out_sf): y as `cast_to_fp8` quantises it, but from FP32; rows: y in BF16 `with_rows`, else None
 
     weight: BF16 or FP32 [hidden]. The sum of squares is held in 64 bits: a token's results do not depend on how many others there are. `out_h`:
-    where h goes with a residual, which may be `residual` or x itself. hidden is a multiple of 32, at most 16384; rows start on 16-byte boundaries."""
+    where h goes with a residual, which may be `residual` or x itself. hidden is a multiple of 32, at most 16384; rows start on 16-byte boundaries.
+    out_sf and rstd may share one allocation."""
     _host_assert(x.is_cuda and x.dim() == 2 and x.stride(1) == 1 and _is_float(x), 'x must be a row-major 2-D BF16 or FP32 tensor on a CUDA device')
     tokens, hidden = x.shape
     _check_norm(x, weight, tokens, hidden)
