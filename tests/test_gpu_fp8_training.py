@@ -7,6 +7,11 @@ dx_l = g w r (p + l p (1 - p)): the terms move by d p and 3 d |l| p (1 - p carri
 normal number where it is below: it moves by at most t = 2^-126 beyond that, dx_r by t |g w l| and dx_l by t |g w r| (1 + |l|). dx is rounded to BF16 once, 2^-8 of the value.
 dw: a sum whose terms pass at most H / 32 + 60 additions."""
 
+import os
+import subprocess
+import sys
+import textwrap
+
 import pytest
 import torch
 
@@ -355,6 +360,34 @@ def test_rows_behind_32_bits():
     assert torch.equal(deep_gemm.cast_from_fp8((kept, sf)), deep_gemm.cast_from_fp8(want))
 
 
+def test_many_rows():
+    """Against torch on the GPU: rows over many CTAs, an odd number of them."""
+    seed_all(10)
+    rows, hidden = 5003, 1408
+    x, g, w = (torch.randn(rows, 2 * hidden, device='cuda') * 2).bfloat16(), torch.randn(rows, hidden, device='cuda').bfloat16(), torch.rand(rows, device='cuda')
+    out, kept = deep_gemm.swiglu_apply_weight_to_fp8_with_checkpoint(x, w)
+    want, want_kept = deep_gemm.swiglu_apply_weight_to_fp8(x, w), deep_gemm.cast_to_fp8(x)
+    for (q, sf), (q1, sf1) in ((out, want), (kept, want_kept)):
+        assert torch.equal(q.view(torch.uint8), q1.view(torch.uint8)) and torch.equal(sf, sf1)
+    dx, dw = deep_gemm.swiglu_apply_weight_grad(g, kept, w)
+    values = deep_gemm.cast_from_fp8(kept, torch.float32).double().requires_grad_()
+    w64 = w.double().requires_grad_()
+    l, r = values[:, :hidden], values[:, hidden:]
+    (l * torch.sigmoid(l) * r * w64[:, None]).backward(g.double())
+    # (2^-8 of the value for the rounding; a few ulp of FP32 times the terms, which are at most |g w| (1 + |l|) (1 + |r|))
+    size = (g.double() * w.double()[:, None]).abs() * (1 + l.abs()) * (1 + r.abs())
+    assert ((dx.double() - values.grad).abs() <= U * values.grad.abs() + 64 * E * torch.cat((size, size), 1)).all()
+    assert ((dw.double() - w64.grad).abs() <= (hidden / 32 + 124) * E * (g.double() * l * r).abs().sum(1)).all()
+    q, sf = deep_gemm.cast_to_fp8(kept, mn_major=True)
+    part = slice(4992, 5003)                                  # the last, ragged tile
+    codes, byte, _ = oracle.cast_fp8_ref(values.detach()[4992:].float().cpu(), 0)
+    assert torch.equal(_bytes(q[part]), codes) and torch.equal(sf[78:].cpu(), oracle.pack_scales(byte, 0))
+    back = deep_gemm.cast_from_fp8((q, sf), torch.float32, mn_major=True).double()
+    amax = torch.nn.functional.pad(values.detach().abs(), (0, 0, 0, -rows % 32)).unflatten(0, (-1, 32)).amax(1).repeat_interleave(32, 0)[:rows]
+    # (half a step of a code is 2^-4 of it, or 2^-10 of a scale, which is at most amax / 224)
+    assert ((back - values.detach()).abs() <= 2.0 ** -4 * values.detach().abs() + 2.0 ** -10 * amax / 224 + 1e-9).all()
+
+
 def test_two_streams_at_once_a_captured_run_and_both_hosts():
     seed_all(12)
     layer = python_layer('quant_ops')
@@ -395,6 +428,46 @@ def test_two_streams_at_once_a_captured_run_and_both_hosts():
     graph.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a.view(torch.uint8) if a.dtype == FP8 else a, b.view(torch.uint8) if b.dtype == FP8 else b) for a, b in zip(held, run(sets[0])))
+
+
+FIRST = textwrap.dedent('''
+    import sys
+    sys.path.insert(0, %r)
+    import torch
+    import deep_gemm
+
+    x, r, w = torch.randn(300, 2048, device='cuda').bfloat16(), torch.randn(300, 2048, device='cuda').bfloat16(), torch.ones(2048, device='cuda')
+    logits, g = torch.randn(300, 64, device='cuda'), torch.randn(300, 4, device='cuda')
+
+
+    def way():
+        (q, sf), rows, h, rstd = deep_gemm.rms_norm_to_fp8(x, w, residual=r, with_rows=True)
+        idx, p = deep_gemm.moe_route(logits, 4, bias=w[:64].contiguous(), num_groups=8, topk_groups=3)
+        out, kept = deep_gemm.swiglu_apply_weight_to_fp8_with_checkpoint(rows, rstd)
+        dx, dw = deep_gemm.swiglu_apply_weight_grad(rows[:, :1024], kept, rstd)
+        mn = deep_gemm.cast_to_fp8(kept, mn_major=True)
+        return [q.view(torch.uint8), sf, rows, h, rstd, idx, p, deep_gemm.moe_route_grad(g, logits, idx), out[0].view(torch.uint8), out[1], dx, dw, mn[0].view(torch.uint8), mn[1],
+                deep_gemm.cast_from_fp8(mn, mn_major=True), *deep_gemm.rms_norm_grad(dx, h, w, rstd, grad_h=r)]
+
+
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = way()
+    graph.replay()
+    torch.cuda.synchronize()
+    with torch.inference_mode():
+        inside = way()
+    for a, b, c in zip(held, way(), inside):
+        assert torch.equal(a, b) and torch.equal(a, c)
+    print('PASS')
+''') % os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), 'deepgemm-ascend_b200')
+
+
+@pytest.mark.parametrize('python_host', ['0', '1'])
+def test_a_capture_that_holds_the_first_call(python_host):
+    proc = subprocess.run([sys.executable, '-c', FIRST], capture_output=True, text=True, timeout=600, env={**os.environ, 'DG_PYTHON_HOST': python_host})
+    assert proc.returncode == 0 and 'PASS' in proc.stdout, proc.stderr[-3000:]
 
 
 # ------------------------------------------------------------------------------------------------------ as they are used

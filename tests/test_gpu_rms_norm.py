@@ -36,7 +36,7 @@ def _check_forward(x, weight, residual=None, eps=1e-6, host=deep_gemm, **kw):
     return (q, sf), rows, h, rstd
 
 
-SHAPES = [(1, 32), (1, 7168), (2, 96), (3, 2048), (37, 1120), (5, 8192), (150, 288), (299, 4096), (3, 16384), (2, 12320), (301, 64)]
+SHAPES = [(1, 32), (1, 7168), (2, 96), (3, 2048), (37, 1120), (5, 8192), (150, 288), (299, 4096), (3, 16384), (2, 12320), (301, 64), (170, 8192), (320, 7168)]
 
 
 @pytest.mark.parametrize('host', quant_hosts)
