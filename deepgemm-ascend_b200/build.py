@@ -15,8 +15,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, 'csrc')
 OUT = os.path.join(HERE, 'deep_gemm', 'libdg_b200.so')
 SOURCES = ['api.cu', 'mx_gemm.cu', 'mx_gemm_k_major.cu', 'mx_gemm_mn_major.cu', 'mx_gemm_decode.cu', 'mx_gemm_bf16.cu', 'mx_gemm_fp4.cu',
-           'few_rows.cu', 'transform_sf.cu', 'quant_ops.cu', 'quant_fp4.cu', 'quant_fp8_mn.cu', 'swiglu_grad.cu', 'norm_ops.cu', 'moe_ops.cu',
-           'moe_route.cu', 'sleep.cu']
+           'few_rows.cu', 'transform_sf.cu', 'quant_ops.cu', 'quant_fp4.cu', 'moe_ops.cu', 'sleep.cu',
+           'quant_fp8_mn.cu', 'swiglu_grad.cu', 'norm_ops.cu', 'moe_route.cu']
 NVCC_FLAGS = ['-gencode', 'arch=compute_100a,code=sm_100a', '-lineinfo', '-O3', '-std=c++17', '--compress-mode=size',
               '-Xcompiler', '-fPIC', '-Xcompiler', '-fvisibility=hidden', '--expt-relaxed-constexpr']
 
