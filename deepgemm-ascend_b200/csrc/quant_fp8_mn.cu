@@ -33,7 +33,7 @@ struct MnArgs {
 };
 
 // Eight values in each of a lane's eight rows -> codes and scale bytes, through FP32.
-__device__ __forceinline__ void quantise_down(const float (&v)[8][8], float floor, uint32_t (&bytes)[2], uint2 (&codes)[8]) {
+__device__ __forceinline__ void quantise_down(const float (&v)[8][8], float floor, uint2& bytes, uint2 (&codes)[8]) {
     uint32_t e[8];
     #pragma unroll
     for (int j = 0; j < 8; ++j) {
@@ -52,12 +52,11 @@ __device__ __forceinline__ void quantise_down(const float (&v)[8][8], float floo
         for (int j = 0; j < 8; ++j) s[j] = v[i][j] * __uint_as_float((254u - min(e[j], 254u)) << 23);
         codes[i] = e4m3_pack8(s, 127u);
     }
-    bytes[0] = e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24;
-    bytes[1] = e[4] | e[5] << 8 | e[6] << 16 | e[7] << 24;
+    bytes = make_uint2(e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24, e[4] | e[5] << 8 | e[6] << 16 | e[7] << 24);
 }
 
 // BF16 rows, two values at a time: magnitudes are compared as whole numbers, products with the inverse scales are exact.
-__device__ __forceinline__ void quantise_down_bf16(const uint4 (&q)[8], float floor, uint32_t (&bytes)[2], uint2 (&codes)[8]) {
+__device__ __forceinline__ void quantise_down_bf16(const uint4 (&q)[8], float floor, uint2& bytes, uint2 (&codes)[8]) {
     uint32_t m[4] = {}, f[4], e[8];
     #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -86,8 +85,7 @@ __device__ __forceinline__ void quantise_down_bf16(const uint4 (&q)[8], float fl
         }
         codes[i] = e4m3_pack8(s, 127u);
     }
-    bytes[0] = e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24;
-    bytes[1] = e[4] | e[5] << 8 | e[6] << 16 | e[7] << 24;
+    bytes = make_uint2(e[0] | e[1] << 8 | e[2] << 16 | e[3] << 24, e[4] | e[5] << 8 | e[6] << 16 | e[7] << 24);
 }
 
 __device__ __forceinline__ uint32_t mul_f16x2(uint32_t a, uint32_t b) {
@@ -107,50 +105,53 @@ __device__ __forceinline__ uint32_t f16x2_to_e4m3(uint32_t v) {
     return (uint32_t)__nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&v), __NV_SATFINITE, __NV_E4M3);
 }
 
-// E4M3 rows with scale bytes b (of this lane's block) through FP16, two values at a time, relative to the largest byte of the warp's rows, `top`: the codes are
-// FP16 numbers h, the rows' factors 2^(b - top) and the columns' 2^(top - e) powers of two. Exact while the former are 2^-15 or more and the latter lie in
-// 2^-14 .. 2^15; answers whether that is so (the same in all lanes), which it is where the magnitudes of a tile's rows and columns lie within a
-// few thousand. The scale bytes of two columns at a time: amax <= 448 s = 1.75 x 2^8 s, so with amax = 1.m x 2^x (m of ten bits) s is 2^(x - 8), or twice that
-// where m is above 0.75, which is an addition to the bits that carries; `least` is the byte of the least amax.
-__device__ __forceinline__ bool quantise_down_fp8(const uint2 (&q)[8], const uint32_t (&b)[8], uint32_t least, uint32_t (&bytes)[2], uint2 (&codes)[8]) {
-    uint32_t top = b[0], low = b[0];
-    #pragma unroll
-    for (int i = 1; i < 8; ++i) { top = max(top, b[i]); low = min(low, b[i]); }
-    top = __reduce_max_sync(0xffffffffu, top);
-    low = __reduce_min_sync(0xffffffffu, low);
+// E4M3 rows through FP16, two values at a time, relative to the largest scale byte of the warp's rows, `top`: the codes are FP16 numbers h, the rows' factors
+// 2^(b - top) and the columns' 2^(top - e) powers of two. Exact while the former are 2^-15 or more and the latter lie in 2^-14 .. 2^15; answers whether that is
+// so (the same in all lanes), which it is where the magnitudes of a tile's rows and columns lie within a few thousand. The scale bytes of two columns at a
+// time: amax <= 448 s = 1.75 x 2^8 s, so with amax = 1.m x 2^x (m of ten bits) s is 2^(x - 8), or twice that where m is above 0.75, which is an addition
+// to the bits that carries; `least` is the byte of the least amax.
+//
+// Whatever a row or a column has once is made once and handed round: `pair` holds the bytes of row `lane` (of the tile's two blocks), `block` says which of them
+// this lane's columns lie in, and of the four words of columns that the lanes of a row share each of the four lanes of a column makes one.
+__device__ __forceinline__ bool quantise_down_fp8(const uint2 (&q)[8], uint32_t pair, uint32_t block, uint32_t least, uint32_t lane, uint2& bytes, uint2 (&codes)[8]) {
+    const uint32_t b0 = pair & 0xffu, b1 = pair >> 8;
+    const uint32_t top = __reduce_max_sync(0xffffffffu, max(b0, b1)), low = __reduce_min_sync(0xffffffffu, min(b0, b1));
     if (top == 255u || low == 0u || top - low > 15u) return false;
-    uint32_t h[8][4], m[4] = {}, f[4];
+    // (2^-15 is a subnormal number of FP16)
+    const uint32_t factors = max((15u - (top - b0)) << 10, 0x0200u) | max((15u - (top - b1)) << 10, 0x0200u) << 16, both = block ? 0x3232u : 0x1010u;
+    uint32_t h[8][4], m[4] = {};
     #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        // (2^-15 is a subnormal number of FP16)
-        const uint32_t d = top - b[i], factor = max((15u - d) << 10, 0x0200u) * 0x10001u;
+        const uint32_t factor = __byte_perm(__shfl_sync(0xffffffffu, factors, i * 4 + lane / 8), 0u, both);
         #pragma unroll
         for (int j = 0; j < 4; ++j) {
             h[i][j] = mul_f16x2(e4m3_to_f16x2((j < 2 ? q[i].x : q[i].y) >> (16 * (j % 2))), factor);
             m[j] = larger_f16x2(m[j], h[i][j]);
         }
     }
-    bool fits = true;
-    const uint32_t offset = ((top - 23u) & 0xffffu) * 0x10001u, floor = least * 0x10001u;
     #pragma unroll
     for (int j = 0; j < 4; ++j) {
         m[j] = larger_f16x2(m[j], __shfl_xor_sync(0xffffffffu, m[j], 8));
         m[j] = larger_f16x2(m[j], __shfl_xor_sync(0xffffffffu, m[j], 16));
-        // (the exponent field is x + 15; a subnormal m stands for no more than top - 22, which `least` covers or the factor shows)
-        const uint32_t some = __vcmpgtu2(m[j], 0u), e = (__vmaxs2(__vadd2(((m[j] + 0x00ff00ffu) >> 10) & 0x003f003fu, offset), floor) & some) | (floor & ~some);
-        const uint32_t x = __vsub2(top * 0x10001u, e), x_in = __vmins2(__vmaxs2(x, 0xfff2fff2u), 0x000f000fu);
-        // (a column of zeros is one under any factor; a NaN is above all codes)
-        fits &= ((x ^ x_in) & some) == 0u && __vmaxu2(m[j], 0x5f005f00u) == 0x5f005f00u;
-        f[j] = __vadd2(x_in, 0x000f000fu) << 10;
-        const uint32_t two = __byte_perm(e, 0u, 0x4420);
-        if (j % 2 == 0) bytes[j / 2] = two & 0xffffu;
-        else bytes[j / 2] |= two << 16;
     }
+    const uint32_t word = lane / 8, mine = word < 2 ? (word == 0 ? m[0] : m[1]) : (word == 2 ? m[2] : m[3]);
+    // (the exponent field is x + 15; a subnormal m stands for no more than top - 22, which `least` covers or the factor shows)
+    const uint32_t some = __vcmpgtu2(mine, 0u), floor = least * 0x10001u;
+    const uint32_t e = (__vmaxs2(__vadd2(((mine + 0x00ff00ffu) >> 10) & 0x003f003fu, ((top - 23u) & 0xffffu) * 0x10001u), floor) & some) | (floor & ~some);
+    const uint32_t x = __vsub2(top * 0x10001u, e), x_in = __vmins2(__vmaxs2(x, 0xfff2fff2u), 0x000f000fu);
+    // (a column of zeros is one under any factor; a NaN is above all codes)
+    const bool fits = ((x ^ x_in) & some) == 0u && __vmaxu2(mine, 0x5f005f00u) == 0x5f005f00u;
     if (!__all_sync(0xffffffffu, fits)) return false;
+    const uint32_t f = __vadd2(x_in, 0x000f000fu) << 10, two = __byte_perm(e, 0u, 0x4420);
+    uint32_t g[4];
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) g[j] = __shfl_sync(0xffffffffu, f, j * 8 + lane % 8);
+    bytes.x = __byte_perm(__shfl_sync(0xffffffffu, two, lane % 8), __shfl_sync(0xffffffffu, two, 8 + lane % 8), 0x5410);
+    bytes.y = __byte_perm(__shfl_sync(0xffffffffu, two, 16 + lane % 8), __shfl_sync(0xffffffffu, two, 24 + lane % 8), 0x5410);
     #pragma unroll
     for (int i = 0; i < 8; ++i)
-        codes[i] = make_uint2(f16x2_to_e4m3(mul_f16x2(h[i][0], f[0])) | f16x2_to_e4m3(mul_f16x2(h[i][1], f[1])) << 16,
-                              f16x2_to_e4m3(mul_f16x2(h[i][2], f[2])) | f16x2_to_e4m3(mul_f16x2(h[i][3], f[3])) << 16);
+        codes[i] = make_uint2(f16x2_to_e4m3(mul_f16x2(h[i][0], g[0])) | f16x2_to_e4m3(mul_f16x2(h[i][1], g[1])) << 16,
+                              f16x2_to_e4m3(mul_f16x2(h[i][2], g[2])) | f16x2_to_e4m3(mul_f16x2(h[i][3], g[3])) << 16);
     return true;
 }
 
@@ -201,20 +202,18 @@ __global__ void __launch_bounds__(kMnThreads, 8) quant_fp8_mn_kernel(const MnArg
                 if (r0 + i * 4 >= row_end) q[i] = Raw{};
         }
     }
-    uint2 codes[8];
-    uint32_t bytes[2];
+    uint2 codes[8], bytes;
     if constexpr (kFromFp8) {
-        // (rows that do not count are zeros and have no scale: the first row lends them its own; nor has the second half of a last, half-used column)
-        const uint32_t lent = __shfl_sync(0xffffffffu, pair, 0), shift = c < a.cols ? lane % 8 / 4 * 8 : 0;
+        // (rows that do not count are zeros and have no scale: the first row lends them its own; the second half of a last, half-used column is lent the first's)
+        const uint32_t lent = __shfl_sync(0xffffffffu, pair, 0), block = c < a.cols ? lane % 8 / 4 : 0u;
         if (warp_row + lane >= row_end) pair = warp_row < row_end ? lent : 0x7f7fu;
-        uint32_t b[8];
-        #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) b[i] = __shfl_sync(0xffffffffu, pair, i * 4 + lane / 8) >> shift & 0xffu;
-        if (!quantise_down_fp8(q, b, a.least, bytes, codes)) {
+        if (warp_col + 32 >= a.cols) pair = (pair & 0xffu) * 0x101u;
+        if (!quantise_down_fp8(q, pair, block, a.least, lane, bytes, codes)) {
             float v[8][8];
             #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) {
-                const float scale = ue8m0_float(r0 + i * 4 < row_end ? b[i] : 127u);
+                const uint32_t b = __shfl_sync(0xffffffffu, pair, i * 4 + lane / 8) >> (block * 8) & 0xffu;
+                const float scale = ue8m0_float(r0 + i * 4 < row_end ? b : 127u);
                 float lo[4], hi[4];
                 e4m3_unpack4(q[i].x, lo);
                 e4m3_unpack4(q[i].y, hi);
@@ -227,7 +226,7 @@ __global__ void __launch_bounds__(kMnThreads, 8) quant_fp8_mn_kernel(const MnArg
         quantise_down_bf16(q, a.floor, bytes, codes);
     }
     // (blocks behind the last row are zero)
-    if (lane < 8) *reinterpret_cast<uint2*>(&sf_smem[half][tc]) = warp_row < a.rows ? make_uint2(bytes[0], bytes[1]) : make_uint2(0u, 0u);
+    if (lane < 8) *reinterpret_cast<uint2*>(&sf_smem[half][tc]) = warp_row < a.rows ? bytes : make_uint2(0u, 0u);
     uint8_t* out = a.out + group * a.out_group_stride + (uint64_t)r0 * a.out_stride + c;
     if (inside) {
         #pragma unroll
