@@ -45,10 +45,15 @@ template <typename T> __device__ __forceinline__ T warp_sum(T v) {
     return v;
 }
 // (NaN counts for nothing here)
-__device__ __forceinline__ float warp_max(float v) {
-    #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, o));
-    return v;
+__device__ __forceinline__ float redux_max(float v) {
+    float m;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
+}
+__device__ __forceinline__ float redux_min(float v) {
+    float m;
+    asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+    return m;
 }
 
 __device__ __forceinline__ float logit_at(const RouteArgs& a, const uint8_t* row, uint32_t e) {
@@ -72,11 +77,11 @@ __device__ __forceinline__ void load_logits(const RouteArgs& a, const uint8_t* r
         if (e >= of.end) continue;
         if (kVec == 4 && a.aligned) {
             if (a.fp32) {
-                const uint4 q = ld_stream_v4(row + (uint64_t)e * 4);
+                const uint4 q = ld_global_v4(row + (uint64_t)e * 4);
                 l[i] = __uint_as_float(q.x);
                 if constexpr (kVec == 4) { l[i + 1] = __uint_as_float(q.y); l[i + 2] = __uint_as_float(q.z); l[i + 3] = __uint_as_float(q.w); }
             } else {
-                const uint2 q = ld_stream_v2(row + (uint64_t)e * 2);
+                const uint2 q = ld_global_v2(row + (uint64_t)e * 2);
                 l[i] = bf16_lo(q.x);
                 if constexpr (kVec == 4) { l[i + 1] = bf16_hi(q.x); l[i + 2] = bf16_lo(q.y); l[i + 3] = bf16_hi(q.y); }
             }
@@ -87,24 +92,22 @@ __device__ __forceinline__ void load_logits(const RouteArgs& a, const uint8_t* r
     }
 }
 
-// Largest logit and sum of e^(l - largest) of a softmax. (Where every expert is masked: 0 and 1, which makes every score 0.)
+// Largest logit and sum of e^(l - largest) of a softmax, which are left in `z`. (Where every expert is masked: 0 and 1, which makes every score 0.)
 struct Softmax { float top, sum; };
 template <uint32_t kItems>
-__device__ __forceinline__ Softmax softmax_of(const float (&l)[kItems]) {
+__device__ __forceinline__ Softmax softmax_of(const float (&l)[kItems], float (&z)[kItems]) {
     Softmax m{-CUDART_INF_F, 0.0f};
     #pragma unroll
     for (uint32_t i = 0; i < kItems; ++i) m.top = fmaxf(m.top, l[i]);
-    m.top = warp_max(m.top);
+    m.top = redux_max(m.top);
+    if (m.top == -CUDART_INF_F) m.top = 0.0f;
     #pragma unroll
-    for (uint32_t i = 0; i < kItems; ++i) m.sum += fast_exp2((l[i] - m.top) * kLog2E);
-    m.sum = warp_sum(m.sum);
-    // (a NaN beside masked experts stays one)
-    if (m.top == -CUDART_INF_F) {
-        bool bad = false;
-        #pragma unroll
-        for (uint32_t i = 0; i < kItems; ++i) bad |= l[i] != l[i];
-        m = __any_sync(kAll, bad) ? Softmax{CUDART_NAN_F, 1.0f} : Softmax{0.0f, 1.0f};
+    for (uint32_t i = 0; i < kItems; ++i) {
+        z[i] = fast_exp2((l[i] - m.top) * kLog2E);
+        m.sum += z[i];
     }
+    m.sum = warp_sum(m.sum);
+    if (m.sum == 0.0f) m.sum = 1.0f;
     return m;
 }
 // (by e^-|l|, so that neither end is lost: scores near 0 keep their bits)
@@ -113,17 +116,6 @@ __device__ __forceinline__ float sigmoid_of(float l) {
     return __fdiv_rn(l < 0.0f ? z : 1.0f, 1.0f + z);
 }
 __device__ __forceinline__ float score_of(bool sigmoid, const Softmax& m, float l) { return sigmoid ? sigmoid_of(l) : __fdiv_rn(expf(l - m.top), m.sum); }
-__device__ __forceinline__ float redux_max(float v) {
-    float m;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
-    return m;
-}
-__device__ __forceinline__ float redux_min(float v) {
-    float m;
-    asm volatile("redux.sync.min.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
-    return m;
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -147,7 +139,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // values, and so is the sum of two scores.
 enum class Choice { kDecided, kOrderOpen, kOpen };
 template <uint32_t kVec, uint32_t kItems, bool kScores>
-__device__ __forceinline__ Choice quick_choice(const RouteArgs& a, const uint8_t* row, const Share<kVec>& of, const float (&l)[kItems], const Softmax& m, uint32_t lane,
+__device__ __forceinline__ Choice quick_choice(const RouteArgs& a, const uint8_t* row, const Share<kVec>& of, const float (&l)[kItems], const Softmax& m, const float (&z)[kItems], uint32_t lane,
                                              int32_t& chosen) {
     float c[kItems], error = 0.0f;
     bool open = false;
@@ -177,7 +169,7 @@ __device__ __forceinline__ Choice quick_choice(const RouteArgs& a, const uint8_t
             float largest = 0.0f;
             #pragma unroll
             for (uint32_t i = 0; i < kItems; ++i) {
-                c[i] = fast_exp2((l[i] - m.top) * kLog2E) * inverse;
+                c[i] = z[i] * inverse;
                 largest = fmaxf(largest, c[i]);
             }
             error = 0x1p-17f * redux_max(largest);
@@ -413,9 +405,10 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const RouteArg
     float l[kItems];
     load_logits(a, row, of, l);
     Softmax m{0.0f, 1.0f};
-    if (!a.sigmoid) m = softmax_of(l);
+    float z[kItems];
+    if (!a.sigmoid) m = softmax_of(l, z);
     int32_t chosen;
-    Choice state = quick_choice<kVec, kItems, kScores>(a, row, of, l, m, lane, chosen);
+    Choice state = quick_choice<kVec, kItems, kScores>(a, row, of, l, m, z, lane, chosen);
     // (a softmax's scores want its sum in 64 bits, and the 33 of 32 choices more lanes)
     if (state == Choice::kOrderOpen) {
         if ((a.sigmoid || a.by_logits) && a.topk < 32) chosen = exact_order(a, row, chosen, lane);
@@ -459,7 +452,8 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_grad_kernel(const Rou
     }
     if (idx < 0) g = 0.0f;
     Softmax m{0.0f, 1.0f};
-    if (!sigmoid) m = softmax_of(l);
+    float z[kItems];
+    if (!sigmoid) m = softmax_of(l, z);
     const float s = idx >= 0 ? score_of(sigmoid, m, mine) : 0.0f;
     // the slope of log s (for a softmax the other part of it is the sum over all experts): 1 - s would lose its bits where s is near 1
     const float slope = sigmoid ? sigmoid_of(-mine) : 1.0f;
@@ -481,7 +475,7 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_grad_kernel(const Rou
         if (e >= of.end) continue;
         float d[kVec];
         #pragma unroll
-        for (uint32_t j = 0; j < kVec; ++j) d[j] = everywhere ? each * fast_exp2((l[i + j] - m.top) * kLog2E) : 0.0f;
+        for (uint32_t j = 0; j < kVec; ++j) d[j] = everywhere ? each * z[i + j] : 0.0f;
         if (kVec == 4 && a.aligned) {
             if (a.fp32) {
                 *reinterpret_cast<float4*>(out + (uint64_t)e * 4) = make_float4(d[0], d[kVec / 4], d[kVec / 2], d[kVec - 1]);
