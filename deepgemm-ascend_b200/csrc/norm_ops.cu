@@ -18,6 +18,7 @@
 namespace dg {
 
 constexpr uint32_t kAll = 0xffffffffu, kMostHidden = 16384;
+constexpr uint64_t kLongestWaitNs = 2000000000ull;
 
 // Eight channels of a lane as they lie in memory.
 template <typename T> struct Piece;
@@ -103,6 +104,14 @@ struct NormArgs {
     double inverse_hidden;
 };
 
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+    if (mbar_try_wait(bar, parity)) return true;
+    const uint64_t t0 = global_timer_ns();
+    while (!mbar_try_wait(bar, parity))
+        if (global_timer_ns() - t0 > kLongestWaitNs) return false;
+    return true;
+}
+
 // 1 / sqrt(m) as the nearest FP32 number (but for one in 10^8): two steps of Newton's method in 64 bits behind the FP32 instruction, where FP32 holds m.
 __device__ __forceinline__ float rsqrt_of(double m) {
     if (m > 0x1p-120 && m < 0x1p120) {
@@ -115,7 +124,8 @@ __device__ __forceinline__ float rsqrt_of(double m) {
 }
 
 // A CTA walks tokens at a distance of the grid, a thread kPieces x 8 channels of each. With kAhead the next token is asked for before the sum over
-// the CTA: what keeps HBM busy over the barrier.
+// the CTA: what keeps HBM busy over the barrier (8192 x 7168 of BF16 with a residual and BF16 rows: 89 us, 5.9 TB/s, where the bytes alone take 81 at the rate of
+// a copy; a CTA for every token took 106, L2 asked for the token behind the next 109). 1 x 7168: 2.4 us, launch and latency.
 template <typename T, uint32_t kPieces, uint32_t kThreads, uint32_t kCtas, bool kAhead>
 __global__ void __launch_bounds__(kThreads, kCtas) rms_norm_fp8_kernel(const NormArgs a) {
     __shared__ double partial[2][32];
@@ -202,8 +212,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) rms_norm_fp8_kernel(const Nor
 // a token, and walks tokens at a distance of all groups; a thread holds its channels' part of dweight in registers (FP32), the groups of a CTA add theirs up,
 // and a second kernel sums the CTAs' in their order: nothing depends on timing.
 //
-// HBM-bound, and what bounds the walk is the way from a token's loads over its barrier to its stores: with kAhead the next token is asked for in front of the
-// barrier.
+// HBM-bound: 8192 x 7168 of BF16 with a gradient of h 75 us, 6.2 TB/s (bytes alone at the rate of a copy 72); 1531 x 2048 of FP32 11.6 us, of which the second
+// kernel and the launches take 3.
 struct NormGradArgs {
     const uint8_t* g; uint64_t g_stride;                                 // BF16 or FP32 as `h` is, or BF16 beside FP32
     const uint8_t *h, *grad_h; uint64_t h_stride, grad_h_stride;         // bytes between rows; grad_h or nullptr
@@ -212,100 +222,217 @@ struct NormGradArgs {
     uint8_t* dx; uint64_t dx_stride;
     float* partial;                                                      // [gridDim.x][hidden]
     uint32_t tokens, hidden;
-    uint32_t groups, threads;                                            // of a CTA; of a group
+    uint32_t groups, threads, stages;                                    // of a CTA; of a group; tokens in shared memory
     float inverse_hidden;
 };
 
-template <typename T, typename G, uint32_t kPieces, uint32_t kThreads, bool kAhead>
+// sum(u n) = rstd sum(u h), and a thread's part of dweight.
+__device__ __forceinline__ void add_dots(const Pair (&h)[4], const Pair (&g)[4], const Pair (&w)[4], Pair scale, Pair& dots, Pair (&sum_w)[4]) {
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        dots = fma2(g[j] * w[j], h[j], dots);
+        sum_w[j] = fma2(g[j], h[j] * scale, sum_w[j]);
+    }
+}
+// dx = rstd u - h (rstd^3 mean(u h)) + grad_h, which `d` holds
+__device__ __forceinline__ void slope_of(const Pair (&h)[4], const Pair (&g)[4], const Pair (&w)[4], Pair scale, Pair slope, Pair (&d)[4]) {
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) d[j] = fma2(h[j], slope, fma2(scale, g[j] * w[j], d[j]));
+}
+__device__ __forceinline__ void store_part(const NormGradArgs& a, uint32_t c, const float (&dw)[8]) {
+    float4* const out = reinterpret_cast<float4*>(a.partial + (uint64_t)blockIdx.x * a.hidden + c);
+    out[0] = make_float4(dw[0], dw[1], dw[2], dw[3]);
+    out[1] = make_float4(dw[4], dw[5], dw[6], dw[7]);
+}
+
+// Short rows: a token in registers, a piece of it a thread. What bounds a walk is the way from a token's loads over its barrier to its stores, so the next token
+// is asked for in front of the barrier.
+template <typename T, typename G, uint32_t kThreads>
 __global__ void __launch_bounds__(kThreads) rms_norm_grad_kernel(const NormGradArgs a) {
     extern __shared__ __align__(16) uint8_t others[];
     __shared__ float sums[2][32];
-    const uint32_t group = threadIdx.x / a.threads, t = threadIdx.x - group * a.threads, warps = a.threads / 32;
+    const uint32_t group = threadIdx.x / a.threads, t = threadIdx.x - group * a.threads, warps = a.threads / 32, c = t * 8;
     const uint64_t stride = (uint64_t)gridDim.x * a.groups, first = (uint64_t)blockIdx.x * a.groups + group;
+    const bool inside = c < a.hidden;
     griddep_wait();
     griddep_launch_dependents();
-    Piece<T> h[kPieces], more[kPieces];
-    Piece<G> g[kPieces];
+    Piece<T> h, more;
+    Piece<G> g;
     float rstd = 0.0f;
     const auto load = [&](uint64_t token) {
-        #pragma unroll
-        for (uint32_t i = 0; i < kPieces; ++i) {
-            const uint32_t c = (i * a.threads + t) * 8;
-            if (c >= a.hidden) continue;
-            h[i].load(a.h + token * a.h_stride + (uint64_t)c * sizeof(T));
-            g[i].load(a.g + token * a.g_stride + (uint64_t)c * sizeof(G));
-            if (a.grad_h) more[i].load(a.grad_h + token * a.grad_h_stride + (uint64_t)c * sizeof(T));
+        if (inside) {
+            h.load(a.h + token * a.h_stride + (uint64_t)c * sizeof(T));
+            g.load(a.g + token * a.g_stride + (uint64_t)c * sizeof(G));
+            if (a.grad_h) more.load(a.grad_h + token * a.grad_h_stride + (uint64_t)c * sizeof(T));
         }
         rstd = __uint_as_float(ld_global_u32(a.rstd + token));
     };
-    Pair sum_w[kPieces][4];
+    h.clear(); g.clear(); more.clear();
+    if (first < a.tokens) load(first);
+    Pair w[4] = {}, sum_w[4];
+    if (inside) weight_at(a.weight, a.weight_fp32, c, w);
     #pragma unroll
-    for (uint32_t i = 0; i < kPieces; ++i) {
-        h[i].clear(); g[i].clear(); more[i].clear();
-        #pragma unroll
-        for (int j = 0; j < 4; ++j) sum_w[i][j] = Pair(0.0f);
-    }
-    if (kAhead && first < a.tokens) load(first);
-    Pair w[4] = {};                                           // (those of several pieces come from L1 each time)
-    const auto weights = [&](uint32_t i) {
-        const uint32_t c = (i * a.threads + t) * 8;
-        if (c < a.hidden) weight_at(a.weight, a.weight_fp32, c, w);
-    };
-    if constexpr (kPieces == 1) weights(0);
+    for (int j = 0; j < 4; ++j) sum_w[j] = Pair(0.0f);
     uint32_t turn = 0;
     for (uint64_t token = first; token < a.tokens; token += stride, turn ^= 1) {
-        if (!kAhead) load(token);
-        Piece<T> h0[kPieces], more0[kPieces];
-        Piece<G> g0[kPieces];
+        Piece<T> h0 = h, more0 = more;
+        const Piece<G> g0 = g;
         const float r = rstd;
         const Pair scale(r);
-        // sum(u n) = rstd sum(u h)
-        Pair dots(0.0f);
-        #pragma unroll
-        for (uint32_t i = 0; i < kPieces; ++i) {
-            h0[i] = h[i]; more0[i] = more[i]; g0[i] = g[i];
-            Pair n[4], u[4];
-            if constexpr (kPieces > 1) weights(i);
-            h0[i].get(n);
-            g0[i].get(u);
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                dots = fma2(u[j] * w[j], n[j], dots);
-                sum_w[i][j] = fma2(u[j], n[j] * scale, sum_w[i][j]);
-            }
-        }
-        if (kAhead && token + stride < a.tokens) load(token + stride);
+        Pair n[4], u[4], dots(0.0f);
+        h0.get(n);
+        g0.get(u);
+        add_dots(n, u, w, scale, dots, sum_w);
+        if (token + stride < a.tokens) load(token + stride);
         float dot, other;
         dots.get(dot, other);
         // (two sets of sums: a warp that is a turn ahead does not write to what another still reads)
         dot = group_sum(dot + other, sums[turn], group * warps, warps, group + 1);
-        // dx = rstd u - h (rstd^3 mean(u h)) + grad_h
-        const Pair slope(-(r * r * (r * (dot * a.inverse_hidden))));
-        // (what several pieces would hold over the barrier is read again: it lies in L2)
-        if constexpr (!kAhead) load(token);
+        if (!inside) continue;
+        Pair d[4];
+        h0.get(n);
+        g0.get(u);
+        more0.get(d);
+        slope_of(n, u, w, scale, Pair(-(r * r * (r * (dot * a.inverse_hidden)))), d);
+        h0.set(d);
+        h0.store(a.dx + token * a.dx_stride + (uint64_t)c * sizeof(T));
+    }
+    float dw[8];
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) sum_w[j].get(dw[2 * j], dw[2 * j + 1]);
+    if (a.groups > 1) {
+        float4* const to = reinterpret_cast<float4*>(others);
+        #pragma unroll
+        for (uint32_t k = 0; k < 2; ++k)
+            if (group > 0) to[((group - 1) * 2 + k) * a.threads + t] = make_float4(dw[4 * k], dw[4 * k + 1], dw[4 * k + 2], dw[4 * k + 3]);
+        __syncthreads();
+        if (group > 0) return;
+        for (uint32_t o = 0; o + 1 < a.groups; ++o)
+            #pragma unroll
+            for (uint32_t k = 0; k < 2; ++k) {
+                const float4 v = to[(o * 2 + k) * a.threads + t];
+                dw[4 * k] += v.x; dw[4 * k + 1] += v.y; dw[4 * k + 2] += v.z; dw[4 * k + 3] += v.w;
+            }
+    }
+    if (inside) store_part(a, c, dw);
+}
+
+// Long rows: tokens come to shared memory by bulk copies that the first thread of a group asks for, as many as fit there (16384 channels of FP32 are 192 KB); a
+// thread takes one piece of its group's token or two. Behind the barrier of a sum all threads of a group have read the token in front of it, whose place the
+// next one takes.
+//
+// From 4096 channels of BF16 and above 2048 of FP32 (8192 tokens; in registers / in shared memory, us): BF16 2048 22.9 / 27.2, 3584 38.6 / 41.3, 4096 58.4 / 46.0,
+// 7168 79.1 / 75.3; FP32 2048 42.0 / 40.9 (1531 tokens 11.6 / 12.3), 2560 76.9 / 49.9, 4096 82.6 / 77.4. Longer ones do not fit in registers: BF16 16384 195, FP32
+// 8192 162, 16384 332 us. (Copies that every thread asks for itself, cp.async, took 120 us for 8192 channels of BF16, where this takes 86: they are issued
+// by the same warps and wait for room.)
+constexpr uint32_t kLongRows = 4096, kLongRowsFp32 = 2080, kLongThreads = 1024, kLongSmem = 226 * 1024, kLongMostStages = 4, kMostGroups = 8;
+
+__device__ __forceinline__ void take(Piece<__nv_bfloat16>& p, const uint8_t* from) { p.q = *reinterpret_cast<const uint4*>(from); }
+__device__ __forceinline__ void take(Piece<float>& p, const uint8_t* from) {
+    p.q = *reinterpret_cast<const uint4*>(from);
+    p.r = *reinterpret_cast<const uint4*>(from + 16);
+}
+
+template <typename T, typename G, uint32_t kPieces>
+__global__ void __launch_bounds__(kLongThreads) rms_norm_grad_long_kernel(const NormGradArgs a) {
+    extern __shared__ __align__(16) uint8_t places[];         // of each token: the rows of h, g and grad_h
+    __shared__ float sums[2][32];
+    __shared__ __align__(8) uint64_t full[kMostGroups * kLongMostStages];
+    // (rows of two pieces leave no room for a second group)
+    const uint32_t groups = kPieces == 1 ? a.groups : 1u, group = kPieces == 1 ? threadIdx.x / a.threads : 0u, t = threadIdx.x - group * a.threads, warps = a.threads / 32;
+    const uint64_t stride = (uint64_t)gridDim.x * groups, first = (uint64_t)blockIdx.x * groups + group;
+    const uint32_t rows_h = a.hidden * sizeof(T), rows_g = a.hidden * sizeof(G), place = rows_h + rows_g + (a.grad_h ? rows_h : 0u);
+    const uint8_t* const mine = places + group * a.stages * place;
+    const uint32_t mine_at = smem_u32(mine), full_at = smem_u32(full + group * a.stages);
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < groups * a.stages; ++s) mbar_init(smem_u32(full + s), 1);
+        fence_mbar_init();
+        fence_proxy_async_smem();
+    }
+    __syncthreads();
+    griddep_wait();
+    griddep_launch_dependents();
+    const auto ask = [&](uint64_t token, uint32_t stage) {
+        const uint32_t to = mine_at + stage * place, bar = full_at + stage * 8;
+        mbar_arrive_expect_tx(bar, place);
+        bulk_copy_to_smem(to, a.h + token * a.h_stride, rows_h, bar);
+        bulk_copy_to_smem(to + rows_h, a.g + token * a.g_stride, rows_g, bar);
+        if (a.grad_h) bulk_copy_to_smem(to + rows_h + rows_g, a.grad_h + token * a.grad_h_stride, rows_h, bar);
+    };
+    if (t == 0)
+        for (uint32_t s = 0; s < a.stages; ++s)
+            if (first + s * stride < a.tokens) ask(first + s * stride, s);
+    Pair w[kPieces][4], sum_w[kPieces][4];
+    #pragma unroll
+    for (uint32_t i = 0; i < kPieces; ++i) {
+        const uint32_t c = (i * a.threads + t) * 8;
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) w[i][j] = sum_w[i][j] = Pair(0.0f);
+        if (c < a.hidden) weight_at(a.weight, a.weight_fp32, c, w[i]);
+    }
+    float next = first < a.tokens ? __uint_as_float(ld_global_u32(a.rstd + first)) : 0.0f;
+    uint32_t turn = 0, stage = 0, before = a.stages - 1, parity = 0;
+    for (uint64_t token = first; token < a.tokens; token += stride, turn ^= 1) {
+        float r = next;
+        if (token + stride < a.tokens) next = __uint_as_float(ld_global_u32(a.rstd + token + stride));
+        // (a copy that never comes shows in the result)
+        if (!wait_for(full_at + stage * 8, parity)) r = __uint_as_float(0x7fc00000u);
+        const Pair scale(r);
+        const uint8_t* const from = mine + stage * place;
+        Pair dots(0.0f);
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
             const uint32_t c = (i * a.threads + t) * 8;
             if (c >= a.hidden) continue;
-            Pair n[4], u[4], d[4];
-            if constexpr (kPieces > 1) weights(i);
-            if constexpr (!kAhead) { h0[i] = h[i]; g0[i] = g[i]; more0[i] = more[i]; }
-            h0[i].get(n);
-            g0[i].get(u);
-            more0[i].get(d);
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) d[j] = fma2(n[j], slope, fma2(scale, u[j] * w[j], d[j]));
-            h0[i].set(d);
-            h0[i].store(a.dx + token * a.dx_stride + (uint64_t)c * sizeof(T));
+            Piece<T> h;
+            Piece<G> g;
+            Pair n[4], u[4];
+            take(h, from + c * sizeof(T));
+            take(g, from + rows_h + c * sizeof(G));
+            h.get(n);
+            g.get(u);
+            add_dots(n, u, w[i], scale, dots, sum_w[i]);
         }
+        float dot, other;
+        dots.get(dot, other);
+        dot = group_sum(dot + other, sums[turn], group * warps, warps, group + 1);
+        // (all threads are done with the token in front)
+        const uint64_t later = token + (a.stages - 1) * stride;
+        if (t == 0 && a.stages > 1 && token != first && later < a.tokens) ask(later, before);
+        const Pair slope(-(r * r * (r * (dot * a.inverse_hidden))));
+        #pragma unroll
+        for (uint32_t i = 0; i < kPieces; ++i) {
+            const uint32_t c = (i * a.threads + t) * 8;
+            if (c >= a.hidden) continue;
+            Piece<T> h, more;
+            Piece<G> g;
+            Pair n[4], u[4], d[4];
+            take(h, from + c * sizeof(T));
+            take(g, from + rows_h + c * sizeof(G));
+            if (a.grad_h) take(more, from + rows_h + rows_g + c * sizeof(T));
+            else more.clear();
+            h.get(n);
+            g.get(u);
+            more.get(d);
+            slope_of(n, u, w[i], scale, slope, d);
+            h.set(d);
+            h.store(a.dx + token * a.dx_stride + (uint64_t)c * sizeof(T));
+        }
+        if (a.stages == 1) {
+            named_bar_sync(group + 1, a.threads);
+            if (t == 0 && token + stride < a.tokens) ask(token + stride, 0);
+        }
+        before = stage;
+        if (++stage == a.stages) { stage = 0; parity ^= 1; }
     }
     float dw[kPieces][8];
     #pragma unroll
     for (uint32_t i = 0; i < kPieces; ++i)
         #pragma unroll
         for (int j = 0; j < 4; ++j) sum_w[i][j].get(dw[i][2 * j], dw[i][2 * j + 1]);
-    if (a.groups > 1) {
-        float4* const to = reinterpret_cast<float4*>(others);
+    if (groups > 1) {
+        __syncthreads();                                      // (nobody reads a token any more)
+        float4* const to = reinterpret_cast<float4*>(places);
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i)
             #pragma unroll
@@ -313,7 +440,7 @@ __global__ void __launch_bounds__(kThreads) rms_norm_grad_kernel(const NormGradA
                 if (group > 0) to[((group - 1) * 2 * kPieces + 2 * i + k) * a.threads + t] = make_float4(dw[i][4 * k], dw[i][4 * k + 1], dw[i][4 * k + 2], dw[i][4 * k + 3]);
         __syncthreads();
         if (group > 0) return;
-        for (uint32_t o = 0; o + 1 < a.groups; ++o)
+        for (uint32_t o = 0; o + 1 < groups; ++o)
             #pragma unroll
             for (uint32_t i = 0; i < kPieces; ++i)
                 #pragma unroll
@@ -325,10 +452,7 @@ __global__ void __launch_bounds__(kThreads) rms_norm_grad_kernel(const NormGradA
     #pragma unroll
     for (uint32_t i = 0; i < kPieces; ++i) {
         const uint32_t c = (i * a.threads + t) * 8;
-        if (c >= a.hidden) continue;
-        float4* const out = reinterpret_cast<float4*>(a.partial + (uint64_t)blockIdx.x * a.hidden + c);
-        out[0] = make_float4(dw[i][0], dw[i][1], dw[i][2], dw[i][3]);
-        out[1] = make_float4(dw[i][4], dw[i][5], dw[i][6], dw[i][7]);
+        if (c < a.hidden) store_part(a, c, dw[i]);
     }
 }
 
@@ -353,16 +477,23 @@ __global__ void __launch_bounds__(kSumThreads) rms_norm_grad_sum_kernel(const fl
 // Threads of a CTA whose threads take `pieces` pieces of a row each.
 static uint32_t norm_threads(uint32_t hidden, uint32_t pieces) { return ((hidden / 8 + pieces - 1) / pieces + 31) / 32 * 32; }
 
-// How the gradient's kernel is laid over the SMs, one CTA each: one piece of a row a thread where that takes at most 896 threads (512 of FP32), in as many groups
-// as fit, else four; as many CTAs as finish together.
-struct NormGradShape { uint32_t pieces, threads, groups, parts; };
-static NormGradShape norm_grad_shape(uint32_t tokens, uint32_t hidden, bool fp32) {
-    const uint32_t most = fp32 ? 512 : 896;
+// How the gradient is laid over the SMs, one CTA each: in as many groups as there are threads for (registers: 896, or 512 of FP32, whose pieces are twice as
+// large), as many CTAs as finish together. (With registers for 1024 threads some go to memory: 117 us where 896 took 84.)
+struct NormGradShape { uint32_t threads, groups, pieces, stages, parts, smem; };   // stages: 0 in registers
+static NormGradShape norm_grad_shape(uint32_t tokens, uint32_t hidden, bool fp32, uint32_t channel_bytes) {
     NormGradShape s{};
-    s.pieces = norm_threads(hidden, 1) <= most ? 1 : 4;
+    const bool whole = hidden < (fp32 ? kLongRowsFp32 : kLongRows);
+    const uint32_t most = !whole ? kLongThreads : fp32 ? 512 : 896, token = hidden * channel_bytes;
+    s.pieces = norm_threads(hidden, 1) <= kLongThreads ? 1 : 2;
     s.threads = norm_threads(hidden, s.pieces);
-    s.groups = s.pieces == 4 ? 1 : most / s.threads < 8 ? most / s.threads : 8;
+    s.groups = most / s.threads < kMostGroups ? most / s.threads : kMostGroups;
     while (s.groups > 1 && (s.groups - 1) * 148 >= tokens) --s.groups;
+    const uint32_t others = (s.groups - 1) * s.threads * s.pieces * 32;
+    if (!whole) {
+        const uint32_t fit = kLongSmem / (token * s.groups);
+        s.stages = fit < kLongMostStages ? fit : kLongMostStages;
+    }
+    s.smem = s.stages * s.groups * token > others ? s.stages * s.groups * token : others;
     const uint32_t wanted = (tokens + s.groups - 1) / s.groups, turns = (wanted + 147) / 148;
     s.parts = turns ? (wanted + turns - 1) / turns : 0;
     return s;
@@ -401,7 +532,9 @@ extern "C" int dg_rms_norm_fp8_launch(const void* x, int is_fp32, uint64_t x_str
     a.sf = reinterpret_cast<uint8_t*>(out_sf); a.sf_col_stride = sf_col_stride * 2;
     a.rstd = rstd; a.tokens = tokens; a.hidden = hidden; a.eps = eps;
     a.inverse_hidden = 1.0 / hidden;
-    // Few tokens: as many threads as a row has pieces. Many of BF16: half as many, and two CTAs on an SM. (FP32 has twice the bytes in each.)
+    // Few tokens: as many threads as a row has pieces (1 / 128 x 7168: 2.4 / 3.0 us, by half as many 2.7 / 3.2). Many of BF16: half as many, and two CTAs on an SM (8192 x
+    // 7168 89 us against 100, x 4096 57 against 73). FP32 has twice the bytes in each (x 7168 158 against 205 with four pieces a thread). Beyond that, four: there
+    // the registers do not hold a next token of FP32.
     const void* fn;
     uint32_t pieces = 1, resident = 1;
     if (norm_threads(hidden, 1) <= (is_fp32 || tokens <= 148 ? 1024 : 448)) {
@@ -422,13 +555,13 @@ extern "C" int dg_rms_norm_fp8_launch(const void* x, int is_fp32, uint64_t x_str
 
 extern "C" uint64_t dg_rms_norm_grad_scratch_bytes(uint32_t tokens, uint32_t hidden) {
     if (hidden == 0) return 0;
-    const uint32_t bf16 = norm_grad_shape(tokens, hidden, false).parts, fp32 = norm_grad_shape(tokens, hidden, true).parts;
-    return (uint64_t)(bf16 > fp32 ? bf16 : fp32) * hidden * 4;
+    return (uint64_t)(tokens < 148 ? tokens : 148) * hidden * 4;
 }
 
 template <typename T, typename G>
-static const void* norm_grad_kernel(uint32_t pieces) {
-    return pieces == 1 ? (const void*)rms_norm_grad_kernel<T, G, 1, sizeof(T) == 4 ? 512 : 896, true> : (const void*)rms_norm_grad_kernel<T, G, 4, 512, false>;
+static const void* norm_grad_kernel(const NormGradShape& s) {
+    return s.stages == 0 ? (const void*)rms_norm_grad_kernel<T, G, sizeof(T) == 4 ? 512 : 896>
+         : s.pieces == 1 ? (const void*)rms_norm_grad_long_kernel<T, G, 1> : (const void*)rms_norm_grad_long_kernel<T, G, 2>;
 }
 
 extern "C" int dg_rms_norm_grad_launch(const void* grad_out, int grad_is_fp32, uint64_t grad_stride, const void* h, int is_fp32, uint64_t h_stride, const void* weight,
@@ -456,14 +589,14 @@ extern "C" int dg_rms_norm_grad_launch(const void* grad_out, int grad_is_fp32, u
     a.partial = static_cast<float*>(scratch);
     a.tokens = tokens; a.hidden = hidden;
     a.inverse_hidden = 1.0f / (float)hidden;
-    const NormGradShape shape = norm_grad_shape(tokens, hidden, is_fp32);
-    a.groups = shape.groups; a.threads = shape.threads;
+    const NormGradShape shape = norm_grad_shape(tokens, hidden, is_fp32, (uint32_t)((grad_h ? 2 * es : es) + (grad_is_fp32 ? 4 : 2)));
+    a.groups = shape.groups; a.threads = shape.threads; a.stages = shape.stages;
     uint32_t parts = shape.parts;
-    const void* fn = !is_fp32 ? norm_grad_kernel<__nv_bfloat16, __nv_bfloat16>(shape.pieces) : grad_is_fp32 ? norm_grad_kernel<float, float>(shape.pieces)
-                                                                                             : norm_grad_kernel<float, __nv_bfloat16>(shape.pieces);
+    const void* fn = !is_fp32 ? norm_grad_kernel<__nv_bfloat16, __nv_bfloat16>(shape) : grad_is_fp32 ? norm_grad_kernel<float, float>(shape)
+                                                                                            : norm_grad_kernel<float, __nv_bfloat16>(shape);
+    if (shape.stages > 0) DG_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLongSmem));
     void* params[] = {&a};
-    if (int rc = launch_overlapped(fn, dim3(parts), dim3(shape.groups * shape.threads), params, static_cast<cudaStream_t>(stream),
-                                   (shape.groups - 1) * shape.threads * shape.pieces * 32)) return rc;
+    if (int rc = launch_overlapped(fn, dim3(parts), dim3(shape.groups * shape.threads), params, static_cast<cudaStream_t>(stream), shape.smem)) return rc;
     const float* from = a.partial;
     void* sum_params[] = {&from, &grad_weight, &parts, &hidden};
     return launch_overlapped((const void*)rms_norm_grad_sum_kernel, dim3(hidden / kSumChannels), dim3(kSumThreads), sum_params, static_cast<cudaStream_t>(stream));

@@ -136,6 +136,23 @@ def test_gradient(host, tokens, hidden, dtype, grad_dtype):
     _check_grad(g, h, weight, rstd, more, host)
 
 
+@pytest.mark.parametrize('dtype,hidden,tokens', [(BF16, 4064, 900), (BF16, 4096, 1500), (BF16, 5120, 1000), (BF16, 8192, 750), (BF16, 16384, 450), (FP32, 2048, 900),
+                                                 (FP32, 2080, 2000), (FP32, 4128, 750), (FP32, 8224, 450), (FP32, 16384, 300)])
+def test_gradient_of_long_rows_in_many_turns(dtype, hidden, tokens):
+    seed_all(tokens)
+    wide = torch.randn(tokens, 2 * hidden + 64).to(dtype)
+    h, g, more = wide[:, 16:16 + hidden], torch.randn(tokens, hidden).to(dtype), wide[:, hidden + 32:2 * hidden + 32]
+    weight = torch.randn(hidden)
+    rstd = oracle.rms_norm_ref(h, weight, 1e-6)[0].float()
+    for grad_h in (None, more):
+        _check_grad(g, h, weight, rstd, grad_h)
+    both = wide.cuda()
+    h, more = both[:, 16:16 + hidden], both[:, hidden + 32:2 * hidden + 32]
+    want = deep_gemm.rms_norm_grad(g.cuda(), h, weight.cuda(), rstd.cuda(), grad_h=more)
+    got = deep_gemm.rms_norm_grad(g.cuda(), h, weight.cuda(), rstd.cuda(), grad_h=more, out=h)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]) and torch.equal(both[:, :16].cpu(), wide[:, :16])
+
+
 def test_gradient_in_place_and_strides():
     seed_all(5)
     for dtype in (BF16, FP32):
