@@ -5,7 +5,8 @@
 // in FP32 in either form (four significant bits times a power of two), so the rounding to E4M3 is the only one. A block that holds an
 // infinity or a NaN gets the scale byte of NaN.
 //
-// HBM-bound: 2 (or 1 + 1/32) bytes read and 1 + 1/32 written per value.
+// HBM-bound: 2 (or 1 + 1/32) bytes read and 1 + 1/32 written per value. 32768 x 7168 from 8 bits 100 us, 5.0 TB/s (the bytes alone 78 at the rate of a copy: the
+// instructions of the conversions fill 63 % of the issue slots); 16384 x 7168 from BF16 50 us, 6.1 TB/s, and back to BF16 55 us, 5.4 TB/s.
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <string.h>
@@ -111,6 +112,8 @@ __device__ __forceinline__ uint32_t f16x2_to_e4m3(uint32_t v) {
 // time: amax <= 448 s = 1.75 x 2^8 s, so with amax = 1.m x 2^x (m of ten bits) s is 2^(x - 8), or twice that where m is above 0.75, which is an addition
 // to the bits that carries; `least` is the byte of the least amax.
 //
+// (Through FP32, which takes every input, 32768 x 7168 takes 173 us, through FP16 102, or 114 where each lane makes its own factors.)
+//
 // Whatever a row or a column has once is made once and handed round: `pair` holds the bytes of row `lane` (of the tile's two blocks), `block` says which of them
 // this lane's columns lie in, and of the four words of columns that the lanes of a row share each of the four lanes of a column makes one.
 __device__ __forceinline__ bool quantise_down_fp8(const uint2 (&q)[8], uint32_t pair, uint32_t block, uint32_t least, uint32_t lane, uint2& bytes, uint2 (&codes)[8]) {
@@ -160,7 +163,7 @@ __device__ __forceinline__ void load_raw(uint4& q, const uint8_t* p) { q = ld_st
 
 // One CTA = 64 rows x 128 columns, a warp 32 rows x 64 columns: lane = (every fourth row, eight columns), so that the maximum down a column takes
 // two shuffles, and a row of the warp's tile is a line of 128 bytes of BF16 or two whole sectors of codes. The 64 columns are one column of the
-// scales of an 8-bit input, whose 32 rows are one read of 64 bytes.
+// scales of an 8-bit input, whose 32 rows are one read of 64 bytes. (32768 x 7168 from 8 bits in CTAs of 256 threads 133 us, of 128 114, before the above.)
 template <bool kFromFp8>
 __global__ void __launch_bounds__(kMnThreads, 8) quant_fp8_mn_kernel(const MnArgs a) {
     __shared__ __align__(8) uint8_t sf_smem[2][kMnCols];
@@ -244,7 +247,7 @@ __global__ void __launch_bounds__(kMnThreads, 8) quant_fp8_mn_kernel(const MnArg
 
 // The way back: code x 2^(byte - 127), rounded once to BF16 or FP32 (which changes nothing but where those have subnormals). One CTA = 32 rows x 256
 // columns, a warp four rows, a lane eight columns. The scales of K-major rows come in runs down the rows, through shared memory; those of an MN-major
-// tile lie along the columns.
+// tile lie along the columns. HBM-bound: 2112 x 7168 there and back 13.9 us, where the bytes alone take 14.0 from HBM (the codes between the two stay in L2).
 template <typename T, bool kMnMajor>
 __global__ void __launch_bounds__(kBackThreads) dequant_fp8_kernel(const MnArgs a) {
     constexpr uint32_t kTileRows = kBackRows, kWarpRows = kTileRows / (kBackThreads / 32);

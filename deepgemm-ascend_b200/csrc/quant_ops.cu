@@ -119,7 +119,9 @@ __global__ void __launch_bounds__(kQuantThreads) quant_fp8_kernel(const QuantArg
 }
 
 // SwiGLU with a checkpoint. A warp takes four tokens x 256 channels and shares nothing with others, so that small CTAs come and go by themselves: the scales of a
-// block's four tokens are collected by shuffles and written in one store of eight bytes where the column starts on a boundary of that.
+// block's four tokens are collected by shuffles and written in one store of eight bytes where the column starts on a boundary of that. HBM-bound, 4 H bytes read and
+// 3 H (1 + 1/32) written: 65536 x 2048 152 us, 6.3 TB/s (the bytes alone 145 at the rate of a copy; 173 in a long row of passes, which draws the power cap). Inside the
+// kernel above, whose CTAs share 32 tokens' scales, it took 190.
 constexpr uint32_t kKeepThreads = 128, kKeepTokens = kWarpTokens * kKeepThreads / 32;
 __device__ __forceinline__ uint32_t cast_piece(const Pair (&v)[4], float floor, uint2& codes) {
     float amax = 0.f;

@@ -148,8 +148,8 @@ def swiglu_apply_weight_grad(grad_out: torch.Tensor, x, topk_weights: Optional[t
                              out: Optional[torch.Tensor] = None, zero_padding: bool = False):
     """Gradients of `swiglu_apply_weight_to_fp8` for grad_out BF16 [tokens, hidden]: (grad_x BF16 [tokens, 2 * hidden], grad_weights float32 like
     topk_weights, or None). x is the BF16 input or the 8-bit pair that `..._with_checkpoint` (or `cast_to_fp8`) made of it. Where the clamp cuts off
-    the gradient is 0. Rows without a value (the padding of a psum layout, rows behind its last group) are not read and have the weights' gradient
-    0; grad_x is not written there, but for the zeros that `zero_padding` puts into the padding. `out`: where grad_x goes. Rows of BF16 start on
+    the gradient is 0. What rows without a value (the padding of a psum layout, rows behind its last group) hold does not matter; their weights
+    have the gradient 0, and grad_x is not written there, but for the zeros that `zero_padding` puts into the padding. `out`: where grad_x goes. Rows of BF16 start on
     16-byte boundaries, those of E4M3 on 8."""
     psum, is_pair = psum_num_tokens_per_expert, isinstance(x, (tuple, list))
     x, sf = x if is_pair else (x, None)
