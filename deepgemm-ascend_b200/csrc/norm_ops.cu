@@ -100,6 +100,7 @@ struct NormArgs {
     uint8_t* sf; uint64_t sf_col_stride;                                 // bytes between scale columns
     float* rstd;
     uint32_t tokens, hidden;
+    uint32_t groups, threads, stages;                                    // long rows: of a CTA; of a group; tokens in shared memory
     float eps;
     double inverse_hidden;
 };
@@ -123,13 +124,62 @@ __device__ __forceinline__ float rsqrt_of(double m) {
     return (float)(1.0 / sqrt(m));
 }
 
-// A CTA walks tokens at a distance of the grid, a thread kPieces x 8 channels of each. With kAhead the next token is asked for before the sum over
-// the CTA: what keeps HBM busy over the barrier (8192 x 7168 of BF16 with a residual and BF16 rows: 89 us, 5.9 TB/s, where the bytes alone take 81 at the rate of
-// a copy; a CTA for every token took 106, L2 asked for the token behind the next 109). 1 x 7168: 2.4 us, launch and latency.
-template <typename T, uint32_t kPieces, uint32_t kThreads, uint32_t kCtas, bool kAhead>
+// h of a piece, and the sum of its squares.
+template <typename T>
+__device__ __forceinline__ void add_piece(const NormArgs& a, uint64_t token, uint32_t c, const Piece<T>& x, const Piece<T>& more, Piece<T>& h, double& sum) {
+    Pair v[4];
+    h = x;
+    if (a.residual) {
+        Pair u[4];
+        x.get(v);
+        more.get(u);
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = v[j] + u[j];
+        h.set(v);
+        if (c < a.hidden) h.store(a.h + token * a.h_stride + (uint64_t)c * sizeof(T));
+    }
+    h.get(v);
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float lo, hi;
+        v[j].get(lo, hi);
+        sum = fma((double)lo, (double)lo, sum);
+        sum = fma((double)hi, (double)hi, sum);
+    }
+}
+// The norm of a piece and its codes. (All lanes of a warp come here.)
+template <typename T>
+__device__ __forceinline__ void finish_piece(const NormArgs& a, uint64_t token, uint32_t c, const Piece<T>& h, Pair scale) {
+    Pair w[4] = {}, v[4];
+    if (c < a.hidden) weight_at(a.weight, a.weight_fp32, c, w);
+    h.get(v);
+    float amax = 0.0f;
+    #pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        v[j] = v[j] * scale * w[j];
+        amax = larger_magnitude(amax, v[j]);
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 2));
+    const uint32_t e = e4m3_scale_byte(amax);
+    // (the second block of a last, half-used scale column is zero)
+    const uint32_t next = __shfl_down_sync(kAll, c < a.hidden ? e : 0u, 4);
+    if (c >= a.hidden) return;
+    *reinterpret_cast<uint2*>(a.out + token * a.out_stride + c) = e4m3_pack8(v, e);
+    if (a.rows) {
+        Piece<__nv_bfloat16> y;
+        y.set(v);
+        y.store(a.rows + token * a.rows_stride + (uint64_t)c * 2);
+    }
+    if (c % 64 == 0) *reinterpret_cast<uint16_t*>(a.sf + (uint64_t)(c / 64) * a.sf_col_stride + token * 2) = (uint16_t)(e | next << 8);
+}
+
+// Few tokens, short rows and some of the middle: a CTA walks tokens at a distance of the grid, a thread kPieces x 8 channels of each. The next token is asked for before
+// the sum over the CTA: what keeps HBM busy over the barrier. 8192 x 7168 of BF16 with a residual and BF16 rows 89 us, 5.9 TB/s, where the bytes alone take 81 at the rate
+// of a copy (a CTA for every token took 106, L2 asked for the token behind the next 109). 1 x 7168: 2.4 us, launch and latency.
+template <typename T, uint32_t kPieces, uint32_t kThreads, uint32_t kCtas>
 __global__ void __launch_bounds__(kThreads, kCtas) rms_norm_fp8_kernel(const NormArgs a) {
     __shared__ double partial[2][32];
-    const uint32_t lane = threadIdx.x % 32;
     griddep_wait();
     griddep_launch_dependents();
     Piece<T> x[kPieces], more[kPieces];
@@ -144,67 +194,84 @@ __global__ void __launch_bounds__(kThreads, kCtas) rms_norm_fp8_kernel(const Nor
     };
     #pragma unroll
     for (uint32_t i = 0; i < kPieces; ++i) { x[i].clear(); more[i].clear(); }
-    if (kAhead) load(blockIdx.x);
+    load(blockIdx.x);
     uint32_t turn = 0;
     for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x, turn ^= 1) {
-        if (!kAhead) load(token);
         Piece<T> h[kPieces];
         double sum = 0.0;
         #pragma unroll
-        for (uint32_t i = 0; i < kPieces; ++i) {
-            const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
-            Pair v[4];
-            h[i] = x[i];
-            if (a.residual) {
-                Pair u[4];
-                x[i].get(v);
-                more[i].get(u);
-                #pragma unroll
-                for (int j = 0; j < 4; ++j) v[j] = v[j] + u[j];
-                h[i].set(v);
-                if (c < a.hidden) h[i].store(a.h + token * a.h_stride + (uint64_t)c * sizeof(T));
-            }
-            h[i].get(v);
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float lo, hi;
-                v[j].get(lo, hi);
-                sum = fma((double)lo, (double)lo, sum);
-                sum = fma((double)hi, (double)hi, sum);
-            }
-        }
-        if (kAhead && token + gridDim.x < a.tokens) load(token + gridDim.x);
+        for (uint32_t i = 0; i < kPieces; ++i) add_piece(a, token, (i * blockDim.x + threadIdx.x) * 8, x[i], more[i], h[i], sum);
+        if (token + gridDim.x < a.tokens) load(token + gridDim.x);
         // (two sets of shared memory: a warp that is a turn ahead does not write to what another still reads)
         sum = group_sum(sum, partial[turn], 0, blockDim.x / 32, 1);
         const float rstd = rsqrt_of(fma(sum, a.inverse_hidden, (double)a.eps));
         if (threadIdx.x == 0) a.rstd[token] = rstd;
-        const Pair scale(rstd);
+        #pragma unroll
+        for (uint32_t i = 0; i < kPieces; ++i) finish_piece(a, token, (i * blockDim.x + threadIdx.x) * 8, h[i], Pair(rstd));
+    }
+}
+
+// Many tokens, and rows too long for the above: the rows of a token come to shared memory by bulk copies, as many tokens ahead as fit there; a group of a CTA's warps
+// takes a token, a thread one piece of it or two. Behind the barrier of the sum nobody reads the rows any more, and the next token takes their place.
+constexpr uint32_t kLongThreads = 1024, kLongSmem = 226 * 1024, kLongMostStages = 4, kMostGroups = 8;
+
+__device__ __forceinline__ void take(Piece<__nv_bfloat16>& p, const uint8_t* from) { p.q = *reinterpret_cast<const uint4*>(from); }
+__device__ __forceinline__ void take(Piece<float>& p, const uint8_t* from) {
+    p.q = *reinterpret_cast<const uint4*>(from);
+    p.r = *reinterpret_cast<const uint4*>(from + 16);
+}
+
+template <typename T, uint32_t kPieces>
+__global__ void __launch_bounds__(kLongThreads) rms_norm_fp8_long_kernel(const NormArgs a) {
+    extern __shared__ __align__(16) uint8_t places[];         // of each token: the rows of x and of the residual
+    __shared__ double partial[2][32];
+    __shared__ __align__(8) uint64_t full[kMostGroups * kLongMostStages];
+    const uint32_t groups = a.groups, group = threadIdx.x / a.threads, t = threadIdx.x - group * a.threads, warps = a.threads / 32;
+    const uint64_t stride = (uint64_t)gridDim.x * groups, first = (uint64_t)blockIdx.x * groups + group;
+    const uint32_t row = a.hidden * sizeof(T), place = a.residual ? 2 * row : row;
+    const uint8_t* const mine = places + group * a.stages * place;
+    const uint32_t mine_at = smem_u32(mine), full_at = smem_u32(full + group * a.stages);
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < groups * a.stages; ++s) mbar_init(smem_u32(full + s), 1);
+        fence_mbar_init();
+        fence_proxy_async_smem();
+    }
+    __syncthreads();
+    griddep_wait();
+    griddep_launch_dependents();
+    const auto ask = [&](uint64_t token, uint32_t stage) {
+        const uint32_t to = mine_at + stage * place, bar = full_at + stage * 8;
+        mbar_arrive_expect_tx(bar, place);
+        bulk_copy_to_smem(to, a.x + token * a.x_stride, row, bar);
+        if (a.residual) bulk_copy_to_smem(to + row, a.residual + token * a.residual_stride, row, bar);
+    };
+    if (t == 0)
+        for (uint32_t s = 0; s < a.stages; ++s)
+            if (first + s * stride < a.tokens) ask(first + s * stride, s);
+    uint32_t turn = 0, stage = 0, parity = 0;
+    for (uint64_t token = first; token < a.tokens; token += stride, turn ^= 1) {
+        // (a copy that never comes shows in the result)
+        double sum = wait_for(full_at + stage * 8, parity) ? 0.0 : (double)__uint_as_float(0x7fc00000u);
+        const uint8_t* const from = mine + stage * place;
+        Piece<T> h[kPieces];
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
-            const uint32_t c = (i * blockDim.x + threadIdx.x) * 8;
-            Pair w[4] = {}, v[4];
-            if (c < a.hidden) weight_at(a.weight, a.weight_fp32, c, w);
-            h[i].get(v);
-            float amax = 0.0f;
-            #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v[j] = v[j] * scale * w[j];
-                amax = larger_magnitude(amax, v[j]);
+            const uint32_t c = (i * a.threads + t) * 8;
+            Piece<T> x, more;
+            x.clear(); more.clear();
+            if (c < a.hidden) {
+                take(x, from + c * sizeof(T));
+                if (a.residual) take(more, from + row + c * sizeof(T));
             }
-            amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(kAll, amax, 2));
-            const uint32_t e = e4m3_scale_byte(amax);
-            // (the second block of a last, half-used scale column is zero)
-            const uint32_t next = __shfl_down_sync(kAll, c < a.hidden ? e : 0u, 4);
-            if (c >= a.hidden) continue;
-            *reinterpret_cast<uint2*>(a.out + token * a.out_stride + c) = e4m3_pack8(v, e);
-            if (a.rows) {
-                Piece<__nv_bfloat16> y;
-                y.set(v);
-                y.store(a.rows + token * a.rows_stride + (uint64_t)c * 2);
-            }
-            if (lane % 8 == 0) *reinterpret_cast<uint16_t*>(a.sf + (uint64_t)(c / 64) * a.sf_col_stride + token * 2) = (uint16_t)(e | next << 8);
+            add_piece(a, token, c, x, more, h[i], sum);
         }
+        sum = group_sum(sum, partial[turn], group * warps, warps, group + 1);
+        if (t == 0 && token + a.stages * stride < a.tokens) ask(token + a.stages * stride, stage);
+        const float rstd = rsqrt_of(fma(sum, a.inverse_hidden, (double)a.eps));
+        if (t == 0) a.rstd[token] = rstd;
+        #pragma unroll
+        for (uint32_t i = 0; i < kPieces; ++i) finish_piece(a, token, (i * a.threads + t) * 8, h[i], Pair(rstd));
+        if (++stage == a.stages) { stage = 0; parity ^= 1; }
     }
 }
 
@@ -212,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) rms_norm_fp8_kernel(const Nor
 // a token, and walks tokens at a distance of all groups; a thread holds its channels' part of dweight in registers (FP32), the groups of a CTA add theirs up,
 // and a second kernel sums the CTAs' in their order: nothing depends on timing.
 //
-// HBM-bound: 8192 x 7168 of BF16 with a gradient of h 75 us, 6.2 TB/s (bytes alone at the rate of a copy 72); 1531 x 2048 of FP32 11.6 us, of which the second
+// HBM-bound: 8192 x 7168 of BF16 with a gradient of h 79 us, 5.9 TB/s (the bytes alone 72 at the rate of a copy); 1531 x 2048 of FP32 11.6 us, of which the second
 // kernel and the launches take 3.
 struct NormGradArgs {
     const uint8_t* g; uint64_t g_stride;                                 // BF16 or FP32 as `h` is, or BF16 beside FP32
@@ -321,17 +388,11 @@ __global__ void __launch_bounds__(kThreads) rms_norm_grad_kernel(const NormGradA
 // thread takes one piece of its group's token or two. Behind the barrier of a sum all threads of a group have read the token in front of it, whose place the
 // next one takes.
 //
-// From 4096 channels of BF16 and above 2048 of FP32 (8192 tokens; in registers / in shared memory, us): BF16 2048 22.9 / 27.2, 3584 38.6 / 41.3, 4096 58.4 / 46.0,
-// 7168 79.1 / 75.3; FP32 2048 42.0 / 40.9 (1531 tokens 11.6 / 12.3), 2560 76.9 / 49.9, 4096 82.6 / 77.4. Longer ones do not fit in registers: BF16 16384 195, FP32
-// 8192 162, 16384 332 us. (Copies that every thread asks for itself, cp.async, took 120 us for 8192 channels of BF16, where this takes 86: they are issued
-// by the same warps and wait for room.)
-constexpr uint32_t kLongRows = 4096, kLongRowsFp32 = 2080, kLongThreads = 1024, kLongSmem = 226 * 1024, kLongMostStages = 4, kMostGroups = 8;
-
-__device__ __forceinline__ void take(Piece<__nv_bfloat16>& p, const uint8_t* from) { p.q = *reinterpret_cast<const uint4*>(from); }
-__device__ __forceinline__ void take(Piece<float>& p, const uint8_t* from) {
-    p.q = *reinterpret_cast<const uint4*>(from);
-    p.r = *reinterpret_cast<const uint4*>(from + 16);
-}
+// From 4096 channels of BF16, but for what is just under the most that fits in registers, and above 2048 of FP32 (8192 tokens; in registers / in shared memory, us in a
+// row of passes): BF16 2048 22.9 / 27.2, 3584 38.6 / 41.3, 4096 59.5 / 50.8, 5120 66.5 / 65.5, 6144 75.2 / 75.7, 7168 83.1 / 85.3; FP32 2048 42.0 / 40.9 (1531 tokens 11.6 / 12.3),
+// 2560 77.5 / 52.1, 4096 87.4 / 82.5. Longer ones do not fit in registers: BF16 16384 195, FP32 8192 162, 16384 332 us. (Copies that every thread asks for itself, cp.async, took
+// 120 us for 8192 channels of BF16, where this takes 86: they are issued by the same warps and wait for room.)
+constexpr uint32_t kLongRows = 4096, kLongRowsFp32 = 2080;
 
 template <typename T, typename G, uint32_t kPieces>
 __global__ void __launch_bounds__(kLongThreads) rms_norm_grad_long_kernel(const NormGradArgs a) {
@@ -482,7 +543,7 @@ static uint32_t norm_threads(uint32_t hidden, uint32_t pieces) { return ((hidden
 struct NormGradShape { uint32_t threads, groups, pieces, stages, parts, smem; };   // stages: 0 in registers
 static NormGradShape norm_grad_shape(uint32_t tokens, uint32_t hidden, bool fp32, uint32_t channel_bytes) {
     NormGradShape s{};
-    const bool whole = hidden < (fp32 ? kLongRowsFp32 : kLongRows);
+    const bool whole = fp32 ? hidden < kLongRowsFp32 : hidden < kLongRows || (hidden > 6144 && hidden <= 7168);
     const uint32_t most = !whole ? kLongThreads : fp32 ? 512 : 896, token = hidden * channel_bytes;
     s.pieces = norm_threads(hidden, 1) <= kLongThreads ? 1 : 2;
     s.threads = norm_threads(hidden, s.pieces);
@@ -532,25 +593,30 @@ extern "C" int dg_rms_norm_fp8_launch(const void* x, int is_fp32, uint64_t x_str
     a.sf = reinterpret_cast<uint8_t*>(out_sf); a.sf_col_stride = sf_col_stride * 2;
     a.rstd = rstd; a.tokens = tokens; a.hidden = hidden; a.eps = eps;
     a.inverse_hidden = 1.0 / hidden;
-    // Few tokens: as many threads as a row has pieces (1 / 128 x 7168: 2.4 / 3.0 us, by half as many 2.7 / 3.2). Many of BF16: half as many, and two CTAs on an SM (8192 x
-    // 7168 89 us against 100, x 4096 57 against 73). FP32 has twice the bytes in each (x 7168 158 against 205 with four pieces a thread). Beyond that, four: there
-    // the registers do not hold a next token of FP32.
-    const void* fn;
-    uint32_t pieces = 1, resident = 1;
-    if (norm_threads(hidden, 1) <= (is_fp32 || tokens <= 148 ? 1024 : 448)) {
-        resident = 896 / norm_threads(hidden, pieces);
-        fn = is_fp32 ? (const void*)rms_norm_fp8_kernel<float, 1, 1024, 1, true> : (const void*)rms_norm_fp8_kernel<__nv_bfloat16, 1, 1024, 1, true>;
-    } else if (!is_fp32 && norm_threads(hidden, 2) <= 448) {
-        pieces = 2;
-        resident = 896 / norm_threads(hidden, pieces);
-        fn = (const void*)rms_norm_fp8_kernel<__nv_bfloat16, 2, 448, 2, true>;
-    } else {
-        pieces = 4;
-        fn = is_fp32 ? (const void*)rms_norm_fp8_kernel<float, 4, 512, 1, false> : (const void*)rms_norm_fp8_kernel<__nv_bfloat16, 4, 512, 1, true>;
-    }
-    resident = resident < 1 ? 1 : resident > 16 ? 16 : resident;
+    // In registers / by bulk copies, us of 8192 tokens: BF16 512 10.3 / 11.5, 1024 18.8 / 16.8, 2048 33.9 / 30.9, 4096 59.3 / 56.1, 7168 89.1 / 92.6; FP32 1024 23.6 / 24.0, 2048
+    // 52.6 / 46.7, 7168 171 / 158, 8192 187 / 159; few turns do not pay for the copies' start: 1024 x 7168 of BF16 12.6 / 15.6, 600 x 2048 4.7 / 5.3, but 2000 x 2048 9.7 / 7.7.
+    // In registers two pieces a thread and two CTAs on an SM for long rows of BF16 (7168 89 us against 100 with one piece) but for few tokens (1 / 128 x 7168 2.4 / 3.0 us
+    // with one piece, 2.7 / 3.2 with two).
+    const uint32_t one = norm_threads(hidden, 1);
+    const bool two = !is_fp32 && one > 448 && one <= 896 && tokens > 148;
     void* params[] = {&a};
-    return launch_overlapped(fn, dim3(tokens < 148 * resident ? tokens : 148 * resident), dim3(norm_threads(hidden, pieces)), params, static_cast<cudaStream_t>(stream));
+    if (one <= 1024 && (hidden < 1024 || tokens <= 1024 || (two && hidden > 4096))) {
+        const uint32_t threads = two ? norm_threads(hidden, 2) : one, resident = 896 / threads < 1 ? 1 : 896 / threads > 16 ? 16 : 896 / threads;
+        return launch_overlapped(two ? (const void*)rms_norm_fp8_kernel<__nv_bfloat16, 2, 448, 2> : is_fp32 ? (const void*)rms_norm_fp8_kernel<float, 1, 1024, 1>
+                                                                                              : (const void*)rms_norm_fp8_kernel<__nv_bfloat16, 1, 1024, 1>,
+                                 dim3(tokens < 148 * resident ? tokens : 148 * resident), dim3(threads), params, static_cast<cudaStream_t>(stream));
+    }
+    // (two pieces a thread of BF16: 7168 104 us with one, 4096 58)
+    const uint32_t pieces = is_fp32 && one <= kLongThreads ? 1 : 2, token = hidden * (uint32_t)(residual ? 2 * es : es);
+    a.threads = norm_threads(hidden, pieces);
+    a.groups = kLongThreads / a.threads < kMostGroups ? kLongThreads / a.threads : kMostGroups;
+    while (a.groups > 1 && (a.groups - 1) * 148 >= tokens) --a.groups;
+    const uint32_t fit = kLongSmem / (token * a.groups), ctas = (tokens + a.groups - 1) / a.groups;
+    a.stages = fit < kLongMostStages ? fit : kLongMostStages;
+    const void* fn = !is_fp32 ? (const void*)rms_norm_fp8_long_kernel<__nv_bfloat16, 2> : pieces == 1 ? (const void*)rms_norm_fp8_long_kernel<float, 1>
+                                                                                                      : (const void*)rms_norm_fp8_long_kernel<float, 2>;
+    DG_CHECK_CUDA(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kLongSmem));
+    return launch_overlapped(fn, dim3(ctas < 148 ? ctas : 148), dim3(a.groups * a.threads), params, static_cast<cudaStream_t>(stream), a.groups * a.stages * token);
 }
 
 extern "C" uint64_t dg_rms_norm_grad_scratch_bytes(uint32_t tokens, uint32_t hidden) {

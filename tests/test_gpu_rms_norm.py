@@ -105,6 +105,25 @@ def test_not_finite():
     assert torch.equal(rows[:1], alone) and rows[1].isnan().all() and rstd[2] == 0 and rows[2, 3].isnan() and (rows[2, 4:] == 0).all()
 
 
+@pytest.mark.parametrize('dtype,hidden,tokens', [(BF16, 992, 1100), (BF16, 1024, 6000), (BF16, 4096, 1100), (BF16, 4128, 1100), (BF16, 7168, 700), (BF16, 7200, 1100), (BF16, 16384, 1100),
+                                                 (FP32, 2048, 2500), (FP32, 8192, 1100), (FP32, 8224, 300), (FP32, 16384, 300)])
+def test_many_tokens_have_the_bits_of_few(dtype, hidden, tokens):
+    torch.manual_seed(hidden)
+    wide = torch.randn(tokens, 2 * hidden + 64, device='cuda').to(dtype)
+    x, residual, w = wide[:, 16:16 + hidden], wide[:, hidden + 32:2 * hidden + 32], torch.randn(hidden, device='cuda')
+    for more in (None, residual):
+        (q, sf), rows, h, rstd = deep_gemm.rms_norm_to_fp8(x, w, residual=more, with_rows=True)
+        for at in range(0, tokens, 97):
+            part = slice(at, min(at + 97, tokens))
+            (q1, sf1), rows1, h1, rstd1 = deep_gemm.rms_norm_to_fp8(x[part], w, residual=None if more is None else more[part], with_rows=True)
+            assert torch.equal(q[part].view(torch.uint8), q1.view(torch.uint8)) and torch.equal(sf[part], sf1) and torch.equal(rstd[part], rstd1)
+            assert torch.equal(rows[part], rows1) and torch.equal(h[part], h1)
+    kept = wide.clone()
+    got = deep_gemm.rms_norm_to_fp8(x, w, residual=residual, with_rows=True, out_h=residual)
+    assert torch.equal(got[1], rows) and torch.equal(got[2], h) and got[2].data_ptr() == residual.data_ptr()
+    assert torch.equal(wide[:, :hidden + 32], kept[:, :hidden + 32]) and torch.equal(wide[:, 2 * hidden + 32:], kept[:, 2 * hidden + 32:])
+
+
 # --------------------------------------------------------------------------------------------------------------- gradient
 def _check_grad(g, h, weight, rstd, grad_h=None, host=deep_gemm, **kw):
     cuda = lambda t: None if t is None else t.cuda()  # noqa: E731
