@@ -1,0 +1,40 @@
+"""Where the router's choice, the norm and SwiGLU's gradient can go wrong: sums that cancel or leave the range, numbers that are not finite, rows next to a
+border of rounding. Against 64 bits on the CPU (oracle/layers.py)."""
+
+import pytest
+import torch
+
+import deep_gemm
+import oracle
+from helpers import seed_all
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24
+
+
+def _routed(logits, topk, scoring='softmax', **kw):
+    """The choices are those of the oracle."""
+    cuda = {k: v.cuda() if isinstance(v, torch.Tensor) else v for k, v in kw.items()}
+    idx, w = deep_gemm.moe_route(logits.cuda(), topk, scoring, **cuda)
+    want, want_w = oracle.moe_route_ref(logits, topk, scoring, **kw)
+    assert torch.equal(idx.cpu(), want)
+    # (24 roundings of a score, 90 of a softmax's with logits that are at most 8 apart: twice that)
+    assert ((w.cpu().double() - want_w).abs() <= 220 * E * want_w.abs()).all()
+    return idx, w
+
+
+# --------------------------------------------------------------------------------------------------------- the router
+@pytest.mark.parametrize('scoring', ['softmax', 'sigmoid'])
+@pytest.mark.parametrize('size', [2, 4, 8])
+def test_groups_whose_large_biases_cancel(scoring, size):
+    """Scores of a group that are sums of a large positive and a large negative number, next to one another."""
+    seed_all(size)
+    for large in (4.0, 16.0, 64.0, 256.0, 5000.0):
+        for groups, taken in ((2, 1), (8, 3)):
+            one = torch.full((size,), -large)
+            one[size // 2] = large
+            first = torch.randn(500, 1, size)
+            logits = (first + 1e-5 * torch.randn(500, groups, size)).flatten(1).contiguous()
+            _routed(logits, 1, scoring, bias=one.repeat(groups), num_groups=groups, topk_groups=taken)
+            _routed(logits, min(4, taken * size), scoring, bias=one.repeat(groups), num_groups=groups, topk_groups=taken, renormalize=True)
