@@ -141,7 +141,7 @@ __device__ __forceinline__ float max3_nan(float a, float b, float c) {
 // value, which moves s by s (1 - s) (|l| + 4) 2^-24 < 1.3 x 2^-24; the addition and the reciprocal by 2^-24 and 2^-23 of s: 4.3 x 2^-24 in all. Softmax: l - top times log2(e) is within
 // 2^-23 of its value x, the exponential 2 ulp more, which moves s by x e^-x 2^-23 + 2^-22 < 2^-21.5 of the largest; the sum likewise, and by
 // at most 64 + 5 additions, 2^-17.8: under 2^-17 of the largest in all. The addition of b and the difference from the largest are within 2^-24 of their
-// values, and so is the sum of two scores: that of a group is within 2 x the error of a score + 2^-23 (|best| + |second|), however small the sum itself.
+// values, and so is the sum of two scores: half that of a group is within the error of a score + 2^-24 (|best| + |second|), however small the sum itself.
 enum class Choice { kDecided, kOrderOpen, kOpen };
 template <uint32_t kVec, uint32_t kItems, bool kScores>
 __device__ __forceinline__ Choice quick_choice(const RouteArgs& a, const uint8_t* row, const Share<kVec>& of, const float (&l)[kItems], const Softmax& m, const float (&z)[kItems], uint32_t lane,
@@ -205,8 +205,9 @@ __device__ __forceinline__ Choice quick_choice(const RouteArgs& a, const uint8_t
             best = fmaxf(best, b);
         }
         // (a group with a single expert that can be chosen counts that one alone)
+        // Half the sum: the largest biases there are do not leave the range.
         const bool two = a.best_two && second > -CUDART_INF_F;
-        const float score = two ? best + second : best;
+        const float score = two ? fmaf(0.5f, second, 0.5f * best) : a.best_two ? 0.5f * best : best;
         // The groups in their order, ties to the lowest: all lanes of a group hold its score.
         float left = group < a.groups ? score : -CUDART_INF_F;
         bool taken = false;
@@ -216,10 +217,10 @@ __device__ __forceinline__ Choice quick_choice(const RouteArgs& a, const uint8_t
             const uint32_t first = __ffs(__ballot_sync(kAll, left == last)) - 1;
             if (group == first >> a.lanes_log2) { taken = true; left = -CUDART_INF_F; }
         }
-        // The groups that are taken stand for those of 64 bits where the least that one of them can be is above the most that another one can (2^-22 instead of
-        // 2^-23: this sum's own rounding). Scores that are logits are exact.
+        // The groups that are taken stand for those of 64 bits where the least that one of them can be is above the most that another one can (1.5 x 2^-23 instead
+        // of 2^-24: these sums' own rounding). Scores that are logits are exact.
         if (kScores) {
-            const float slack = 2.0f * error + 0x1p-22f * (fabsf(best) + (two ? fabsf(second) : 0.0f));
+            const float slack = error + 0x1.8p-23f * fabsf(best) + (two ? 0x1.8p-23f * fabsf(second) : 0.0f);
             const float least = redux_min(taken ? score - slack : CUDART_INF_F), most = redux_max(taken || best == -CUDART_INF_F ? -CUDART_INF_F : score + slack);
             open |= most > -CUDART_INF_F && least <= most;
         }

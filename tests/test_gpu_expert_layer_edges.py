@@ -1,6 +1,8 @@
 """Where the router's choice, the norm and SwiGLU's gradient can go wrong: sums that cancel or leave the range, numbers that are not finite, rows next to a
 border of rounding. Against 64 bits on the CPU (oracle/layers.py)."""
 
+import math
+
 import pytest
 import torch
 
@@ -11,6 +13,7 @@ from helpers import seed_all
 pytestmark = pytest.mark.gpu
 
 E = 2.0 ** -24
+INF = math.inf
 
 
 def _routed(logits, topk, scoring='softmax', **kw):
@@ -38,3 +41,20 @@ def test_groups_whose_large_biases_cancel(scoring, size):
             logits = (first + 1e-5 * torch.randn(500, groups, size)).flatten(1).contiguous()
             _routed(logits, 1, scoring, bias=one.repeat(groups), num_groups=groups, topk_groups=taken)
             _routed(logits, min(4, taken * size), scoring, bias=one.repeat(groups), num_groups=groups, topk_groups=taken, renormalize=True)
+
+
+def test_groups_whose_sums_leave_the_range():
+    """The largest numbers of FP32 as biases: their sums are infinite in 32 bits, and are told apart in 64."""
+    seed_all(1)
+    logits, lowest = torch.randn(5, 16), torch.finfo(torch.float32).min
+    for scoring in ('softmax', 'sigmoid'):
+        _routed(logits, 3, scoring, bias=torch.tensor([2e38] * 4 + [3e38] * 4 + [2.5e38] * 4 + [-1.0] * 4), num_groups=4, topk_groups=2)
+        _routed(logits, 6, scoring, bias=torch.tensor([-3e38] * 4 + [-2e38] * 4 + [-2.5e38] * 8), num_groups=4, topk_groups=2)
+        # every expert, and all but one of a group, masked by the least number
+        for topk in (1, 2, 6):
+            _routed(logits, topk, scoring, bias=torch.full((16,), lowest), num_groups=4, topk_groups=2)
+            bias = torch.full((16,), lowest)
+            bias[[9, 14]] = 0.0
+            _routed(logits, topk, scoring, bias=bias, num_groups=4, topk_groups=2)
+            bias[:4] = -INF
+            _routed(logits, topk, scoring, bias=bias, num_groups=4, topk_groups=2)
