@@ -121,6 +121,8 @@ __device__ __forceinline__ float sigmoid_of(float l) {
     return __fdiv_rn(l < 0.0f ? z : 1.0f, 1.0f + z);
 }
 __device__ __forceinline__ float score_of(bool sigmoid, const Softmax& m, float l) { return sigmoid ? sigmoid_of(l) : __fdiv_rn(expf(l - m.top), m.sum); }
+// (a NaN stays one)
+__device__ __forceinline__ float divisor_of(float sum) { return sum < kLeastSum ? kLeastSum : sum; }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -429,10 +431,10 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_kernel(const RouteArg
     if (lane >= a.topk) chosen = -1;
     float w = 0.0f;
     if (chosen >= 0) w = score_of(a.sigmoid != 0, m, logit_at(a, row, (uint32_t)chosen));
-    if (a.renormalize) w = __fdiv_rn(w, fmaxf(warp_sum(w), kLeastSum));
+    if (a.renormalize) w = __fdiv_rn(w, divisor_of(warp_sum(w)));
     if (lane < a.topk) {
         static_cast<int32_t*>(a.idx)[(uint64_t)token * a.topk + lane] = chosen;
-        a.weights[(uint64_t)token * a.topk + lane] = w * a.scale;
+        a.weights[(uint64_t)token * a.topk + lane] = chosen >= 0 ? w * a.scale : 0.0f;
     }
 }
 
@@ -470,8 +472,8 @@ __global__ void __launch_bounds__(kRouteThreads) moe_route_grad_kernel(const Rou
     const float slope = sigmoid ? sigmoid_of(-mine) : 1.0f;
     float from_choice, from_all = 0.0f;
     if (a.renormalize) {
-        const float sum = warp_sum(s), q = __fdiv_rn(s, fmaxf(sum, kLeastSum)), dot = warp_sum(g * q);
-        from_choice = q * (sum > kLeastSum ? g - dot : g) * slope;
+        const float sum = warp_sum(s), q = __fdiv_rn(s, divisor_of(sum)), dot = warp_sum(g * q);
+        from_choice = q * (sum <= kLeastSum ? g : g - dot) * slope;
     } else {
         from_choice = g * s * slope;
         if (!sigmoid) from_all = warp_sum(g * s);

@@ -115,7 +115,7 @@ def moe_route(logits: torch.Tensor, topk: int, scoring: str = 'softmax', bias: O
 
     With groups (num_groups of the same number of neighbouring experts) the score of a group is the sum of its `group_best` (1 or 2) largest c, and
     only the experts of the `topk_groups` best groups can be chosen. The weights are s of the chosen, divided by their sum (1e-20 or more)
-    with `renormalize`, times `scale`. c is compared in 64 bits, ties go to the lowest index (the lowest group), NaN counts as the largest, as in torch.topk.
+    with `renormalize` (NaN where one of them is), times `scale`. c is compared in 64 bits, ties go to the lowest index (the lowest group), NaN counts as the largest, as in torch.topk.
     An expert whose logit or bias is -inf is never chosen; where fewer than topk are left, -1 with the weight 0 takes their place: `moe_sort`
     gives it no row, so a padded token is one whose logits are all -inf. At most 1024 experts, 32 groups, 32 choices. The two tensors may share one
     allocation."""

@@ -362,7 +362,7 @@ int dg_dequant_fp4_launch(const void* codes, uint64_t code_stride, uint64_t code
  * elements between rows. score s = 1 / (1 + e^-l) (sigmoid) or softmax(l); c = s + bias[e] (NULL: 0). With num_groups > 1 the experts lie in groups of
  * experts / num_groups, whose scores are the sums of their group_best (1 or 2) largest c, and the topk_groups best groups stay. The topk largest c
  * are chosen (compared in 64 bits; NaN is the largest; ties to the lowest index), the largest first; weights[t, j] = s, divided by max(1e-20, the
- * sum of the token's) with `renormalize`, times `scale`. Logits and biases of -inf are never chosen: -1 with the weight 0 takes their place.
+ * sum of the token's) with `renormalize` (NaN where one of them is), times `scale`. Logits and biases of -inf are never chosen: -1 with the weight 0 takes their place.
  * At most 1024 experts, 32 groups, 32 choices.
  * dg_moe_route_grad_launch: the gradient of the weights with respect to the logits for given choices (those outside [0, experts) count for nothing,
  * equal ones add up), in the type of the logits. Bias and groups have no part in it. grad_logits may be the logits themselves. */

@@ -8,12 +8,13 @@ import torch
 
 import deep_gemm
 import oracle
+from both_hosts import moe_hosts
 from helpers import seed_all
 
 pytestmark = pytest.mark.gpu
 
 E = 2.0 ** -24
-INF = math.inf
+INF, NAN = math.inf, math.nan
 
 
 def _routed(logits, topk, scoring='softmax', **kw):
@@ -58,3 +59,27 @@ def test_groups_whose_sums_leave_the_range():
             _routed(logits, topk, scoring, bias=bias, num_groups=4, topk_groups=2)
             bias[:4] = -INF
             _routed(logits, topk, scoring, bias=bias, num_groups=4, topk_groups=2)
+
+
+@pytest.mark.parametrize('host', moe_hosts)
+def test_a_sum_that_is_not_a_number_shows(host):
+    """Weights that are divided by a sum with a NaN in it are NaN, and so are their gradients; places without a choice have the weight 0 all the same."""
+    seed_all(2)
+    logits = torch.randn(5, 40)
+    logits[1, 7] = NAN
+    logits[2, 4:] = -INF
+    logits[2, 1] = NAN
+    logits[3, 9] = INF
+    logits[4] = -INF
+    g = torch.randn(5, 6)
+    for scoring in ('softmax', 'sigmoid'):
+        idx, w = host.moe_route(logits.cuda(), 6, scoring, renormalize=True, scale=2.5)
+        want, want_w = oracle.moe_route_ref(logits, 6, scoring, renormalize=True, scale=2.5)
+        assert torch.equal(idx.cpu(), want) and torch.equal(w.isnan().cpu(), want_w.isnan())
+        assert w[1].isnan().all() and w[2, :4].isnan().all() and (w[2, 4:] == 0).all() and (w[4] == 0).all()
+        got = host.moe_route_grad(g.cuda(), logits.cuda(), idx, scoring, True, 2.5).cpu()
+        chosen = torch.zeros(5, 40, dtype=torch.bool)
+        for t in range(5):
+            chosen[t, [e for e in want[t].tolist() if e >= 0]] = True
+        bad = torch.tensor([False, True, True, scoring == 'softmax', False])
+        assert torch.equal(got.isnan(), chosen & bad[:, None]) and (got[~chosen] == 0).all()
