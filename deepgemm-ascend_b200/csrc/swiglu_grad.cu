@@ -4,7 +4,7 @@
 // r = min(max(x_r, -clamp), clamp), p = 1 / (1 + e^-l):
 //     dx_l = g w r p (1 + l (1 - p)) where x_l <= clamp (else 0)      dx_r = g w l p where |x_r| <= clamp (else 0)
 //     dw = sum over the row of g l p r
-// all in FP32 (the fast exponential and reciprocal: p within a few ulp, and not below 2^-126), dx rounded once to BF16.
+// all in FP32 (the fast exponential and reciprocal: p within a few ulp, and 0 below 2^-126), dx rounded once to BF16.
 //
 // HBM-bound: 2 H + 2 H + H / 16 bytes read (6 H from BF16) and 4 H written per row; the arithmetic, two channels an instruction, is two thirds of that time.
 // 65536 x 2048 from 8 bits 179 us, 6.0 TB/s (the bytes alone 165 at the rate of a copy; 199 in a long row of passes, which draws the power cap); 77 x 2048 from BF16
@@ -88,9 +88,21 @@ template <> struct Tile8<true> {
             v[2 * h + 1] = Pair(four[2], four[3]) * s;
         }
     }
+    // The lowest numbers of BF16 round to codes that stand for -2^128, -inf in FP32: the lowest finite number for it, so that a closed gate is no infinity times 0.
+    // As whole numbers -inf is the first one above that; a NaN that the conversion and the product make is a positive one and stays.
+    static __device__ __forceinline__ void lowest_for_infinity(Pair (&v)[4]) {
+        #pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float a, b;
+            v[j].get(a, b);
+            v[j] = Pair(__uint_as_float(min(__float_as_uint(a), 0xff7fffffu)), __uint_as_float(min(__float_as_uint(b), 0xff7fffffu)));
+        }
+    }
     __device__ __forceinline__ void get(uint32_t shift, Pair (&lv)[4], Pair (&rv)[4]) const {
         values(l, ue8m0_float(e >> shift & 0xffu), lv);
         values(r, ue8m0_float(e >> (shift + 16) & 0xffu), rv);
+        lowest_for_infinity(lv);
+        lowest_for_infinity(rv);
     }
 };
 
@@ -156,16 +168,19 @@ __global__ void __launch_bounds__(kGradThreads, 8) swiglu_grad_kernel(const Swig
                 l[j] = Pair(lv[0], lv[1]);
                 r[j] = Pair(rv[0], rv[1]);
             }
-            // (the reciprocal of a number beyond 2^126 would be 0, and its product with that an invalid one; 1 - p would lose its bits where p is near 1)
-            float x0, x1;
-            (l[j] * exponent).get(x0, x1);
-            const Pair z(fast_exp2(fminf(x0, 126.0f)), fast_exp2(fminf(x1, 126.0f)));
-            (z + one).get(x0, x1);
-            const Pair p(fast_reciprocal(x0), fast_reciprocal(x1)), rest = z * p, silu = l[j] * p, g(bf16_lo(gw[j]), bf16_hi(gw[j]));
-            const Pair gs = g * silu, gr = g * r[j];
+            // (beyond 2^126 p is 0, as it has to be for l down to the type's lowest number, and so is any product with it but that of an infinity; 1 - p would
+            // lose its bits where p is near 1)
+            float z0, z1, x0, x1;
+            (l[j] * exponent).get(z0, z1);
+            z0 = fast_exp2(z0);
+            z1 = fast_exp2(z1);
+            (Pair(z0, z1) + one).get(x0, x1);
+            const Pair p(fast_reciprocal(x0), fast_reciprocal(x1)), rest = Pair(fminf(z0, 0x1p126f), fminf(z1, 0x1p126f)) * p, silu = l[j] * p, g(bf16_lo(gw[j]), bf16_hi(gw[j]));
+            const Pair gs = g * silu;
             sum = fma2(gs, r[j], sum);
             float v[4];
-            (gr * weights * fma2(silu, rest, p)).get(v[0], v[1]);
+            // (r times the slope first: 0 for a closed gate, whatever r is, where the gradient times r could leave the range)
+            (g * weights * (r[j] * fma2(silu, rest, p))).get(v[0], v[1]);
             (gs * weights).get(v[2], v[3]);
             if constexpr (kClamp) {
                 #pragma unroll

@@ -8,13 +8,14 @@ import torch
 
 import deep_gemm
 import oracle
-from both_hosts import moe_hosts
+from both_hosts import moe_hosts, quant_hosts
 from helpers import seed_all
 
 pytestmark = pytest.mark.gpu
 
 E = 2.0 ** -24
 INF, NAN = math.inf, math.nan
+BF16 = torch.bfloat16
 
 
 def _routed(logits, topk, scoring='softmax', **kw):
@@ -83,3 +84,44 @@ def test_a_sum_that_is_not_a_number_shows(host):
             chosen[t, [e for e in want[t].tolist() if e >= 0]] = True
         bad = torch.tensor([False, True, True, scoring == 'softmax', False])
         assert torch.equal(got.isnan(), chosen & bad[:, None]) and (got[~chosen] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------------- SwiGLU's gradient
+@pytest.mark.parametrize('host', quant_hosts)
+@pytest.mark.parametrize('clamp', [None, 7.0])
+def test_gates_far_below_zero_have_no_gradient(host, clamp):
+    """silu(l) and its slope are 0 in FP32 from about l = -110 on, down to the type's lowest number."""
+    seed_all(3)
+    far = torch.tensor([-128.0, -1e4, -1e20, -1e30, -1e37, -1e38, -3e38, torch.finfo(BF16).min])
+    x, g, w = torch.randn(4, 512).bfloat16(), torch.randn(4, 256).bfloat16(), torch.rand(4) + 0.5
+    x[:, 32:40] = far.bfloat16()
+    x[2, :256] = torch.finfo(BF16).min
+    x[3] = torch.finfo(BF16).min
+    pair = deep_gemm.cast_to_fp8(x.cuda())
+    # (code times scale in 64 bits: the lowest number of BF16 becomes -2^128)
+    byte = torch.stack((pair[1].cpu().int() & 255, (pair[1].cpu().int() >> 8) & 255), 2).flatten(1)
+    kept = pair[0].cpu().double() * torch.exp2((byte - 127).double()).repeat_interleave(32, 1)
+    assert kept.min() == -2.0 ** 128
+    for arg, values in ((x.cuda(), x.double()), (pair, kept)):
+        dx, dw = host.swiglu_apply_weight_grad(g.cuda(), arg, w.cuda(), clamp_value=clamp)
+        dx, dw = dx.cpu(), dw.cpu()
+        none = values[:, :256] <= -128
+        assert (dx[:, :256][none] == 0).all() and (dx[:, 256:][none] == 0).all() and torch.isfinite(dx).all()
+        l, r = values[:, :256], values[:, 256:]
+        if clamp:
+            l, r = l.clamp(max=clamp), r.clamp(-clamp, clamp)
+        terms = g.double() * l * torch.sigmoid(l) * r
+        # (64 roundings, of 32 channels a lane and of each term)
+        assert ((dw.double() - terms.sum(1)).abs() <= 128 * E * terms.abs().sum(1)).all() and (dw[2:] == 0).all()
+
+
+def test_codes_that_are_not_numbers_show_in_the_gradient():
+    """A NaN code of either sign, and the NaN scale, in both halves of the 8-bit input."""
+    codes, sf = torch.full((6, 256), 0x38, dtype=torch.uint8), torch.full((4, 6), 0x7F7F, dtype=torch.int16)
+    codes[0, 3], codes[1, 3], codes[2, 131], codes[3, 131] = 0x7F, 0xFF, 0x7F, 0xFF
+    sf[0, 4], sf[2, 5] = -129, -129                                  # 0xFF7F: columns 32 to 63 of a half
+    dx, dw = deep_gemm.swiglu_apply_weight_grad(torch.ones(6, 128, dtype=BF16, device='cuda'), (codes.cuda().view(torch.float8_e4m3fn), sf.cuda().t()), torch.ones(6, device='cuda'))
+    bad = torch.zeros(6, 256, dtype=torch.bool)
+    bad[:2, 3] = bad[:2, 131] = bad[2:4, 3] = True
+    bad[4, 32:64] = bad[4, 160:192] = bad[5, 32:64] = True
+    assert torch.equal(dx.isnan().cpu(), bad) and dw.isnan().all()
