@@ -293,18 +293,19 @@ struct NormGradArgs {
     float inverse_hidden;
 };
 
-// sum(u n) = rstd sum(u h), and a thread's part of dweight.
+// sum(u n), and a thread's part of dweight. (With n and not with h, whose products with u and whose rstd^2 leave the range of FP32 long before dx does.)
 __device__ __forceinline__ void add_dots(const Pair (&h)[4], const Pair (&g)[4], const Pair (&w)[4], Pair scale, Pair& dots, Pair (&sum_w)[4]) {
     #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        dots = fma2(g[j] * w[j], h[j], dots);
-        sum_w[j] = fma2(g[j], h[j] * scale, sum_w[j]);
+        const Pair n = h[j] * scale;
+        dots = fma2(g[j] * w[j], n, dots);
+        sum_w[j] = fma2(g[j], n, sum_w[j]);
     }
 }
-// dx = rstd u - h (rstd^3 mean(u h)) + grad_h, which `d` holds
+// dx = rstd u - n (rstd mean(u n)) + grad_h, which `d` holds
 __device__ __forceinline__ void slope_of(const Pair (&h)[4], const Pair (&g)[4], const Pair (&w)[4], Pair scale, Pair slope, Pair (&d)[4]) {
     #pragma unroll
-    for (int j = 0; j < 4; ++j) d[j] = fma2(h[j], slope, fma2(scale, g[j] * w[j], d[j]));
+    for (int j = 0; j < 4; ++j) d[j] = fma2(h[j] * scale, slope, fma2(scale, g[j] * w[j], d[j]));
 }
 __device__ __forceinline__ void store_part(const NormGradArgs& a, uint32_t c, const float (&dw)[8]) {
     float4* const out = reinterpret_cast<float4*>(a.partial + (uint64_t)blockIdx.x * a.hidden + c);
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(kThreads) rms_norm_grad_kernel(const NormGradA
         h0.get(n);
         g0.get(u);
         more0.get(d);
-        slope_of(n, u, w, scale, Pair(-(r * r * (r * (dot * a.inverse_hidden)))), d);
+        slope_of(n, u, w, scale, Pair(-(r * (dot * a.inverse_hidden))), d);
         h0.set(d);
         h0.store(a.dx + token * a.dx_stride + (uint64_t)c * sizeof(T));
     }
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_grad_long_kernel(const 
         // (all threads are done with the token in front)
         const uint64_t later = token + (a.stages - 1) * stride;
         if (t == 0 && a.stages > 1 && token != first && later < a.tokens) ask(later, before);
-        const Pair slope(-(r * r * (r * (dot * a.inverse_hidden))));
+        const Pair slope(-(r * (dot * a.inverse_hidden)));
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
             const uint32_t c = (i * a.threads + t) * 8;

@@ -10,6 +10,7 @@ import deep_gemm
 import oracle
 from both_hosts import moe_hosts, quant_hosts
 from helpers import seed_all
+from test_gpu_rms_norm import _check_grad
 
 pytestmark = pytest.mark.gpu
 
@@ -125,3 +126,16 @@ def test_codes_that_are_not_numbers_show_in_the_gradient():
     bad[:2, 3] = bad[:2, 131] = bad[2:4, 3] = True
     bad[4, 32:64] = bad[4, 160:192] = bad[5, 32:64] = True
     assert torch.equal(dx.isnan().cpu(), bad) and dw.isnan().all()
+
+
+# ---------------------------------------------------------------------------------------------------------- the norm
+@pytest.mark.parametrize('dtype,hidden', [(BF16, 96), (BF16, 2048), (BF16, 4096), (BF16, 7168), (BF16, 8224), (torch.float32, 96), (torch.float32, 2048),
+                                          (torch.float32, 4128), (torch.float32, 8224)])
+@pytest.mark.parametrize('size,grad_size', [(1e-25, 1.0), (1e30, 1e10), (1e-30, 1e-5)])
+def test_gradient_of_rows_far_from_one(dtype, hidden, size, grad_size):
+    """rstd^2 and the products of h and its gradient leave the range of FP32, dx does not."""
+    seed_all(hidden)
+    for tokens in (3, 400):
+        h, g = (torch.randn(tokens, hidden) * size).to(dtype), (torch.randn(tokens, hidden) * grad_size).to(dtype)
+        weight = 1 + 0.1 * torch.randn(hidden)
+        _check_grad(g, h, weight, oracle.rms_norm_ref(h, weight, 0.0)[0].float())
