@@ -2,8 +2,7 @@
 // one UE8M0 scale per 32 channels in the layout the GEMM reads (and in BF16 where a router or a dispatch wants it), and its gradient.
 //
 // h is rounded to its type before the norm sees it: what the residual stream holds is what the gradient is taken at. The sum of squares is held in
-// 64 bits, so that 1 / sqrt comes out as the same FP32 number however a row is spread over threads: a token's bits do not depend on how many
-// others there are. y = (h * rstd) * weight in FP32, one rounding each, then one to E4M3 (values times the inverse of the scale of quant.cuh, which is
+// 64 bits and made in one order however a row is spread over threads (row_sum): a token's bits do not depend on how many others there are. y = (h * rstd) * weight in FP32, one rounding each, then one to E4M3 (values times the inverse of the scale of quant.cuh, which is
 // a power of two) and one to BF16.
 //
 // HBM-bound: BF16 with a residual 4 H bytes read, 2 H + H + H / 32 written per token (2 H more for the BF16 rows).
@@ -78,14 +77,38 @@ __device__ __forceinline__ void weight_at(const void* weight, uint32_t fp32, uin
 }
 
 // The sum over a group of `warps` warps, of which `first` is the first, in all its threads. `partial`: a place for each warp of the CTA that nobody reads any more.
-template <typename S>
-__device__ __forceinline__ S group_sum(S v, S* partial, uint32_t first, uint32_t warps, uint32_t barrier) {
+__device__ __forceinline__ float group_sum(float v, float* partial, uint32_t first, uint32_t warps, uint32_t barrier) {
     const uint32_t warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
     if (lane == 0) partial[warp] = v;
     named_bar_sync(barrier, warps * 32);
-    v = lane < warps ? partial[first + lane] : (S)0;
+    v = lane < warps ? partial[first + lane] : 0.0f;
+    #pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+    return v;
+}
+
+// The sum over a group of the sums of squares of a thread's pieces, in an order that depends on the row's length alone: pairs of a piece's lanes, then pairs of
+// the places that stand 32 pieces (256 channels) apart, whichever thread holds them. `partial`: as above, kPieces places for each warp.
+template <uint32_t kPieces>
+__device__ __forceinline__ double row_sum(const double (&of)[kPieces], double* partial, uint32_t first, uint32_t warps, uint32_t barrier) {
+    const uint32_t warp = threadIdx.x / 32 - first, lane = threadIdx.x % 32;
+    partial += first * kPieces;
+    double v;
+    if constexpr (kPieces == 1) {
+        v = of[0] + __shfl_xor_sync(kAll, of[0], 16);
+    } else {
+        // (the lower lanes carry on with the first piece, the upper ones with the second)
+        v = lane < 16 ? of[0] : of[1];
+        v += __shfl_xor_sync(kAll, lane < 16 ? of[1] : of[0], 16);
+    }
+    #pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
+    if (lane % (32 / kPieces) == 0) partial[lane / (32 / kPieces) * warps + warp] = v;
+    named_bar_sync(barrier, warps * 32);
+    v = lane < kPieces * warps ? partial[lane] : 0.0;
+    if (kPieces > 1 && lane + 32 < kPieces * warps) v += partial[lane + 32];
     #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kAll, v, o);
     return v;
@@ -179,7 +202,7 @@ __device__ __forceinline__ void finish_piece(const NormArgs& a, uint64_t token, 
 // of a copy (a CTA for every token took 106, L2 asked for the token behind the next 109). 1 x 7168: 2.4 us, launch and latency.
 template <typename T, uint32_t kPieces, uint32_t kThreads, uint32_t kCtas>
 __global__ void __launch_bounds__(kThreads, kCtas) rms_norm_fp8_kernel(const NormArgs a) {
-    __shared__ double partial[2][32];
+    __shared__ double partial[2][kPieces * (kThreads / 32)];
     griddep_wait();
     griddep_launch_dependents();
     Piece<T> x[kPieces], more[kPieces];
@@ -198,12 +221,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) rms_norm_fp8_kernel(const Nor
     uint32_t turn = 0;
     for (uint64_t token = blockIdx.x; token < a.tokens; token += gridDim.x, turn ^= 1) {
         Piece<T> h[kPieces];
-        double sum = 0.0;
+        double sums[kPieces] = {};
         #pragma unroll
-        for (uint32_t i = 0; i < kPieces; ++i) add_piece(a, token, (i * blockDim.x + threadIdx.x) * 8, x[i], more[i], h[i], sum);
+        for (uint32_t i = 0; i < kPieces; ++i) add_piece(a, token, (i * blockDim.x + threadIdx.x) * 8, x[i], more[i], h[i], sums[i]);
         if (token + gridDim.x < a.tokens) load(token + gridDim.x);
         // (two sets of shared memory: a warp that is a turn ahead does not write to what another still reads)
-        sum = group_sum(sum, partial[turn], 0, blockDim.x / 32, 1);
+        const double sum = row_sum(sums, partial[turn], 0, blockDim.x / 32, 1);
         const float rstd = rsqrt_of(fma(sum, a.inverse_hidden, (double)a.eps));
         if (threadIdx.x == 0) a.rstd[token] = rstd;
         #pragma unroll
@@ -213,7 +236,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) rms_norm_fp8_kernel(const Nor
 
 // Many tokens, and rows too long for the above: the rows of a token come to shared memory by bulk copies, as many tokens ahead as fit there; a group of a CTA's warps
 // takes a token, a thread one piece of it or two. Behind the barrier of the sum nobody reads the rows any more, and the next token takes their place.
-constexpr uint32_t kLongThreads = 1024, kLongSmem = 226 * 1024, kLongMostStages = 4, kMostGroups = 8;
+constexpr uint32_t kLongThreads = 1024, kLongSmem = 225 * 1024, kLongMostStages = 4, kMostGroups = 8;
 
 __device__ __forceinline__ void take(Piece<__nv_bfloat16>& p, const uint8_t* from) { p.q = *reinterpret_cast<const uint4*>(from); }
 __device__ __forceinline__ void take(Piece<float>& p, const uint8_t* from) {
@@ -224,7 +247,7 @@ __device__ __forceinline__ void take(Piece<float>& p, const uint8_t* from) {
 template <typename T, uint32_t kPieces>
 __global__ void __launch_bounds__(kLongThreads) rms_norm_fp8_long_kernel(const NormArgs a) {
     extern __shared__ __align__(16) uint8_t places[];         // of each token: the rows of x and of the residual
-    __shared__ double partial[2][32];
+    __shared__ double partial[2][kPieces * (kLongThreads / 32)];
     __shared__ __align__(8) uint64_t full[kMostGroups * kLongMostStages];
     const uint32_t groups = a.groups, group = threadIdx.x / a.threads, t = threadIdx.x - group * a.threads, warps = a.threads / 32;
     const uint64_t stride = (uint64_t)gridDim.x * groups, first = (uint64_t)blockIdx.x * groups + group;
@@ -251,9 +274,10 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_fp8_long_kernel(const N
     uint32_t turn = 0, stage = 0, parity = 0;
     for (uint64_t token = first; token < a.tokens; token += stride, turn ^= 1) {
         // (a copy that never comes shows in the result)
-        double sum = wait_for(full_at + stage * 8, parity) ? 0.0 : (double)__uint_as_float(0x7fc00000u);
+        const double none = wait_for(full_at + stage * 8, parity) ? 0.0 : (double)__uint_as_float(0x7fc00000u);
         const uint8_t* const from = mine + stage * place;
         Piece<T> h[kPieces];
+        double sums[kPieces];
         #pragma unroll
         for (uint32_t i = 0; i < kPieces; ++i) {
             const uint32_t c = (i * a.threads + t) * 8;
@@ -263,9 +287,10 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_fp8_long_kernel(const N
                 take(x, from + c * sizeof(T));
                 if (a.residual) take(more, from + row + c * sizeof(T));
             }
-            add_piece(a, token, c, x, more, h[i], sum);
+            sums[i] = none;
+            add_piece(a, token, c, x, more, h[i], sums[i]);
         }
-        sum = group_sum(sum, partial[turn], group * warps, warps, group + 1);
+        const double sum = row_sum(sums, partial[turn], group * warps, warps, group + 1);
         if (t == 0 && token + a.stages * stride < a.tokens) ask(token + a.stages * stride, stage);
         const float rstd = rsqrt_of(fma(sum, a.inverse_hidden, (double)a.eps));
         if (t == 0) a.rstd[token] = rstd;

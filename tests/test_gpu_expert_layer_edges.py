@@ -139,3 +139,34 @@ def test_gradient_of_rows_far_from_one(dtype, hidden, size, grad_size):
         h, g = (torch.randn(tokens, hidden) * size).to(dtype), (torch.randn(tokens, hidden) * grad_size).to(dtype)
         weight = 1 + 0.1 * torch.randn(hidden)
         _check_grad(g, h, weight, oracle.rms_norm_ref(h, weight, 0.0)[0].float())
+
+
+def _rows_near_a_border(count, hidden, eps):
+    """BF16 rows whose 1 / sqrt(mean(h^2) + eps) lies within a few 2^-53 of the middle between two FP32 numbers, with squares whose sum depends on its order."""
+    rows = (torch.randn(count, hidden) * torch.exp2(torch.randint(-14, 15, (count, hidden)).float())).bfloat16()
+    spare, nothing = torch.randperm(hidden)[:10], torch.zeros((), dtype=BF16)
+    rows[:, spare] = 0
+    eps = float(torch.tensor(eps))
+    for row, steps in zip(rows, torch.randint(-4, 5, (count,)).tolist()):
+        base = math.fsum((row.double() ** 2).tolist())
+        low = torch.tensor(1 / math.sqrt(base / hidden + eps))
+        low = torch.nextafter(torch.nextafter(low, torch.zeros(())), torch.zeros(()))
+        middle = (float(low) + float(torch.nextafter(low, torch.ones(()) * 9e9))) / 2
+        left = (1 / middle ** 2 - eps) * hidden * (1 + steps * 2.0 ** -53) - base
+        for c in spare:
+            v = torch.tensor(math.sqrt(max(left, 0.0)), dtype=torch.float64).bfloat16()
+            if float(v) ** 2 > left:
+                v = torch.nextafter(v, nothing)
+            row[c] = v
+            left -= float(v) ** 2
+    return rows
+
+
+@pytest.mark.parametrize('hidden', [2048, 4096, 7168])
+def test_rows_next_to_a_border_do_not_depend_on_their_number(hidden):
+    """The sum of squares is made in one order, whatever the number of tokens."""
+    seed_all(hidden)
+    x, w = _rows_near_a_border(400, hidden, 1e-6).cuda(), torch.ones(hidden, device='cuda')
+    few = torch.cat([deep_gemm.rms_norm_to_fp8(x[i:i + 100], w)[3] for i in range(0, 400, 100)])
+    assert torch.equal(deep_gemm.rms_norm_to_fp8(x, w)[3], few)
+    assert torch.equal(deep_gemm.rms_norm_to_fp8(x.repeat(3, 1), w)[3], few.repeat(3))
