@@ -12,6 +12,8 @@ namespace dg {
 
 void set_last_error(const char* fmt, ...);
 void count_kernel_launch(unsigned n = 1);
+// The status word of the norm's kernels (norm_ops.cu): fills `status` where it is 0.
+int take_norm_status(int32_t* status);
 // Are kernels launched with programmatic stream serialisation (see mx_gemm.cu)?
 bool overlap_launches_enabled();
 

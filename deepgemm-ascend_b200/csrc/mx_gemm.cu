@@ -281,5 +281,5 @@ extern "C" int dg_device_status(int32_t* out_status) {
     DG_CHECK_CUDA(cudaDeviceSynchronize());
     DG_CHECK_CUDA(cudaMemcpy(out_status, p, sizeof(int32_t), cudaMemcpyDeviceToHost));
     if (*out_status != 0) DG_CHECK_CUDA(cudaMemset(p, 0, sizeof(int32_t)));
-    return DG_OK;
+    return dg::take_norm_status(out_status);
 }

@@ -17,7 +17,14 @@
 namespace dg {
 
 constexpr uint32_t kAll = 0xffffffffu, kMostHidden = 16384;
-constexpr uint64_t kLongestWaitNs = 2000000000ull;
+// How long a wait for a bulk copy may take. (0: every one gives up at once, for a test of what happens then)
+#ifndef DG_NORM_LONGEST_WAIT_NS
+#define DG_NORM_LONGEST_WAIT_NS 2000000000ull
+#endif
+constexpr uint64_t kLongestWaitNs = DG_NORM_LONGEST_WAIT_NS, kLongestDrainNs = 2000000000ull;
+constexpr int32_t kStatusTimeoutRows = 108;
+// 0, or that a wait gave up: a word of this file's own, which its kernels reach without an argument. dg_device_status reads it.
+__device__ int32_t g_norm_status = 0;
 
 // Eight channels of a lane as they lie in memory.
 template <typename T> struct Piece;
@@ -129,12 +136,25 @@ struct NormArgs {
 };
 
 __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+    if (kLongestWaitNs == 0) return false;
     if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = global_timer_ns();
     while (!mbar_try_wait(bar, parity))
         if (global_timer_ns() - t0 > kLongestWaitNs) return false;
     return true;
 }
+// A wait gave up: a group takes no more tokens. Its first thread says so and lets the copies that were asked for, `asked` from `stage` on, land (again with a limit)
+// before the CTA leaves its shared memory to another. Out of line: no launch that works runs it.
+static __device__ __noinline__ void report_and_drain(uint32_t full_at, uint32_t stages, uint32_t stage, uint32_t parity, uint64_t asked) {
+    atomicCAS(&g_norm_status, 0, kStatusTimeoutRows);
+    const uint64_t t0 = global_timer_ns();
+    for (uint64_t i = 0; i < asked; ++i) {
+        while (!mbar_try_wait(full_at + stage * 8, parity) && global_timer_ns() - t0 < kLongestDrainNs) {}
+        if (++stage == stages) { stage = 0; parity ^= 1; }
+    }
+}
+// How many tokens from `token` on there are, `most` at most.
+__device__ __forceinline__ uint64_t tokens_ahead(uint64_t token, uint64_t tokens, uint64_t stride, uint32_t most) { return min((tokens - token + stride - 1) / stride, (uint64_t)most); }
 
 // 1 / sqrt(m) as the nearest FP32 number (but for one in 10^8): two steps of Newton's method in 64 bits behind the FP32 instruction, where FP32 holds m.
 __device__ __forceinline__ float rsqrt_of(double m) {
@@ -249,6 +269,7 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_fp8_long_kernel(const N
     extern __shared__ __align__(16) uint8_t places[];         // of each token: the rows of x and of the residual
     __shared__ double partial[2][kPieces * (kLongThreads / 32)];
     __shared__ __align__(8) uint64_t full[kMostGroups * kLongMostStages];
+    __shared__ volatile uint32_t gave_up[2][kMostGroups];     // set in front of the barrier of a turn, read behind it: two sets, as of the sums
     const uint32_t groups = a.groups, group = threadIdx.x / a.threads, t = threadIdx.x - group * a.threads, warps = a.threads / 32;
     const uint64_t stride = (uint64_t)gridDim.x * groups, first = (uint64_t)blockIdx.x * groups + group;
     const uint32_t row = a.hidden * sizeof(T), place = a.residual ? 2 * row : row;
@@ -256,6 +277,7 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_fp8_long_kernel(const N
     const uint32_t mine_at = smem_u32(mine), full_at = smem_u32(full + group * a.stages);
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < groups * a.stages; ++s) mbar_init(smem_u32(full + s), 1);
+        for (uint32_t g = 0; g < groups; ++g) gave_up[0][g] = gave_up[1][g] = 0;
         fence_mbar_init();
         fence_proxy_async_smem();
     }
@@ -273,8 +295,7 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_fp8_long_kernel(const N
             if (first + s * stride < a.tokens) ask(first + s * stride, s);
     uint32_t turn = 0, stage = 0, parity = 0;
     for (uint64_t token = first; token < a.tokens; token += stride, turn ^= 1) {
-        // (a copy that never comes shows in the result)
-        const double none = wait_for(full_at + stage * 8, parity) ? 0.0 : (double)__uint_as_float(0x7fc00000u);
+        if (!wait_for(full_at + stage * 8, parity)) gave_up[turn][group] = 1;
         const uint8_t* const from = mine + stage * place;
         Piece<T> h[kPieces];
         double sums[kPieces];
@@ -287,10 +308,16 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_fp8_long_kernel(const N
                 take(x, from + c * sizeof(T));
                 if (a.residual) take(more, from + row + c * sizeof(T));
             }
-            sums[i] = none;
+            sums[i] = 0.0;
             add_piece(a, token, c, x, more, h[i], sums[i]);
         }
         const double sum = row_sum(sums, partial[turn], group * warps, warps, group + 1);
+        if (gave_up[turn][group] != 0) {
+            if (t != 0) return;
+            report_and_drain(full_at, a.stages, stage, parity, tokens_ahead(token, a.tokens, stride, a.stages));
+            for (; token < a.tokens; token += stride) a.rstd[token] = __uint_as_float(0x7fc00000u);
+            return;
+        }
         if (t == 0 && token + a.stages * stride < a.tokens) ask(token + a.stages * stride, stage);
         const float rstd = rsqrt_of(fma(sum, a.inverse_hidden, (double)a.eps));
         if (t == 0) a.rstd[token] = rstd;
@@ -425,6 +452,7 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_grad_long_kernel(const 
     extern __shared__ __align__(16) uint8_t places[];         // of each token: the rows of h, g and grad_h
     __shared__ float sums[2][32];
     __shared__ __align__(8) uint64_t full[kMostGroups * kLongMostStages];
+    __shared__ volatile uint32_t gave_up[2][kMostGroups];     // set in front of the barrier of a turn, read behind it: two sets, as of the sums
     // (rows of two pieces leave no room for a second group)
     const uint32_t groups = kPieces == 1 ? a.groups : 1u, group = kPieces == 1 ? threadIdx.x / a.threads : 0u, t = threadIdx.x - group * a.threads, warps = a.threads / 32;
     const uint64_t stride = (uint64_t)gridDim.x * groups, first = (uint64_t)blockIdx.x * groups + group;
@@ -433,6 +461,7 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_grad_long_kernel(const 
     const uint32_t mine_at = smem_u32(mine), full_at = smem_u32(full + group * a.stages);
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < groups * a.stages; ++s) mbar_init(smem_u32(full + s), 1);
+        for (uint32_t g = 0; g < groups; ++g) gave_up[0][g] = gave_up[1][g] = 0;
         fence_mbar_init();
         fence_proxy_async_smem();
     }
@@ -459,11 +488,11 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_grad_long_kernel(const 
     }
     float next = first < a.tokens ? __uint_as_float(ld_global_u32(a.rstd + first)) : 0.0f;
     uint32_t turn = 0, stage = 0, before = a.stages - 1, parity = 0;
+    bool complete = true;
     for (uint64_t token = first; token < a.tokens; token += stride, turn ^= 1) {
-        float r = next;
+        const float r = next;
         if (token + stride < a.tokens) next = __uint_as_float(ld_global_u32(a.rstd + token + stride));
-        // (a copy that never comes shows in the result)
-        if (!wait_for(full_at + stage * 8, parity)) r = __uint_as_float(0x7fc00000u);
+        if (!wait_for(full_at + stage * 8, parity)) gave_up[turn][group] = 1;
         const Pair scale(r);
         const uint8_t* const from = mine + stage * place;
         Pair dots(0.0f);
@@ -483,6 +512,13 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_grad_long_kernel(const 
         float dot, other;
         dots.get(dot, other);
         dot = group_sum(dot + other, sums[turn], group * warps, warps, group + 1);
+        if (gave_up[turn][group] != 0) {
+            complete = false;
+            // (behind the first token, the last stage's next one has not been asked for yet)
+            if (t == 0) report_and_drain(full_at, a.stages, stage, parity, tokens_ahead(token, a.tokens, stride, token == first || a.stages == 1 ? a.stages : a.stages - 1));
+            __syncwarp();
+            break;
+        }
         // (all threads are done with the token in front)
         const uint64_t later = token + (a.stages - 1) * stride;
         if (t == 0 && a.stages > 1 && token != first && later < a.tokens) ask(later, before);
@@ -516,7 +552,10 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_grad_long_kernel(const 
     #pragma unroll
     for (uint32_t i = 0; i < kPieces; ++i)
         #pragma unroll
-        for (int j = 0; j < 4; ++j) sum_w[i][j].get(dw[i][2 * j], dw[i][2 * j + 1]);
+        for (int j = 0; j < 4; ++j) {
+            if (!complete) sum_w[i][j] = Pair(__uint_as_float(0x7fc00000u));
+            sum_w[i][j].get(dw[i][2 * j], dw[i][2 * j + 1]);
+        }
     if (groups > 1) {
         __syncthreads();                                      // (nobody reads a token any more)
         float4* const to = reinterpret_cast<float4*>(places);
@@ -595,6 +634,17 @@ static int norm_checks(uint32_t tokens, uint32_t hidden) {
     DG_CHECK_ARG(tokens <= 0x7fffffffu, "rms_norm: too many tokens");
     return DG_OK;
 }
+// Adds to dg_device_status what these kernels recorded, and forgets it. (The device has been waited for.)
+namespace dg {
+int take_norm_status(int32_t* status) {
+    int32_t code = 0;
+    const int32_t none = 0;
+    DG_CHECK_CUDA(cudaMemcpyFromSymbol(&code, g_norm_status, sizeof(code)));
+    if (code != 0) DG_CHECK_CUDA(cudaMemcpyToSymbol(g_norm_status, &none, sizeof(none)));
+    if (*status == 0) *status = code;
+    return DG_OK;
+}
+}  // namespace dg
 static bool aligned16(const void* p, uint64_t stride_bytes) { return (reinterpret_cast<uintptr_t>(p) | stride_bytes) % 16 == 0; }
 
 extern "C" int dg_rms_norm_fp8_launch(const void* x, int is_fp32, uint64_t x_stride, const void* residual, uint64_t residual_stride, void* h, uint64_t h_stride,

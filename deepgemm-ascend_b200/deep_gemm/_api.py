@@ -847,7 +847,8 @@ def einsum(expr, a, b, d, c=None, use_cublaslt=False, epilogue=None, *, config=N
 
 def device_status() -> int:
     """0, or the code of the first problem a kernel recorded since the last call: 101..107 = a bounded wait inside a
-    GEMM kernel gave up (its output is incomplete), 201 = a scale-factor transform met an FP32 scale that is negative
+    GEMM kernel gave up (its output is incomplete), 108 = one of the norm's or its gradient's (rows were left out; their rstd, or the
+    gradient of the weight, is NaN), 201 = a scale-factor transform met an FP32 scale that is negative
     or not a power of two (the reference's device assert, transform_sf.hpp:13-21). Synchronises the device; the
     record is cleared. After a wait that gave up the split-K scratch may hold partial sums, so it is dropped and
     the next split-K launch starts from a fresh zeroed buffer."""

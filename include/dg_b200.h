@@ -441,7 +441,7 @@ uint32_t dg_resident_clusters(uint32_t cluster_size);
 int dg_l2_flush_launch(void* buffer, size_t bytes, void* stream);
 
 /* Device-side status word of the most recent kernels on this device: 0, or a code recorded by a
- * bounded wait that gave up. Reading it synchronises the device. */
+ * bounded wait that gave up (101 to 107 a GEMM's, 108 the norm's or its gradient's). Reading it synchronises the device. */
 int dg_device_status(int32_t* out_status);
 
 /* Number of kernels this library has enqueued in this process (all devices, all threads). Benchmarks

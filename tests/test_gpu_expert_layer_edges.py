@@ -1,7 +1,11 @@
 """Where the router's choice, the norm and SwiGLU's gradient can go wrong: sums that cancel or leave the range, numbers that are not finite, rows next to a
 border of rounding. Against 64 bits on the CPU (oracle/layers.py)."""
 
+import ctypes as C
 import math
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -9,6 +13,7 @@ import torch
 import deep_gemm
 import oracle
 from both_hosts import moe_hosts, quant_hosts
+from deep_gemm import _lib as L
 from helpers import seed_all
 from test_gpu_rms_norm import _check_grad
 
@@ -170,3 +175,46 @@ def test_rows_next_to_a_border_do_not_depend_on_their_number(hidden):
     few = torch.cat([deep_gemm.rms_norm_to_fp8(x[i:i + 100], w)[3] for i in range(0, 400, 100)])
     assert torch.equal(deep_gemm.rms_norm_to_fp8(x, w)[3], few)
     assert torch.equal(deep_gemm.rms_norm_to_fp8(x.repeat(3, 1), w)[3], few.repeat(3))
+
+
+WAITS = '''
+#include "%s"
+namespace dg {
+void set_last_error(const char*, ...) {}
+void count_kernel_launch(unsigned) {}
+bool overlap_launches_enabled() { return false; }
+}
+extern "C" int take_status() { int code = 0; return cudaDeviceSynchronize() == cudaSuccess && dg::take_norm_status(&code) == 0 ? code : -1; }
+'''
+
+
+def test_a_wait_that_gives_up_is_reported(tmp_path):
+    """The norm's kernels, built so that no wait for a bulk copy lasts: they let the copies land, say so, and leave NaN; the device goes on."""
+    nvcc = shutil.which('nvcc') or '/usr/local/cuda/bin/nvcc'
+    if not os.path.exists(nvcc):
+        pytest.skip('no nvcc')
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(deep_gemm.__file__))), 'csrc')
+    (tmp_path / 'waits.cu').write_text(WAITS % os.path.join(csrc, 'norm_ops.cu'))
+    subprocess.run([nvcc, '-gencode', 'arch=compute_100a,code=sm_100a', '-O3', '-std=c++17', '--expt-relaxed-constexpr', '-DDG_NORM_LONGEST_WAIT_NS=0', '-Xcompiler', '-fPIC',
+                    '-Xlinker', '-Bsymbolic', '-shared', '-o', str(tmp_path / 'waits.so'), str(tmp_path / 'waits.cu')], check=True, timeout=300)
+    lib = C.CDLL(str(tmp_path / 'waits.so'))
+    for name in ('dg_rms_norm_fp8_launch', 'dg_rms_norm_grad_launch'):
+        getattr(lib, name).restype, getattr(lib, name).argtypes = L._PROTOTYPES[name]
+    stream = torch.cuda.current_stream().cuda_stream
+    # four, one and two tokens ahead; several groups of a CTA, and one; one turn, and many
+    for dtype, tokens, hidden in ((BF16, 1100, 1024), (BF16, 1100, 16384), (torch.float32, 100, 16384), (torch.float32, 1100, 4096), (torch.float32, 1100, 2080)):
+        x, w, fp32 = torch.randn(tokens, hidden, device='cuda').to(dtype), torch.randn(hidden, device='cuda'), int(dtype == torch.float32)
+        q, sf = torch.zeros(tokens, hidden, dtype=torch.uint8, device='cuda'), torch.zeros(hidden // 64 + 1, tokens, dtype=torch.int16, device='cuda')
+        rstd, h = torch.zeros(tokens, device='cuda'), torch.zeros_like(x)
+        assert lib.dg_rms_norm_fp8_launch(x.data_ptr(), fp32, hidden, x.data_ptr(), hidden, h.data_ptr(), hidden, w.data_ptr(), 1, 1e-6, tokens, hidden, q.data_ptr(), hidden,
+                                          sf.data_ptr(), tokens, None, 0, rstd.data_ptr(), stream) == 0
+        assert lib.take_status() == 108 and lib.take_status() == 0 and rstd.isnan().all() and (q == 0).all()
+        ones = torch.ones(tokens, device='cuda')
+        dx, dw, scratch = torch.zeros_like(x), torch.zeros(hidden, device='cuda'), torch.empty(148 * hidden, device='cuda')
+        assert lib.dg_rms_norm_grad_launch(x.data_ptr(), fp32, hidden, x.data_ptr(), fp32, hidden, w.data_ptr(), 1, ones.data_ptr(), x.data_ptr(), hidden,
+                                           tokens, hidden, dx.data_ptr(), hidden, dw.data_ptr(), scratch.data_ptr(), scratch.numel() * 4, stream) == 0
+        long = dtype == torch.float32 or hidden >= 4096
+        assert lib.take_status() == (108 if long else 0) and dw.isnan().all() == long and (dx == 0).all() == long
+        # the library itself reports nothing, and works
+        want = deep_gemm.rms_norm_to_fp8(x, w)[3]
+        assert deep_gemm.device_status() == 0 and not want.isnan().any()
