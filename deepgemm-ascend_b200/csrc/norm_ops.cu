@@ -441,12 +441,8 @@ __global__ void __launch_bounds__(kThreads) rms_norm_grad_kernel(const NormGradA
 // thread takes one piece of its group's token or two. Behind the barrier of a sum all threads of a group have read the token in front of it, whose place the
 // next one takes.
 //
-// From 4096 channels of BF16, but for what is just under the most that fits in registers, and above 2048 of FP32 (8192 tokens; in registers / in shared memory, us in a
-// row of passes): BF16 2048 22.9 / 27.2, 3584 38.6 / 41.3, 4096 59.5 / 50.8, 5120 66.5 / 65.5, 6144 75.2 / 75.7, 7168 83.1 / 85.3; FP32 2048 42.0 / 40.9 (1531 tokens 11.6 / 12.3),
-// 2560 77.5 / 52.1, 4096 87.4 / 82.5. Longer ones do not fit in registers: BF16 16384 195, FP32 8192 162, 16384 332 us. (Copies that every thread asks for itself, cp.async, took
-// 120 us for 8192 channels of BF16, where this takes 86: they are issued by the same warps and wait for room.)
-constexpr uint32_t kLongRows = 4096, kLongRowsFp32 = 2080;
-
+// Longer rows than fit in registers: BF16 16384 195, FP32 8192 159, 16384 332 us of 8192 tokens. (Copies that every thread asks for itself, cp.async, took 120 us for 8192
+// channels of BF16, where this takes 86: they are issued by the same warps and wait for room.)
 template <typename T, typename G, uint32_t kPieces>
 __global__ void __launch_bounds__(kLongThreads) rms_norm_grad_long_kernel(const NormGradArgs a) {
     extern __shared__ __align__(16) uint8_t places[];         // of each token: the rows of h, g and grad_h
@@ -605,12 +601,29 @@ static uint32_t norm_threads(uint32_t hidden, uint32_t pieces) { return ((hidden
 
 // How the gradient is laid over the SMs, one CTA each: in as many groups as there are threads for (registers: 896, or 512 of FP32, whose pieces are twice as
 // large), as many CTAs as finish together. (With registers for 1024 threads some go to memory: 117 us where 896 took 84.)
+//
+// In registers or in shared memory goes by the groups that each has threads for. Two or more in registers: these. One: of BF16 registers all the same (their next token needs no
+// barrier), but not where shared memory holds two and the walks are long; of FP32 shared memory. In registers / in shared memory, us:
+//   BF16, tokens     3616 channels       4096           4608           5120           6144           6656          7168
+//    1500                           13.7 / 16.0    14.2 / 17.1    14.9 / 17.7    16.2 / 19.6    17.0 / 21.1    17.6 / 21.6
+//    3000          21.2 / 22.2      21.7 / 23.0    22.9 / 28.0    23.7 / 28.5    26.2 / 31.3    28.1 / 34.1
+//    4500                           29.8 / 30.3
+//    6000          38.8 / 36.2      40.5 / 37.1
+//    8192          54.5 / 45.6      58.2 / 46.6    61.8 / 63.6    65.1 / 63.9    72.3 / 70.4    76.0 / 78.0    79.3 / 79.9
+//   16384         108.6 / 83.5     112.3 / 84.5   118.1 / 119.3  124.8 / 119.6  138.5 / 133.0  146.6 / 147.3  152.8 / 154.0
+//   FP32, tokens     2080 channels       2560           4096
+//    1000          12.0 / 9.8       13.8 / 11.2    13.8 / 15.8
+//    4500          38.3 / 25.8      45.9 / 29.7    46.9 / 47.2
+//    8192          64.7 / 39.8      76.5 / 49.3    82.3 / 77.7
+// Two in registers, 8192 tokens: BF16 2048 22.9 / 27.2, 3584 38.6 / 41.3; FP32 2048 42.0 / 40.9, 1531 tokens 11.6 / 12.3.
+constexpr uint32_t kLongWalk = 32;                            // turns of one group on every SM
 struct NormGradShape { uint32_t threads, groups, pieces, stages, parts, smem; };   // stages: 0 in registers
 static NormGradShape norm_grad_shape(uint32_t tokens, uint32_t hidden, bool fp32, uint32_t channel_bytes) {
     NormGradShape s{};
-    const bool whole = fp32 ? hidden < kLongRowsFp32 : hidden < kLongRows || (hidden > 6144 && hidden <= 7168);
+    const uint32_t one = norm_threads(hidden, 1), in_registers = (fp32 ? 512 : 896) / one, in_smem = kLongThreads / one;
+    const bool whole = in_registers > 1 || (in_registers == 1 && !fp32 && (in_smem == 1 || tokens <= kLongWalk * 148));
     const uint32_t most = !whole ? kLongThreads : fp32 ? 512 : 896, token = hidden * channel_bytes;
-    s.pieces = norm_threads(hidden, 1) <= kLongThreads ? 1 : 2;
+    s.pieces = one <= kLongThreads ? 1 : 2;
     s.threads = norm_threads(hidden, s.pieces);
     s.groups = most / s.threads < kMostGroups ? most / s.threads : kMostGroups;
     while (s.groups > 1 && (s.groups - 1) * 148 >= tokens) --s.groups;
@@ -669,20 +682,23 @@ extern "C" int dg_rms_norm_fp8_launch(const void* x, int is_fp32, uint64_t x_str
     a.sf = reinterpret_cast<uint8_t*>(out_sf); a.sf_col_stride = sf_col_stride * 2;
     a.rstd = rstd; a.tokens = tokens; a.hidden = hidden; a.eps = eps;
     a.inverse_hidden = 1.0 / hidden;
-    // In registers / by bulk copies, us of 8192 tokens: BF16 512 10.3 / 11.5, 1024 18.8 / 16.8, 2048 33.9 / 30.9, 4096 59.3 / 56.1, 7168 89.1 / 92.6; FP32 1024 23.6 / 24.0, 2048
-    // 52.6 / 46.7, 7168 171 / 158, 8192 187 / 159; few turns do not pay for the copies' start: 1024 x 7168 of BF16 12.6 / 15.6, 600 x 2048 4.7 / 5.3, but 2000 x 2048 9.7 / 7.7.
+    // In registers / by bulk copies, us of 8192 tokens: BF16 512 10.3 / 11.5, 1024 16.1 / 17.5, 1536 27.1 / 24.2, 2048 32.8 / 29.6, 2560 45.8 / 36.5, 3584 49.8 / 50.9, 4096 53.2 / 53.1,
+    // 7168 89.1 / 92.6; FP32 1024 23.6 / 24.0, 2048 52.6 / 46.7, 7168 171 / 158, 8192 187 / 159. Few turns do not pay for the copies' start. Between 1024 and 2000 tokens it goes by
+    // how the last turn is filled: BF16 x 2048 of 1024 tokens 6.0 / 4.8, 1300 6.2 / 7.6, 1700 7.9 / 7.8, 2300 10.7 / 8.1; x 2560 of 600 to 1100 about the same, 1300 9.1 / 7.5, 2300 14.3 /
+    // 11.7; FP32 x 2048 of 1100 9.5 / 7.3, 1300 9.6 / 10.1, 1700 12.5 / 11.2; x 7168 of 1300 26.4 / 28.5, 2300 45.2 / 45.8. With two pieces a thread, and up to 1024 channels, registers
+    // win with any number of tokens: BF16 x 4096 of 1300 8.9 / 12.0, 3000 18.9 / 25.7, 16384 101.8 / 100.7; x 1024 of 1700 4.8 / 5.3, 6000 12.5 / 14.0, 16384 31.0 / 33.8.
     // In registers two pieces a thread and two CTAs on an SM for long rows of BF16 (7168 89 us against 100 with one piece) but for few tokens (1 / 128 x 7168 2.4 / 3.0 us
     // with one piece, 2.7 / 3.2 with two).
     const uint32_t one = norm_threads(hidden, 1);
     const bool two = !is_fp32 && one > 448 && one <= 896 && tokens > 148;
     void* params[] = {&a};
-    if (one <= 1024 && (hidden < 1024 || tokens <= 1024 || (two && hidden > 4096))) {
+    if (one <= 1024 && (hidden <= 1024 || tokens <= 1024 || two)) {
         const uint32_t threads = two ? norm_threads(hidden, 2) : one, resident = 896 / threads < 1 ? 1 : 896 / threads > 16 ? 16 : 896 / threads;
         return launch_overlapped(two ? (const void*)rms_norm_fp8_kernel<__nv_bfloat16, 2, 448, 2> : is_fp32 ? (const void*)rms_norm_fp8_kernel<float, 1, 1024, 1>
                                                                                               : (const void*)rms_norm_fp8_kernel<__nv_bfloat16, 1, 1024, 1>,
                                  dim3(tokens < 148 * resident ? tokens : 148 * resident), dim3(threads), params, static_cast<cudaStream_t>(stream));
     }
-    // (two pieces a thread of BF16: 7168 104 us with one, 4096 58)
+    // (two pieces a thread of BF16: 7168 104 us with one)
     const uint32_t pieces = is_fp32 && one <= kLongThreads ? 1 : 2, token = hidden * (uint32_t)(residual ? 2 * es : es);
     a.threads = norm_threads(hidden, pieces);
     a.groups = kLongThreads / a.threads < kMostGroups ? kLongThreads / a.threads : kMostGroups;

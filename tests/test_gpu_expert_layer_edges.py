@@ -177,6 +177,15 @@ def test_rows_next_to_a_border_do_not_depend_on_their_number(hidden):
     assert torch.equal(deep_gemm.rms_norm_to_fp8(x.repeat(3, 1), w)[3], few.repeat(3))
 
 
+@pytest.mark.parametrize('tokens,hidden', [(4736, 3616), (4737, 3616), (5003, 4096), (5003, 4128)])
+def test_gradient_on_both_sides_of_a_long_walk(tokens, hidden):
+    """BF16 rows of which a CTA holds one in registers and two in shared memory."""
+    seed_all(tokens + hidden)
+    h, g, more = torch.randn(tokens, hidden).bfloat16(), torch.randn(tokens, hidden).bfloat16(), torch.randn(tokens, hidden).bfloat16()
+    weight = torch.randn(hidden)
+    _check_grad(g, h, weight, oracle.rms_norm_ref(h, weight, 1e-6)[0].float(), more)
+
+
 WAITS = '''
 #include "%s"
 namespace dg {
@@ -201,20 +210,20 @@ def test_a_wait_that_gives_up_is_reported(tmp_path):
     for name in ('dg_rms_norm_fp8_launch', 'dg_rms_norm_grad_launch'):
         getattr(lib, name).restype, getattr(lib, name).argtypes = L._PROTOTYPES[name]
     stream = torch.cuda.current_stream().cuda_stream
-    # four, one and two tokens ahead; several groups of a CTA, and one; one turn, and many
-    for dtype, tokens, hidden in ((BF16, 1100, 1024), (BF16, 1100, 16384), (torch.float32, 100, 16384), (torch.float32, 1100, 4096), (torch.float32, 1100, 2080)):
+    # four, one and two tokens ahead; several groups of a CTA, and one; one turn, and many; whether the norm and its gradient have bulk copies there
+    for dtype, tokens, hidden, forward, backward in ((BF16, 1100, 1056, True, False), (BF16, 1100, 16384, True, True), (torch.float32, 100, 16384, True, True),
+                                                     (torch.float32, 1100, 4096, True, True), (torch.float32, 1100, 2080, True, True), (BF16, 5000, 4096, False, True)):
         x, w, fp32 = torch.randn(tokens, hidden, device='cuda').to(dtype), torch.randn(hidden, device='cuda'), int(dtype == torch.float32)
         q, sf = torch.zeros(tokens, hidden, dtype=torch.uint8, device='cuda'), torch.zeros(hidden // 64 + 1, tokens, dtype=torch.int16, device='cuda')
         rstd, h = torch.zeros(tokens, device='cuda'), torch.zeros_like(x)
         assert lib.dg_rms_norm_fp8_launch(x.data_ptr(), fp32, hidden, x.data_ptr(), hidden, h.data_ptr(), hidden, w.data_ptr(), 1, 1e-6, tokens, hidden, q.data_ptr(), hidden,
                                           sf.data_ptr(), tokens, None, 0, rstd.data_ptr(), stream) == 0
-        assert lib.take_status() == 108 and lib.take_status() == 0 and rstd.isnan().all() and (q == 0).all()
+        assert lib.take_status() == (108 if forward else 0) and lib.take_status() == 0 and rstd.isnan().all() == forward and (q == 0).all() == forward
         ones = torch.ones(tokens, device='cuda')
         dx, dw, scratch = torch.zeros_like(x), torch.zeros(hidden, device='cuda'), torch.empty(148 * hidden, device='cuda')
         assert lib.dg_rms_norm_grad_launch(x.data_ptr(), fp32, hidden, x.data_ptr(), fp32, hidden, w.data_ptr(), 1, ones.data_ptr(), x.data_ptr(), hidden,
                                            tokens, hidden, dx.data_ptr(), hidden, dw.data_ptr(), scratch.data_ptr(), scratch.numel() * 4, stream) == 0
-        long = dtype == torch.float32 or hidden >= 4096
-        assert lib.take_status() == (108 if long else 0) and dw.isnan().all() == long and (dx == 0).all() == long
+        assert lib.take_status() == (108 if backward else 0) and dw.isnan().all() == backward and (dx == 0).all() == backward
         # the library itself reports nothing, and works
         want = deep_gemm.rms_norm_to_fp8(x, w)[3]
         assert deep_gemm.device_status() == 0 and not want.isnan().any()
