@@ -119,7 +119,8 @@ __device__ __forceinline__ uint32_t f16x2_to_e4m3(uint32_t v) {
 __device__ __forceinline__ bool quantise_down_fp8(const uint2 (&q)[8], uint32_t pair, uint32_t block, uint32_t least, uint32_t lane, uint2& bytes, uint2 (&codes)[8]) {
     const uint32_t b0 = pair & 0xffu, b1 = pair >> 8;
     const uint32_t top = __reduce_max_sync(0xffffffffu, max(b0, b1)), low = __reduce_min_sync(0xffffffffu, min(b0, b1));
-    if (top == 255u || low == 0u || top - low > 15u) return false;
+    // (from 2^120 on codes stand for numbers beyond FP32, which are infinities there whatever else the tile holds)
+    if (top > 246u || low == 0u || top - low > 15u) return false;
     // (2^-15 is a subnormal number of FP16)
     const uint32_t factors = max((15u - (top - b0)) << 10, 0x0200u) | max((15u - (top - b1)) << 10, 0x0200u) << 16, both = block ? 0x3232u : 0x1010u;
     uint32_t h[8][4], m[4] = {};

@@ -133,6 +133,23 @@ def test_codes_that_are_not_numbers_show_in_the_gradient():
     assert torch.equal(dx.isnan().cpu(), bad) and dw.isnan().all()
 
 
+@pytest.mark.parametrize('host', quant_hosts)
+def test_codes_beyond_the_range_are_infinities_whatever_lies_beside_them(host):
+    """-256 x 2^120, what the lowest BF16 number becomes, in tiles whose other rows have scales near to that one and far from it."""
+    for other in (247, 240, 200, 0):
+        codes, byte = torch.full((64, 64), 0x30, dtype=torch.uint8), torch.full((64, 2), other, dtype=torch.int32)
+        codes[5, 3], codes[5, 40], codes[9, 7] = 0xF8, 0x78, 0x77             # -256, 256, and 240, which is within
+        byte[5] = byte[9] = 247
+        sf = (byte[:, :1] | byte[:, 1:] << 8)
+        sf = torch.where(sf >= 32768, sf - 65536, sf).to(torch.int16)
+        q, out = host.cast_to_fp8((codes.cuda().view(torch.float8_e4m3fn), sf.cuda()), mn_major=True)
+        first = out.cpu().int() & 255
+        want = oracle.cast_fp8_ref((codes.view(torch.float8_e4m3fn).double() * torch.exp2((byte - 127).double()).repeat_interleave(32, 1)).float(), 0, 1e-4)
+        assert torch.equal(first[0], want[1][0].int()) and first[0, 3] == first[0, 40] == 255 and first[0, 7] == 247
+        fine = (want[1] != 255).repeat_interleave(32, 0)
+        assert torch.equal(q.view(torch.uint8).cpu()[fine], want[0][fine])
+
+
 # ---------------------------------------------------------------------------------------------------------- the norm
 @pytest.mark.parametrize('dtype,hidden', [(BF16, 96), (BF16, 2048), (BF16, 4096), (BF16, 7168), (BF16, 8224), (torch.float32, 96), (torch.float32, 2048),
                                           (torch.float32, 4128), (torch.float32, 8224)])
