@@ -6,6 +6,7 @@ import math
 import os
 import shutil
 import subprocess
+import sys
 
 import pytest
 import torch
@@ -244,3 +245,36 @@ def test_a_wait_that_gives_up_is_reported(tmp_path):
         # the library itself reports nothing, and works
         want = deep_gemm.rms_norm_to_fp8(x, w)[3]
         assert deep_gemm.device_status() == 0 and not want.isnan().any()
+
+
+FIRST = '''
+import sys
+sys.path.insert(0, %r)
+import torch
+import deep_gemm
+x, w, g = torch.randn(1100, 2048, device='cuda').bfloat16(), torch.ones(2048, device='cuda'), torch.randn(1100, 4096, device='cuda')
+wide = torch.ones(4096, device='cuda')
+
+
+def way():
+    (q, sf), rows, h, rstd = deep_gemm.rms_norm_to_fp8(x, w, residual=x, with_rows=True)
+    return [q.view(torch.uint8), sf, rows, h, rstd, *deep_gemm.rms_norm_grad(g, g, wide, rstd, grad_h=g)]
+
+
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    held = way()
+graph.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(held, way())) and deep_gemm.device_status() == 0
+print('PASS')
+'''
+
+
+def test_bulk_copies_in_a_capture_that_holds_the_first_call():
+    """The norm's forms that raise a limit of shared memory, in the first call of a process."""
+    package = os.path.dirname(os.path.dirname(os.path.abspath(deep_gemm.__file__)))
+    for host in '01':
+        proc = subprocess.run([sys.executable, '-c', FIRST % package], capture_output=True, text=True, timeout=600, env={**os.environ, 'DG_PYTHON_HOST': host})
+        assert proc.returncode == 0 and 'PASS' in proc.stdout, proc.stderr[-3000:]
