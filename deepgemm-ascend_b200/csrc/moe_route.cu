@@ -14,9 +14,10 @@
 // One warp a token, nothing shared between warps. A group of experts lies in 32 / num_groups lanes (rounded down to a power of two), so that a
 // lane holds experts of one group only and a group that is not taken is dropped by its lanes.
 //
-// Bound by instructions, about 800 of a warp for a token of 256 experts and 8 choices: 16384 tokens (sigmoid, bias, 4 of 8 groups, FP32) 17.2 to 17.9 us, where the bytes
-// alone take 2.7; 128 tokens 2.6 us, launch and latency. (A maximum of scores and then one of the indices that hold it took 43.6, whole-number keys 24 to 26; all
-// 64-bit scores where only the order is open 24 where those of the chosen take 19.) The gradient, 16384 x 256 of a softmax that is not renormalised, 6.7 us, 5.2 TB/s.
+// Bound by instructions, about 800 of a warp for a token of 256 experts and 8 choices: 16384 tokens (sigmoid, bias, 4 of 8 groups, FP32) 17.1 to 19.9 us by
+// the input, where the bytes alone take 2.7; without a bias 19.7, of a softmax without groups 13.4 (BF16, whose logits are often equal, 20.3); 128 tokens 2.6 us, launch and latency. (A maximum of scores and then one of the indices that hold it took 43.6, whole-number keys 24 to 26; all
+// 64-bit scores where only the order is open 24 where those of the chosen take 19.) The gradient, 16384 x 256 of a softmax that is not renormalised, 6.5 us, 5.4 TB/s.
+// (Every form has a frame of 136 bytes for the arguments of what is out of line; 64 experts a lane, one at a time, spill 76 bytes besides.)
 #include <cuda_runtime.h>
 #include <math_constants.h>
 #include <stdint.h>

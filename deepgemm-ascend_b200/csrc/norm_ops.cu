@@ -219,7 +219,7 @@ __device__ __forceinline__ void finish_piece(const NormArgs& a, uint64_t token, 
 
 // Few tokens, short rows and some of the middle: a CTA walks tokens at a distance of the grid, a thread kPieces x 8 channels of each. The next token is asked for before
 // the sum over the CTA: what keeps HBM busy over the barrier. 8192 x 7168 of BF16 with a residual and BF16 rows 89 us, 5.9 TB/s, where the bytes alone take 81 at the rate
-// of a copy (a CTA for every token took 106, L2 asked for the token behind the next 109). 1 x 7168: 2.4 us, launch and latency.
+// of a copy (a CTA for every token took 106, L2 asked for the token behind the next 109). 1 x 7168: 2.4 to 2.7 us, launch and latency.
 template <typename T, uint32_t kPieces, uint32_t kThreads, uint32_t kCtas>
 __global__ void __launch_bounds__(kThreads, kCtas) rms_norm_fp8_kernel(const NormArgs a) {
     __shared__ double partial[2][kPieces * (kThreads / 32)];
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kLongThreads) rms_norm_fp8_long_kernel(const N
 // a token, and walks tokens at a distance of all groups; a thread holds its channels' part of dweight in registers (FP32), the groups of a CTA add theirs up,
 // and a second kernel sums the CTAs' in their order: nothing depends on timing.
 //
-// HBM-bound: 8192 x 7168 of BF16 with a gradient of h 79 us, 5.9 TB/s (the bytes alone 72 at the rate of a copy); 1531 x 2048 of FP32 11.6 us, of which the second
+// HBM-bound: 8192 x 7168 of BF16 with a gradient of h 79 us, 5.9 TB/s (the bytes alone 72 at the rate of a copy); 1531 x 2048 of FP32 11.4 us, of which the second
 // kernel and the launches take 3.
 struct NormGradArgs {
     const uint8_t* g; uint64_t g_stride;                                 // BF16 or FP32 as `h` is, or BF16 beside FP32

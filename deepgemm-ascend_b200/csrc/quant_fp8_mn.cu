@@ -6,7 +6,8 @@
 // infinity or a NaN gets the scale byte of NaN.
 //
 // HBM-bound: 2 (or 1 + 1/32) bytes read and 1 + 1/32 written per value. 32768 x 7168 from 8 bits 100 us, 5.0 TB/s (the bytes alone 78 at the rate of a copy: the
-// instructions of the conversions fill 63 % of the issue slots); 16384 x 7168 from BF16 50 us, 6.1 TB/s, and back to BF16 55 us, 5.4 TB/s.
+// instructions of the conversions fill 63 % of the issue slots); 16384 x 7168 from BF16 54 us, 6.6 TB/s, and back to BF16 56 us, 6.4 TB/s, from
+// scales along the rows 54.
 #include <cuda_runtime.h>
 #include <stdint.h>
 #include <string.h>
@@ -112,7 +113,7 @@ __device__ __forceinline__ uint32_t f16x2_to_e4m3(uint32_t v) {
 // time: amax <= 448 s = 1.75 x 2^8 s, so with amax = 1.m x 2^x (m of ten bits) s is 2^(x - 8), or twice that where m is above 0.75, which is an addition
 // to the bits that carries; `least` is the byte of the least amax.
 //
-// (Through FP32, which takes every input, 32768 x 7168 takes 173 us, through FP16 102, or 114 where each lane makes its own factors.)
+// (Through FP32, which takes every input, 32768 x 7168 takes 173 us, through FP16 100, or 114 where each lane makes its own factors. 40 bytes are spilled.)
 //
 // Whatever a row or a column has once is made once and handed round: `pair` holds the bytes of row `lane` (of the tile's two blocks), `block` says which of them
 // this lane's columns lie in, and of the four words of columns that the lanes of a row share each of the four lanes of a column makes one.

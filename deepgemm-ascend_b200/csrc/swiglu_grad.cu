@@ -4,11 +4,12 @@
 // r = min(max(x_r, -clamp), clamp), p = 1 / (1 + e^-l):
 //     dx_l = g w r p (1 + l (1 - p)) where x_l <= clamp (else 0)      dx_r = g w l p where |x_r| <= clamp (else 0)
 //     dw = sum over the row of g l p r
+// A NaN is on no side of the clamp here and shows in all three; the forward pass, which takes minima and maxima, makes the clamp of it.
 // all in FP32 (the fast exponential and reciprocal: p within a few ulp, and 0 below 2^-126), dx rounded once to BF16.
 //
 // HBM-bound: 2 H + 2 H + H / 16 bytes read (6 H from BF16) and 4 H written per row; the arithmetic, two channels an instruction, is two thirds of that time.
-// 65536 x 2048 from 8 bits 179 us, 6.0 TB/s (the bytes alone 165 at the rate of a copy; 199 in a long row of passes, which draws the power cap); 77 x 2048 from BF16
-// 2.6 us, launch and latency.
+// 65536 x 2048 from 8 bits 178 us, 6.1 TB/s (the bytes alone 165 at the rate of a copy; 200 in a long row of passes, which draws the power cap), from BF16 212 us, 6.3 TB/s; 77 x 2048
+// from BF16 2.7 us, launch and latency, with weights 4.3 (a second launch). At 64 registers it spills 40 bytes from BF16, 24 from 8 bits with a clamp.
 #include <cuda_runtime.h>
 #include <stdint.h>
 
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(kGradThreads, 8) swiglu_grad_kernel(const Swig
         for (int j = 0; j < 4; ++j) {
             bool outside_l[2] = {}, outside_r[2] = {};
             if constexpr (kClamp) {
-                // (a NaN is on no side of the clamp, and stays one)
+                // (a NaN is on no side of it, and stays one)
                 float lv[2], rv[2];
                 l[j].get(lv[0], lv[1]);
                 r[j].get(rv[0], rv[1]);

@@ -149,8 +149,9 @@ def swiglu_apply_weight_grad(grad_out: torch.Tensor, x, topk_weights: Optional[t
     """Gradients of `swiglu_apply_weight_to_fp8` for grad_out BF16 [tokens, hidden]: (grad_x BF16 [tokens, 2 * hidden], grad_weights float32 like
     topk_weights, or None). x is the BF16 input or the 8-bit pair that `..._with_checkpoint` (or `cast_to_fp8`) made of it. Where the clamp cuts off
     the gradient is 0. What rows without a value (the padding of a psum layout, rows behind its last group) hold does not matter; their weights
-    have the gradient 0, and grad_x is not written there, but for the zeros that `zero_padding` puts into the padding. `out`: where grad_x goes. Rows of BF16 start on
-    16-byte boundaries, those of E4M3 on 8."""
+    have the gradient 0, and grad_x is not written there, but for the zeros that `zero_padding` puts into the padding. `out`: where grad_x goes, which may overlap
+    nothing else. Rows of BF16 start on 16-byte boundaries, those of E4M3 on 8. A NaN in x shows here whether there is a clamp or not; the forward pass takes minima
+    and maxima, and makes the clamp of it."""
     psum, is_pair = psum_num_tokens_per_expert, isinstance(x, (tuple, list))
     x, sf = x if is_pair else (x, None)
     _host_assert(grad_out.is_cuda and grad_out.dim() == 2 and grad_out.stride(1) == 1 and grad_out.dtype == torch.bfloat16,
@@ -241,7 +242,7 @@ def _check_scales(x, sf, groups, run, k64, mn_major):
 
 def cast_from_fp8(x, out_dtype: torch.dtype = torch.bfloat16, mn_major: bool = False):
     """The pair that `cast_to_fp8` makes (or any E4M3 operand with packed scales) -> [.., rows, cols] BF16 or FP32: the values that a product with it
-    sees, code times scale."""
+    sees, code times scale. (What lies beyond FP32, such as the -2^128 that the lowest BF16 number becomes, is an infinity.)"""
     codes, sf = x
     _host_assert(codes.is_cuda and codes.dim() in (2, 3) and codes.dtype == torch.float8_e4m3fn and codes.stride(-1) == 1,
                  'x must be a row-major 2-D or 3-D E4M3 tensor on a CUDA device, with its scales')
@@ -271,7 +272,7 @@ def rms_norm_to_fp8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[to
 
     weight: BF16 or FP32 [hidden]. The sum of squares is held in 64 bits: a token's results do not depend on how many others there are. `out_h`:
     where h goes with a residual, which may be `residual` or x itself. hidden is a multiple of 32, at most 16384; rows start on 16-byte boundaries.
-    out_sf and rstd may share one allocation."""
+    out_sf and rstd may share one allocation: keeping rstd keeps the scales."""
     _host_assert(x.is_cuda and x.dim() == 2 and x.stride(1) == 1 and _is_float(x), 'x must be a row-major 2-D BF16 or FP32 tensor on a CUDA device')
     tokens, hidden = x.shape
     _check_norm(x, weight, tokens, hidden)

@@ -301,7 +301,7 @@ int dg_swiglu_checkpoint_launch(const void* x, uint64_t x_stride, uint32_t token
 
 /* Its gradient. grad_out BF16 [tokens, hidden]; x [tokens, 2 * hidden] BF16 (x_sf NULL), or E4M3 with the scales that
  * dg_swiglu_checkpoint_launch writes; grad_x BF16 [tokens, 2 * hidden]; grad_weights float [tokens] or NULL (0 for rows without a value). Where the
- * clamp cuts off, the gradient is 0. What rows of the psum layout's padding, and behind its last group, hold does not matter; `zero_padding`
+ * clamp cuts off, the gradient is 0; a NaN, of which the forward pass makes the clamp, is a NaN. What rows of the psum layout's padding, and behind its last group, hold does not matter; `zero_padding`
  * writes zeros to the former. grad_x may not overlap anything else. `scratch`: with grad_weights, dg_swiglu_grad_scratch_bytes (0 for short rows) of device memory that
  * the call may use until it has run. hidden % 64 == 0; rows 16-byte aligned (8 for E4M3). */
 uint64_t dg_swiglu_grad_scratch_bytes(uint32_t tokens, uint32_t hidden);
